@@ -21,7 +21,7 @@ LIB = os.path.join(HERE, "libnvfp4kv.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 SOURCES = ["abi_common.cu", "nvfp4_append.cu", "nvfp4_gather.cu", "nvfp4_rope.cu", "nvfp4_indexer.cu", "nvfp4_mla_decode.cu",
-           "nvfp4_mla_decode_fp4.cu", "nvfp4_mla_decode_static.cu"]
+           "nvfp4_mla_decode_fp4.cu", "nvfp4_mla_decode_static.cu", "rotary.cu", "cache_pages.cu", "mla_prefill.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
               "-I", INCLUDE]
@@ -35,7 +35,7 @@ def nvcc() -> str:
 
 
 def _deps_mtime() -> float:
-    newest = os.path.getmtime(os.path.join(INCLUDE, "nvfp4kv.h"))
+    newest = max(os.path.getmtime(os.path.join(INCLUDE, h)) for h in ("nvfp4kv.h", "nvfp4kv_serving.h"))
     for f in os.listdir(CSRC):
         if f.endswith((".cuh", ".h")):
             newest = max(newest, os.path.getmtime(os.path.join(CSRC, f)))

@@ -23,6 +23,7 @@ stream; nothing synchronises the host and nothing falls back to the CPU.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 
 import torch
@@ -595,3 +596,325 @@ def index_scores_buffer(device=None) -> torch.Tensor | None:
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     ws = _bufs.get(("index_ws", dev.index))
     return None if ws is None else ws.view(torch.float32)
+
+
+# ------------------------------------------------------------------ rotary positions
+_ROPE_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
+_INDEX_DTYPES = {torch.int64: _lib.INDEX_I64, torch.int32: _lib.INDEX_I32}
+
+
+def rope_cos_sin(max_positions: int, rotary_dim: int = ROPE, base: float = 10000.0, factor: float = 1.0,
+                 original_positions: int | None = None, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                 attention_factor: float | None = None, device=None) -> torch.Tensor:
+    """The cos | sin table of the rotary operators, float32 [max_positions, rotary_dim], computed
+    in float64.  ``factor`` > 1 stretches the positions for long contexts: by it alone
+    (position interpolation), or, with ``original_positions`` (the trained length), by the YaRN
+    rule: dims that turn more than ``beta_fast`` times over the trained length keep their
+    frequency, those that turn less than ``beta_slow`` times are divided by ``factor``, the ones
+    between are blended linearly, and cos and sin carry ``attention_factor`` (default
+    0.1 ln(factor) + 1)."""
+    if rotary_dim < 2 or rotary_dim % 2 or max_positions < 1:
+        raise ValueError("rotary_dim must be even and >= 2, max_positions >= 1")
+    half = rotary_dim // 2
+    inv = base ** (-torch.arange(half, dtype=torch.float64) / half)
+    gain = 1.0
+    if factor != 1.0 and original_positions is None:
+        inv = inv / factor
+    elif factor != 1.0:
+        def dim_of(turns):      # the dim that turns `turns` times over the trained length
+            return half * math.log(original_positions / (turns * 2 * math.pi)) / math.log(base)
+
+        lo, hi = max(math.floor(dim_of(beta_fast)), 0), min(math.ceil(dim_of(beta_slow)), half - 1)
+        blend = ((torch.arange(half, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        inv = inv * (1 - blend) + inv / factor * blend
+        gain = 0.1 * math.log(factor) + 1.0 if attention_factor is None else attention_factor
+    angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * inv.to(device)
+    return (torch.cat([angle.cos(), angle.sin()], 1) * gain).float()
+
+
+def _check_angles(cos_sin: torch.Tensor, positions: torch.Tensor, T: int, rotary_dim: int):
+    _require_cuda(cos_sin, "cos_sin")
+    _require_cuda(positions, "positions")
+    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != rotary_dim \
+            or not cos_sin.is_contiguous():
+        raise ValueError(f"cos_sin must be a contiguous float32 [positions, {rotary_dim}] table")
+    pos = positions.reshape(-1).contiguous()
+    if pos.numel() != T:
+        raise ValueError(f"positions has {pos.numel()} entries for {T} tokens")
+    if pos.dtype not in _INDEX_DTYPES:
+        raise TypeError("positions must be int64 or int32")
+    return pos, _INDEX_DTYPES[pos.dtype]
+
+
+def apply_rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, rope_offset: int | None = None,
+               interleaved: bool = True, inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions: x [T, H, D] or [T, D] (bf16, fp16 or fp32, last dim contiguous), dims
+    [rope_offset, rope_offset + cos_sin.shape[1]) of every head rotated by its token's angles
+    (default: the last dims), the others copied.  ``interleaved`` pairs dims (2i, 2i + 1), else
+    (i, i + half).  ``inverse`` rotates back: the gradient with respect to x.  ``out`` may be x;
+    a position outside the table leaves its token as it is and is flagged in the device error
+    word.  cos_sin: see rope_cos_sin."""
+    _require_cuda(x, "x")
+    if x.dtype not in _ROPE_DTYPES:
+        raise TypeError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
+    if x.dim() not in (2, 3) or x.stride(-1) != 1:
+        raise ValueError("x must be [T, H, D] or [T, D] with a contiguous last dimension")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _require_cuda(out, "out")
+    if out.shape != x.shape or out.dtype != x.dtype or out.stride(-1) != 1:
+        raise ValueError("out must have x's shape and dtype and a contiguous last dimension")
+    T, D = x.shape[0], x.shape[-1]
+    H = x.shape[1] if x.dim() == 3 else 1
+    r = cos_sin.shape[-1]
+    off = D - r if rope_offset is None else int(rope_offset)
+    pos, pdt = _check_angles(cos_sin, positions, T, r)
+    if T == 0 or H == 0:
+        return out
+    dev = x.device
+    with _on_device(dev):
+        rc = _lib.lib().nvfp4kv_rope(x.data_ptr(), _ROPE_DTYPES[x.dtype], T, H, D, x.stride(0),
+                                     x.stride(1) if x.dim() == 3 else D, pos.data_ptr(), pdt, cos_sin.data_ptr(),
+                                     cos_sin.shape[0], r, off, int(interleaved), int(inverse), out.data_ptr(),
+                                     out.stride(0), out.stride(1) if x.dim() == 3 else D, _err_word(dev).data_ptr(),
+                                     _stream(dev))
+    _lib.check(rc, "nvfp4kv_rope")
+    return out
+
+
+def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                             positions: torch.Tensor, cos_sin: torch.Tensor, q_pe: torch.Tensor | None = None,
+                             q_out: torch.Tensor | None = None, interleaved: bool = True) -> torch.Tensor | None:
+    """The rope part of a step in one launch: k_pe [T, 64] bf16, rotated by its tokens' angles,
+    into the rope side-pool at slot_mapping (as write_nvfp4_rope), and the queries' rope dims
+    q_pe [T, H, 64] bf16 rotated into q_out (default: in place).  Returns q_out."""
+    T = k_pe.shape[0]
+    _require_cuda(k_pe, "k_pe")
+    _require_cuda(rope_cache, "rope_cache")
+    if k_pe.dtype != torch.bfloat16 or k_pe.dim() != 2 or k_pe.shape[1] < ROPE or k_pe.stride(1) != 1:
+        raise ValueError("k_pe must be bf16 [T, >=64] with a contiguous last dimension")
+    rope = rope_cache.view(-1, ROPE)
+    if rope.dtype != torch.bfloat16:
+        raise TypeError("rope_cache must be bf16")
+    slot = slot_mapping.reshape(-1).contiguous()
+    if slot.numel() != T:
+        raise ValueError(f"slot_mapping has {slot.numel()} entries for {T} tokens")
+    if slot.dtype not in _INDEX_DTYPES:
+        raise TypeError("slot_mapping must be int64 or int32")
+    pos, pdt = _check_angles(cos_sin, positions, T, ROPE)
+    H, qs, qos = 0, (0, 0), (0, 0)
+    if q_pe is not None:
+        q_out = q_pe if q_out is None else q_out
+        for name, t in (("q_pe", q_pe), ("q_out", q_out)):
+            _require_cuda(t, name)
+            if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[0] != T or t.shape[2] != ROPE or t.stride(2) != 1:
+                raise ValueError(f"{name} must be bf16 [T, H, 64] with a contiguous last dimension")
+        if q_out.shape != q_pe.shape:
+            raise ValueError("q_out must have q_pe's shape")
+        H, qs, qos = q_pe.shape[1], q_pe.stride()[:2], q_out.stride()[:2]
+    elif q_out is not None:
+        raise ValueError("q_out without q_pe")
+    if T == 0:
+        return q_out
+    dev = k_pe.device
+    with _on_device(dev):
+        rc = _lib.lib().nvfp4kv_append_rope_rotated(
+            k_pe.data_ptr(), T, k_pe.stride(0), rope.data_ptr(), rope.shape[0], slot.data_ptr(),
+            _INDEX_DTYPES[slot.dtype], pos.data_ptr(), pdt, cos_sin.data_ptr(), cos_sin.shape[0], int(interleaved),
+            q_pe.data_ptr() if H else None, H, *qs, q_out.data_ptr() if H else None, *qos,
+            _err_word(dev).data_ptr(), _stream(dev))
+    _lib.check(rc, "nvfp4kv_append_rope_rotated")
+    return q_out
+
+
+# ------------------------------------------------------------------ chunk attention
+def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: torch.Tensor | None,
+                kv_lora_rank: int, qk_rope_head_dim: int, block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                seq_lens: torch.Tensor, max_q_len: int, max_seq_len: int, out: torch.Tensor | None = None,
+                bmm1_scale: float = 1.0, bmm2_scale: float = 1.0, rope_cache: torch.Tensor | None = None,
+                return_lse: bool = False):
+    """Causal MLA attention of a ragged batch of new tokens over the paged pool, whose rows
+    already hold them: chunked prefill, speculative steps and single tokens in one call.
+
+    query [T, H, kv_lora_rank + qk_rope_head_dim] bf16: the new tokens of sequence b are
+    cu_seqlens_q[b] .. cu_seqlens_q[b + 1], the last of its seq_lens[b] tokens; each sees the
+    tokens up to itself.  kv_cache, block_tables, rope_cache and workspace_buffer as in
+    mla_decode (dense).  max_q_len and max_seq_len bound the device-side lengths; nothing
+    synchronises the host.  Returns out [T, H, kv_lora_rank] bf16, with ``return_lse`` also
+    lse [T, H] float32 (natural log; -inf for a row that sees no token, whose out is zeros)."""
+    _require_cuda(query, "query")
+    _require_cuda(kv_cache, "kv_cache")
+    if isinstance(bmm1_scale, torch.Tensor) or isinstance(bmm2_scale, torch.Tensor):
+        raise TypeError("bmm1_scale / bmm2_scale must be Python floats (a device scalar would need a sync)")
+    if query.dtype != torch.bfloat16 or query.dim() != 3 or query.stride(2) != 1:
+        raise ValueError("query must be bf16 [T, H, D] with a contiguous last dimension")
+    T, H, D = query.shape
+    if kv_lora_rank != LATENT or D != kv_lora_rank + qk_rope_head_dim:
+        raise ValueError(f"query dim {D} must equal kv_lora_rank (512) + qk_rope_head_dim")
+    pool = kv_cache.view(-1, NV_BYTES)
+    page_size = kv_cache.shape[-2] if kv_cache.dim() >= 3 else 64
+    for name, t in (("block_tables", block_tables), ("cu_seqlens_q", cu_seqlens_q), ("seq_lens", seq_lens)):
+        _require_cuda(t, name)
+        if t.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32")
+    B = seq_lens.numel()
+    if block_tables.dim() != 2 or block_tables.shape[0] != B or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be [B, width] with a contiguous last dimension")
+    if cu_seqlens_q.numel() != B + 1:
+        raise ValueError("cu_seqlens_q must have one entry more than seq_lens")
+    if block_tables.shape[1] * page_size < max_seq_len:
+        raise ValueError("block_tables too narrow for max_seq_len")
+    if out is None:
+        out = torch.empty(T, H, LATENT, dtype=torch.bfloat16, device=query.device)
+    elif out.shape != (T, H, LATENT) or out.dtype != torch.bfloat16 or out.stride(2) != 1:
+        raise ValueError("out must be bf16 [T, H, 512] with a contiguous last dimension")
+    rope = None
+    if rope_cache is not None:
+        _require_cuda(rope_cache, "rope_cache")
+        rope = rope_cache.reshape(-1, ROPE)
+        if rope.dtype != torch.bfloat16 or rope.shape[0] != pool.shape[0] or not rope.is_contiguous():
+            raise ValueError("rope_cache must be a contiguous bf16 [pool rows, 64] side-pool")
+    lse = torch.empty(T, H, dtype=torch.float32, device=query.device) if return_lse else None
+    dev = query.device
+    if T > 0 and B > 0:
+        with _on_device(dev):
+            key = ("prefill", B, T, H, int(max_q_len), int(max_seq_len), dev.index)
+            need = _ws_sizes.get(key)
+            if need is None:
+                n = ctypes.c_size_t(0)
+                _lib.check(_lib.lib().nvfp4kv_mla_prefill_workspace_size(B, T, H, int(max_q_len), int(max_seq_len),
+                                                                         ctypes.byref(n)),
+                           "nvfp4kv_mla_prefill_workspace_size")
+                need = _ws_sizes[key] = int(n.value)
+            ws = workspace_buffer
+            if need and (ws is None or not ws.is_cuda or not ws.is_contiguous() or ws.data_ptr() % 256
+                         or ws.numel() * ws.element_size() < need):
+                ws = _stream_buffer(dev, "prefill_ws", need, torch.uint8)
+            cu, sl = cu_seqlens_q.contiguous(), seq_lens.contiguous()
+            rc = _lib.lib().nvfp4kv_mla_prefill(
+                query.data_ptr(), query.stride(0), query.stride(1), pool.data_ptr(), pool.shape[0],
+                rope.data_ptr() if rope is not None else None, block_tables.data_ptr(), block_tables.stride(0),
+                cu.data_ptr(), sl.data_ptr(), B, T, H, D, kv_lora_rank, int(page_size), int(max_q_len),
+                int(max_seq_len), float(bmm1_scale), float(bmm2_scale), out.data_ptr(), out.stride(0), out.stride(1),
+                lse.data_ptr() if lse is not None else None, ws.data_ptr() if need else None, need,
+                _err_word(dev).data_ptr(), _stream(dev))
+        _lib.check(rc, "nvfp4kv_mla_prefill")
+    return (out, lse) if return_lse else out
+
+
+# ------------------------------------------------------------------ page upkeep
+def _cache_list(caches):
+    """(device pointers, bytes per page, pages, page size) of pools [num_pages, page_size, ...]."""
+    if not caches:
+        raise ValueError("caches must name at least one pool")
+    pages, size = caches[0].shape[0], caches[0].shape[1]
+    for c in caches:
+        _require_cuda(c, "caches")
+        if c.dim() < 3 or c.shape[0] != pages or c.shape[1] != size or not c.is_contiguous():
+            raise ValueError("caches must be contiguous [num_pages, page_size, ...] pools of one geometry")
+    n = len(caches)
+    ptrs = (ctypes.c_void_p * n)(*[c.data_ptr() for c in caches])
+    sizes = (ctypes.c_int64 * n)(*[c.numel() // pages * c.element_size() if pages else size for c in caches])
+    return ptrs, sizes, n, pages, size
+
+
+def _check_int32(**tensors):
+    for name, t in tensors.items():
+        _require_cuda(t, name)
+        if t.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32")
+        if name.endswith("tables"):
+            if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+                raise ValueError(f"{name} must be [slots, width] with a contiguous last dimension")
+        elif t.dim() != 1 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous vector")
+
+
+def _stream_buffer(dev: torch.device, name: str, n: int, dtype: torch.dtype) -> torch.Tensor:
+    """A persistent buffer of the current stream, so that calls on two streams never share one."""
+    key = (name, dev.index, torch.cuda.current_stream(dev).cuda_stream)
+    ws = _bufs.get(key)
+    if ws is None or ws.numel() < n:
+        ws = _bufs[key] = torch.empty(n, dtype=dtype, device=dev)
+    return ws
+
+
+def copy_pages(caches, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Pages src[k] -> dst[k] (int32) of every pool in ``caches`` ([num_pages, page_size, ...] each:
+    latent rows, rope rows, indexer rows).  Negative ids skip the pair.  A page may not be a
+    source and a destination, nor a destination twice."""
+    ptrs, sizes, n, pages, _ = _cache_list(caches)
+    _check_int32(src=src, dst=dst)
+    if src.numel() != dst.numel():
+        raise ValueError("src and dst must have the same length")
+    dev = caches[0].device
+    with _on_device(dev):
+        rc = _lib.lib().nvfp4kv_copy_pages(ptrs, sizes, n, pages, src.data_ptr(), dst.data_ptr(), src.numel(),
+                                           _err_word(dev).data_ptr(), _stream(dev))
+    _lib.check(rc, "nvfp4kv_copy_pages")
+
+
+def free_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, slots: torch.Tensor,
+               ref_counts: torch.Tensor) -> None:
+    """Empties the sequences in ``slots``: their pages lose one reference each (0 = free), their
+    rows of block_tables [num_slots, width] become -1 and their seq_lens 0, in place."""
+    _check_int32(block_tables=block_tables, seq_lens=seq_lens, slots=slots, ref_counts=ref_counts)
+    if seq_lens.numel() != block_tables.shape[0]:
+        raise ValueError("seq_lens must have one entry per row of block_tables")
+    dev = block_tables.device
+    with _on_device(dev):
+        rc = _lib.lib().nvfp4kv_free_pages(block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
+                                           block_tables.shape[0], seq_lens.data_ptr(), slots.data_ptr(), slots.numel(),
+                                           ref_counts.data_ptr(), ref_counts.numel(), _err_word(dev).data_ptr(),
+                                           _stream(dev))
+    _lib.check(rc, "nvfp4kv_free_pages")
+
+
+def fork_pages(caches, block_tables: torch.Tensor, seq_lens: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+               ref_counts: torch.Tensor) -> None:
+    """Makes the empty slot dst[k] a copy of the sequence in slot src[k], for every k, in place:
+    full pages are shared (one reference more each), the filled rows of a partly filled last
+    page are copied in every pool of ``caches`` into the lowest free page (ref_counts == 0), in
+    order of k.  Beams and samples that share a prompt; see free_pages for the way back."""
+    ptrs, sizes, n, pages, size = _cache_list(caches)
+    _check_int32(block_tables=block_tables, seq_lens=seq_lens, src=src, dst=dst, ref_counts=ref_counts)
+    if src.numel() != dst.numel():
+        raise ValueError("src and dst must have the same length")
+    if seq_lens.numel() != block_tables.shape[0] or ref_counts.numel() != pages:
+        raise ValueError("seq_lens must have one entry per row of block_tables, ref_counts one per page")
+    dev = block_tables.device
+    ws = _stream_buffer(dev, "fork_ws", max(3 * src.numel(), 1024), torch.int32)
+    with _on_device(dev):
+        rc = _lib.lib().nvfp4kv_fork_pages(ptrs, sizes, n, size, block_tables.data_ptr(), block_tables.stride(0),
+                                           block_tables.shape[1], block_tables.shape[0], seq_lens.data_ptr(),
+                                           src.data_ptr(), dst.data_ptr(), src.numel(), ref_counts.data_ptr(), pages,
+                                           ws.data_ptr(), ws.numel(), _err_word(dev).data_ptr(), _stream(dev))
+    _lib.check(rc, "nvfp4kv_fork_pages")
+
+
+def compact_pages(caches, block_tables: torch.Tensor, ref_counts: torch.Tensor, out_tables: torch.Tensor | None = None,
+                  out_ref_counts: torch.Tensor | None = None) -> torch.Tensor:
+    """Moves the pages in use (ref_counts > 0) to the front of every pool of ``caches``: the k-th of
+    those past their number goes to the k-th free page before it.  The tables and counts that go
+    with it are written to out_tables / out_ref_counts (default: in place; an engine whose
+    running step still reads the old tables gives others).  Returns the number of pages in use,
+    int32 [] on the device."""
+    ptrs, sizes, n, pages, _ = _cache_list(caches)
+    out_tables = block_tables if out_tables is None else out_tables
+    out_ref_counts = ref_counts if out_ref_counts is None else out_ref_counts
+    _check_int32(block_tables=block_tables, ref_counts=ref_counts, out_tables=out_tables, out_ref_counts=out_ref_counts)
+    if ref_counts.numel() != pages or out_ref_counts.numel() != pages or out_tables.shape != block_tables.shape:
+        raise ValueError("ref_counts must have one entry per page, out_tables block_tables' shape")
+    dev = block_tables.device
+    live = torch.empty((), dtype=torch.int32, device=dev)
+    need = ctypes.c_int64(0)
+    _lib.check(_lib.lib().nvfp4kv_compact_workspace_ints(pages, ctypes.byref(need)), "nvfp4kv_compact_workspace_ints")
+    ws = _stream_buffer(dev, "compact_ws", need.value, torch.int32)
+    with _on_device(dev):
+        rc = _lib.lib().nvfp4kv_compact_pages(ptrs, sizes, n, block_tables.data_ptr(), block_tables.stride(0),
+                                              block_tables.shape[1], block_tables.shape[0], ref_counts.data_ptr(), pages,
+                                              out_tables.data_ptr(), out_tables.stride(0), out_ref_counts.data_ptr(),
+                                              live.data_ptr(), ws.data_ptr(), ws.numel(), _err_word(dev).data_ptr(),
+                                              _stream(dev))
+    _lib.check(rc, "nvfp4kv_compact_pages")
+    return live
