@@ -28,7 +28,11 @@
 //
 // Warps: 0-7 softmax (a row's 256 scores over four of them), 8-15 producers, 16 issues MMAs (in
 // the leading CTA).  Every wait is bounded (common.cuh).
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <math.h>
+
+#include <mutex>
 
 #include "../../include/nvfp4kv_serving.h"
 #include "abi_common.h"
@@ -43,12 +47,16 @@ constexpr int kDim = kLatent + kRope;
 constexpr int kUnitRows = 128;                  // query rows of a work unit
 constexpr int kCtaRows = 64;
 constexpr int kTile = 256;                      // tokens per tile
-constexpr int kStages = 7;
+constexpr int kStages = 7;                      // ring stages with an image,
+constexpr int kDirectStages = 3;                // and without: the rest of the ring holds raw rows
 constexpr int kStageBytes = 16384;              // 128 rows x 128 B
+constexpr int kRawSlots = 3;
+constexpr int kRawBytes = 128 * (128 + 16);     // 128 rows: 256 dims' codes and scales (or 64 rope dims)
 constexpr int kVStages = 8;                     // V stages of a tile: 4 x 64 tokens x 2 x 128 dims a CTA
-constexpr int kSoftmaxWarps = 8, kProducerWarp0 = 8, kMmaWarp = 16;
+static_assert(kRawSlots * kRawBytes + kDirectStages * kStageBytes <= kStages * kStageBytes, "ring area");
+constexpr int kSoftmaxWarps = 8, kProducerWarp0 = 8, kProducerWarps = 8, kMmaWarp = 16;
 constexpr int kThreads = 20 * 32;
-constexpr uint32_t kRegsSoftmax = 144, kRegsProducer = 72, kRegsCtl = 48;
+constexpr uint32_t kRegsSoftmax = 152, kRegsProducer = 64, kRegsCtl = 48;
 static_assert(256 * kRegsSoftmax + 256 * kRegsProducer + 128 * kRegsCtl <= kThreads * 96,
               "the register split stays within what the block is launched with");
 constexpr float kRescaleLog2 = 8.0f;
@@ -71,7 +79,9 @@ constexpr int B_S_FREE = B_S_FULL + 2;         // [2] leader: S read by both CTA
 constexpr int B_P_FULL = B_S_FREE + 2;         // leader: P written in both CTAs
 constexpr int B_PV_DONE = B_P_FULL + 1;        // both: O stable, P free
 constexpr int B_DRAIN = B_PV_DONE + 1;         // both: every MMA complete
-constexpr int kNumBars = B_DRAIN + 1;
+constexpr int B_RAW_FULL = B_DRAIN + 1;        // [kRawSlots] own: raw rows landed
+constexpr int B_RAW_EMPTY = B_RAW_FULL + kRawSlots;      // own: the producers have read them
+constexpr int kNumBars = B_RAW_EMPTY + kRawSlots;
 constexpr int kSmemBytes = SM_BARS + kNumBars * 8 + 1024;    // slack to align the base
 static_assert(kSmemBytes <= 232448, "shared memory budget");
 
@@ -90,7 +100,7 @@ struct PrefillParams {
     const int32_t* cu;
     const int32_t* seq_lens;
     int batch, total_q, heads, page_shift, max_q_len, max_seq_len;
-    int units, splits;
+    int units, splits, box_rows;
     float scale_log2, out_scale;
     __nv_bfloat16* out;
     int64_t o_st, o_sh;
@@ -209,24 +219,19 @@ __device__ __forceinline__ int64_t pool_row(const PrefillParams& p, const int32_
     return (static_cast<int64_t>(pg) << p.page_shift) | (pos & ((1 << p.page_shift) - 1));
 }
 
-// Stages in the order the MMAs take them: K of tile 0, then K of tile i and V of tile i - 1.
+// Pieces in the order the MMAs take them: the k_pieces of K of tile 0, then those of K of tile i and
+// the v_pieces of V of tile i - 1.
 struct Cursor {
-    int u, i, s;      // stage number; s < k_stages: K stage s of tile i, else V stage s - k_stages of tile i - 1
+    int u, i, s;      // piece number; s < k_pieces: K piece s of tile i, else V piece s - k_pieces of tile i - 1
 };
-__device__ __forceinline__ void advance(Cursor& c, int k_stages, int n_tiles) {
+__device__ __forceinline__ void advance(Cursor& c, int k_pieces, int v_pieces, int n_tiles) {
     ++c.u;
     ++c.s;
-    if (c.i == 0 ? c.s == k_stages : c.s == k_stages + kVStages) {
+    if (c.i == 0 ? c.s == k_pieces : c.s == k_pieces + v_pieces) {
         ++c.i;
-        c.s = c.i < n_tiles ? 0 : k_stages;
+        c.s = c.i < n_tiles ? 0 : k_pieces;
     }
 }
-
-// One producer thread's share of a stage: 64 latent dims of a row (32 code bytes, 4 scales).
-struct RowPiece {
-    uint4 lo, hi;
-    uint32_t scales;
-};
 
 // The image of the sequences with many units: their tokens dequantised once for all of them, as
 // the ring stages the attention kernel copies.  Block = 128 tokens: [8 latent atoms (+ the rope
@@ -289,7 +294,8 @@ __global__ void __launch_bounds__(256) prefill_image_kernel(const __grid_constan
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
+mla_prefill_kernel(const __grid_constant__ PrefillParams p, const __grid_constant__ CUtensorMap tm_codes,
+                   const __grid_constant__ CUtensorMap tm_scales, const __grid_constant__ CUtensorMap tm_rope) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const uint32_t sbase = smem_u32(smem);
@@ -328,7 +334,8 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
     const int tiles = (end + kTile - 1) / kTile;
     const int tile0 = static_cast<int>(static_cast<int64_t>(split) * tiles / p.splits);
     const int n_tiles = static_cast<int>(static_cast<int64_t>(split + 1) * tiles / p.splits) - tile0;
-    const int k_stages = p.rope ? 9 : 8;
+    const int k_stages = p.rope ? 9 : 8, stages = image ? kStages : kDirectStages;
+    const int ring = image ? SM_RING : SM_RING + kRawSlots * kRawBytes;
     const int image_last = image0 + (L + kImageTok - 1) / kImageTok - 1;      // (tokens past it are masked)
 
     if (threadIdx.x == 0) {
@@ -341,6 +348,10 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         for (int k = 0; k < 2; ++k) {
             mbar_init(bar(B_S_FULL + k), 1);
             mbar_init(bar(B_S_FREE + k), 2 * kSoftmaxWarps);
+        }
+        for (int k = 0; k < kRawSlots; ++k) {
+            mbar_init(bar(B_RAW_FULL + k), 1);
+            mbar_init(bar(B_RAW_EMPTY + k), kProducerWarps);
         }
         mbar_init(bar(B_P_FULL), 2 * kSoftmaxWarps);
         mbar_init(bar(B_PV_DONE), 1);
@@ -404,12 +415,12 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 // ==================================================== MMA issue
                 const uint64_t dq = smem_desc_sw128(sbase + SM_Q, 16, 1024);
                 const uint64_t dp = smem_desc_sw128(sbase + SM_P, 16, 1024);
-                const uint64_t dk = smem_desc_sw128(sbase + SM_RING, 16, 1024);
-                const uint64_t dv = smem_desc_sw128(sbase + SM_RING, 8192, 1024);
+                const uint64_t dk = smem_desc_sw128(sbase + ring, 16, 1024);
+                const uint64_t dv = smem_desc_sw128(sbase + ring, 8192, 1024);
                 int slot = 0;
                 uint32_t phase = 0;
                 auto next = [&] {
-                    if (++slot == kStages) {
+                    if (++slot == stages) {
                         slot = 0;
                         phase ^= 1;
                     }
@@ -468,7 +479,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             Cursor cur{0, 0, 0};
             int slot = warp - kMmaWarp - 1;
             uint32_t phase = 0;
-            if (slot == 1) advance(cur, k_stages, n_tiles);
+            if (slot == 1) advance(cur, k_stages, kVStages, n_tiles);
             griddep_wait();                       // the image kernel's writes
             int issued = -1;                      // last stage copied
 #pragma unroll 1
@@ -490,8 +501,8 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 }
                 __syncwarp();
                 issued = cur.u;
-                advance(cur, k_stages, n_tiles);
-                advance(cur, k_stages, n_tiles);
+                advance(cur, k_stages, kVStages, n_tiles);
+                advance(cur, k_stages, kVStages, n_tiles);
                 slot += 2;
                 if (slot >= kStages) {
                     slot -= kStages;
@@ -503,7 +514,63 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             const int from = max(0, cur.u >= total ? total - kStages : issued - kStages + 1);
             for (int u = from; u <= issued; ++u)
                 if ((u & 1) == (issued & 1)) mbar_drain_wait(bar(B_FULL + u % kStages), (u / kStages) & 1);
-        } else if (image && cta == 1) {
+        } else if (!image && warp == kMmaWarp + 1) {
+            // ======================================================== raw rows
+            // Piece: 128 tokens x 128 code bytes + their 16 scales (K: half of this CTA's tokens' dims; V:
+            // half of the tile's tokens, this CTA's dims), or the 64 rope dims of the K tokens; boxes of up
+            // to a page, a lane each.  A missing page, and a box past the end, is addressed out of range
+            // and reads as zeros, so a slot always receives the same bytes.
+            const int kp = p.rope ? 3 : 2, total = n_tiles * (kp + 2), box = p.box_rows, boxes = kImageTok / box;
+            auto box_row = [&](const Cursor& c, int r) {
+                const int pos = c.s < kp ? (tile0 + c.i) * kTile + 128 * cta : (tile0 + c.i - 1) * kTile + 128 * (c.s - kp);
+                const int64_t row = pool_row(p, table, pos + r * box, end);
+                return row < 0 ? -box : static_cast<int>(row);
+            };
+            if (lane == 0) {
+                tma_prefetch_desc(&tm_codes);
+                tma_prefetch_desc(&tm_scales);
+            }
+            Cursor cur{0, 0, 0};
+            int slot = 0, y = total > 0 ? box_row(cur, min(lane, boxes - 1)) : 0;
+            uint32_t phase = 0;
+#pragma unroll 1
+            while (cur.u < total) {
+                if (cur.u >= kRawSlots && !mbar_wait(bar(B_RAW_EMPTY + slot), phase ^ 1, abort_flag, p.err)) break;
+                fence_proxy_async_smem();
+                const uint32_t dst = sbase + SM_RING + slot * kRawBytes, full = bar(B_RAW_FULL + slot);
+                const bool rope = p.rope && cur.s == 2;
+                const int half = cur.s < kp ? cur.s : cta;      // which 256 dims
+                const bool scale_boxes = box >= 8;              // a copy starts on a multiple of 128 bytes
+                if (!scale_boxes && !rope) {
+                    for (int r = lane; r < kImageTok; r += 32) {
+                        const int row = box_row(cur, r / box) + r % box;
+                        *reinterpret_cast<uint4*>(smem + SM_RING + slot * kRawBytes + kStageBytes + 16 * r) =
+                            row >= 0 ? ldg_nc_v4(p.pool + static_cast<int64_t>(row) * kRowBytes + 256 + 16 * half) : make_uint4(0, 0, 0, 0);
+                    }
+                    __syncwarp();
+                }
+                if (lane == 0) mbar_arrive_expect_tx(full, rope || !scale_boxes ? kStageBytes : kRawBytes);
+                __syncwarp();
+                for (int r = lane; r < boxes; r += 32) {
+                    if (r >= 32) y = box_row(cur, r);
+                    if (rope) {
+                        tma_load_2d(dst + r * box * 128, &tm_rope, 0, y, full);
+                    } else {
+                        tma_load_2d(dst + r * box * 128, &tm_codes, 128 * half, y, full);
+                        if (scale_boxes) tma_load_2d(dst + kStageBytes + r * box * 16, &tm_scales, 256 + 16 * half, y, full);
+                    }
+                }
+                __syncwarp();
+                advance(cur, kp, 2, n_tiles);
+                if (cur.u < total) y = box_row(cur, min(lane, boxes - 1));
+                if (++slot == kRawSlots) {
+                    slot = 0;
+                    phase ^= 1;
+                }
+            }
+            for (int u = max(0, cur.u - kRawSlots); u < cur.u; ++u)      // every copy lands before the CTA can exit
+                mbar_drain_wait(bar(B_RAW_FULL + u % kRawSlots), (u / kRawSlots) & 1);
+        } else if (image && cta == 1 && warp == kMmaWarp + 3) {
             // ======================================================== relay: this CTA's copies, to the leader
             const int total = n_tiles * (k_stages + kVStages);
             int slot = 0;
@@ -523,78 +590,58 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         warpgroup_reg_dealloc<kRegsProducer>();
         if (!image) {
         // ============================================================ producers
-        // Two groups of four warps take the stages in turn.  Stage order: K of tile 0, then K of
-        // tile i and V of tile i - 1.  Thread t writes row t of a stage: K: token 128 c + t of the
-        // tile, dims 64 j ..; V: token 64 (s / 2) + t % 64, dims 256 c + 128 (s % 2) + 64 (t / 64) .. .
+        // Two groups of four warps take the stages in turn.  Thread t writes row t of a stage: K: token
+        // 128 c + t of the tile, dims 64 s ..; V: token 64 (s / 2) + t % 64, dims 256 c + 128 (s % 2) +
+        // 64 (t / 64) .. : 32 code bytes and 4 scales of a raw row.
         const int grp = (warp - kProducerWarp0) >> 2, t = threadIdx.x & 127;
-        const int total = n_tiles * (k_stages + kVStages);
-        auto locate = [&](const Cursor& c, int* dims) -> int64_t {      // the thread's pool row of a stage
-            if (c.s < k_stages) {
-                *dims = 64 * c.s;
-                return pool_row(p, table, (tile0 + c.i) * kTile + 128 * cta + t, end);
-            }
-            const int s = c.s - k_stages;
-            *dims = 256 * cta + 128 * (s & 1) + 64 * (t >> 6);
-            return pool_row(p, table, (tile0 + c.i - 1) * kTile + 64 * (s >> 1) + (t & 63), end);
-        };
-        auto load = [&](const Cursor& c) -> RowPiece {
-            RowPiece r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0), 0};
-            if (c.u >= total) return r;
-            int dims;
-            const int64_t row = locate(c, &dims);
-            if (row < 0 || (c.s == 8 && p.rope)) return r;                          // (the rope stage is copied when it is written)
-            const uint8_t* src = p.pool + row * kRowBytes;
-            r.lo = __ldg(reinterpret_cast<const uint4*>(src + dims / 2));
-            r.hi = __ldg(reinterpret_cast<const uint4*>(src + dims / 2) + 1);
-            r.scales = __ldg(reinterpret_cast<const uint32_t*>(src + 256 + dims / 16));
-            return r;
-        };
+        const int kp = p.rope ? 3 : 2, total = n_tiles * (kp + 2);
         Cursor cur{0, 0, 0};
-        if (grp == 1) advance(cur, k_stages, n_tiles);
-        Cursor ahead = cur;
-        RowPiece buf[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            buf[k] = load(ahead);
-            advance(ahead, k_stages, n_tiles);
-            advance(ahead, k_stages, n_tiles);
-        }
-        int slot = grp;
-        uint32_t phase = 0;
-        uint8_t* dst_row = smem + SM_RING + t * 128;
+        int raw = 0, slot = 0, n = 0;          // raw slot; ring slot and number of the next stage
+        uint32_t raw_phase = 0, phase = 0;
+        auto next = [&] {
+            ++n;
+            if (++slot == kDirectStages) {
+                slot = 0;
+                phase ^= 1;
+            }
+        };
 #pragma unroll 1
         while (cur.u < total) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                if (cur.u >= total) break;
-                const RowPiece r = buf[k];
-                const Cursor c = cur;
-                buf[k] = load(ahead);
-                advance(ahead, k_stages, n_tiles);
-                advance(ahead, k_stages, n_tiles);
-                advance(cur, k_stages, n_tiles);
-                advance(cur, k_stages, n_tiles);
-                uint8_t* dst = dst_row + slot * kStageBytes;
-                if (c.s == 8 && p.rope) {
-                    int dims;
-                    const int64_t row = locate(c, &dims);
+            mbar_wait(bar(B_RAW_FULL + raw), raw_phase, abort_flag, p.err);
+            const uint8_t* src = smem + SM_RING + raw * kRawBytes;
+            if (p.rope && cur.s == 2) {
+                if ((n & 1) == grp) {
                     uint4 v[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        v[j] = row >= 0 ? __ldg(reinterpret_cast<const uint4*>(p.rope + row * kRope) + j) : make_uint4(0, 0, 0, 0);
-                    if (c.u >= kStages) mbar_wait(bar(B_EMPTY + slot), phase ^ 1, abort_flag, p.err);
+                    for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const uint4*>(src + t * 128 + 16 * j);
+                    if (n >= kDirectStages) mbar_wait(bar(B_EMPTY + slot), phase ^ 1, abort_flag, p.err);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(dst + ((j ^ (t & 7)) << 4)) = v[j];
-                } else {
-                    const uint32_t code[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
-                    uint32_t s2[2] = {e4m3x2_to_f16x2(static_cast<uint16_t>(r.scales)), e4m3x2_to_f16x2(static_cast<uint16_t>(r.scales >> 16))};
-                    if (c.s >= k_stages) {
+                    for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(smem + ring + slot * kStageBytes + t * 128 + 16 * j) = v[j];
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) leader_arrive(bar(B_FULL + slot));
+                }
+                next();
+            } else {
+                const bool is_v = cur.s >= kp;
+#pragma unroll 1
+                for (int s = 0; s < 4; ++s, next()) {
+                    if ((n & 1) != grp) continue;
+                    // raw row, its 32-byte piece
+                    const int r = is_v ? 64 * (s >> 1) + (t & 63) : t, piece = is_v ? 2 * (s & 1) + (t >> 6) : s;
+                    const uint4 lo = *reinterpret_cast<const uint4*>(src + r * 128 + (((2 * piece) ^ (r & 7)) << 4));
+                    const uint4 hi = *reinterpret_cast<const uint4*>(src + r * 128 + (((2 * piece + 1) ^ (r & 7)) << 4));
+                    const uint32_t sc4 = *reinterpret_cast<const uint32_t*>(src + kStageBytes + r * 16 + 4 * piece);
+                    const uint32_t code[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                    uint32_t s2[2] = {e4m3x2_to_f16x2(static_cast<uint16_t>(sc4)), e4m3x2_to_f16x2(static_cast<uint16_t>(sc4 >> 16))};
+                    if (is_v) {
                         // a NaN block scale counts as 0 in V: rows that see the token are NaN by its score,
                         // rows that do not (probability 0) stay clear of it
                         s2[0] = max_f16x2(s2[0], 0u);
                         s2[1] = max_f16x2(s2[1], 0u);
                     }
-                    if (c.u >= kStages) mbar_wait(bar(B_EMPTY + slot), phase ^ 1, abort_flag, p.err);
+                    if (n >= kDirectStages) mbar_wait(bar(B_EMPTY + slot), phase ^ 1, abort_flag, p.err);
+                    uint8_t* dst = smem + ring + slot * kStageBytes + t * 128;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {                       // chunk j: dims 8 j .. of the 64
                         const uint32_t two = s2[j >> 2];
@@ -604,15 +651,17 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                         *reinterpret_cast<uint4*>(dst + ((j ^ (t & 7)) << 4)) =
                             make_uint4(hmul2_u32(h[0], sc), hmul2_u32(h[1], sc), hmul2_u32(h[2], sc), hmul2_u32(h[3], sc));
                     }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) leader_arrive(bar(B_FULL + slot));
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) leader_arrive(bar(B_FULL + slot));
-                slot += 2;
-                if (slot >= kStages) {
-                    slot -= kStages;
-                    phase ^= 1;
-                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(B_RAW_EMPTY + raw));
+            advance(cur, kp, 2, n_tiles);
+            if (++raw == kRawSlots) {
+                raw = 0;
+                raw_phase ^= 1;
             }
         }
         }
@@ -631,33 +680,39 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         const int lim = real ? min(L, L - n_new + tok + 1) : 0;        // tokens the row sees
         const float factor = qs[row];
         float m_ref = -INFINITY, l = 0.0f;
-        // Tokens of the quarter that exist (bits[0], bits[1]) and, with an image, that hold a NaN (bits[2], [3]).
-        auto token_bits = [&](int i, uint32_t (&bits)[4]) {
-            bits[2] = bits[3] = 0;
+        // What the next tile's token masks are made of, loaded a tile ahead.  Image: the bits of the
+        // quarter's tokens that exist and of those that hold a NaN; else: the page ids of tokens lane
+        // and 32 + lane.
+        auto load_masks = [&](int i, uint32_t (&w)[4]) {
+            const int tok0 = (tile0 + i) * kTile + 64 * q4;
             if (image) {
-                const int tok0 = (tile0 + i) * kTile + 64 * q4;
-                const int blk = min(image0 + tok0 / kImageTok, image_last), w = (tok0 & (kImageTok - 1)) >> 5;
-                const uint2 have = *reinterpret_cast<const uint2*>(p.image_bits + 8 * static_cast<int64_t>(blk) + w);
-                const uint2 nans = *reinterpret_cast<const uint2*>(p.image_bits + 8 * static_cast<int64_t>(blk) + 4 + w);
-                bits[0] = have.x; bits[1] = have.y; bits[2] = nans.x; bits[3] = nans.y;
-                return;
-            }
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int pos = (tile0 + i) * kTile + 64 * q4 + 32 * k + lane;
-                const bool ok = i < n_tiles && pool_row(p, table, pos, end) >= 0;
-                if (i < n_tiles && pos < end && !ok) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
-                bits[k] = __ballot_sync(0xFFFFFFFFu, ok);
+                const int blk = min(image0 + tok0 / kImageTok, image_last), k = (tok0 & (kImageTok - 1)) >> 5;
+                const uint2 have = *reinterpret_cast<const uint2*>(p.image_bits + 8 * static_cast<int64_t>(blk) + k);
+                const uint2 nans = *reinterpret_cast<const uint2*>(p.image_bits + 8 * static_cast<int64_t>(blk) + 4 + k);
+                w[0] = have.x; w[1] = have.y; w[2] = nans.x; w[3] = nans.y;
+            } else {
+                w[0] = tok0 + lane < end ? __ldg(table + ((tok0 + lane) >> p.page_shift)) : 0;
+                w[1] = tok0 + 32 + lane < end ? __ldg(table + ((tok0 + 32 + lane) >> p.page_shift)) : 0;
             }
         };
         if (image) griddep_wait();
-        uint32_t bits[4], next_bits[4];
-        token_bits(0, next_bits);
+        uint32_t ahead[4];
+        load_masks(0, ahead);
 #pragma unroll 1
         for (int i = 0; i < n_tiles; ++i) {
+            uint32_t bits[4] = {ahead[0], ahead[1], 0, 0};
+            if (image) {
+                bits[2] = ahead[2];
+                bits[3] = ahead[3];
+            } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) bits[k] = next_bits[k];
-            token_bits(i + 1, next_bits);
+                for (int k = 0; k < 2; ++k) {
+                    const bool missing = static_cast<int64_t>(ahead[k]) >= p.num_pages;      // (a negative id is a large one)
+                    if (missing) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
+                    bits[k] = __ballot_sync(0xFFFFFFFFu, !missing);
+                }
+            }
+            load_masks(i + 1, ahead);
             const int see = lim - ((tile0 + i) * kTile + 64 * q4);     // tokens of the quarter the row sees
             mbar_wait(bar(B_S_FULL + (i & 1)), (i >> 1) & 1, abort_flag, p.err);
             tc_fence_after();
@@ -855,6 +910,33 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_const
         make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+    static std::once_flag once;
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    std::call_once(once, [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    });
+    return fn;
+}
+
+// Map of [rows][row_bytes] bytes with boxes of box_x bytes x box_y rows.
+int make_row_map(CUtensorMap* m, const void* base, int64_t rows, int row_bytes, int box_x, int box_y, bool swizzle) {
+    auto enc = tensor_map_encoder();
+    if (!enc) return fail(NVFP4KV_ECUDA, "mla_prefill: cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_x), static_cast<cuuint32_t>(box_y)}, step[2] = {1, 1};
+    const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, step,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(NVFP4KV_ECUDA, "mla_prefill: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return NVFP4KV_OK;
+}
+
 struct PrefillPlan {
     int units, splits, image_blocks;
     size_t image_bytes, part_bytes, ws_bytes;
@@ -924,8 +1006,8 @@ extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_
         return fail(NVFP4KV_EINVAL, "mla_prefill: page_size must be a power of two <= 4096 (got %d)", page_size);
     if (batch == 0 || total_q == 0) return NVFP4KV_OK;
     if (!q || !pool || !tables || !cu_seqlens_q || !seq_lens || !out) return fail(NVFP4KV_EINVAL, "mla_prefill: null pointer");
-    if (pool_rows <= 0 || pool_rows % page_size)
-        return fail(NVFP4KV_EINVAL, "mla_prefill: pool_rows %lld not a positive multiple of page_size %d",
+    if (pool_rows <= 0 || pool_rows % page_size || pool_rows > 0x7FFFFFFFll)
+        return fail(NVFP4KV_EINVAL, "mla_prefill: pool_rows %lld not a multiple of page_size %d in [1, 2^31)",
                     (long long)pool_rows, page_size);
     if (static_cast<int64_t>(max_q_len) * num_heads > 0x3FFFFFFF || static_cast<int64_t>(total_q) * num_heads > 0x7FFFFFFF)
         return fail(NVFP4KV_EINVAL, "mla_prefill: too many query rows");
@@ -958,16 +1040,21 @@ extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t e = cudaFuncSetAttribute(mla_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "mla_prefill: %s", cudaGetErrorString(e));
-    int rc = NVFP4KV_OK;
+    p.box_rows = page_size < kImageTok ? page_size : kImageTok;
+    CUtensorMap tm_codes{}, tm_scales{}, tm_rope{};
+    int rc = make_row_map(&tm_codes, pool, pool_rows, kRowBytes, 128, p.box_rows, true);
+    if (rc == NVFP4KV_OK) rc = make_row_map(&tm_scales, pool, pool_rows, kRowBytes, 16, p.box_rows, false);
+    if (rc == NVFP4KV_OK && rope_pool) rc = make_row_map(&tm_rope, rope_pool, pool_rows, 2 * kRope, 2 * kRope, p.box_rows, true);
+    if (rc != NVFP4KV_OK) return rc;
     if (pl.image_blocks > 0) {
         prefill_image_kernel<<<pl.image_blocks, 256, 0, st>>>(p);
         if ((rc = check_launch("nvfp4kv_mla_prefill image")) != NVFP4KV_OK) return rc;
     }
     const dim3 grid(static_cast<unsigned>(2 * pl.units * pl.splits));
     if (pl.image_blocks > 0)      // its set-up overlaps the image kernel, all else it reads was there before that one
-        e = launch_dependent(mla_prefill_kernel, grid, dim3(kThreads), kSmemBytes, st, p);
+        e = launch_dependent(mla_prefill_kernel, grid, dim3(kThreads), kSmemBytes, st, p, tm_codes, tm_scales, tm_rope);
     else
-        mla_prefill_kernel<<<grid, kThreads, kSmemBytes, st>>>(p);
+        mla_prefill_kernel<<<grid, kThreads, kSmemBytes, st>>>(p, tm_codes, tm_scales, tm_rope);
     if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill launch failed: %s", cudaGetErrorString(e));
     rc = check_launch("nvfp4kv_mla_prefill");
     if (rc != NVFP4KV_OK || pl.splits == 1) return rc;

@@ -100,6 +100,9 @@ CASES = [
     ([130], [130], 3, 16, True), ([64], [1000], 20, 128, True), ([2, 0, 33, 1], [2, 50, 520, 0], 5, 16, True),
     ([9], [700], 128, 64, True), ([1, 1, 1, 1, 1], [1, 255, 256, 257, 2000], 64, 64, True), ([40], [300], 7, 1, False),
     ([257], [513], 64, 64, True), ([100, 3], [100, 4097], 32, 256, True),
+    # few rows per sequence (no image) with every page size
+    ([1], [300], 8, 1, True), ([2], [530], 4, 2, False), ([1, 1], [301, 65], 16, 4, True), ([3], [700], 16, 8, True),
+    ([2], [900], 32, 32, False), ([1], [1300], 64, 4096, True), ([1, 4], [2050, 770], 16, 256, True),
 ]
 
 
