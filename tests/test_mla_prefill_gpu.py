@@ -103,6 +103,9 @@ CASES = [
     # few rows per sequence (no image) with every page size
     ([1], [300], 8, 1, True), ([2], [530], 4, 2, False), ([1, 1], [301, 65], 16, 4, True), ([3], [700], 16, 8, True),
     ([2], [900], 32, 32, False), ([1], [1300], 64, 4096, True), ([1, 4], [2050, 770], 16, 256, True),
+    # more units than CTA pairs: several to a pair, cut anywhere, with and without images in turn
+    ([150], [1500], 128, 64, True), ([1, 9, 2, 33, 1, 0, 17, 4] * 12, [300, 9, 700, 40, 1, 5, 260, 513] * 12, 32, 16, True),
+    ([3] * 200, list(range(3, 203)), 64, 64, False),
 ]
 
 
