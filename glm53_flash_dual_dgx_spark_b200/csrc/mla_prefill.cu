@@ -16,12 +16,16 @@
 //   QK: B = tokens: CTA c holds tokens [128 c, 128 c + 128) of a 256-token tile
 //   PV: B = latent dims: CTA c holds dims [256 c, 256 c + 256) of all 256 tokens
 // in 16 KB ring stages (64 dims x 128 tokens, or 128 dims x 64 tokens), each 128 rows of 128 bytes,
-// 128-byte swizzled, and four MMAs of 64 cycles.  Two ways fill them:
-//   - producer warps read the raw rows (whole 128-byte runs of codes, two or three of them ahead in
-//     registers) and dequantise them: a sequence with few units;
-//   - bulk copies from an image of the sequence in the workspace, dequantised once by a kernel
-//     before: a sequence with many units, which would repeat that arithmetic in each (an image
-//     costs its 1,152 bytes a token written, the copies 17 stages of 16 KB a tile from L2).
+// 128-byte swizzled, and four MMAs of 64 cycles.
+//
+// The stages are bulk copies from an image of the context in the workspace: a kernel before the
+// attention dequantises every token once, into the very bytes of the stages (1,152 a token).  A pair
+// needs every latent byte twice (K and V lie in different CTAs), and 64 heads make a unit of every
+// two new tokens, so dequantising in the attention kernel repeats the work once per unit and twice
+// in it: producer warps that did so held a tile to 13,000 cycles (issue slots) where the copies take
+// 6,400, and already a batch of single tokens gains nothing by them.  Copies from L2 reach 70 bytes a
+// cycle and SM with two warps issuing (46 with one); what bounds a tile then is shared memory: 40 KB
+// written and read per stage, 320 of the 256 cycles its MMAs take.
 //
 // The work of a call, all (unit, tile) pairs in order and one more per unit for its set-up, is cut
 // into one equal range per CTA pair, so that no pair waits for another's longer sequence; a unit cut
@@ -29,8 +33,8 @@
 // the device-side lengths in closed form, in every CTA.
 //
 // Dims are permuted within each half h of the latent: column 8 p + e of dim atom 4 h + s is dim
-// 256 h + 32 p + 8 s + e, so that a thread's 16 code bytes (32 dims) give 8 dims to each of four
-// stages; the queries and the output use the same order.
+// 256 h + 32 p + 8 s + e, so that 16 code bytes (32 dims) of a row give 16 bytes to each of four
+// atoms; the queries and the output use the same order.
 //
 // Numbers: a code times its e4m3 scale is exact in fp16, q is scaled per row by a power of two and
 // then exact in fp16 (but for parts below 2^-35 of the row's largest), the rope part stays bf16;
@@ -38,9 +42,9 @@
 // the output's own rounding), their sums fp32 and of the unrounded values.  A row's maximum moves
 // only when a tile exceeds it by 2^8, so O is rarely rescaled and P stays far from fp16's largest.
 //
-// Warps: 0-7 softmax (a row's 256 scores over four of them) and epilogue, 8-15 producers and Q,
-// 16 issues the MMAs (in the leading CTA), 17-18 image copies, 19 their relay to the leader.
-// Every wait is bounded (common.cuh).
+// Warps: 0-7 softmax (a row's 256 scores over four of them) and epilogue, 8-11 Q, 12 issues the
+// MMAs (in the leading CTA), 13-14 image copies, 15 hands landed copies to the leader.  Every wait is
+// bounded (common.cuh).
 #include <math.h>
 
 #include "../../include/nvfp4kv_serving.h"
@@ -59,15 +63,14 @@ constexpr int kTile = 256;                      // tokens per tile
 constexpr int kStages = 7;
 constexpr int kStageBytes = 16384;              // 128 rows x 128 B
 constexpr int kVStages = 8;                     // V stages of a tile: 4 x 64 tokens x 2 x 128 dims a CTA
-constexpr int kSoftmaxWarps = 8, kProducerWarp0 = 8, kProducerWarps = 8, kMmaWarp = 16, kCopyWarp0 = 17, kRelayWarp = 19;
-constexpr int kThreads = 20 * 32;
-constexpr uint32_t kRegsSoftmax = 128, kRegsProducer = 88, kRegsCtl = 48;
-static_assert(256 * kRegsSoftmax + 256 * kRegsProducer + 128 * kRegsCtl <= kThreads * 96,
+constexpr int kSoftmaxWarps = 8, kQWarp0 = 8, kQWarps = 4, kMmaWarp = 12, kCopyWarp0 = 13, kRelayWarp = 15;
+constexpr int kThreads = 16 * 32;
+constexpr uint32_t kRegsLaunch = 128, kRegsSoftmax = 168, kRegsQ = 96, kRegsCtl = 80;
+static_assert(256 * kRegsSoftmax + 128 * kRegsQ + 128 * kRegsCtl <= kThreads * kRegsLaunch,
               "the register split stays within what the block is launched with");
 constexpr float kRescaleLog2 = 8.0f;
 constexpr int kMaxPairs = 128;
 constexpr int kImageTok = 128;                  // tokens of an image block
-constexpr int kImageUnits = 2;                  // sequences with at least this many units read an image
 
 constexpr int SM_Q = 0;                                      // 9 dim atoms x [64 rows x 128 B]
 constexpr int SM_P = SM_Q + 9 * kCtaRows * 128;              // 4 token atoms x [64 rows x 128 B]
@@ -76,19 +79,19 @@ constexpr int SM_RED = SM_RING + kStages * kStageBytes;      // 2 x 4 x 64 f32: 
 constexpr int SM_LSUM = SM_RED + 2 * 4 * 64 * 4;             // 4 x 64 f32
 constexpr int SM_QS = SM_LSUM + 4 * 64 * 4;                  // 2 x 64 f32: score factor (log2 units) of a row
 constexpr int SM_FLAGS = SM_QS + 2 * 64 * 4;                 // [0] TMEM base, [1] abort
-constexpr int SM_SCHED = SM_FLAGS + 16;                      // where this pair's range begins
-constexpr int SM_BARS = SM_SCHED + 48;
-constexpr int B_FULL = 0;                      // [kStages] leader: stage ready in both CTAs
+constexpr int SM_WORK = SM_FLAGS + 16;                       // a Work per warp
+constexpr int kWorkBytes = 96;
+constexpr int SM_BARS = SM_WORK + (kThreads / 32) * kWorkBytes;
+constexpr int B_FULL = 0;                      // [kStages] leader: stage landed in both CTAs
 constexpr int B_EMPTY = B_FULL + kStages;      // [kStages] both: the MMAs have read the stage
 constexpr int B_LAND = B_EMPTY + kStages;      // [kStages] own: an image copy landed
 constexpr int B_S_FULL = B_LAND + kStages;     // [2] both: S of a tile complete
 constexpr int B_S_FREE = B_S_FULL + 2;         // [2] leader: S read by both CTAs
 constexpr int B_P_FULL = B_S_FREE + 2;         // leader: P written in both CTAs
 constexpr int B_PV_DONE = B_P_FULL + 1;        // both: O stable, P free
-constexpr int B_Q_FULL = B_PV_DONE + 1;        // leader: Q written in both CTAs, and the ring handed over
+constexpr int B_Q_FULL = B_PV_DONE + 1;        // leader: Q written in both CTAs
 constexpr int B_Q_FREE = B_Q_FULL + 1;         // both: the last QK of a part complete
-constexpr int B_PART_DONE = B_Q_FREE + 1;      // both: the last PV of a part complete, its stages read
-constexpr int B_O_FREE = B_PART_DONE + 1;      // leader: O read by both CTAs
+constexpr int B_O_FREE = B_Q_FREE + 1;         // leader: O read by both CTAs
 constexpr int B_DRAIN = B_O_FREE + 1;          // both: every MMA complete
 constexpr int kNumBars = B_DRAIN + 1;
 constexpr int kSmemBytes = SM_BARS + kNumBars * 8 + 1024;    // slack to align the base
@@ -115,7 +118,7 @@ struct PrefillParams {
     const int32_t* cu;
     const int32_t* seq_lens;
     int batch, total_q, heads, page_shift, max_q_len, max_seq_len;
-    int pairs, image_blocks;
+    int pairs;
     float scale_log2, out_scale;
     __nv_bfloat16* out;
     int64_t o_st, o_sh;
@@ -123,8 +126,8 @@ struct PrefillParams {
     PartInfo* parts;    // [pairs][2]: the range's first part of a unit, and its last one
     float* part_ml;     // [pairs][2][128][2]: maximum (log2 units), sum
     float* part_o;      // [pairs][2][128][512]
-    uint8_t* image;     // [image_blocks][8 or 9 atoms][128 tokens x 128 B]
-    uint32_t* image_bits;   // [image_blocks][8]: 128 bits of tokens that exist, 128 of those that hold a NaN
+    uint8_t* image;     // [blocks][8 or 9 atoms][128 tokens x 128 B]
+    uint32_t* image_bits;   // [blocks][8]: 128 bits of tokens that exist, 128 of those that hold a NaN
     int32_t* err;
 };
 
@@ -146,22 +149,29 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
 }
-// Arrive `count` times on the leading CTA's barrier.  What the arrival publishes is this CTA's own
-// shared and tensor memory, ordered before it by fence.proxy.async or tcgen05.fence and read by the
-// tensor core only, so the plain (CTA-scoped) release does; a cluster-scoped one is a full fence
-// that takes about 900 cycles (measured: one per stage held the kernel to 0.38 of its rate).
-__device__ __forceinline__ void leader_arrive(uint32_t bar, uint32_t count = 1) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_map(bar, 0)), "r"(count) : "memory");
+// Arrive on the leading CTA's barrier.  What the arrival publishes is this CTA's own shared and
+// tensor memory, ordered before it by fence.proxy.async or tcgen05.fence and read by the tensor
+// core only, so the plain (CTA-scoped) release does; a cluster-scoped one is a full fence that
+// takes about 900 cycles (measured: one per stage held the kernel to 0.38 of its rate).
+__device__ __forceinline__ void leader_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_map(bar, 0)) : "memory");
 }
-__device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
+// One 32-byte store (dst 32-byte aligned).
+__device__ __forceinline__ void st_global_v8(void* dst, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 // Instruction descriptors: fp32 accumulators, M = 128 (a pair's rows), N = 256.
 constexpr uint32_t kIdescQk = idesc_f16_f32(128, 256, false, false);
 constexpr uint32_t kIdescRope = kIdescQk | (1u << 7) | (1u << 10);      // both operands bf16
 constexpr uint32_t kIdescPv = idesc_f16_f32(128, 256, false, true);
+
+// A warpgroup's registers per thread from here on (a decrease may not go up, nor an increase down).
+template <uint32_t kRegs>
+__device__ __forceinline__ void set_registers() {
+    if constexpr (kRegs > kRegsLaunch) warpgroup_reg_alloc<kRegs>();
+    if constexpr (kRegs < kRegsLaunch) warpgroup_reg_dealloc<kRegs>();
+}
 
 // ------------------------------------------------------------------ the work and its ranges
 struct Seq {
@@ -180,8 +190,8 @@ __device__ __forceinline__ Seq load_seq(const PrefillParams& p, int b) {
     s.units = (s.rows + kUnitRows - 1) / kUnitRows;
     return s;
 }
-__device__ __forceinline__ int image_blocks_of(const PrefillParams& p, const Seq& s) {
-    return s.units >= kImageUnits && p.image_blocks > 0 ? (s.L + kImageTok - 1) / kImageTok : 0;
+__device__ __forceinline__ int image_blocks_of(const Seq& s) {
+    return s.units > 0 ? (s.L + kImageTok - 1) / kImageTok : 0;
 }
 // Tokens that unit k of the sequence sees: those of its last row.
 __device__ __forceinline__ int unit_end(const PrefillParams& p, const Seq& s, int k) {
@@ -241,7 +251,7 @@ __device__ __forceinline__ Range find_range(const PrefillParams& p, int pair) {
         Seq s{};
         if (b0 + lane < p.batch) s = load_seq(p, b0 + lane);
         const int64_t w = weight_before(p, s, s.units);
-        const int blocks = image_blocks_of(p, s);
+        const int blocks = image_blocks_of(s);
         const int64_t upto = before + warp_inclusive_sum(w, lane);
         const int img = r.image0 + warp_inclusive_sum(blocks, lane);
         const uint32_t hit = __ballot_sync(0xFFFFFFFFu, lo < upto);
@@ -276,15 +286,15 @@ struct Part {
     int first, n, L, rows;  // of the sequence
     int end;                // tokens the unit sees
     int tile0, n_tiles;
-    int image;              // the sequence's first image block, -1 without an image
-    bool head, tail;        // it begins / ends the unit
+    int image;              // the sequence's first image block
+    int head, tail;         // it begins / ends the unit
 };
 // The next part of the range; parts without tiles are given only where they are a whole unit (one
 // that sees no token).
-__device__ __forceinline__ bool next_part(const PrefillParams& p, Range& r, Part& t) {
+__device__ __forceinline__ bool next_part_of(const PrefillParams& p, Range& r, Part& t) {
     while (r.left > 0) {
         const Seq s = load_seq(p, r.b);
-        const int blocks = image_blocks_of(p, s);
+        const int blocks = image_blocks_of(s);
         if (r.k >= s.units) {
             ++r.b;
             r.k = 0;
@@ -299,7 +309,7 @@ __device__ __forceinline__ bool next_part(const PrefillParams& p, Range& r, Part
         t.n_tiles = r.offset + take - 1 - t.tile0;
         t.b = r.b; t.block = r.k;
         t.first = s.first; t.n = s.n; t.L = s.L; t.rows = s.rows;
-        t.image = blocks > 0 && r.image0 + blocks <= p.image_blocks ? r.image0 : -1;
+        t.image = r.image0;
         t.head = t.tile0 == 0;
         t.tail = t.tile0 + t.n_tiles == tiles;
         r.left -= take;
@@ -312,6 +322,27 @@ __device__ __forceinline__ bool next_part(const PrefillParams& p, Range& r, Part
     }
     return false;
 }
+// A warp's place in its pair's range and its current part, in shared memory: read where they are
+// used, they cost no registers in the loops over tiles.
+struct Work {
+    Range range;
+    int more;
+    Part part;
+};
+static_assert(sizeof(Work) <= kWorkBytes, "a warp's work record");
+__device__ __forceinline__ bool next_part(const PrefillParams& p, Work* w) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+        Range r = w->range;
+        Part t;
+        const bool more = next_part_of(p, r, t);
+        w->range = r;
+        w->more = more;
+        if (more) w->part = t;
+    }
+    __syncwarp();
+    return *reinterpret_cast<volatile int*>(&w->more) != 0;
+}
 
 // Pool row of position pos < end of a sequence, -1 for a missing page or past the end.
 __device__ __forceinline__ int64_t pool_row(const PrefillParams& p, const int32_t* table, int pos, int end) {
@@ -321,36 +352,16 @@ __device__ __forceinline__ int64_t pool_row(const PrefillParams& p, const int32_
     return (static_cast<int64_t>(pg) << p.page_shift) | (pos & ((1 << p.page_shift) - 1));
 }
 
-// Part j begins once every warp that fills the ring, whether in this part or not, has arrived on
-// B_Q_FULL.  Before that it waits for the last QK of part j - 1 (then Q is free, and every earlier
-// part done), and where the ring changes hands, because only one of the two parts has an image,
-// for the end of part j - 1.  So no barrier is ever more than one phase past the one waited for: a
-// parity wait could not tell.
-struct RingTurn {
-    int parts = 0;          // parts with tiles so far
-    bool image = false;     // the last one's kind
-};
-__device__ __forceinline__ bool take_ring(RingTurn& r, bool image, uint32_t bar_q_free, uint32_t bar_part_done,
-                                          volatile int* abort_flag, int32_t* err) {
-    const int j = r.parts++;
-    const bool change = image != r.image;
-    r.image = image;
-    if (j == 0) return true;
-    return mbar_wait(bar_q_free, (j - 1) & 1, abort_flag, err) &&
-           (!change || mbar_wait(bar_part_done, (j - 1) & 1, abort_flag, err));
-}
-
-// Pieces in the order the MMAs take them: the k_pieces of K of tile 0, then those of K of tile i and
-// the v_pieces of V of tile i - 1.
+// Stages in the order the MMAs take them: K of tile 0, then K of tile i and V of tile i - 1.
 struct Cursor {
-    int u, i, s;      // piece number; s < k_pieces: K piece s of tile i, else V piece s - k_pieces of tile i - 1
+    int u, i, s;      // stage number; s < k_stages: K stage s of tile i, else V stage s - k_stages of tile i - 1
 };
-__device__ __forceinline__ void advance(Cursor& c, int k_pieces, int v_pieces, int n_tiles) {
+__device__ __forceinline__ void advance(Cursor& c, int k_stages, int n_tiles) {
     ++c.u;
     ++c.s;
-    if (c.i == 0 ? c.s == k_pieces : c.s == k_pieces + v_pieces) {
+    if (c.i == 0 ? c.s == k_stages : c.s == k_stages + kVStages) {
         ++c.i;
-        c.s = c.i < n_tiles ? 0 : k_pieces;
+        c.s = c.i < n_tiles ? 0 : k_stages;
     }
 }
 
@@ -362,28 +373,29 @@ __device__ __forceinline__ uint4 dequant8(uint32_t code, uint32_t scale2) {
 }
 
 // ------------------------------------------------------------------ image
-// The image of the sequences with many units: their tokens dequantised once for all of them, as
-// the ring stages the attention kernel copies.  Block = 128 tokens: [8 latent atoms (+ the rope
-// part)][128 tokens x 128 B], 128-byte swizzled, zeros for tokens that do not exist and for blocks
-// with a NaN scale (the token's bit says so instead: a NaN in V would reach rows that do not see it).
+// The image: every token of the sequences with new ones dequantised, as the ring stages the attention
+// kernel copies.  Block = 128 tokens: [8 latent atoms (+ the rope part)][128 tokens x 128 B], 128-byte
+// swizzled, zeros for tokens that do not exist and for blocks with a NaN scale (the token's bit says
+// so instead: a NaN in V would reach rows that do not see it).  Eight lanes read a row's half (128
+// code bytes), a thread writes its 32 dims as 16 bytes to each of four atoms, a warp whole 128-byte
+// rows; all of a block's loads are in flight before the first is used.
 __global__ void __launch_bounds__(256) prefill_image_kernel(const __grid_constant__ PrefillParams p) {
-    __shared__ int64_t rows[kImageTok];
     __shared__ uint32_t bits[8];
     __shared__ int b_s, pos_s;
     griddep_launch_dependents();
-    if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
+    const int tid = threadIdx.x, lp = tid & 7, r0 = tid >> 3;
+    if (tid < 32) {
+        const int lane = tid;
         int base = 0, b = -1, pos = 0;
         for (int b0 = 0; b0 < p.batch && b < 0; b0 += 32) {
             int blocks = 0;
-            if (b0 + lane < p.batch) blocks = image_blocks_of(p, load_seq(p, b0 + lane));
+            if (b0 + lane < p.batch) blocks = image_blocks_of(load_seq(p, b0 + lane));
             const int upto = base + warp_inclusive_sum(blocks, lane);
             const uint32_t hit = __ballot_sync(0xFFFFFFFFu, static_cast<int>(blockIdx.x) < upto);
             if (hit) {
-                const int src = __ffs(hit) - 1, last = __shfl_sync(0xFFFFFFFFu, upto, src);
+                const int src = __ffs(hit) - 1;
                 b = b0 + src;
-                pos = kImageTok * (static_cast<int>(blockIdx.x) - (last - __shfl_sync(0xFFFFFFFFu, blocks, src)));
-                if (last > p.image_blocks) b = -2;      // a sequence that does not fit has no image
+                pos = kImageTok * (static_cast<int>(blockIdx.x) - __shfl_sync(0xFFFFFFFFu, upto - blocks, src));
             }
             base = __shfl_sync(0xFFFFFFFFu, upto, 31);
         }
@@ -391,51 +403,61 @@ __global__ void __launch_bounds__(256) prefill_image_kernel(const __grid_constan
             b_s = b;
             pos_s = pos;
         }
+        if (lane < 8) bits[lane] = 0;
     }
-    if (threadIdx.x < 8) bits[threadIdx.x] = 0;
     __syncthreads();
     if (b_s < 0) return;
-    const int L = load_seq(p, b_s).L, tid = threadIdx.x;
-    if (tid < kImageTok) {
-        const int pos = pos_s + tid;
-        const int64_t row = pool_row(p, p.tables + b_s * p.tables_stride, pos, L);
-        rows[tid] = row;
-        if (row >= 0) atomicOr(&bits[tid >> 5], 1u << (tid & 31));
-        else if (pos < L) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
+    const int L = load_seq(p, b_s).L;
+    const int32_t* table = p.tables + b_s * p.tables_stride;
+    int64_t row[4];
+    uint4 code[4][2], rope[4];
+    uint16_t scale[4][2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) row[k] = pool_row(p, table, pos_s + r0 + 32 * k, L);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        rope[k] = code[k][0] = code[k][1] = make_uint4(0, 0, 0, 0);
+        scale[k][0] = scale[k][1] = 0;
+        if (row[k] >= 0) {
+            const uint8_t* src = p.pool + row[k] * kRowBytes;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                code[k][h] = ldg_nc_v4(src + 128 * h + 16 * lp);
+                scale[k][h] = __ldg(reinterpret_cast<const uint16_t*>(src + 256 + 16 * h + 2 * lp));
+            }
+            if (p.rope) rope[k] = ldg_nc_v4(p.rope + row[k] * kRope + 8 * lp);
+        }
     }
-    __syncthreads();
     const int atoms = p.rope ? 9 : 8;
-    uint4* dst = reinterpret_cast<uint4*>(p.image + static_cast<int64_t>(blockIdx.x) * atoms * kStageBytes);
-#pragma unroll 4
-    for (int k = tid; k < atoms * 1024; k += 256) {      // 16-byte chunk of the image
-        const int atom = k >> 10, t = (k >> 3) & 127, c = (k & 7) ^ (t & 7);
-        const int64_t row = rows[t];
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row >= 0) {
-            if (atom == 8) {
-                v = ldg_nc_v4(p.rope + row * kRope + 8 * c);
-            } else {
-                const int h = atom >> 2, s = atom & 3;      // dims 256 h + 32 c + 8 s ..
-                const uint8_t* src = p.pool + row * kRowBytes;
-                const uint32_t code = __ldg(reinterpret_cast<const uint32_t*>(src + 128 * h + 16 * c + 4 * s));
-                const uint32_t sb = src[256 + 16 * h + 2 * c + (s >> 1)];
-                if ((sb & 0x7F) == 0x7F) atomicOr(&bits[4 + (t >> 5)], 1u << (t & 31));
-                else v = dequant8(code, e4m3x2_to_f16x2(static_cast<uint16_t>(sb | sb << 8)));
+    uint8_t* dst = p.image + static_cast<int64_t>(blockIdx.x) * atoms * kStageBytes + r0 * 128 + ((lp ^ (r0 & 7)) << 4);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int t = r0 + 32 * k;
+        uint32_t nan = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t word[4] = {code[k][h].x, code[k][h].y, code[k][h].z, code[k][h].w};
+            const uint32_t s2 = e4m3x2_to_f16x2(scale[k][h]);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const bool bad = ((scale[k][h] >> (s & 2 ? 8 : 0)) & 0x7F) == 0x7F;
+                nan |= bad;
+                const uint4 v = dequant8(word[s], __byte_perm(s2, s2, s & 2 ? 0x3232 : 0x1010));
+                *reinterpret_cast<uint4*>(dst + (4 * h + s) * kStageBytes + 4096 * k) = bad ? make_uint4(0, 0, 0, 0) : v;
             }
         }
-        dst[k] = v;
+        if (p.rope) *reinterpret_cast<uint4*>(dst + 8 * kStageBytes + 4096 * k) = rope[k];
+        if (nan) atomicOr(&bits[4 + k], 1u << (t & 31));
+        if (lp == 0) {
+            if (row[k] >= 0) atomicOr(&bits[k], 1u << (t & 31));
+            else if (pos_s + t < L) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
+        }
     }
     __syncthreads();
     if (tid < 8) p.image_bits[8 * static_cast<int64_t>(blockIdx.x) + tid] = bits[tid];
 }
 
 // ------------------------------------------------------------------ attention
-// Raw pieces a producer thread holds: four rows' 32 latent dims (16 code bytes, two scales) or 8 rope dims.
-struct Raw {
-    uint4 v[4];
-    uint32_t scales[2];     // row k: half k & 1 of word k >> 1
-};
-
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -451,13 +473,13 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         const Range r = find_range(p, pair);
         if (lane == 0) {
             flags[1] = 0;
-            *reinterpret_cast<Range*>(smem + SM_SCHED) = r;
+            for (int k = 0; k < kThreads / 32; ++k) reinterpret_cast<Work*>(smem + SM_WORK + k * kWorkBytes)->range = r;
             if (cta == 0) p.parts[2 * pair].used = p.parts[2 * pair + 1].used = 0;
         }
     }
     if (threadIdx.x == 32) {
         for (int k = 0; k < kStages; ++k) {
-            mbar_init(bar(B_FULL + k), 2 * kProducerWarps);      // (an image copy arrives as often)
+            mbar_init(bar(B_FULL + k), 2);
             mbar_init(bar(B_EMPTY + k), 1);
             mbar_init(bar(B_LAND + k), 1);
         }
@@ -467,26 +489,25 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         }
         mbar_init(bar(B_P_FULL), 2 * kSoftmaxWarps);
         mbar_init(bar(B_PV_DONE), 1);
-        mbar_init(bar(B_Q_FULL), 2 * (kProducerWarps + 2));
+        mbar_init(bar(B_Q_FULL), 2 * kQWarps);
         mbar_init(bar(B_Q_FREE), 1);
-        mbar_init(bar(B_PART_DONE), 1);
         mbar_init(bar(B_O_FREE), 2 * kSoftmaxWarps);
         mbar_init(bar(B_DRAIN), 1);
         mbar_fence_init();
     }
     __syncthreads();
-    Range range = *reinterpret_cast<const Range*>(smem + SM_SCHED);
-    if (range.left <= 0) return;       // nothing for this pair: the whole cluster
+    Work* work = reinterpret_cast<Work*>(smem + SM_WORK + warp * kWorkBytes);
+    const volatile Part& t = work->part;
+    if (reinterpret_cast<volatile Work*>(work)->range.left <= 0) return;       // nothing for this pair: the whole cluster
     if (warp == kMmaWarp) pair_tmem_alloc(sbase + SM_FLAGS, kTmemCols);
     tc_fence_before();
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem = static_cast<uint32_t>(flags[0]);
     const int k_stages = p.rope ? 9 : 8;
-    Part t;
 
     if (warp >= kMmaWarp) {
-        warpgroup_reg_dealloc<kRegsCtl>();
+        set_registers<kRegsCtl>();
         if (warp == kMmaWarp) {
             if (cta == 0) {
                 // ==================================================== MMA issue
@@ -503,12 +524,13 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                     }
                 };
 #pragma unroll 1
-                while (next_part(p, range, t) && !*abort_flag) {
-                    if (t.n_tiles == 0) continue;
+                while (next_part(p, work) && !*abort_flag) {
+                    const int n_tiles = t.n_tiles;
+                    if (n_tiles == 0) continue;
                     mbar_wait(bar(B_Q_FULL), parts & 1, abort_flag, p.err);
 #pragma unroll 1
-                    for (int i = 0; i <= t.n_tiles; ++i, ++tile) {
-                        if (i < t.n_tiles) {
+                    for (int i = 0; i <= n_tiles; ++i, ++tile) {
+                        if (i < n_tiles) {
                             const uint32_t d = tmem + kTS + 128 * (tile & 1);
                             if (tile >= 2) mbar_wait(bar(B_S_FREE + (tile & 1)), ((tile >> 1) - 1) & 1, abort_flag, p.err);
 #pragma unroll 1
@@ -523,7 +545,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                                     pair_commit(bar(B_EMPTY + slot));
                                     if (j == k_stages - 1) {
                                         pair_commit(bar(B_S_FULL + (tile & 1)));
-                                        if (i == t.n_tiles - 1) pair_commit(bar(B_Q_FREE));
+                                        if (i == n_tiles - 1) pair_commit(bar(B_Q_FREE));
                                     }
                                 }
                                 __syncwarp();
@@ -543,10 +565,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
 #pragma unroll
                                     for (int k = 0; k < 4; ++k) pair_mma_f16(d, a + 2 * k, b + 128 * k, kIdescPv, ((i - 1) | (s >> 1) | k) != 0);
                                     pair_commit(bar(B_EMPTY + slot));
-                                    if (s == kVStages - 1) {
-                                        pair_commit(bar(B_PV_DONE));
-                                        if (i == t.n_tiles) pair_commit(bar(B_PART_DONE));
-                                    }
+                                    if (s == kVStages - 1) pair_commit(bar(B_PV_DONE));
                                 }
                                 __syncwarp();
                                 next();
@@ -563,248 +582,128 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             mbar_drain_wait(bar(B_DRAIN), 0);
         } else {
             // ======================================================== image copies and their relay
-            // Two warps take the stages in turn (one issues at most about 46 bytes a cycle); a third
-            // hands each landed stage to the leader.
+            // Two warps take the stages in turn, a third hands each landed stage to the leader.
             const int64_t image_bytes = static_cast<int64_t>(k_stages) * kStageBytes;
             const bool relay = warp == kRelayWarp;
             const int mine = warp - kCopyWarp0;
-            int u0 = 0;                           // stages of the parts before
-            uint32_t land = 0;                    // parity of each slot's next landing
+            int u = 0, slot = 0;                  // stage number and its ring slot
+            uint32_t phase = 0;
             bool ok = true;
-            RingTurn turn;
             griddep_wait();                       // the image kernel's writes
 #pragma unroll 1
-            while (ok && next_part(p, range, t)) {
-                const int total = t.n_tiles * (k_stages + kVStages);
-                if (total > 0 && !relay) {
-                    ok = take_ring(turn, t.image >= 0, bar(B_Q_FREE), bar(B_PART_DONE), abort_flag, p.err);
-                    if (lane == 0) leader_arrive(bar(B_Q_FULL));
-                }
-                if (ok && t.image >= 0) {
-                    const int last = t.image + (t.L + kImageTok - 1) / kImageTok - 1;      // (tokens past it are masked)
-                    int slot = u0 % kStages;
-                    uint32_t phase = (u0 / kStages) & 1;
-                    Cursor c{0, 0, 0};
+            while (ok && next_part(p, work)) {
+                const int n_tiles = t.n_tiles, total = n_tiles * (k_stages + kVStages), image = t.image, tile0 = t.tile0;
+                const int last = image + (t.L + kImageTok - 1) / kImageTok - 1;      // (tokens past it are masked)
+                Cursor c{0, 0, 0};
 #pragma unroll 1
-                    for (; c.u < total; advance(c, k_stages, kVStages, t.n_tiles)) {
-                        if (relay) {
-                            if (!(ok = mbar_wait(bar(B_LAND + slot), (land >> slot) & 1, abort_flag, p.err))) break;
-                            if (lane == 0) leader_arrive(bar(B_FULL + slot), kProducerWarps);
-                            __syncwarp();
-                        } else if (((u0 + c.u) & 1) == mine) {
-                            if (u0 + c.u >= kStages && !(ok = mbar_wait(bar(B_EMPTY + slot), phase ^ 1, abort_flag, p.err))) break;
-                            const uint32_t dst = sbase + SM_RING + slot * kStageBytes, landed = bar(B_LAND + slot);
-                            if (elect_one()) {
-                                mbar_arrive_expect_tx(landed, kStageBytes);
-                                if (c.s < k_stages) {
-                                    const int blk = min(t.image + 2 * (t.tile0 + c.i) + cta, last);
-                                    bulk_copy_g2s(dst, p.image + blk * image_bytes + c.s * kStageBytes, kStageBytes, landed);
-                                } else {
-                                    const int v = c.s - k_stages;      // tokens 64 (v / 2) .., dim atoms 4 c + 2 (v % 2), + 1
-                                    const int blk = min(t.image + 2 * (t.tile0 + c.i - 1) + (v >> 2), last);
-                                    const uint8_t* src = p.image + blk * image_bytes + (4 * cta + 2 * (v & 1)) * kStageBytes + ((v >> 1) & 1) * 8192;
-                                    bulk_copy_g2s(dst, src, 8192, landed);
-                                    bulk_copy_g2s(dst + 8192, src + kStageBytes, 8192, landed);
-                                }
+                for (; c.u < total; advance(c, k_stages, n_tiles)) {
+                    if (relay) {
+                        if (!(ok = mbar_wait(bar(B_LAND + slot), phase, abort_flag, p.err))) break;
+                        if (lane == 0) leader_arrive(bar(B_FULL + slot));
+                        __syncwarp();
+                    } else if ((u & 1) == mine) {
+                        // (a release waited for by the other warp in between is earlier than this one's: no
+                        // phase is skipped unseen)
+                        if (u >= kStages && !(ok = mbar_wait(bar(B_EMPTY + slot), phase ^ 1, abort_flag, p.err))) break;
+                        const uint32_t dst = sbase + SM_RING + slot * kStageBytes, landed = bar(B_LAND + slot);
+                        if (elect_one()) {
+                            mbar_arrive_expect_tx(landed, kStageBytes);
+                            if (c.s < k_stages) {
+                                const int blk = min(image + 2 * (tile0 + c.i) + cta, last);
+                                bulk_copy_g2s(dst, p.image + blk * image_bytes + c.s * kStageBytes, kStageBytes, landed);
+                            } else {
+                                const int v = c.s - k_stages;      // tokens 64 (v / 2) .., dim atoms 4 c + 2 (v % 2), + 1
+                                const int blk = min(image + 2 * (tile0 + c.i - 1) + (v >> 2), last);
+                                const uint8_t* src = p.image + blk * image_bytes + (4 * cta + 2 * (v & 1)) * kStageBytes + ((v >> 1) & 1) * 8192;
+                                bulk_copy_g2s(dst, src, 8192, landed);
+                                bulk_copy_g2s(dst + 8192, src + kStageBytes, 8192, landed);
                             }
-                            __syncwarp();
                         }
-                        land ^= 1u << slot;
-                        if (++slot == kStages) {
-                            slot = 0;
-                            phase ^= 1;
-                        }
+                        __syncwarp();
+                    }
+                    ++u;
+                    if (++slot == kStages) {
+                        slot = 0;
+                        phase ^= 1;
                     }
                 }
-                u0 += total;
             }
             // Every copy has landed once the MMAs that read it are done; after a timed-out wait the ones in
-            // flight are awaited here, so that the CTA does not exit under them.
+            // flight (the stages before u) are awaited here, so that the CTA does not exit under them.
             if (!relay && *abort_flag)
-                for (int k = 0; k < kStages; ++k) mbar_drain_wait(bar(B_LAND + k), ((land >> k) & 1) ^ 1);
+                for (int k = max(0, u - kStages); k < u; ++k) mbar_drain_wait(bar(B_LAND + k % kStages), (k / kStages) & 1);
         }
-    } else if (warp >= kProducerWarp0) {
-        warpgroup_reg_dealloc<kRegsProducer>();
-        // ============================================================ producers: Q, and the stages of parts without an image
-        // Raw pieces of a tile: K, 256 dims of this CTA's 128 tokens: four stages, twice (+ the rope
-        // dims: one); V, this CTA's 256 dims of 128 tokens: four stages, twice.  Eight lanes read a row's 128
-        // code bytes, a thread the rows r0 + 32 k; its 32 dims give 8 to each K stage, 16 to each V stage.
-        const int tid = threadIdx.x - 32 * kProducerWarp0, lp = tid & 7, r0 = tid >> 3;
-        const int kp = p.rope ? 3 : 2;
-        const uint32_t swz = static_cast<uint32_t>((lp ^ (r0 & 7)) << 4);
-        int parts = 0, slot = 0;
-        uint32_t phase = 0;
-        int n = 0;                              // stages so far
-        RingTurn turn;
+    } else if (warp >= kQWarp0) {
+        set_registers<kRegsQ>();
+        // ============================================================ Q of each part
+        int parts = 0;
 #pragma unroll 1
-        while (next_part(p, range, t)) {
+        while (next_part(p, work)) {
             if (t.n_tiles == 0) continue;
-            const int32_t* table = p.tables + t.b * p.tables_stride;
-            const int total = t.image < 0 ? t.n_tiles * (kp + 2) : 0;
-            auto load = [&](const Cursor& c) -> Raw {
-                Raw r;
-                const bool v = c.s >= kp;
-                const int pos0 = v ? (t.tile0 + c.i - 1) * kTile + 128 * (c.s - kp) : (t.tile0 + c.i) * kTile + 128 * cta;
-                const int half = v ? cta : c.s;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int64_t row = c.u < total ? pool_row(p, table, pos0 + r0 + 32 * k, t.end) : -1;
-                    uint32_t sc = 0;
-                    r.v[k] = make_uint4(0, 0, 0, 0);
-                    if (row >= 0) {
-                        if (!v && c.s == 2) {
-                            r.v[k] = __ldg(reinterpret_cast<const uint4*>(p.rope + row * kRope + 8 * lp));
-                        } else {
-                            const uint8_t* src = p.pool + row * kRowBytes;
-                            r.v[k] = __ldg(reinterpret_cast<const uint4*>(src + 128 * half + 16 * lp));
-                            sc = __ldg(reinterpret_cast<const uint16_t*>(src + 256 + 16 * half + 2 * lp));
-                        }
-                    }
-                    r.scales[k >> 1] = (k & 1) ? r.scales[k >> 1] | sc << 16 : sc;
-                }
-                return r;
-            };
-            Cursor cur{0, 0, 0}, ahead{0, 0, 0};
-            Raw buf[3];
-#pragma unroll
-            for (int k = 0; k < 3; ++k) {
-                buf[k] = load(ahead);
-                advance(ahead, kp, 2, t.n_tiles);
-            }
             // Q: 64 rows -> fp16 after a power of two per row that brings its largest |q| to [2^10, 2^11)
-            // (the rope part by the same factor, in bf16); a warp per row, 16 + 2 dims per lane
-            take_ring(turn, t.image >= 0, bar(B_Q_FREE), bar(B_PART_DONE), abort_flag, p.err);
+            // (the rope part by the same factor, in bf16); a warp per row, 16 + 2 dims per lane, four rows
+            // in flight (the first four from before the last part's QK is done)
+            const int rows = t.rows, q_row0 = t.block * kUnitRows + kCtaRows * cta, first = t.first;
             float* qs = reinterpret_cast<float*>(smem + SM_QS) + 64 * (parts & 1);
-#pragma unroll 2
-            for (int r = warp - kProducerWarp0; r < kCtaRows; r += kProducerWarps) {
-                uint4 u[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-                uint32_t rw = 0;
-                const int row = t.block * kUnitRows + kCtaRows * cta + r;
-                if (row < t.rows) {
-                    const int tok = row / p.heads;
-                    const __nv_bfloat16* src = p.q + static_cast<int64_t>(t.first + tok) * p.q_st + static_cast<int64_t>(row - tok * p.heads) * p.q_sh;
-                    u[0] = ldg_nc_v4(src + 16 * lane);
-                    u[1] = ldg_nc_v4(src + 16 * lane + 8);
-                    if (p.rope) rw = __ldg(reinterpret_cast<const uint32_t*>(src + kLatent) + lane);
-                }
-                const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
-                float amax = 0.0f;
+#pragma unroll 1
+            for (int rr = warp - kQWarp0; rr < kCtaRows; rr += 4 * kQWarps) {
+                uint4 u[4][2];
+                uint32_t rw[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xFFFF0000u))));
-#pragma unroll
-                for (int o = 16; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-                const int eb = static_cast<int>((__float_as_uint(amax) >> 23) & 0xFFu);
-                const int e = eb > 0 && eb < 255 ? max(eb - 127 - 10, -100) : 0;
-                float factor = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-                float mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                mul = p.scale_log2 < 0.0f ? -mul : mul;
-                if (factor == 0.0f) {              // every score 0: zero queries, and a factor that keeps a hidden score's -inf
-                    factor = 1.0f;
-                    mul = 0.0f;
+                for (int j = 0; j < 4; ++j) {
+                    u[j][0] = u[j][1] = make_uint4(0, 0, 0, 0);
+                    rw[j] = 0;
+                    const int row = q_row0 + rr + j * kQWarps;
+                    if (row < rows) {
+                        const int tok = row / p.heads;
+                        const __nv_bfloat16* src = p.q + static_cast<int64_t>(first + tok) * p.q_st + static_cast<int64_t>(row - tok * p.heads) * p.q_sh;
+                        u[j][0] = ldg_nc_v4(src + 16 * lane);
+                        u[j][1] = ldg_nc_v4(src + 16 * lane + 8);
+                        if (p.rope) rw[j] = __ldg(reinterpret_cast<const uint32_t*>(src + kLatent) + lane);
+                    }
                 }
-                uint32_t h[8];
+                if (rr < kQWarps && parts > 0) mbar_wait(bar(B_Q_FREE), (parts - 1) & 1, abort_flag, p.err);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[j] = pack_half2(__uint_as_float(w[j] << 16) * mul, __uint_as_float(w[j] & 0xFFFF0000u) * mul);
-                // dims 16 lane + 8 c: half lane / 16, piece (lane / 2) % 8, chunk 2 (lane % 2) + c
-                uint8_t* dst = smem + SM_Q + ((lane >> 4) * 4 + 2 * (lane & 1)) * (kCtaRows * 128) + r * 128 + ((((lane >> 1) & 7) ^ (r & 7)) << 4);
-                *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
-                *reinterpret_cast<uint4*>(dst + kCtaRows * 128) = make_uint4(h[4], h[5], h[6], h[7]);
-                if (p.rope) {
-                    const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(rw << 16) * mul, __uint_as_float(rw & 0xFFFF0000u) * mul);
-                    *reinterpret_cast<uint32_t*>(smem + SM_Q + 8 * (kCtaRows * 128) + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)) =
-                        *reinterpret_cast<const uint32_t*>(&two);
+                for (int j = 0; j < 4; ++j) {
+                    const int r = rr + j * kQWarps;
+                    const uint32_t w[8] = {u[j][0].x, u[j][0].y, u[j][0].z, u[j][0].w, u[j][1].x, u[j][1].y, u[j][1].z, u[j][1].w};
+                    float amax = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
+#pragma unroll
+                    for (int o = 16; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+                    const int eb = static_cast<int>((__float_as_uint(amax) >> 23) & 0xFFu);
+                    const int e = eb > 0 && eb < 255 ? max(eb - 127 - 10, -100) : 0;
+                    float factor = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                    float mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                    mul = p.scale_log2 < 0.0f ? -mul : mul;
+                    if (factor == 0.0f) {          // every score 0: zero queries, and a factor that keeps a hidden score's -inf
+                        factor = 1.0f;
+                        mul = 0.0f;
+                    }
+                    uint32_t h[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) h[i] = pack_half2(__uint_as_float(w[i] << 16) * mul, __uint_as_float(w[i] & 0xFFFF0000u) * mul);
+                    // dims 16 lane + 8 c: half lane / 16, piece (lane / 2) % 8, chunk 2 (lane % 2) + c
+                    uint8_t* dst = smem + SM_Q + ((lane >> 4) * 4 + 2 * (lane & 1)) * (kCtaRows * 128) + r * 128 + ((((lane >> 1) & 7) ^ (r & 7)) << 4);
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(dst + kCtaRows * 128) = make_uint4(h[4], h[5], h[6], h[7]);
+                    if (p.rope) {
+                        const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(rw[j] << 16) * mul, __uint_as_float(rw[j] & 0xFFFF0000u) * mul);
+                        *reinterpret_cast<uint32_t*>(smem + SM_Q + 8 * (kCtaRows * 128) + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)) =
+                            *reinterpret_cast<const uint32_t*>(&two);
+                    }
+                    if (lane == 0) qs[r] = factor;
                 }
-                if (lane == 0) qs[r] = factor;
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) leader_arrive(bar(B_Q_FULL));
             ++parts;
-            if (t.image >= 0) {
-                const int all = t.n_tiles * (k_stages + kVStages);
-                n += all;
-                slot = n % kStages;
-                phase = (n / kStages) & 1;
-                continue;
-            }
-            // one stage's address once its slot is free
-            auto take = [&]() -> uint8_t* {
-                if (n >= kStages) mbar_wait(bar(B_EMPTY + slot), phase ^ 1, abort_flag, p.err);
-                uint8_t* dst = smem + SM_RING + slot * kStageBytes;
-                ++n;
-                if (++slot == kStages) {
-                    slot = 0;
-                    phase ^= 1;
-                }
-                return dst;
-            };
-            auto publish = [&](int count) {      // the last `count` stages taken
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0)
-                    for (int k = count; k >= 1; --k) leader_arrive(bar(B_FULL + (slot >= k ? slot - k : slot - k + kStages)));
-            };
-#pragma unroll 1
-            while (cur.u < total) {
-#pragma unroll
-                for (int b = 0; b < 3; ++b) {
-                    if (cur.u >= total) break;
-                    const Raw& r = buf[b];
-                    if (cur.s == 2 && kp == 3) {
-                        uint8_t* dst = take() + r0 * 128 + swz;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(dst + 4096 * k) = r.v[k];
-                        publish(1);
-                    } else {
-                        const bool v = cur.s >= kp;
-                        uint32_t s2[4];      // row k's two block scales
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            s2[k] = e4m3x2_to_f16x2(static_cast<uint16_t>(r.scales[k >> 1] >> (16 * (k & 1))));
-                            // a NaN block scale counts as 0 in V: rows that see the token are NaN by its score,
-                            // rows that do not (probability 0) stay clear of it
-                            if (v) s2[k] = max_f16x2(s2[k], 0u);
-                        }
-                        if (!v) {
-#pragma unroll
-                            for (int s = 0; s < 4; s += 2) {      // stages s, s + 1: chunk s, s + 1 of each row (one block scale)
-                                uint8_t* d0 = take() + r0 * 128 + swz;
-                                uint8_t* d1 = take() + r0 * 128 + swz;
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    const uint32_t sc = __byte_perm(s2[k], s2[k], s ? 0x3232 : 0x1010);
-                                    *reinterpret_cast<uint4*>(d0 + 4096 * k) = dequant8(s ? r.v[k].z : r.v[k].x, sc);
-                                    *reinterpret_cast<uint4*>(d1 + 4096 * k) = dequant8(s ? r.v[k].w : r.v[k].y, sc);
-                                }
-                                publish(2);
-                            }
-                        } else {
-#pragma unroll
-                            for (int q = 0; q < 2; ++q) {         // 64 tokens: stages of chunks 0, 1 and 2, 3
-                                uint8_t* d0 = take() + r0 * 128 + swz;
-                                uint8_t* d1 = take() + r0 * 128 + swz;
-#pragma unroll
-                                for (int j = 0; j < 2; ++j) {
-                                    const int k = 2 * q + j;
-                                    const uint32_t lo = __byte_perm(s2[k], s2[k], 0x1010), hi = __byte_perm(s2[k], s2[k], 0x3232);
-                                    *reinterpret_cast<uint4*>(d0 + 4096 * j) = dequant8(r.v[k].x, lo);
-                                    *reinterpret_cast<uint4*>(d0 + 4096 * j + 8192) = dequant8(r.v[k].y, lo);
-                                    *reinterpret_cast<uint4*>(d1 + 4096 * j) = dequant8(r.v[k].z, hi);
-                                    *reinterpret_cast<uint4*>(d1 + 4096 * j + 8192) = dequant8(r.v[k].w, hi);
-                                }
-                                publish(2);
-                            }
-                        }
-                    }
-                    buf[b] = load(ahead);
-                    advance(ahead, kp, 2, t.n_tiles);
-                    advance(cur, kp, 2, t.n_tiles);
-                }
-            }
         }
     } else {
-        warpgroup_reg_alloc<kRegsSoftmax>();
+        set_registers<kRegsSoftmax>();
         // ============================================================ softmax
         // warp: TMEM lanes 32 sp .., columns 64 ch .. of a tile's 128: row 32 (sp & 1) + lane, token
         // quarter q4; the four warps of a row exchange their maxima in shared memory
@@ -817,46 +716,28 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         bool first_part = true;
         griddep_wait();                          // the image kernel's token bits
 #pragma unroll 1
-        while (next_part(p, range, t)) {
-            const int32_t* table = p.tables + t.b * p.tables_stride;
-            const int grow = t.block * kUnitRows + kCtaRows * cta + row;      // row of the sequence
-            const bool real = grow < t.rows;
-            const int tok = real ? grow / p.heads : 0;
-            const int lim = real ? min(t.L, t.L - t.n + tok + 1) : 0;         // tokens the row sees
+        while (next_part(p, work)) {
+            const int n_tiles = t.n_tiles, tile0 = t.tile0, image = t.image;
+            int lim = 0;                                                      // tokens the row sees
+            {
+                const int grow = t.block * kUnitRows + kCtaRows * cta + row;  // row of the sequence
+                if (grow < t.rows) lim = min(t.L, t.L - t.n + grow / p.heads + 1);
+            }
             float factor = 1.0f, m_ref = -INFINITY, l = 0.0f;
-            // What the next tile's token masks are made of, loaded a tile ahead.  Image: the bits of the
-            // quarter's tokens that exist and of those that hold a NaN; else: the page ids of tokens lane
-            // and 32 + lane.
-            auto load_masks = [&](int i, uint32_t (&w)[4]) {
-                const int tok0 = (t.tile0 + i) * kTile + 64 * q4;
-                if (t.image >= 0) {
-                    const int blk = t.image + min(tok0, t.L - 1) / kImageTok, k = (tok0 & (kImageTok - 1)) >> 5;
-                    const uint2 have = *reinterpret_cast<const uint2*>(p.image_bits + 8 * static_cast<int64_t>(blk) + k);
-                    const uint2 nans = *reinterpret_cast<const uint2*>(p.image_bits + 8 * static_cast<int64_t>(blk) + 4 + k);
-                    w[0] = have.x; w[1] = have.y; w[2] = nans.x; w[3] = nans.y;
-                } else {
-                    w[0] = tok0 + lane < t.end ? __ldg(table + ((tok0 + lane) >> p.page_shift)) : 0;
-                    w[1] = tok0 + 32 + lane < t.end ? __ldg(table + ((tok0 + 32 + lane) >> p.page_shift)) : 0;
-                }
+            // bits of the quarter's tokens that exist, and of those that hold a NaN, loaded a tile ahead
+            auto load_bits = [&](int i, uint2 (&w)[2]) {
+                const int tok0 = (tile0 + i) * kTile + 64 * q4;
+                const uint32_t* src = p.image_bits + 8 * static_cast<int64_t>(image + min(tok0, t.L - 1) / kImageTok) + ((tok0 & (kImageTok - 1)) >> 5);
+                w[0] = *reinterpret_cast<const uint2*>(src);
+                w[1] = *reinterpret_cast<const uint2*>(src + 4);
             };
-            uint32_t ahead[4];
-            if (t.n_tiles > 0) load_masks(0, ahead);
+            uint2 ahead[2];
+            if (n_tiles > 0) load_bits(0, ahead);
 #pragma unroll 1
-            for (int i = 0; i < t.n_tiles; ++i, ++tile) {
-                uint32_t bits[4] = {ahead[0], ahead[1], 0, 0};
-                if (t.image >= 0) {
-                    bits[2] = ahead[2];
-                    bits[3] = ahead[3];
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const bool missing = static_cast<int64_t>(ahead[k]) >= p.num_pages;      // (a negative id is a large one)
-                        if (missing) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
-                        bits[k] = __ballot_sync(0xFFFFFFFFu, !missing);
-                    }
-                }
-                if (i + 1 < t.n_tiles) load_masks(i + 1, ahead);
-                const int see = lim - ((t.tile0 + i) * kTile + 64 * q4);     // tokens of the quarter the row sees
+            for (int i = 0; i < n_tiles; ++i, ++tile) {
+                const uint2 have = ahead[0], nan = ahead[1];
+                if (i + 1 < n_tiles) load_bits(i + 1, ahead);
+                const int see = lim - ((tile0 + i) * kTile + 64 * q4);     // tokens of the quarter the row sees
                 mbar_wait(bar(B_S_FULL + (tile & 1)), (tile >> 1) & 1, abort_flag, p.err);
                 tc_fence_after();
                 if (i == 0) factor = reinterpret_cast<const float*>(smem + SM_QS)[64 * (parts & 1) + row];
@@ -867,11 +748,11 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) leader_arrive(bar(B_S_FREE + (tile & 1)));
-                if (!__all_sync(0xFFFFFFFFu, see >= 64 && (bits[0] & bits[1]) == 0xFFFFFFFFu && (bits[2] | bits[3]) == 0)) {
+                if (!__all_sync(0xFFFFFFFFu, see >= 64 && (have.x & have.y) == 0xFFFFFFFFu && (nan.x | nan.y) == 0)) {
 #pragma unroll
                     for (int k = 0; k < 64; ++k) {
-                        if ((bits[2 + (k >> 5)] >> (k & 31)) & 1u) x[k] = __int_as_float(0x7FFFFFFF);
-                        if (k >= see || !((bits[k >> 5] >> (k & 31)) & 1u)) x[k] = -INFINITY;
+                        if (((k < 32 ? nan.x : nan.y) >> (k & 31)) & 1u) x[k] = __int_as_float(0x7FFFFFFF);
+                        if (k >= see || !(((k < 32 ? have.x : have.y) >> (k & 31)) & 1u)) x[k] = -INFINITY;
                     }
                 }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -892,10 +773,10 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < 32; ++k) {
-                    const float a = ex2_approx(fmaf(x[2 * k], factor, -base)), c = ex2_approx(fmaf(x[2 * k + 1], factor, -base));
+                    const float a = ex2_approx(fmaf(x[2 * k], factor, -base)), b = ex2_approx(fmaf(x[2 * k + 1], factor, -base));
                     sum[k & 1] += a;
-                    sum[2 + (k & 1)] += c;
-                    pk[k] = pack_half2(a, c);
+                    sum[2 + (k & 1)] += b;
+                    pk[k] = pack_half2(a, b);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 if (i > 0) {
@@ -928,26 +809,30 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             lsum[64 * q4 + row] = l;
             named_bar_sync(1 + (sp & 1), 128);
             l = (lsum[row] + lsum[64 + row]) + (lsum[128 + row] + lsum[192 + row]);
-            if (t.n_tiles > 0) mbar_wait(bar(B_PV_DONE), (tile - 1) & 1, abort_flag, p.err);
+            if (n_tiles > 0) mbar_wait(bar(B_PV_DONE), (tile - 1) & 1, abort_flag, p.err);
             tc_fence_after();
             const bool any = l > 0.0f || l != l, whole = t.head && t.tail;
-            const int head = grow - tok * p.heads;
-            const int64_t part = 2 * pair + (first_part ? 0 : 1);
+            const int grow = t.block * kUnitRows + kCtaRows * cta + row;
+            const bool real = grow < t.rows;
+            const int tok = real ? grow / p.heads : 0, head = grow - tok * p.heads;
+            const int64_t part_row = (2 * pair + (first_part ? 0 : 1)) * kUnitRows + kCtaRows * cta + row;
             const float mul = whole ? (any ? p.out_scale / l : 0.0f) : 1.0f;
-            __nv_bfloat16* out = p.out + static_cast<int64_t>(t.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh;
-            float* part_o = p.part_o + (part * kUnitRows + kCtaRows * cta + row) * kLatent;
             if (q4 == 0) {
                 if (!whole)
-                    *reinterpret_cast<float2*>(p.part_ml + 2 * (part * kUnitRows + kCtaRows * cta + row)) = make_float2(m_ref, l);
+                    *reinterpret_cast<float2*>(p.part_ml + 2 * part_row) = make_float2(m_ref, l);
                 else if (p.lse && real)
                     p.lse[static_cast<int64_t>(t.first + tok) * p.heads + head] = any ? 0.69314718055994531f * (m_ref + log2f(l)) : -INFINITY;
             }
             if (!whole && threadIdx.x == 0 && cta == 0)
-                p.parts[part] = PartInfo{1, t.head, t.tail, t.first, t.n, t.block};
+                p.parts[2 * pair + (first_part ? 0 : 1)] = PartInfo{1, t.head, t.tail, t.first, t.n, t.block};
+            // 32 bytes a store: with 16 the stores took twice as long, a wavefront per row and store
+            __nv_bfloat16* out = p.out + static_cast<int64_t>(t.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh + 256 * (sp >> 1) + 16 * ch;
+            float* part_o = p.part_o + part_row * kLatent + 256 * (sp >> 1) + 16 * ch;
+            const bool wide = (reinterpret_cast<uintptr_t>(p.out) % 32 == 0) && p.o_st % 16 == 0 && p.o_sh % 16 == 0;
 #pragma unroll 1
             for (int pp = 0; pp < 8; pp += 2) {         // pieces pp, pp + 1: 16 dims of each, in columns 8 pp .. and 64 + 8 pp ..
                 uint32_t o[2][16];
-                if (t.n_tiles > 0) {
+                if (n_tiles > 0) {
                     tmem_ld16(tmem + kTO + 128 * ch + 8 * pp + lanes, o[0]);
                     tmem_ld16(tmem + kTO + 128 * ch + 64 + 8 * pp + lanes, o[1]);
                     tmem_wait_ld();
@@ -955,27 +840,30 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 if (!real) continue;
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const int d = 256 * (sp >> 1) + 32 * (pp + j) + 16 * ch;
-                    float v[16];
+                    uint32_t v[16];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) v[k] = any ? __uint_as_float(o[k >> 3][8 * j + (k & 7)]) * mul : 0.0f;
+                    for (int k = 0; k < 16; ++k) v[k] = any ? __float_as_uint(__uint_as_float(o[k >> 3][8 * j + (k & 7)]) * mul) : 0u;
                     if (whole) {
                         uint32_t w[8];
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+                            const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
                             w[k] = *reinterpret_cast<const uint32_t*>(&two);
                         }
-                        *reinterpret_cast<uint4*>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
-                        *reinterpret_cast<uint4*>(out + d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                        __nv_bfloat16* dst = out + 32 * (pp + j);
+                        if (wide) {
+                            st_global_v8(dst, w);
+                        } else {
+                            *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                        }
                     } else if (any) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            *reinterpret_cast<float4*>(part_o + d + 4 * k) = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                        st_global_v8(part_o + 32 * (pp + j), v);
+                        st_global_v8(part_o + 32 * (pp + j) + 8, v + 8);
                     }
                 }
             }
-            if (t.n_tiles > 0) {
+            if (n_tiles > 0) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) leader_arrive(bar(B_O_FREE));
@@ -1063,34 +951,32 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_const
 }
 
 struct PrefillPlan {
+    int group;               // sequences per pass over the workspace
     int pairs, image_blocks;
     size_t image_bytes, bits_bytes, o_bytes, ml_bytes, ws_bytes;
 };
 
-constexpr size_t kImageCap = size_t(1) << 30;      // images take at most this, or one sequence's
+// Images take at most this, or one sequence's; a larger batch runs in groups of sequences.
+constexpr size_t kImageCap = size_t(1) << 30;
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
 PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_len, int max_seq_len) {
     PrefillPlan pl{};
-    // no more pairs than tiles there can be
+    const int64_t one = (static_cast<int64_t>(max_seq_len) + kImageTok - 1) / kImageTok;
+    const int64_t cap = static_cast<int64_t>(kImageCap / (9 * kStageBytes));
+    const int64_t fit = one > 0 ? cap / one : batch;
+    pl.group = static_cast<int>(fit < 1 ? 1 : (fit < batch ? fit : batch));
+    // no more pairs than tiles there can be in a group
     const int64_t longest = max_q_len < total_q ? max_q_len : total_q;
-    const int64_t by_seq = (longest * num_heads + kUnitRows - 1) / kUnitRows * batch;
-    const int64_t by_rows = (static_cast<int64_t>(total_q) * num_heads + static_cast<int64_t>(batch) * (kUnitRows - 1)) / kUnitRows;
-    const int64_t units = by_seq < by_rows ? by_seq : by_rows;
-    const int64_t tiles = units * ((static_cast<int64_t>(max_seq_len) + kTile - 1) / kTile);
+    const int64_t by_seq = (longest * num_heads + kUnitRows - 1) / kUnitRows * pl.group;
+    const int64_t by_rows = (static_cast<int64_t>(total_q) * num_heads + static_cast<int64_t>(pl.group) * (kUnitRows - 1)) / kUnitRows;
+    const int64_t tiles = (by_seq < by_rows ? by_seq : by_rows) * ((static_cast<int64_t>(max_seq_len) + kTile - 1) / kTile);
     int64_t pairs = device_sm_count() / 2;
     pairs = pairs > kMaxPairs ? kMaxPairs : pairs;
     pairs = pairs > tiles ? tiles : pairs;
     pl.pairs = static_cast<int>(pairs < 1 ? 1 : pairs);
-    // only sequences of at least kImageUnits units have an image
-    const int64_t least = static_cast<int64_t>(kImageUnits - 1) * kUnitRows / num_heads + 1;      // their new tokens
-    int64_t seqs = longest >= least ? total_q / least : 0;
-    seqs = seqs > batch ? batch : seqs;
-    const int64_t one = (static_cast<int64_t>(max_seq_len) + kImageTok - 1) / kImageTok;
-    const int64_t cap = static_cast<int64_t>(kImageCap / (9 * kStageBytes));
-    int64_t blocks = seqs * one;
-    if (blocks > cap) blocks = cap > one ? cap : one;
+    const int64_t blocks = one * pl.group;
     pl.image_blocks = static_cast<int>(blocks);
     pl.image_bytes = static_cast<size_t>(blocks) * 9 * kStageBytes;
     pl.bits_bytes = round256(static_cast<size_t>(blocks) * 32);
@@ -1167,7 +1053,7 @@ extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
     p.scale_log2 = bmm1_scale * 1.4426950408889634f; p.out_scale = bmm2_scale;
     p.out = static_cast<__nv_bfloat16*>(out); p.o_st = out_stride_t; p.o_sh = out_stride_h;
-    p.lse = lse; p.err = err_flag; p.pairs = pl.pairs; p.image_blocks = pl.image_blocks;
+    p.lse = lse; p.err = err_flag; p.pairs = pl.pairs;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     p.image = ws;
     p.image_bits = reinterpret_cast<uint32_t*>(ws += pl.image_bytes);
@@ -1177,19 +1063,27 @@ extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     int rc = set_smem_limit();
     if (rc != NVFP4KV_OK) return rc;
-    const dim3 grid(2 * pl.pairs);
-    cudaError_t e = cudaSuccess;
-    if (pl.image_blocks > 0) {
-        prefill_image_kernel<<<pl.image_blocks, 256, 0, st>>>(p);
-        if ((rc = check_launch("nvfp4kv_mla_prefill image")) != NVFP4KV_OK) return rc;
-        // its set-up overlaps the image kernel; all else it reads was there before that one
-        e = launch_dependent(mla_prefill_kernel, grid, dim3(kThreads), kSmemBytes, st, p);
-    } else {
-        mla_prefill_kernel<<<grid, kThreads, kSmemBytes, st>>>(p);
+    for (int b0 = 0; b0 < batch; b0 += pl.group) {
+        p.batch = batch - b0 < pl.group ? batch - b0 : pl.group;
+        p.tables = tables + b0 * tables_stride;
+        p.cu = cu_seqlens_q + b0;
+        p.seq_lens = seq_lens + b0;
+        const dim3 grid(2 * pl.pairs);
+        cudaError_t e = cudaSuccess;
+        if (pl.image_blocks > 0) {
+            prefill_image_kernel<<<pl.image_blocks, 256, 0, st>>>(p);
+            if ((rc = check_launch("nvfp4kv_mla_prefill image")) != NVFP4KV_OK) return rc;
+            // its set-up overlaps the image kernel; all else it reads was there before that one
+            e = launch_dependent(mla_prefill_kernel, grid, dim3(kThreads), kSmemBytes, st, p);
+        } else {
+            mla_prefill_kernel<<<grid, kThreads, kSmemBytes, st>>>(p);
+        }
+        if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill launch failed: %s", cudaGetErrorString(e));
+        if ((rc = check_launch("nvfp4kv_mla_prefill")) != NVFP4KV_OK) return rc;
+        if (pl.pairs == 1) continue;
+        e = launch_dependent(prefill_combine_kernel, dim3(pl.pairs * kUnitRows), dim3(128), 0, st, p);
+        if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill combine launch failed: %s", cudaGetErrorString(e));
+        if ((rc = check_launch("nvfp4kv_mla_prefill combine")) != NVFP4KV_OK) return rc;
     }
-    if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill launch failed: %s", cudaGetErrorString(e));
-    if ((rc = check_launch("nvfp4kv_mla_prefill")) != NVFP4KV_OK || pl.pairs == 1) return rc;
-    e = launch_dependent(prefill_combine_kernel, dim3(pl.pairs * kUnitRows), dim3(128), 0, st, p);
-    if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill combine launch failed: %s", cudaGetErrorString(e));
-    return check_launch("nvfp4kv_mla_prefill combine");
+    return NVFP4KV_OK;
 }
