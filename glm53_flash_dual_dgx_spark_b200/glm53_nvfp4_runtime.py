@@ -598,6 +598,33 @@ def index_scores_buffer(device=None) -> torch.Tensor | None:
     return None if ws is None else ws.view(torch.float32)
 
 
+# ------------------------------------------------------------------ serving operators: the call
+# A few tokens' operators run for less time on the device than their call takes on the host, so the
+# call below uses torch's raw getters: 3 us less than the stream object and device guard.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_err_ptrs: dict = {}
+
+
+def _call(name: str, index: int, *args) -> None:
+    """The C entry ``name`` on device ``index``'s current stream, with the device error word; raises
+    on a non-OK code."""
+    err = _err_ptrs.get(index)
+    if err is None:
+        err = _err_ptrs[index] = _err_word(torch.device("cuda", index)).data_ptr()
+    fn = getattr(_lib.lib(), name)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, err, _raw_stream(index))
+    else:
+        with _on_device(torch.device("cuda", index)):
+            rc = fn(*args, err, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _vector(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
+
+
 # ------------------------------------------------------------------ rotary positions
 _ROPE_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
 _INDEX_DTYPES = {torch.int64: _lib.INDEX_I64, torch.int32: _lib.INDEX_I32}
@@ -638,12 +665,13 @@ def _check_angles(cos_sin: torch.Tensor, positions: torch.Tensor, T: int, rotary
     if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != rotary_dim \
             or not cos_sin.is_contiguous():
         raise ValueError(f"cos_sin must be a contiguous float32 [positions, {rotary_dim}] table")
-    pos = positions.reshape(-1).contiguous()
-    if pos.numel() != T:
-        raise ValueError(f"positions has {pos.numel()} entries for {T} tokens")
-    if pos.dtype not in _INDEX_DTYPES:
+    pos = _vector(positions)
+    if pos.shape[0] != T:
+        raise ValueError(f"positions has {pos.shape[0]} entries for {T} tokens")
+    dtype = _INDEX_DTYPES.get(pos.dtype)
+    if dtype is None:
         raise TypeError("positions must be int64 or int32")
-    return pos, _INDEX_DTYPES[pos.dtype]
+    return pos, dtype
 
 
 def apply_rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, rope_offset: int | None = None,
@@ -655,30 +683,27 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, 
     a position outside the table leaves its token as it is and is flagged in the device error
     word.  cos_sin: see rope_cos_sin."""
     _require_cuda(x, "x")
-    if x.dtype not in _ROPE_DTYPES:
+    dtype = _ROPE_DTYPES.get(x.dtype)
+    if dtype is None:
         raise TypeError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
-    if x.dim() not in (2, 3) or x.stride(-1) != 1:
+    shape, st = x.shape, x.stride()
+    if len(shape) not in (2, 3) or st[-1] != 1:
         raise ValueError("x must be [T, H, D] or [T, D] with a contiguous last dimension")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
     _require_cuda(out, "out")
-    if out.shape != x.shape or out.dtype != x.dtype or out.stride(-1) != 1:
+    ost = out.stride()
+    if out.shape != shape or out.dtype != x.dtype or ost[-1] != 1:
         raise ValueError("out must have x's shape and dtype and a contiguous last dimension")
-    T, D = x.shape[0], x.shape[-1]
-    H = x.shape[1] if x.dim() == 3 else 1
-    r = cos_sin.shape[-1]
-    off = D - r if rope_offset is None else int(rope_offset)
+    T, D = shape[0], shape[-1]
+    H, sh, osh = (shape[1], st[1], ost[1]) if len(shape) == 3 else (1, D, D)
+    P, r = cos_sin.shape
     pos, pdt = _check_angles(cos_sin, positions, T, r)
     if T == 0 or H == 0:
         return out
-    dev = x.device
-    with _on_device(dev):
-        rc = _lib.lib().nvfp4kv_rope(x.data_ptr(), _ROPE_DTYPES[x.dtype], T, H, D, x.stride(0),
-                                     x.stride(1) if x.dim() == 3 else D, pos.data_ptr(), pdt, cos_sin.data_ptr(),
-                                     cos_sin.shape[0], r, off, int(interleaved), int(inverse), out.data_ptr(),
-                                     out.stride(0), out.stride(1) if x.dim() == 3 else D, _err_word(dev).data_ptr(),
-                                     _stream(dev))
-    _lib.check(rc, "nvfp4kv_rope")
+    _call("nvfp4kv_rope", x.get_device(), x.data_ptr(), dtype, T, H, D, st[0], sh, pos.data_ptr(), pdt,
+          cos_sin.data_ptr(), P, r, D - r if rope_offset is None else int(rope_offset), int(interleaved),
+          int(inverse), out.data_ptr(), ost[0], osh)
     return out
 
 
@@ -696,10 +721,11 @@ def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_
     rope = rope_cache.view(-1, ROPE)
     if rope.dtype != torch.bfloat16:
         raise TypeError("rope_cache must be bf16")
-    slot = slot_mapping.reshape(-1).contiguous()
-    if slot.numel() != T:
-        raise ValueError(f"slot_mapping has {slot.numel()} entries for {T} tokens")
-    if slot.dtype not in _INDEX_DTYPES:
+    slot = _vector(slot_mapping)
+    if slot.shape[0] != T:
+        raise ValueError(f"slot_mapping has {slot.shape[0]} entries for {T} tokens")
+    sdt = _INDEX_DTYPES.get(slot.dtype)
+    if sdt is None:
         raise TypeError("slot_mapping must be int64 or int32")
     pos, pdt = _check_angles(cos_sin, positions, T, ROPE)
     H, qs, qos = 0, (0, 0), (0, 0)
@@ -711,19 +737,15 @@ def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_
                 raise ValueError(f"{name} must be bf16 [T, H, 64] with a contiguous last dimension")
         if q_out.shape != q_pe.shape:
             raise ValueError("q_out must have q_pe's shape")
-        H, qs, qos = q_pe.shape[1], q_pe.stride()[:2], q_out.stride()[:2]
+        H, qs, qos = q_pe.shape[1], q_pe.stride(), q_out.stride()
     elif q_out is not None:
         raise ValueError("q_out without q_pe")
     if T == 0:
         return q_out
-    dev = k_pe.device
-    with _on_device(dev):
-        rc = _lib.lib().nvfp4kv_append_rope_rotated(
-            k_pe.data_ptr(), T, k_pe.stride(0), rope.data_ptr(), rope.shape[0], slot.data_ptr(),
-            _INDEX_DTYPES[slot.dtype], pos.data_ptr(), pdt, cos_sin.data_ptr(), cos_sin.shape[0], int(interleaved),
-            q_pe.data_ptr() if H else None, H, *qs, q_out.data_ptr() if H else None, *qos,
-            _err_word(dev).data_ptr(), _stream(dev))
-    _lib.check(rc, "nvfp4kv_append_rope_rotated")
+    _call("nvfp4kv_append_rope_rotated", k_pe.get_device(), k_pe.data_ptr(), T, k_pe.stride(0), rope.data_ptr(),
+          rope.shape[0], slot.data_ptr(), sdt, pos.data_ptr(), pdt, cos_sin.data_ptr(), cos_sin.shape[0],
+          int(interleaved), q_pe.data_ptr() if H else None, H, qs[0], qs[1], q_out.data_ptr() if H else None,
+          qos[0], qos[1])
     return q_out
 
 
@@ -751,16 +773,19 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
     T, H, D = query.shape
     if kv_lora_rank != LATENT or D != kv_lora_rank + qk_rope_head_dim:
         raise ValueError(f"query dim {D} must equal kv_lora_rank (512) + qk_rope_head_dim")
-    pool = kv_cache.view(-1, NV_BYTES)
+    if kv_cache.shape[-1] != NV_BYTES or not kv_cache.is_contiguous():
+        raise ValueError("kv_cache must be a contiguous pool of 288-byte rows")
+    rows = kv_cache.numel() // NV_BYTES
     page_size = kv_cache.shape[-2] if kv_cache.dim() >= 3 else 64
     for name, t in (("block_tables", block_tables), ("cu_seqlens_q", cu_seqlens_q), ("seq_lens", seq_lens)):
         _require_cuda(t, name)
         if t.dtype != torch.int32:
             raise TypeError(f"{name} must be int32")
-    B = seq_lens.numel()
-    if block_tables.dim() != 2 or block_tables.shape[0] != B or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+    cu, sl = _vector(cu_seqlens_q), _vector(seq_lens)
+    B, ts = sl.shape[0], block_tables.stride()
+    if block_tables.dim() != 2 or block_tables.shape[0] != B or (block_tables.shape[1] > 1 and ts[1] != 1):
         raise ValueError("block_tables must be [B, width] with a contiguous last dimension")
-    if cu_seqlens_q.numel() != B + 1:
+    if cu.shape[0] != B + 1:
         raise ValueError("cu_seqlens_q must have one entry more than seq_lens")
     if block_tables.shape[1] * page_size < max_seq_len:
         raise ValueError("block_tables too narrow for max_seq_len")
@@ -771,34 +796,30 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
     rope = None
     if rope_cache is not None:
         _require_cuda(rope_cache, "rope_cache")
-        rope = rope_cache.reshape(-1, ROPE)
-        if rope.dtype != torch.bfloat16 or rope.shape[0] != pool.shape[0] or not rope.is_contiguous():
+        if rope_cache.dtype != torch.bfloat16 or rope_cache.numel() != rows * ROPE or not rope_cache.is_contiguous():
             raise ValueError("rope_cache must be a contiguous bf16 [pool rows, 64] side-pool")
+        rope = rope_cache.data_ptr()
     lse = torch.empty(T, H, dtype=torch.float32, device=query.device) if return_lse else None
-    dev = query.device
     if T > 0 and B > 0:
-        with _on_device(dev):
-            key = ("prefill", B, T, H, int(max_q_len), int(max_seq_len), dev.index)
-            need = _ws_sizes.get(key)
-            if need is None:
-                n = ctypes.c_size_t(0)
+        index = query.get_device()
+        key = ("prefill", B, T, H, max_q_len, max_seq_len, index)
+        need = _ws_sizes.get(key)
+        if need is None:
+            n = ctypes.c_size_t(0)
+            with _on_device(query.device):
                 _lib.check(_lib.lib().nvfp4kv_mla_prefill_workspace_size(B, T, H, int(max_q_len), int(max_seq_len),
                                                                          ctypes.byref(n)),
                            "nvfp4kv_mla_prefill_workspace_size")
-                need = _ws_sizes[key] = int(n.value)
-            ws = workspace_buffer
-            if need and (ws is None or not ws.is_cuda or not ws.is_contiguous() or ws.data_ptr() % 256
-                         or ws.numel() * ws.element_size() < need):
-                ws = _stream_buffer(dev, "prefill_ws", need, torch.uint8)
-            cu, sl = cu_seqlens_q.contiguous(), seq_lens.contiguous()
-            rc = _lib.lib().nvfp4kv_mla_prefill(
-                query.data_ptr(), query.stride(0), query.stride(1), pool.data_ptr(), pool.shape[0],
-                rope.data_ptr() if rope is not None else None, block_tables.data_ptr(), block_tables.stride(0),
-                cu.data_ptr(), sl.data_ptr(), B, T, H, D, kv_lora_rank, int(page_size), int(max_q_len),
-                int(max_seq_len), float(bmm1_scale), float(bmm2_scale), out.data_ptr(), out.stride(0), out.stride(1),
-                lse.data_ptr() if lse is not None else None, ws.data_ptr() if need else None, need,
-                _err_word(dev).data_ptr(), _stream(dev))
-        _lib.check(rc, "nvfp4kv_mla_prefill")
+            need = _ws_sizes[key] = int(n.value)
+        ws = workspace_buffer
+        if ws is None or not ws.is_cuda or not ws.is_contiguous() or ws.data_ptr() % 256 \
+                or ws.numel() * ws.element_size() < need:
+            ws = _stream_buffer(index, "prefill_ws", need, torch.uint8)
+        qs, os = query.stride(), out.stride()
+        _call("nvfp4kv_mla_prefill", index, query.data_ptr(), qs[0], qs[1], kv_cache.data_ptr(), rows, rope,
+              block_tables.data_ptr(), ts[0], cu.data_ptr(), sl.data_ptr(), B, T, H, D, kv_lora_rank, page_size,
+              int(max_q_len), int(max_seq_len), bmm1_scale, bmm2_scale, out.data_ptr(), os[0], os[1],
+              None if lse is None else lse.data_ptr(), ws.data_ptr(), need)
     return (out, lse) if return_lse else out
 
 
@@ -814,7 +835,7 @@ def _cache_list(caches):
             raise ValueError("caches must be contiguous [num_pages, page_size, ...] pools of one geometry")
     n = len(caches)
     ptrs = (ctypes.c_void_p * n)(*[c.data_ptr() for c in caches])
-    sizes = (ctypes.c_int64 * n)(*[c.numel() // pages * c.element_size() if pages else size for c in caches])
+    sizes = (ctypes.c_int64 * n)(*[c.stride(0) * c.element_size() for c in caches])
     return ptrs, sizes, n, pages, size
 
 
@@ -830,12 +851,12 @@ def _check_int32(**tensors):
             raise ValueError(f"{name} must be a contiguous vector")
 
 
-def _stream_buffer(dev: torch.device, name: str, n: int, dtype: torch.dtype) -> torch.Tensor:
+def _stream_buffer(index: int, name: str, n: int, dtype: torch.dtype) -> torch.Tensor:
     """A persistent buffer of the current stream, so that calls on two streams never share one."""
-    key = (name, dev.index, torch.cuda.current_stream(dev).cuda_stream)
+    key = (name, index, _raw_stream(index))
     ws = _bufs.get(key)
     if ws is None or ws.numel() < n:
-        ws = _bufs[key] = torch.empty(n, dtype=dtype, device=dev)
+        ws = _bufs[key] = torch.empty(n, dtype=dtype, device=torch.device("cuda", index))
     return ws
 
 
@@ -847,11 +868,8 @@ def copy_pages(caches, src: torch.Tensor, dst: torch.Tensor) -> None:
     _check_int32(src=src, dst=dst)
     if src.numel() != dst.numel():
         raise ValueError("src and dst must have the same length")
-    dev = caches[0].device
-    with _on_device(dev):
-        rc = _lib.lib().nvfp4kv_copy_pages(ptrs, sizes, n, pages, src.data_ptr(), dst.data_ptr(), src.numel(),
-                                           _err_word(dev).data_ptr(), _stream(dev))
-    _lib.check(rc, "nvfp4kv_copy_pages")
+    _call("nvfp4kv_copy_pages", caches[0].get_device(), ptrs, sizes, n, pages, src.data_ptr(), dst.data_ptr(),
+          src.shape[0])
 
 
 def free_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, slots: torch.Tensor,
@@ -861,13 +879,9 @@ def free_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, slots: torch.
     _check_int32(block_tables=block_tables, seq_lens=seq_lens, slots=slots, ref_counts=ref_counts)
     if seq_lens.numel() != block_tables.shape[0]:
         raise ValueError("seq_lens must have one entry per row of block_tables")
-    dev = block_tables.device
-    with _on_device(dev):
-        rc = _lib.lib().nvfp4kv_free_pages(block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1],
-                                           block_tables.shape[0], seq_lens.data_ptr(), slots.data_ptr(), slots.numel(),
-                                           ref_counts.data_ptr(), ref_counts.numel(), _err_word(dev).data_ptr(),
-                                           _stream(dev))
-    _lib.check(rc, "nvfp4kv_free_pages")
+    S, width = block_tables.shape
+    _call("nvfp4kv_free_pages", block_tables.get_device(), block_tables.data_ptr(), block_tables.stride(0), width, S,
+          seq_lens.data_ptr(), slots.data_ptr(), slots.shape[0], ref_counts.data_ptr(), ref_counts.shape[0])
 
 
 def fork_pages(caches, block_tables: torch.Tensor, seq_lens: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
@@ -882,14 +896,12 @@ def fork_pages(caches, block_tables: torch.Tensor, seq_lens: torch.Tensor, src: 
         raise ValueError("src and dst must have the same length")
     if seq_lens.numel() != block_tables.shape[0] or ref_counts.numel() != pages:
         raise ValueError("seq_lens must have one entry per row of block_tables, ref_counts one per page")
-    dev = block_tables.device
-    ws = _stream_buffer(dev, "fork_ws", max(3 * src.numel(), 1024), torch.int32)
-    with _on_device(dev):
-        rc = _lib.lib().nvfp4kv_fork_pages(ptrs, sizes, n, size, block_tables.data_ptr(), block_tables.stride(0),
-                                           block_tables.shape[1], block_tables.shape[0], seq_lens.data_ptr(),
-                                           src.data_ptr(), dst.data_ptr(), src.numel(), ref_counts.data_ptr(), pages,
-                                           ws.data_ptr(), ws.numel(), _err_word(dev).data_ptr(), _stream(dev))
-    _lib.check(rc, "nvfp4kv_fork_pages")
+    index, num = block_tables.get_device(), src.shape[0]
+    ws = _stream_buffer(index, "fork_ws", max(3 * num, 1024), torch.int32)
+    S, width = block_tables.shape
+    _call("nvfp4kv_fork_pages", index, ptrs, sizes, n, size, block_tables.data_ptr(), block_tables.stride(0), width, S,
+          seq_lens.data_ptr(), src.data_ptr(), dst.data_ptr(), num, ref_counts.data_ptr(), pages, ws.data_ptr(),
+          ws.shape[0])
 
 
 def compact_pages(caches, block_tables: torch.Tensor, ref_counts: torch.Tensor, out_tables: torch.Tensor | None = None,
@@ -905,16 +917,13 @@ def compact_pages(caches, block_tables: torch.Tensor, ref_counts: torch.Tensor, 
     _check_int32(block_tables=block_tables, ref_counts=ref_counts, out_tables=out_tables, out_ref_counts=out_ref_counts)
     if ref_counts.numel() != pages or out_ref_counts.numel() != pages or out_tables.shape != block_tables.shape:
         raise ValueError("ref_counts must have one entry per page, out_tables block_tables' shape")
-    dev = block_tables.device
-    live = torch.empty((), dtype=torch.int32, device=dev)
+    index = block_tables.get_device()
+    live = torch.empty((), dtype=torch.int32, device=block_tables.device)
     need = ctypes.c_int64(0)
     _lib.check(_lib.lib().nvfp4kv_compact_workspace_ints(pages, ctypes.byref(need)), "nvfp4kv_compact_workspace_ints")
-    ws = _stream_buffer(dev, "compact_ws", need.value, torch.int32)
-    with _on_device(dev):
-        rc = _lib.lib().nvfp4kv_compact_pages(ptrs, sizes, n, block_tables.data_ptr(), block_tables.stride(0),
-                                              block_tables.shape[1], block_tables.shape[0], ref_counts.data_ptr(), pages,
-                                              out_tables.data_ptr(), out_tables.stride(0), out_ref_counts.data_ptr(),
-                                              live.data_ptr(), ws.data_ptr(), ws.numel(), _err_word(dev).data_ptr(),
-                                              _stream(dev))
-    _lib.check(rc, "nvfp4kv_compact_pages")
+    ws = _stream_buffer(index, "compact_ws", need.value, torch.int32)
+    S, width = block_tables.shape
+    _call("nvfp4kv_compact_pages", index, ptrs, sizes, n, block_tables.data_ptr(), block_tables.stride(0), width, S,
+          ref_counts.data_ptr(), pages, out_tables.data_ptr(), out_tables.stride(0), out_ref_counts.data_ptr(),
+          live.data_ptr(), ws.data_ptr(), ws.shape[0])
     return live
