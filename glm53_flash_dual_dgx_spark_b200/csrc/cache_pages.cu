@@ -69,7 +69,7 @@ __device__ __forceinline__ void copy_bytes(uint8_t* dst, const uint8_t* src, int
 }
 
 // Pairs (src[k], dst[k]): blockIdx.y = cache, blocks of x stride over the pairs, whose number is
-// on the host (num) or on the device (num_dev).
+// on the host (num) or on the device (num_dev).  For pages that bulk copies cannot move.
 __global__ void __launch_bounds__(256)
 copy_pages_kernel(const __grid_constant__ Caches c, int64_t num_pages, const int32_t* __restrict__ src,
                   const int32_t* __restrict__ dst, int64_t num, const int32_t* __restrict__ num_dev,
@@ -87,6 +87,81 @@ copy_pages_kernel(const __grid_constant__ Caches c, int64_t num_pages, const int
         }
         copy_bytes(base + d * pb, base + s * pb, pb, threadIdx.x, blockDim.x);
     }
+}
+
+// The same with bulk copies through shared memory: a block is one warp that keeps kCopyStages pieces
+// in flight, loads ahead of stores, and no data passes registers (256 threads with four 16-byte
+// loads each moved 3.6 TB/s).  Piece q of a pair: kCopyBytes of one cache's page (the last one of a
+// page shorter); the blocks take the pieces of all pairs in turn.
+constexpr int kCopyStages = 8, kCopyBytes = 8192;
+struct CopyPieces {
+    int first[NVFP4KV_MAX_CACHES + 1];      // a pair's first piece in each cache
+};
+__global__ void __launch_bounds__(32)
+bulk_copy_pages_kernel(const __grid_constant__ Caches c, const __grid_constant__ CopyPieces pieces, int64_t num_pages,
+                       const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int64_t num,
+                       const int32_t* __restrict__ num_dev, int32_t* __restrict__ err) {
+    extern __shared__ __align__(128) uint8_t stage[];
+    __shared__ __align__(8) uint64_t bars[kCopyStages];
+    __shared__ int abort_flag;
+    if (threadIdx.x != 0) return;
+    for (int k = 0; k < kCopyStages; ++k) mbar_init(smem_u32(&bars[k]), 1);
+    abort_flag = 0;
+    mbar_fence_init();
+    griddep_wait();
+    const int per = pieces.first[c.num];
+    const int64_t total = (num_dev ? static_cast<int64_t>(*num_dev) : num) * per;
+    // piece i: where it comes from and goes to, 0 bytes for a pair that is skipped
+    auto locate = [&](int64_t i, const uint8_t** from, uint8_t** to) -> uint32_t {
+        const int64_t k = i / per;
+        const int q = static_cast<int>(i - k * per);
+        const int s = __ldg(src + k), d = __ldg(dst + k);
+        if (s < 0 || d < 0) return 0;
+        if (s >= num_pages || d >= num_pages) {
+            set_error(err, NVFP4KV_DEVERR_BAD_PAGE);
+            return 0;
+        }
+        int cache = 0;
+        while (q >= pieces.first[cache + 1]) ++cache;
+        const int64_t pb = c.page_bytes[cache], at = static_cast<int64_t>(q - pieces.first[cache]) * kCopyBytes;
+        *from = c.base[cache] + s * pb + at;
+        *to = c.base[cache] + d * pb + at;
+        return static_cast<uint32_t>(pb - at < kCopyBytes ? pb - at : kCopyBytes);
+    };
+    // Piece i of this block (blockIdx.x + i gridDim.x) uses stage i % kCopyStages.  Loads run kAhead
+    // pieces ahead; the stage a load takes was last stored from kCopyStages - kAhead pieces ago.
+    constexpr int kAhead = kCopyStages / 2;
+    const int64_t mine = total > blockIdx.x ? (total - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+    uint8_t* to[kCopyStages];
+    uint32_t bytes[kCopyStages];
+    auto load = [&](int64_t i, int st) {
+        bytes[st] = 0;
+        if (i >= mine) return;
+        const uint8_t* from = nullptr;
+        bytes[st] = locate(blockIdx.x + i * gridDim.x, &from, &to[st]);
+        mbar_arrive_expect_tx(smem_u32(&bars[st]), bytes[st]);      // (a skipped pair's phase completes at once)
+        if (bytes[st]) bulk_copy_g2s(smem_u32(stage) + st * kCopyBytes, from, bytes[st], smem_u32(&bars[st]));
+    };
+#pragma unroll
+    for (int st = 0; st < kAhead; ++st) load(st, st);
+    uint32_t phase = 0;
+    for (int64_t i0 = 0; i0 < mine; i0 += kCopyStages, phase ^= 1) {
+#pragma unroll
+        for (int st = 0; st < kCopyStages; ++st) {
+            if (i0 + st >= mine) break;
+            if (!mbar_wait(smem_u32(&bars[st]), phase, &abort_flag, err)) break;
+            if (bytes[st]) bulk_copy_s2g(to[st], smem_u32(stage) + st * kCopyBytes, bytes[st]);
+            bulk_commit_group();
+            asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kCopyStages - kAhead) : "memory");
+            load(i0 + st + kAhead, (st + kAhead) % kCopyStages);
+        }
+        if (abort_flag) break;
+    }
+    bulk_wait_group_read0();
+    // (after a timed-out wait: the loads in flight land before the block's shared memory goes)
+    if (abort_flag)
+        for (int st = 0; st < kCopyStages; ++st)
+            if (bytes[st]) mbar_drain_wait(smem_u32(&bars[st]), phase);
 }
 
 // ------------------------------------------------------------------ freeing
@@ -277,68 +352,122 @@ struct CompactArgs {
     int64_t num_pages;
     int32_t* num_live;
     int32_t* moves;      // number of pages that move
+    int32_t* counts;     // [blocks]: live pages of each block's pages
     int32_t* src;        // [num_pages]
     int32_t* dst;
     int32_t* src_refs;
-    int32_t* remap;      // page -> its new id, -1 for a free one
+    int32_t* remap;      // page -> its new id, -1 for a free one, -2 - k for the k-th that moves
+    const int32_t* tables;
+    int64_t stride, num_slots, out_stride;
+    int width;
+    int32_t* out_tables;
+    int32_t* err;
 };
+constexpr int kPer = 4, kBlockPages = kPlanThreads * kPer;      // pages of a thread, of a block
 
-// One block, two passes over the counts: how many pages are live (n), then the k-th live page
-// past n with the k-th hole before it.
+// kPer consecutive counts of a thread (0 past the end).
+__device__ __forceinline__ void load_counts(const int32_t* refs, int64_t i0, int64_t num, int (&r)[kPer]) {
+    if (i0 + kPer <= num && reinterpret_cast<uintptr_t>(refs) % 16 == 0) {
+        const int4 v = *reinterpret_cast<const int4*>(refs + i0);
+        r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) r[j] = i0 + j < num ? refs[i0 + j] : 0;
+    }
+}
+
+__global__ void __launch_bounds__(kPlanThreads) compact_count_kernel(const __grid_constant__ CompactArgs p) {
+    __shared__ int sums[32];
+    int r[kPer], live = 0, total;
+    load_counts(p.refs, static_cast<int64_t>(blockIdx.x) * kBlockPages + threadIdx.x * kPer, p.num_pages, r);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) live += r[j] > 0;
+    block_exclusive_scan(live, sums, &total);
+    if (threadIdx.x == 0) p.counts[blockIdx.x] = total;
+    griddep_launch_dependents();
+}
+
+// With n = live pages in all: the k-th live page past n goes to the k-th hole before it.  A page's
+// number among the live ones is the live pages of the blocks before its own plus a scan; that of a
+// hole before n is its index less that; that of a live page past n is that less the live pages
+// before n, which every block counts for itself.  (In place, only counts of free pages and of
+// pages past n change, which no other block's counting depends on.)
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid_constant__ CompactArgs p) {
-    __shared__ int sums[2][32];
-    const int tid = threadIdx.x;
-    int live = 0;
-    for (int64_t i = tid; i < p.num_pages; i += kPlanThreads) live += p.refs[i] > 0;
-    int n;
-    block_exclusive_scan(live, sums[0], &n);
+    __shared__ int sums[3][32];
+    const int tid = threadIdx.x, blocks = gridDim.x;
+    griddep_wait();
+    int mine[2] = {0, 0}, n, before;
+    for (int b = tid; b < blocks; b += kPlanThreads) {
+        const int c = p.counts[b];
+        mine[0] += c;
+        if (b < static_cast<int>(blockIdx.x)) mine[1] += c;
+    }
+    block_exclusive_scan(mine[0], sums[0], &n);
+    block_exclusive_scan(mine[1], sums[1], &before);
+    // live pages before page n: whole blocks, and the part of n's own
+    const int nb = n / kBlockPages;
+    int part = 0, live_low;
+    for (int b = tid; b < nb; b += kPlanThreads) part += p.counts[b];
+    int r[kPer];
+    const int64_t at = static_cast<int64_t>(nb) * kBlockPages + tid * kPer;
+    load_counts(p.refs, at, n, r);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) part += r[j] > 0;
+    block_exclusive_scan(part, sums[2], &live_low);
+    const int64_t i0 = static_cast<int64_t>(blockIdx.x) * kBlockPages + tid * kPer;
+    load_counts(p.refs, i0, p.num_pages, r);
+    int live = 0, total;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) live += r[j] > 0;
     __syncthreads();
-    int holes = 0, movers = 0;
-    for (int64_t i0 = 0; i0 < p.num_pages; i0 += kPlanThreads) {
-        const int64_t i = i0 + tid;
-        const int r = i < p.num_pages ? p.refs[i] : 0;
-        const bool in = i < p.num_pages;
-        const bool hole = in && i < n && r <= 0, mover = in && i >= n && r > 0;
-        int th, tm;
-        const int h = holes + block_exclusive_scan(hole, sums[0], &th);
-        const int m = movers + block_exclusive_scan(mover, sums[1], &tm);
-        if (hole) p.dst[h] = static_cast<int>(i);
-        if (mover) {
-            p.src[m] = static_cast<int>(i);
-            p.src_refs[m] = r;
+    int rank = before + block_exclusive_scan(live, sums[0], &total);      // live pages before the thread's first
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int64_t i = i0 + j;
+        if (i >= p.num_pages) break;
+        if (r[j] > 0) {
+            if (i >= n) {
+                const int k = rank - live_low;
+                p.src[k] = static_cast<int>(i);
+                p.src_refs[k] = r[j];
+                p.remap[i] = -2 - k;
+                p.out_refs[i] = 0;
+            } else {
+                p.remap[i] = static_cast<int>(i);
+                p.out_refs[i] = r[j];
+            }
+            ++rank;
+        } else {
+            if (i < n) p.dst[i - rank] = static_cast<int>(i);      // (its count comes with the page that moves in)
+            else p.out_refs[i] = 0;
+            p.remap[i] = -1;
         }
-        if (in) p.remap[i] = r > 0 ? static_cast<int>(i) : -1;
-        if (in && !hole) p.out_refs[i] = mover ? 0 : r > 0 ? r : 0;
-        holes += th;
-        movers += tm;
-        __syncthreads();
     }
-    for (int k = tid; k < movers; k += kPlanThreads) {
-        p.remap[p.src[k]] = p.dst[k];
-        p.out_refs[p.dst[k]] = p.src_refs[k];
-    }
-    if (tid == 0) {
+    if (blockIdx.x == 0 && tid == 0) {
         *p.num_live = n;
-        *p.moves = movers;
+        *p.moves = n - live_low;
     }
     griddep_launch_dependents();
 }
 
-__global__ void __launch_bounds__(256)
-remap_tables_kernel(const int32_t* tables, int64_t stride, int width, int64_t num_slots, int32_t* out,
-                    int64_t out_stride, const int32_t* __restrict__ remap, int64_t num_pages, int32_t* err) {
+// The tables by the new ids, and the counts of the pages that moved.
+__global__ void __launch_bounds__(256) compact_tables_kernel(const __grid_constant__ CompactArgs p) {
     griddep_wait();
-    const int64_t n = num_slots * width;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t s = i / width, j = i - s * width;
-        const int p = tables[s * stride + j];
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+    const int64_t n = p.num_slots * p.width;
+    for (int64_t i = first; i < n; i += step) {
+        const int64_t s = i / p.width, j = i - s * p.width;
+        const int pg = p.tables[s * p.stride + j];
         int q = -1;
-        if (p >= 0) {
-            if (p < num_pages) q = remap[p];
-            if (q < 0) set_error(err, NVFP4KV_DEVERR_BAD_PAGE);
+        if (pg >= 0) {
+            if (pg < p.num_pages) q = p.remap[pg];
+            if (q <= -2) q = p.dst[-2 - q];
+            if (q < 0) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
         }
-        out[s * out_stride + j] = q;
+        p.out_tables[s * p.out_stride + j] = q;
     }
+    const int moves = *p.moves;
+    for (int64_t k = first; k < moves; k += step) p.out_refs[p.dst[k]] = p.src_refs[k];
 }
 
 int gather_caches(const char* what, const void* const* caches, const int64_t* page_bytes, int num, int page_size, Caches* c) {
@@ -367,11 +496,32 @@ int check_tables(const char* what, const void* tables, int64_t stride, int width
     return NVFP4KV_OK;
 }
 
+// Moves (with a pad), counts of the blocks, and four lists of pages.
+int64_t compact_ints(int64_t num_pages) { return 4 + (num_pages + kBlockPages - 1) / kBlockPages + 4 * num_pages; }
+
 int launch_copy(const Caches& c, int64_t num_pages, const int32_t* src, const int32_t* dst, int64_t num,
-                const int32_t* num_dev, int64_t blocks, int32_t* err, cudaStream_t st) {
+                const int32_t* num_dev, int64_t most_pairs, int32_t* err, cudaStream_t st) {
     if (c.num == 0) return NVFP4KV_OK;
-    const cudaError_t e = launch_dependent(copy_pages_kernel, dim3(static_cast<unsigned>(blocks), c.num), dim3(256), 0,
-                                           st, c, num_pages, src, dst, num, num_dev, err);
+    uint64_t align = 0;
+    CopyPieces pieces{};
+    for (int k = 0; k < c.num; ++k) {
+        align |= reinterpret_cast<uint64_t>(c.base[k]) | static_cast<uint64_t>(c.page_bytes[k]);
+        pieces.first[k + 1] = pieces.first[k] + static_cast<int>((c.page_bytes[k] + kCopyBytes - 1) / kCopyBytes);
+    }
+    cudaError_t e;
+    if (align % 16 == 0) {      // what a bulk copy can move
+        static_assert(kCopyStages * kCopyBytes * 3 <= 227 * 1024, "three blocks on an SM");
+        e = cudaFuncSetAttribute(bulk_copy_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCopyStages * kCopyBytes);
+        int64_t blocks = 3 * device_sm_count();
+        blocks = blocks < most_pairs * pieces.first[c.num] ? blocks : most_pairs * pieces.first[c.num];
+        if (e == cudaSuccess)
+            e = launch_dependent(bulk_copy_pages_kernel, dim3(static_cast<unsigned>(blocks)), dim3(32), kCopyStages * kCopyBytes, st, c,
+                                 pieces, num_pages, src, dst, num, num_dev, err);
+    } else {
+        const int64_t blocks = most_pairs < 8 * device_sm_count() ? most_pairs : 8 * device_sm_count();
+        e = launch_dependent(copy_pages_kernel, dim3(static_cast<unsigned>(blocks), c.num), dim3(256), 0, st, c, num_pages, src, dst,
+                             num, num_dev, err);
+    }
     if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "page copy launch failed: %s", cudaGetErrorString(e));
     return check_launch("page copy");
 }
@@ -390,8 +540,7 @@ extern "C" int nvfp4kv_copy_pages(const void* const* caches, const int64_t* page
     if (num_pairs == 0) return NVFP4KV_OK;
     if (!src || !dst) return fail(NVFP4KV_EINVAL, "nvfp4kv_copy_pages: null pointer");
     if (num_pages < 1 || num_pages >= 0x7FFFFFFFll) return fail(NVFP4KV_EINVAL, "nvfp4kv_copy_pages: bad num_pages");
-    return launch_copy(c, num_pages, src, dst, num_pairs, nullptr, num_pairs < 65536 ? num_pairs : 65536, err_flag,
-                       reinterpret_cast<cudaStream_t>(stream));
+    return launch_copy(c, num_pages, src, dst, num_pairs, nullptr, num_pairs, err_flag, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int nvfp4kv_free_pages(int32_t* block_tables, int64_t tables_stride, int table_width, int64_t num_slots,
@@ -442,7 +591,7 @@ extern "C" int nvfp4kv_compact_workspace_ints(int64_t num_pages, int64_t* ints) 
     using namespace nvfp4kv;
     if (!ints) return fail(NVFP4KV_EINVAL, "nvfp4kv_compact_workspace_ints: null output");
     if (num_pages < 1) return fail(NVFP4KV_EINVAL, "nvfp4kv_compact_workspace_ints: bad num_pages");
-    *ints = 4 * num_pages + 4;
+    *ints = compact_ints(num_pages);
     return NVFP4KV_OK;
 }
 
@@ -460,23 +609,25 @@ extern "C" int nvfp4kv_compact_pages(const void* const* caches, const int64_t* p
     if (rc != NVFP4KV_OK) return rc;
     if (!out_tables || !out_ref_counts || !num_live || out_tables_stride < table_width)
         return fail(NVFP4KV_EINVAL, "nvfp4kv_compact_pages: null or too narrow output");
-    if (!workspace || workspace_ints < 4 * num_pages + 4)
+    if (!workspace || workspace_ints < compact_ints(num_pages))
         return fail(NVFP4KV_EWORKSPACE, "nvfp4kv_compact_pages: workspace %lld ints < %lld required",
-                    (long long)workspace_ints, (long long)(4 * num_pages + 4));
+                    (long long)workspace_ints, (long long)compact_ints(num_pages));
     CompactArgs a{};
     a.refs = ref_counts; a.out_refs = out_ref_counts; a.num_pages = num_pages; a.num_live = num_live;
-    a.moves = workspace; a.src = workspace + 4; a.dst = a.src + num_pages; a.src_refs = a.dst + num_pages;
-    a.remap = a.src_refs + num_pages;
+    const int blocks = static_cast<int>((num_pages + kBlockPages - 1) / kBlockPages);
+    a.moves = workspace; a.counts = workspace + 4; a.src = a.counts + blocks; a.dst = a.src + num_pages;
+    a.src_refs = a.dst + num_pages; a.remap = a.src_refs + num_pages;
+    a.tables = block_tables; a.stride = tables_stride; a.width = table_width; a.num_slots = num_slots;
+    a.out_tables = out_tables; a.out_stride = out_tables_stride; a.err = err_flag;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
-    rc = check_launch("nvfp4kv_compact_pages plan");
+    compact_count_kernel<<<blocks, kPlanThreads, 0, st>>>(a);
+    rc = check_launch("nvfp4kv_compact_pages count");
     if (rc != NVFP4KV_OK) return rc;
-    const int64_t entries = num_slots * table_width;
-    const int64_t want = (entries + 255) / 256;
-    const cudaError_t e = launch_dependent(remap_tables_kernel, dim3(static_cast<unsigned>(want < 1184 ? want : 1184)),
-                                           dim3(256), 0, st, block_tables, tables_stride, table_width, num_slots,
-                                           out_tables, out_tables_stride, a.remap, num_pages, err_flag);
+    const int64_t want = (num_slots * table_width + 255) / 256, most = 8 * device_sm_count();
+    cudaError_t e = launch_dependent(compact_plan_kernel, dim3(blocks), dim3(kPlanThreads), 0, st, a);
+    if (e == cudaSuccess)
+        e = launch_dependent(compact_tables_kernel, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(256), 0, st, a);
     if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_compact_pages launch failed: %s", cudaGetErrorString(e));
-    if ((rc = check_launch("nvfp4kv_compact_pages tables")) != NVFP4KV_OK) return rc;
-    return launch_copy(c, num_pages, a.src, a.dst, 0, a.moves, device_sm_count() * 8, err_flag, st);
+    if ((rc = check_launch("nvfp4kv_compact_pages")) != NVFP4KV_OK) return rc;
+    return launch_copy(c, num_pages, a.src, a.dst, 0, a.moves, num_pages, err_flag, st);
 }

@@ -97,62 +97,96 @@ __device__ __forceinline__ void rotate_halves(Vec<T>& xa, Vec<T>& xb, const floa
     }
 }
 
+// Quotients by a number the host knows, for the small dividends of one block (up to a few thousand
+// plus the divisor): a multiplication by ceil(2^32 / d).
+constexpr int kMostDivisor = 32768;
+struct SmallDiv {
+    uint32_t d, magic;
+};
+__device__ __forceinline__ uint32_t quotient(uint32_t n, const SmallDiv& v) { return v.d == 1 ? n : __umulhi(n, v.magic); }
+
 struct RopeArgs {
     const void* x;
     void* out;
     int64_t x_st, x_sh, o_st, o_sh;
     const void* positions;
     const float* cos_sin;
-    int64_t max_positions;
+    int64_t max_positions, tokens, total;      // total: units of the call
     int heads, dim, rotary, offset;
-    int heads_per_block, head_blocks;
+    int before, rotated;    // units of a head: copies before the rotated part, rotated ones, copies after it
+    SmallDiv units, by_heads;
     int pos_i64, inverse, in_place;
     int32_t* err;
 };
+constexpr int kRopeSteps = 2;
 
-// One block: heads_per_block heads of one token, a 16-byte vector per thread and step.  In half
-// layout the thread of a lower-half vector does its partner too.
+// A unit is a 16-byte vector of a head (a rotated one of the half layout: the pair of vectors that
+// turn together).  The units of the call are dealt flat, two to a thread and 256 apart: every warp
+// moves 512 contiguous bytes, every block is full, and two loads in flight per thread are enough at
+// the occupancy that leaves (8,192 tokens x 64 heads x 576 bf16, 1.2 GB: 176 us against 203 with one
+// and 178 with four; 225 with blocks of whole heads, whose last steps are part empty).
 template <typename T, bool kInterleaved>
-__global__ void __launch_bounds__(256) rope_vec_kernel(const RopeArgs p) {
+__global__ void __launch_bounds__(256) rope_vec_kernel(const __grid_constant__ RopeArgs p) {
     constexpr int N = Vec<T>::kN;
-    const int64_t t = blockIdx.x / p.head_blocks;
-    const int h0 = static_cast<int>(blockIdx.x % p.head_blocks) * p.heads_per_block;
-    const int heads = min(p.heads_per_block, p.heads - h0);
-    const int64_t pos = load_index(p.positions, p.pos_i64, t);
-    const bool turn = pos >= 0 && pos < p.max_positions;
-    if (!turn && threadIdx.x == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
-    const float* cs = p.cos_sin + (turn ? pos : 0) * p.rotary;
+    const int64_t u0 = static_cast<int64_t>(blockIdx.x) * (256 * kRopeSteps);
+    int64_t row0, t0;       // the block's first head row, its token
+    if (p.total < (1ll << 32)) {
+        row0 = static_cast<uint32_t>(u0) / p.units.d;
+        t0 = static_cast<uint32_t>(row0) / p.by_heads.d;
+    } else {
+        row0 = u0 / p.units.d;
+        t0 = row0 / p.by_heads.d;
+    }
+    const uint32_t j0 = static_cast<uint32_t>(u0 - row0 * p.units.d), h0 = static_cast<uint32_t>(row0 - t0 * p.by_heads.d);
     const int half = p.rotary / 2;
-    const float sign = p.inverse ? -1.0f : 1.0f;
-    // in place only the rotated dims are visited
-    const int d0 = p.in_place ? p.offset : 0;
-    const int per = (p.in_place ? p.rotary : p.dim) / N;
-    const T* x = static_cast<const T*>(p.x) + t * p.x_st + h0 * p.x_sh + d0;
-    T* o = static_cast<T*>(p.out) + t * p.o_st + h0 * p.o_sh + d0;
-    for (int u = threadIdx.x; u < heads * per; u += blockDim.x) {
-        const int h = u / per, d = (u - h * per) * N;
-        const T* xp = x + h * p.x_sh + d;
-        T* op = o + h * p.o_sh + d;
-        const int r = d0 + d - p.offset;          // dim within the rotated part
-        if (r < 0 || r >= p.rotary || !turn) {
-            store_vec(op, load_vec(xp));
-        } else if (kInterleaved) {
-            store_vec(op, rotate_pairs(load_vec(xp), cs + r / 2, half, sign));
-        } else if (r < half) {
-            Vec<T> a = load_vec(xp), b = load_vec(xp + half);
-            rotate_halves(a, b, cs + r, half, sign);
-            store_vec(op, a);
-            store_vec(op + half, b);
+    Vec<T> a[kRopeSteps], b[kRopeSteps];
+    int64_t t[kRopeSteps], at[kRopeSteps];
+    int r[kRopeSteps];      // dim within the rotated part, -1 for a copy, -2 past the end
+#pragma unroll
+    for (int k = 0; k < kRopeSteps; ++k) {
+        const uint32_t l = j0 + threadIdx.x + 256 * k, lr = quotient(l, p.units);
+        const int j = static_cast<int>(l - lr * p.units.d);
+        const uint32_t lh = h0 + lr, lt = quotient(lh, p.by_heads), h = lh - lt * p.by_heads.d;
+        t[k] = t0 + lt;
+        const int q = j - p.before;
+        r[k] = q < 0 || q >= p.rotated ? -1 : q * N;
+        const int d = q < 0 ? j * N : q < p.rotated ? p.offset + q * N : p.offset + p.rotary + (q - p.rotated) * N;
+        at[k] = t[k] * p.o_st + h * p.o_sh + d;
+        if (u0 + threadIdx.x + 256 * k < p.total) {
+            const T* xp = static_cast<const T*>(p.x) + t[k] * p.x_st + h * p.x_sh + d;
+            a[k] = load_vec(xp);
+            if (!kInterleaved && r[k] >= 0) b[k] = load_vec(xp + half);
+        } else {
+            r[k] = -2;
         }
+    }
+#pragma unroll
+    for (int k = 0; k < kRopeSteps; ++k) {
+        if (r[k] == -2) break;
+        T* op = static_cast<T*>(p.out) + at[k];
+        if (r[k] >= 0) {
+            const int64_t pos = load_index(p.positions, p.pos_i64, t[k]);
+            const bool turn = pos >= 0 && pos < p.max_positions;
+            if (!turn) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
+            const float* cs = p.cos_sin + (turn ? pos : 0) * p.rotary + (kInterleaved ? r[k] / 2 : r[k]);
+            const float sign = p.inverse ? -1.0f : 1.0f;
+            if (kInterleaved) {
+                if (turn) a[k] = rotate_pairs(a[k], cs, half, sign);
+            } else {
+                if (turn) rotate_halves(a[k], b[k], cs, half, sign);
+                store_vec(op + half, b[k]);
+            }
+        }
+        store_vec(op, a[k]);
     }
 }
 
 // Any strides, alignment and sizes: one element (a rotated dim: its pair) per thread and step.
 template <typename T, bool kInterleaved>
-__global__ void __launch_bounds__(256) rope_elem_kernel(const RopeArgs p) {
-    const int64_t t = blockIdx.x / p.head_blocks;
-    const int h0 = static_cast<int>(blockIdx.x % p.head_blocks) * p.heads_per_block;
-    const int heads = min(p.heads_per_block, p.heads - h0);
+__global__ void __launch_bounds__(256) rope_elem_kernel(const __grid_constant__ RopeArgs p, int head_blocks, int heads_per_block) {
+    const int64_t t = blockIdx.x / head_blocks;
+    const int h0 = static_cast<int>(blockIdx.x % head_blocks) * heads_per_block;
+    const int heads = min(heads_per_block, p.heads - h0);
     const int64_t pos = load_index(p.positions, p.pos_i64, t);
     const bool turn = pos >= 0 && pos < p.max_positions;
     if (!turn && threadIdx.x == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
@@ -187,25 +221,34 @@ int launch_rope(RopeArgs a, int64_t tokens, bool interleaved, cudaStream_t st) {
     // 16-byte vectors need every row, and each rotated vector's partner, on a 16-byte boundary
     const bool vec = bases % 16 == 0 && reinterpret_cast<uintptr_t>(a.cos_sin) % 16 == 0 && a.x_st % N == 0 &&
                      a.x_sh % N == 0 && a.o_st % N == 0 && a.o_sh % N == 0 && a.dim % N == 0 && a.offset % N == 0 &&
-                     a.rotary % (interleaved ? N : 2 * N) == 0;
-    const int per_head = vec ? (a.in_place ? a.rotary : a.dim) / N : a.dim;
-    // about four steps a thread: enough loads in flight, and blocks for every SM from a few tokens on
-    int hb = 1024 / per_head;
-    hb = hb < 1 ? 1 : (hb > a.heads ? a.heads : hb);
-    a.head_blocks = (a.heads + hb - 1) / hb;
-    a.heads_per_block = (a.heads + a.head_blocks - 1) / a.head_blocks;
-    const int64_t blocks = tokens * a.head_blocks;
-    if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: too many rows for one call");
-    const dim3 grid(static_cast<unsigned>(blocks));
+                     a.rotary % (interleaved ? N : 2 * N) == 0 &&
+                     a.heads <= kMostDivisor && a.dim <= kMostDivisor;
+    int64_t blocks;
     if (vec) {
-        if (interleaved) rope_vec_kernel<T, true><<<grid, 256, 0, st>>>(a);
-        else rope_vec_kernel<T, false><<<grid, 256, 0, st>>>(a);
+        // in place only the rotated dims are visited
+        a.rotated = a.rotary / (interleaved ? N : 2 * N);
+        a.before = a.in_place ? 0 : a.offset / N;
+        const uint32_t units = a.rotated + (a.in_place ? 0 : (a.dim - a.rotary) / N), heads = a.heads;
+        a.units = {units, static_cast<uint32_t>(((1ull << 32) + units - 1) / units)};
+        a.by_heads = {heads, static_cast<uint32_t>(((1ull << 32) + heads - 1) / heads)};
+        a.total = tokens * heads * units;
+        blocks = (a.total + 256 * kRopeSteps - 1) / (256 * kRopeSteps);
+        if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: too many rows for one call");
+        if (interleaved) rope_vec_kernel<T, true><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+        else rope_vec_kernel<T, false><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
     } else {
-        if (interleaved) rope_elem_kernel<T, true><<<grid, 256, 0, st>>>(a);
-        else rope_elem_kernel<T, false><<<grid, 256, 0, st>>>(a);
+        int hb = 1024 / a.dim;
+        hb = hb < 1 ? 1 : (hb > a.heads ? a.heads : hb);
+        const int head_blocks = (a.heads + hb - 1) / hb, per_block = (a.heads + head_blocks - 1) / head_blocks;
+        blocks = tokens * head_blocks;
+        if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: too many rows for one call");
+        if (interleaved) rope_elem_kernel<T, true><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, head_blocks, per_block);
+        else rope_elem_kernel<T, false><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, head_blocks, per_block);
     }
     return check_launch("nvfp4kv_rope");
 }
+
+constexpr int kAppendSteps = 2;
 
 struct RopeAppendArgs {
     const __nv_bfloat16* k;
@@ -220,70 +263,81 @@ struct RopeAppendArgs {
     __nv_bfloat16* qo;
     int64_t q_st, q_sh, qo_st, qo_sh;
     int heads;                 // 0 without queries
+    SmallDiv rows_of_token;    // heads + 1
     int slot_i64, pos_i64;
     int32_t* err;
 };
 
-// 64 dims of a row from `x` to `o`, the part of them that belongs to unit `u` of 8 (interleaved:
-// dims 8u..) or 4 (half layout: dims 8u.. and 32 + 8u..).
-template <bool kInterleaved, bool kVec>
-__device__ __forceinline__ void rotate_unit(const __nv_bfloat16* x, __nv_bfloat16* o, const float* cs, bool turn, int u) {
-    using V = Vec<__nv_bfloat16>;
-    auto get = [](const __nv_bfloat16* p) {
-        if constexpr (kVec) {
-            return load_vec(p);
-        } else {
-            V r;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) r.v[k] = p[k];
-            return r;
-        }
-    };
-    auto put = [](__nv_bfloat16* p, const V& r) {
-        if constexpr (kVec) {
-            store_vec(p, r);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) p[k] = r.v[k];
-        }
-    };
-    if constexpr (kInterleaved) {
-        V a = get(x + 8 * u);
-        if (turn) a = rotate_pairs(a, cs + 4 * u, 32, 1.0f);
-        put(o + 8 * u, a);
+// 8 bf16, as one 16-byte access or element by element.
+template <bool kVec> __device__ __forceinline__ Vec<__nv_bfloat16> get8(const __nv_bfloat16* p) {
+    if constexpr (kVec) {
+        return load_vec(p);
     } else {
-        V a = get(x + 8 * u), b = get(x + 32 + 8 * u);
-        if (turn) rotate_halves(a, b, cs + 8 * u, 32, 1.0f);
-        put(o + 8 * u, a);
-        put(o + 32 + 8 * u, b);
+        Vec<__nv_bfloat16> r;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) r.v[k] = p[k];
+        return r;
+    }
+}
+template <bool kVec> __device__ __forceinline__ void put8(__nv_bfloat16* p, const Vec<__nv_bfloat16>& r) {
+    if constexpr (kVec) {
+        store_vec(p, r);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) p[k] = r.v[k];
     }
 }
 
-// Thread = unit of one row: the token's key (row 0) or a head of its query (rows 1..heads).
+// The units (8 dims of a row, half layout: 8 and their partners) of all rows, dealt flat as in
+// rope_vec_kernel; a token's rows are its key and the heads of its query.
 template <bool kInterleaved, bool kVec>
-__global__ void __launch_bounds__(256) rope_append_rotated_kernel(const RopeAppendArgs p) {
-    constexpr int kU = kInterleaved ? 8 : 4;
-    const int64_t g = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const int u = static_cast<int>(g % kU);
-    const int64_t row = g / kU;
-    const int64_t t = row / (p.heads + 1);
-    const int h = static_cast<int>(row - t * (p.heads + 1)) - 1;
-    if (t >= p.tokens) return;
-    const int64_t pos = load_index(p.positions, p.pos_i64, t);
-    const bool turn = pos >= 0 && pos < p.max_positions;
-    const float* cs = p.cos_sin + (turn ? pos : 0) * NVFP4KV_ROPE;
-    if (h >= 0) {
-        rotate_unit<kInterleaved, kVec>(p.q + t * p.q_st + h * p.q_sh, p.qo + t * p.qo_st + h * p.qo_sh, cs, turn, u);
-        return;
+__global__ void __launch_bounds__(256) rope_append_rotated_kernel(const __grid_constant__ RopeAppendArgs p) {
+    using V = Vec<__nv_bfloat16>;
+    constexpr int kU = kInterleaved ? 8 : 4, kSteps = kAppendSteps, kRows = 256 / kU;      // rows of a block and step
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kRows * kSteps);
+    const int64_t t0 = row0 < (1ll << 32) ? static_cast<int64_t>(static_cast<uint32_t>(row0) / p.rows_of_token.d) : row0 / p.rows_of_token.d;
+    const uint32_t first = static_cast<uint32_t>(row0 - t0 * p.rows_of_token.d);
+    const int u = threadIdx.x % kU;
+    V a[kSteps], b[kSteps];
+    int64_t t[kSteps];
+    int h[kSteps];          // head, -1 for the key
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+        const uint32_t l = first + threadIdx.x / kU + kRows * k, lt = quotient(l, p.rows_of_token);
+        t[k] = t0 + lt;
+        h[k] = static_cast<int>(l - lt * p.rows_of_token.d) - 1;
+        if (t[k] >= p.tokens) continue;
+        const __nv_bfloat16* src = h[k] < 0 ? p.k + t[k] * p.k_st : p.q + t[k] * p.q_st + h[k] * p.q_sh;
+        a[k] = get8<kVec>(src + 8 * u);
+        if (!kInterleaved) b[k] = get8<kVec>(src + 32 + 8 * u);
     }
-    if (!turn && u == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
-    const int64_t slot = load_index(p.slots, p.slot_i64, t);
-    if (slot < 0) return;
-    if (slot >= p.rows) {
-        if (u == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_SLOT);
-        return;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+        if (t[k] >= p.tokens) break;
+        const int64_t pos = load_index(p.positions, p.pos_i64, t[k]);
+        const bool turn = pos >= 0 && pos < p.max_positions;
+        const float* cs = p.cos_sin + (turn ? pos : 0) * NVFP4KV_ROPE;
+        __nv_bfloat16* dst;
+        if (h[k] < 0) {
+            if (!turn && u == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
+            const int64_t slot = load_index(p.slots, p.slot_i64, t[k]);
+            if (slot < 0) continue;
+            if (slot >= p.rows) {
+                if (u == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_SLOT);
+                continue;
+            }
+            dst = p.pool + slot * NVFP4KV_ROPE;
+        } else {
+            dst = p.qo + t[k] * p.qo_st + h[k] * p.qo_sh;
+        }
+        if (kInterleaved) {
+            if (turn) a[k] = rotate_pairs(a[k], cs + 4 * u, 32, 1.0f);
+        } else {
+            if (turn) rotate_halves(a[k], b[k], cs + 8 * u, 32, 1.0f);
+            put8<kVec>(dst + 32 + 8 * u, b[k]);
+        }
+        put8<kVec>(dst + 8 * u, a[k]);
     }
-    rotate_unit<kInterleaved, kVec>(p.k + t * p.k_st, p.pool + slot * NVFP4KV_ROPE, cs, turn, u);
 }
 
 }  // namespace
@@ -342,7 +396,8 @@ extern "C" int nvfp4kv_append_rope_rotated(const void* k_pe, int64_t num_tokens,
         return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: k_stride %lld < 64", (long long)k_stride);
     if (pool_rows <= 0 || max_positions < 1)
         return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: empty rope pool or cos_sin table");
-    if (q_pe && num_heads < 1) return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: num_heads must be >= 1");
+    if (q_pe && (num_heads < 1 || num_heads >= kMostDivisor))
+        return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: num_heads %d not in [1, %d)", num_heads, kMostDivisor);
     if (reinterpret_cast<uintptr_t>(rope_pool) % 16 || reinterpret_cast<uintptr_t>(cos_sin) % 16 ||
         (reinterpret_cast<uintptr_t>(k_pe) | reinterpret_cast<uintptr_t>(q_pe) | reinterpret_cast<uintptr_t>(q_out)) % 2)
         return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: rope pool and cos_sin must be 16-byte aligned");
@@ -360,8 +415,9 @@ extern "C" int nvfp4kv_append_rope_rotated(const void* k_pe, int64_t num_tokens,
     const bool vec = reinterpret_cast<uintptr_t>(k_pe) % 16 == 0 && k_stride % 8 == 0 &&
                      (!q_pe || ((reinterpret_cast<uintptr_t>(q_pe) | reinterpret_cast<uintptr_t>(q_out)) % 16 == 0 &&
                                 (q_stride_t | q_stride_h | qo_stride_t | qo_stride_h) % 8 == 0));
-    const int64_t threads = num_tokens * (a.heads + 1) * (interleaved ? 8 : 4);
-    const int64_t blocks = (threads + 255) / 256;
+    const uint32_t per_token = a.heads + 1;
+    a.rows_of_token = {per_token, static_cast<uint32_t>(((1ull << 32) + per_token - 1) / per_token)};
+    const int64_t per_block = kAppendSteps * 256 / (interleaved ? 8 : 4), blocks = (num_tokens * per_token + per_block - 1) / per_block;
     if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: too many rows for one call");
     const dim3 grid(static_cast<unsigned>(blocks));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -841,6 +841,9 @@ def _cache_list(caches):
 
 def _check_int32(**tensors):
     for name, t in tensors.items():
+        st = t.stride()
+        if t.dtype is torch.int32 and t.is_cuda and st[-1] == 1 and len(st) == (2 if name.endswith("tables") else 1):
+            continue
         _require_cuda(t, name)
         if t.dtype != torch.int32:
             raise TypeError(f"{name} must be int32")
