@@ -65,7 +65,8 @@ constexpr int kStageBytes = 16384;              // 128 rows x 128 B
 constexpr int kVStages = 8;                     // V stages of a tile: 4 x 64 tokens x 2 x 128 dims a CTA
 constexpr int kSoftmaxWarps = 8, kQWarp0 = 8, kQWarps = 4, kMmaWarp = 12, kCopyWarp0 = 13, kRelayWarp = 15;
 constexpr int kThreads = 16 * 32;
-constexpr uint32_t kRegsLaunch = 128, kRegsSoftmax = 168, kRegsQ = 96, kRegsCtl = 80;
+constexpr uint32_t kRegsLaunch = 128, kRegsSoftmax = 160, kRegsQ = 128, kRegsCtl = 64;
+constexpr int kQRows = 4;                       // rows of Q a warp converts at a time
 static_assert(256 * kRegsSoftmax + 128 * kRegsQ + 128 * kRegsCtl <= kThreads * kRegsLaunch,
               "the register split stays within what the block is launched with");
 constexpr float kRescaleLog2 = 8.0f;
@@ -118,6 +119,7 @@ struct PrefillParams {
     const int32_t* cu;
     const int32_t* seq_lens;
     int batch, total_q, heads, page_shift, max_q_len, max_seq_len;
+    uint32_t heads_magic;      // ceil(2^32 / heads)
     int pairs;
     float scale_log2, out_scale;
     __nv_bfloat16* out;
@@ -148,6 +150,27 @@ __device__ __forceinline__ void pair_mma_f16(uint32_t d, uint64_t a, uint64_t b,
 __device__ __forceinline__ void pair_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+// mbar_wait whose polls sleep until the phase completes, or for about 20 us.
+__device__ __forceinline__ bool try_wait_asleep(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
+    if (try_wait_asleep(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    while (!try_wait_asleep(bar, parity)) {
+        if (*abort_flag) return false;
+        if (globaltimer_ns() - t0 > NVFP4KV_WAIT_TIMEOUT_NS) {
+            *abort_flag = 1;
+            set_error(err, NVFP4KV_DEVERR_TIMEOUT);
+            return false;
+        }
+    }
+    return true;
 }
 // Arrive on the leading CTA's barrier.  What the arrival publishes is this CTA's own shared and
 // tensor memory, ordered before it by fence.proxy.async or tcgen05.fence and read by the tensor
@@ -233,13 +256,15 @@ struct Range {
     int b, k, offset;   // sequence, unit, weight of the unit done before
     int image0;         // image blocks of the sequences before b
 };
-// Where pair `pair` of p.pairs begins.  Run by one warp.
+// Where pair `pair` of p.pairs begins.  Run by one warp, a sequence per lane (and pass, past 32).
 __device__ __forceinline__ Range find_range(const PrefillParams& p, int pair) {
     const int lane = threadIdx.x & 31;
-    int64_t total = 0;
+    Seq s{};
+    int64_t w = 0, total = 0;
     for (int b = lane; b < p.batch; b += 32) {
-        const Seq s = load_seq(p, b);
-        total += weight_before(p, s, s.units);
+        s = load_seq(p, b);
+        w = weight_before(p, s, s.units);
+        total += w;
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
@@ -248,9 +273,11 @@ __device__ __forceinline__ Range find_range(const PrefillParams& p, int pair) {
     if (hi <= lo) return r;
     int64_t before = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        Seq s{};
-        if (b0 + lane < p.batch) s = load_seq(p, b0 + lane);
-        const int64_t w = weight_before(p, s, s.units);
+        if (p.batch > 32) {       // (else the first pass left them here)
+            s = Seq{};
+            if (b0 + lane < p.batch) s = load_seq(p, b0 + lane);
+            w = weight_before(p, s, s.units);
+        }
         const int blocks = image_blocks_of(s);
         const int64_t upto = before + warp_inclusive_sum(w, lane);
         const int img = r.image0 + warp_inclusive_sum(blocks, lane);
@@ -260,7 +287,12 @@ __device__ __forceinline__ Range find_range(const PrefillParams& p, int pair) {
             r.b = b0 + src;
             r.image0 = __shfl_sync(0xFFFFFFFFu, img - blocks, src);
             const int64_t x = lo - __shfl_sync(0xFFFFFFFFu, upto - w, src);
-            const Seq t = load_seq(p, r.b);
+            Seq t;
+            t.n = __shfl_sync(0xFFFFFFFFu, s.n, src);
+            t.L = __shfl_sync(0xFFFFFFFFu, s.L, src);
+            t.rows = __shfl_sync(0xFFFFFFFFu, s.rows, src);
+            t.units = __shfl_sync(0xFFFFFFFFu, s.units, src);
+            t.first = 0;
             int k = 0, len = t.units;
             while (len > 1) {                          // the last unit that begins at or before x, 32 candidates a step
                 const int step = (len + 31) / 32, cand = k + lane * step;
@@ -641,39 +673,58 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         while (next_part(p, work)) {
             if (t.n_tiles == 0) continue;
             // Q: 64 rows -> fp16 after a power of two per row that brings its largest |q| to [2^10, 2^11)
-            // (the rope part by the same factor, in bf16); a warp per row, 16 + 2 dims per lane, four rows
-            // in flight (the first four from before the last part's QK is done)
-            const int rows = t.rows, q_row0 = t.block * kUnitRows + kCtaRows * cta, first = t.first;
+            // (the rope part by the same factor, in bf16); a warp per row, 16 + 2 dims per lane, the next
+            // kQRows rows on their way meanwhile (the first ones from before the last part's QK is done)
+            const int rows = t.rows, q_row0 = t.block * kUnitRows + kCtaRows * cta + warp - kQWarp0, first = t.first;
             float* qs = reinterpret_cast<float*>(smem + SM_QS) + 64 * (parts & 1);
-#pragma unroll 1
-            for (int rr = warp - kQWarp0; rr < kCtaRows; rr += 4 * kQWarps) {
-                uint4 u[4][2];
-                uint32_t rw[4];
+            uint4 u[kQRows][2];
+            uint32_t rw[kQRows];
+            auto load = [&](int r0) {      // rows r0, r0 + kQWarps, ... of this warp
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < kQRows; ++j) {
                     u[j][0] = u[j][1] = make_uint4(0, 0, 0, 0);
                     rw[j] = 0;
-                    const int row = q_row0 + rr + j * kQWarps;
-                    if (row < rows) {
-                        const int tok = row / p.heads;
+                    const int row = q_row0 + r0 + j * kQWarps;
+                    if (row < rows && r0 < kCtaRows) {
+                        int tok = p.heads == 1 ? row : static_cast<int>(__umulhi(row, p.heads_magic));      // row / heads, or one more
+                        tok -= tok * p.heads > row;
                         const __nv_bfloat16* src = p.q + static_cast<int64_t>(first + tok) * p.q_st + static_cast<int64_t>(row - tok * p.heads) * p.q_sh;
                         u[j][0] = ldg_nc_v4(src + 16 * lane);
                         u[j][1] = ldg_nc_v4(src + 16 * lane + 8);
                         if (p.rope) rw[j] = __ldg(reinterpret_cast<const uint32_t*>(src + kLatent) + lane);
                     }
                 }
-                if (rr < kQWarps && parts > 0) mbar_wait(bar(B_Q_FREE), (parts - 1) & 1, abort_flag, p.err);
+            };
+            load(0);
+            if (parts > 0) wait_phase(bar(B_Q_FREE), (parts - 1) & 1, abort_flag, p.err);
+#pragma unroll 1
+            for (int r0 = 0; r0 < kCtaRows; r0 += kQRows * kQWarps) {
+                uint32_t w[kQRows][8], rope_w[kQRows];
+                float amax[kQRows];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = rr + j * kQWarps;
-                    const uint32_t w[8] = {u[j][0].x, u[j][0].y, u[j][0].z, u[j][0].w, u[j][1].x, u[j][1].y, u[j][1].z, u[j][1].w};
-                    float amax = 0.0f;
+                for (int j = 0; j < kQRows; ++j) {
+                    w[j][0] = u[j][0].x; w[j][1] = u[j][0].y; w[j][2] = u[j][0].z; w[j][3] = u[j][0].w;
+                    w[j][4] = u[j][1].x; w[j][5] = u[j][1].y; w[j][6] = u[j][1].z; w[j][7] = u[j][1].w;
+                    rope_w[j] = rw[j];
+                    // |bf16 pairs| by their largest: as integers, the order of |x|
+                    uint32_t hi = 0, lo = 0;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xFFFF0000u))));
+                    for (int i = 0; i < 8; ++i) {
+                        hi = max(hi, w[j][i] & 0x7FFF0000u);
+                        lo = max(lo, w[j][i] & 0x7FFFu);
+                    }
+                    amax[j] = __uint_as_float(max(hi, lo << 16));
+                }
+                load(r0 + kQRows * kQWarps);
 #pragma unroll
-                    for (int o = 16; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-                    const int eb = static_cast<int>((__float_as_uint(amax) >> 23) & 0xFFu);
+                for (int o = 16; o >= 1; o >>= 1)
+#pragma unroll
+                    for (int j = 0; j < kQRows; ++j)
+                        amax[j] = __uint_as_float(max(__float_as_uint(amax[j]), __shfl_xor_sync(0xFFFFFFFFu, __float_as_uint(amax[j]), o)));
+#pragma unroll
+                for (int j = 0; j < kQRows; ++j) {
+                    const int r = warp - kQWarp0 + r0 + j * kQWarps;
+                    const int eb = static_cast<int>((__float_as_uint(amax[j]) >> 23) & 0xFFu);      // 255: inf or NaN
                     const int e = eb > 0 && eb < 255 ? max(eb - 127 - 10, -100) : 0;
                     float factor = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
                     float mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
@@ -684,13 +735,14 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                     }
                     uint32_t h[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) h[i] = pack_half2(__uint_as_float(w[i] << 16) * mul, __uint_as_float(w[i] & 0xFFFF0000u) * mul);
+                    for (int i = 0; i < 8; ++i)
+                        h[i] = pack_half2(__uint_as_float(w[j][i] << 16) * mul, __uint_as_float(w[j][i] & 0xFFFF0000u) * mul);
                     // dims 16 lane + 8 c: half lane / 16, piece (lane / 2) % 8, chunk 2 (lane % 2) + c
                     uint8_t* dst = smem + SM_Q + ((lane >> 4) * 4 + 2 * (lane & 1)) * (kCtaRows * 128) + r * 128 + ((((lane >> 1) & 7) ^ (r & 7)) << 4);
                     *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
                     *reinterpret_cast<uint4*>(dst + kCtaRows * 128) = make_uint4(h[4], h[5], h[6], h[7]);
                     if (p.rope) {
-                        const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(rw[j] << 16) * mul, __uint_as_float(rw[j] & 0xFFFF0000u) * mul);
+                        const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(rope_w[j] << 16) * mul, __uint_as_float(rope_w[j] & 0xFFFF0000u) * mul);
                         *reinterpret_cast<uint32_t*>(smem + SM_Q + 8 * (kCtaRows * 128) + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)) =
                             *reinterpret_cast<const uint32_t*>(&two);
                     }
@@ -738,7 +790,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 const uint2 have = ahead[0], nan = ahead[1];
                 if (i + 1 < n_tiles) load_bits(i + 1, ahead);
                 const int see = lim - ((tile0 + i) * kTile + 64 * q4);     // tokens of the quarter the row sees
-                mbar_wait(bar(B_S_FULL + (tile & 1)), (tile >> 1) & 1, abort_flag, p.err);
+                wait_phase(bar(B_S_FULL + (tile & 1)), (tile >> 1) & 1, abort_flag, p.err);
                 tc_fence_after();
                 if (i == 0) factor = reinterpret_cast<const float*>(smem + SM_QS)[64 * (parts & 1) + row];
                 float x[64];
@@ -780,7 +832,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 if (i > 0) {
-                    mbar_wait(bar(B_PV_DONE), (tile - 1) & 1, abort_flag, p.err);
+                    wait_phase(bar(B_PV_DONE), (tile - 1) & 1, abort_flag, p.err);
                     if (__any_sync(0xFFFFFFFFu, alpha != 1.0f)) {          // the row's O: this warp's lanes, block ch
                         tc_fence_after();
 #pragma unroll 1
@@ -809,7 +861,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             lsum[64 * q4 + row] = l;
             named_bar_sync(1 + (sp & 1), 128);
             l = (lsum[row] + lsum[64 + row]) + (lsum[128 + row] + lsum[192 + row]);
-            if (n_tiles > 0) mbar_wait(bar(B_PV_DONE), (tile - 1) & 1, abort_flag, p.err);
+            if (n_tiles > 0) wait_phase(bar(B_PV_DONE), (tile - 1) & 1, abort_flag, p.err);
             tc_fence_after();
             const bool any = l > 0.0f || l != l, whole = t.head && t.tail;
             const int grow = t.block * kUnitRows + kCtaRows * cta + row;
@@ -825,21 +877,22 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             }
             if (!whole && threadIdx.x == 0 && cta == 0)
                 p.parts[2 * pair + (first_part ? 0 : 1)] = PartInfo{1, t.head, t.tail, t.first, t.n, t.block};
-            // 32 bytes a store: with 16 the stores took twice as long, a wavefront per row and store
+            // 64 columns a step in registers, 32-byte stores by the lanes that hold the rows (whole rows
+            // staged in shared memory and stored by warps took 9,000 cycles for barriers and latency)
             __nv_bfloat16* out = p.out + static_cast<int64_t>(t.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh + 256 * (sp >> 1) + 16 * ch;
             float* part_o = p.part_o + part_row * kLatent + 256 * (sp >> 1) + 16 * ch;
             const bool wide = (reinterpret_cast<uintptr_t>(p.out) % 32 == 0) && p.o_st % 16 == 0 && p.o_sh % 16 == 0;
 #pragma unroll 1
-            for (int pp = 0; pp < 8; pp += 2) {         // pieces pp, pp + 1: 16 dims of each, in columns 8 pp .. and 64 + 8 pp ..
-                uint32_t o[2][16];
+            for (int p0 = 0; p0 < 8; p0 += 4) {         // pieces p0 .. p0 + 3: 16 dims of each, in columns 8 p0 .. and 64 + 8 p0 ..
+                uint32_t o[2][32];
                 if (n_tiles > 0) {
-                    tmem_ld16(tmem + kTO + 128 * ch + 8 * pp + lanes, o[0]);
-                    tmem_ld16(tmem + kTO + 128 * ch + 64 + 8 * pp + lanes, o[1]);
+                    tmem_ld32(tmem + kTO + 128 * ch + 8 * p0 + lanes, o[0]);
+                    tmem_ld32(tmem + kTO + 128 * ch + 64 + 8 * p0 + lanes, o[1]);
                     tmem_wait_ld();
                 }
                 if (!real) continue;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < 4; ++j) {
                     uint32_t v[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) v[k] = any ? __float_as_uint(__uint_as_float(o[k >> 3][8 * j + (k & 7)]) * mul) : 0u;
@@ -850,7 +903,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                             const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
                             w[k] = *reinterpret_cast<const uint32_t*>(&two);
                         }
-                        __nv_bfloat16* dst = out + 32 * (pp + j);
+                        __nv_bfloat16* dst = out + 32 * (p0 + j);
                         if (wide) {
                             st_global_v8(dst, w);
                         } else {
@@ -858,8 +911,8 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                             *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
                         }
                     } else if (any) {
-                        st_global_v8(part_o + 32 * (pp + j), v);
-                        st_global_v8(part_o + 32 * (pp + j) + 8, v + 8);
+                        st_global_v8(part_o + 32 * (p0 + j), v);
+                        st_global_v8(part_o + 32 * (p0 + j) + 8, v + 8);
                     }
                 }
             }
@@ -1054,6 +1107,7 @@ extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_
     p.scale_log2 = bmm1_scale * 1.4426950408889634f; p.out_scale = bmm2_scale;
     p.out = static_cast<__nv_bfloat16*>(out); p.o_st = out_stride_t; p.o_sh = out_stride_h;
     p.lse = lse; p.err = err_flag; p.pairs = pl.pairs;
+    p.heads_magic = num_heads > 1 ? static_cast<uint32_t>(((1ull << 32) + num_heads - 1) / num_heads) : 0xFFFFFFFFu;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     p.image = ws;
     p.image_bits = reinterpret_cast<uint32_t*>(ws += pl.image_bytes);
