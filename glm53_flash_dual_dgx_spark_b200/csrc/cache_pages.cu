@@ -91,11 +91,12 @@ copy_pages_kernel(const __grid_constant__ Caches c, int64_t num_pages, const int
 
 // The same with bulk copies through shared memory: a block is one warp that keeps kCopyStages pieces
 // in flight, loads ahead of stores, and no data passes registers (256 threads with four 16-byte
-// loads each moved 3.6 TB/s).  Piece q of a pair: kCopyBytes of one cache's page (the last one of a
-// page shorter); the blocks take the pieces of all pairs in turn.
-constexpr int kCopyStages = 8, kCopyBytes = 8192;
+// loads each moved 3.6 TB/s).  A page is cut into equal pieces of at most kCopyBytes; the blocks take
+// the pieces of all pairs in turn.
+constexpr int kCopyStages = 8, kCopyBytes = 9216;
 struct CopyPieces {
     int first[NVFP4KV_MAX_CACHES + 1];      // a pair's first piece in each cache
+    int bytes[NVFP4KV_MAX_CACHES];          // of a piece
 };
 __global__ void __launch_bounds__(32)
 bulk_copy_pages_kernel(const __grid_constant__ Caches c, const __grid_constant__ CopyPieces pieces, int64_t num_pages,
@@ -123,10 +124,11 @@ bulk_copy_pages_kernel(const __grid_constant__ Caches c, const __grid_constant__
         }
         int cache = 0;
         while (q >= pieces.first[cache + 1]) ++cache;
-        const int64_t pb = c.page_bytes[cache], at = static_cast<int64_t>(q - pieces.first[cache]) * kCopyBytes;
+        const int size = pieces.bytes[cache];
+        const int64_t pb = c.page_bytes[cache], at = static_cast<int64_t>(q - pieces.first[cache]) * size;
         *from = c.base[cache] + s * pb + at;
         *to = c.base[cache] + d * pb + at;
-        return static_cast<uint32_t>(pb - at < kCopyBytes ? pb - at : kCopyBytes);
+        return static_cast<uint32_t>(pb - at < size ? pb - at : size);
     };
     // Piece i of this block (blockIdx.x + i gridDim.x) uses stage i % kCopyStages.  Loads run kAhead
     // pieces ahead; the stage a load takes was last stored from kCopyStages - kAhead pieces ago.
@@ -506,7 +508,9 @@ int launch_copy(const Caches& c, int64_t num_pages, const int32_t* src, const in
     CopyPieces pieces{};
     for (int k = 0; k < c.num; ++k) {
         align |= reinterpret_cast<uint64_t>(c.base[k]) | static_cast<uint64_t>(c.page_bytes[k]);
-        pieces.first[k + 1] = pieces.first[k] + static_cast<int>((c.page_bytes[k] + kCopyBytes - 1) / kCopyBytes);
+        const int64_t cut = (c.page_bytes[k] + kCopyBytes - 1) / kCopyBytes;
+        pieces.bytes[k] = static_cast<int>(((c.page_bytes[k] + cut - 1) / cut + 15) / 16 * 16);
+        pieces.first[k + 1] = pieces.first[k] + static_cast<int>((c.page_bytes[k] + pieces.bytes[k] - 1) / pieces.bytes[k]);
     }
     cudaError_t e;
     if (align % 16 == 0) {      // what a bulk copy can move

@@ -713,14 +713,16 @@ def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_
     """The rope part of a step in one launch: k_pe [T, 64] bf16, rotated by its tokens' angles,
     into the rope side-pool at slot_mapping (as write_nvfp4_rope), and the queries' rope dims
     q_pe [T, H, 64] bf16 rotated into q_out (default: in place).  Returns q_out."""
-    T = k_pe.shape[0]
     _require_cuda(k_pe, "k_pe")
     _require_cuda(rope_cache, "rope_cache")
-    if k_pe.dtype != torch.bfloat16 or k_pe.dim() != 2 or k_pe.shape[1] < ROPE or k_pe.stride(1) != 1:
+    ks = k_pe.stride()
+    if k_pe.dtype != torch.bfloat16 or len(ks) != 2 or k_pe.shape[1] < ROPE or ks[1] != 1:
         raise ValueError("k_pe must be bf16 [T, >=64] with a contiguous last dimension")
-    rope = rope_cache.view(-1, ROPE)
-    if rope.dtype != torch.bfloat16:
+    if rope_cache.dtype != torch.bfloat16:
         raise TypeError("rope_cache must be bf16")
+    if not rope_cache.is_contiguous() or rope_cache.numel() % ROPE:
+        raise ValueError("rope_cache must be contiguous rows of 64")
+    T = k_pe.shape[0]
     slot = _vector(slot_mapping)
     if slot.shape[0] != T:
         raise ValueError(f"slot_mapping has {slot.shape[0]} entries for {T} tokens")
@@ -728,24 +730,26 @@ def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_
     if sdt is None:
         raise TypeError("slot_mapping must be int64 or int32")
     pos, pdt = _check_angles(cos_sin, positions, T, ROPE)
-    H, qs, qos = 0, (0, 0), (0, 0)
+    H, qs, qos, q_ptr, qo_ptr = 0, (0, 0), (0, 0), None, None
     if q_pe is not None:
         q_out = q_pe if q_out is None else q_out
-        for name, t in (("q_pe", q_pe), ("q_out", q_out)):
-            _require_cuda(t, name)
-            if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[0] != T or t.shape[2] != ROPE or t.stride(2) != 1:
-                raise ValueError(f"{name} must be bf16 [T, H, 64] with a contiguous last dimension")
-        if q_out.shape != q_pe.shape:
-            raise ValueError("q_out must have q_pe's shape")
-        H, qs, qos = q_pe.shape[1], q_pe.stride(), q_out.stride()
+        _require_cuda(q_pe, "q_pe")
+        _require_cuda(q_out, "q_out")
+        shape, qs, qos = q_pe.shape, q_pe.stride(), q_out.stride()
+        if len(shape) != 3 or shape[0] != T or shape[2] != ROPE or qs[2] != 1 or q_pe.dtype != torch.bfloat16:
+            raise ValueError("q_pe must be bf16 [T, H, 64] with a contiguous last dimension")
+        if q_out.shape != shape or qos[2] != 1 or q_out.dtype != torch.bfloat16:
+            raise ValueError("q_out must be bf16 of q_pe's shape with a contiguous last dimension")
+        H = shape[1]
+        if H:
+            q_ptr, qo_ptr = q_pe.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q_pe")
     if T == 0:
         return q_out
-    _call("nvfp4kv_append_rope_rotated", k_pe.get_device(), k_pe.data_ptr(), T, k_pe.stride(0), rope.data_ptr(),
-          rope.shape[0], slot.data_ptr(), sdt, pos.data_ptr(), pdt, cos_sin.data_ptr(), cos_sin.shape[0],
-          int(interleaved), q_pe.data_ptr() if H else None, H, qs[0], qs[1], q_out.data_ptr() if H else None,
-          qos[0], qos[1])
+    _call("nvfp4kv_append_rope_rotated", k_pe.get_device(), k_pe.data_ptr(), T, ks[0], rope_cache.data_ptr(),
+          rope_cache.numel() // ROPE, slot.data_ptr(), sdt, pos.data_ptr(), pdt, cos_sin.data_ptr(),
+          cos_sin.shape[0], int(interleaved), q_ptr, H, qs[0], qs[1], qo_ptr, qos[0], qos[1])
     return q_out
 
 
@@ -828,14 +832,16 @@ def _cache_list(caches):
     """(device pointers, bytes per page, pages, page size) of pools [num_pages, page_size, ...]."""
     if not caches:
         raise ValueError("caches must name at least one pool")
-    pages, size = caches[0].shape[0], caches[0].shape[1]
-    for c in caches:
-        _require_cuda(c, "caches")
-        if c.dim() < 3 or c.shape[0] != pages or c.shape[1] != size or not c.is_contiguous():
-            raise ValueError("caches must be contiguous [num_pages, page_size, ...] pools of one geometry")
+    pages, size = caches[0].shape[:2]
     n = len(caches)
-    ptrs = (ctypes.c_void_p * n)(*[c.data_ptr() for c in caches])
-    sizes = (ctypes.c_int64 * n)(*[c.stride(0) * c.element_size() for c in caches])
+    ptrs, sizes = (ctypes.c_void_p * n)(), (ctypes.c_int64 * n)()
+    for k, c in enumerate(caches):
+        _require_cuda(c, "caches")
+        shape = c.shape
+        if len(shape) < 3 or shape[0] != pages or shape[1] != size or not c.is_contiguous():
+            raise ValueError("caches must be contiguous [num_pages, page_size, ...] pools of one geometry")
+        ptrs[k] = c.data_ptr()
+        sizes[k] = c.nbytes // pages if pages else size
     return ptrs, sizes, n, pages, size
 
 
