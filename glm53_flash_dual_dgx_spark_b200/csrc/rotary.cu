@@ -126,7 +126,7 @@ constexpr int kRopeSteps = 2;
 // the occupancy that leaves (8,192 tokens x 64 heads x 576 bf16, 1.2 GB: 176 us against 203 with one
 // and 178 with four; 225 with blocks of whole heads, whose last steps are part empty).
 template <typename T, bool kInterleaved>
-__global__ void __launch_bounds__(256) rope_vec_kernel(const __grid_constant__ RopeArgs p) {
+__global__ void __launch_bounds__(256, kInterleaved && sizeof(T) == 2 ? 8 : 4) rope_vec_kernel(const __grid_constant__ RopeArgs p) {
     constexpr int N = Vec<T>::kN;
     const int64_t u0 = static_cast<int64_t>(blockIdx.x) * (256 * kRopeSteps);
     int64_t row0, t0;       // the block's first head row, its token
