@@ -411,82 +411,89 @@ __device__ __forceinline__ uint4 dequant8(uint32_t code, uint32_t scale2) {
 // so instead: a NaN in V would reach rows that do not see it).  Eight lanes read a row's half (128
 // code bytes), a thread writes its 32 dims as 16 bytes to each of four atoms, a warp whole 128-byte
 // rows; all of a block's loads are in flight before the first is used.
+// The blocks of the grid take the image's in turn (their number is on the device).
 __global__ void __launch_bounds__(256) prefill_image_kernel(const __grid_constant__ PrefillParams p) {
     __shared__ uint32_t bits[8];
-    __shared__ int b_s, pos_s;
+    __shared__ int b_s, pos_s, total_s;
     griddep_launch_dependents();
     const int tid = threadIdx.x, lp = tid & 7, r0 = tid >> 3;
-    if (tid < 32) {
-        const int lane = tid;
-        int base = 0, b = -1, pos = 0;
-        for (int b0 = 0; b0 < p.batch && b < 0; b0 += 32) {
-            int blocks = 0;
-            if (b0 + lane < p.batch) blocks = image_blocks_of(load_seq(p, b0 + lane));
-            const int upto = base + warp_inclusive_sum(blocks, lane);
-            const uint32_t hit = __ballot_sync(0xFFFFFFFFu, static_cast<int>(blockIdx.x) < upto);
-            if (hit) {
-                const int src = __ffs(hit) - 1;
-                b = b0 + src;
-                pos = kImageTok * (static_cast<int>(blockIdx.x) - __shfl_sync(0xFFFFFFFFu, upto - blocks, src));
+    int total = 0x7FFFFFFF;
+    for (int item = blockIdx.x; item < total; item += gridDim.x) {
+        if (tid < 32) {
+            const int lane = tid;
+            int base = 0, b = -1, pos = 0;
+            for (int b0 = 0; b0 < p.batch; b0 += 32) {
+                int blocks = 0;
+                if (b0 + lane < p.batch) blocks = image_blocks_of(load_seq(p, b0 + lane));
+                const int upto = base + warp_inclusive_sum(blocks, lane);
+                const uint32_t hit = __ballot_sync(0xFFFFFFFFu, item < upto);
+                if (hit && b < 0) {
+                    const int src = __ffs(hit) - 1;
+                    b = b0 + src;
+                    pos = kImageTok * (item - __shfl_sync(0xFFFFFFFFu, upto - blocks, src));
+                }
+                base = __shfl_sync(0xFFFFFFFFu, upto, 31);
             }
-            base = __shfl_sync(0xFFFFFFFFu, upto, 31);
+            if (lane == 0) {
+                b_s = b;
+                pos_s = pos;
+                total_s = base;
+            }
+            if (lane < 8) bits[lane] = 0;
         }
-        if (lane == 0) {
-            b_s = b;
-            pos_s = pos;
+        __syncthreads();
+        if (b_s < 0) return;
+        total = total_s;
+        const int L = load_seq(p, b_s).L;
+        const int32_t* table = p.tables + b_s * p.tables_stride;
+        int64_t row[4];
+        uint4 code[4][2], rope[4];
+        uint16_t scale[4][2];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) row[k] = pool_row(p, table, pos_s + r0 + 32 * k, L);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            rope[k] = code[k][0] = code[k][1] = make_uint4(0, 0, 0, 0);
+            scale[k][0] = scale[k][1] = 0;
+            if (row[k] >= 0) {
+                const uint8_t* src = p.pool + row[k] * kRowBytes;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    code[k][h] = ldg_nc_v4(src + 128 * h + 16 * lp);
+                    scale[k][h] = __ldg(reinterpret_cast<const uint16_t*>(src + 256 + 16 * h + 2 * lp));
+                }
+                if (p.rope) rope[k] = ldg_nc_v4(p.rope + row[k] * kRope + 8 * lp);
+            }
         }
-        if (lane < 8) bits[lane] = 0;
-    }
-    __syncthreads();
-    if (b_s < 0) return;
-    const int L = load_seq(p, b_s).L;
-    const int32_t* table = p.tables + b_s * p.tables_stride;
-    int64_t row[4];
-    uint4 code[4][2], rope[4];
-    uint16_t scale[4][2];
+        const int atoms = p.rope ? 9 : 8;
+        uint8_t* dst = p.image + static_cast<int64_t>(item) * atoms * kStageBytes + r0 * 128 + ((lp ^ (r0 & 7)) << 4);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) row[k] = pool_row(p, table, pos_s + r0 + 32 * k, L);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        rope[k] = code[k][0] = code[k][1] = make_uint4(0, 0, 0, 0);
-        scale[k][0] = scale[k][1] = 0;
-        if (row[k] >= 0) {
-            const uint8_t* src = p.pool + row[k] * kRowBytes;
+        for (int k = 0; k < 4; ++k) {
+            const int t = r0 + 32 * k;
+            uint32_t nan = 0;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                code[k][h] = ldg_nc_v4(src + 128 * h + 16 * lp);
-                scale[k][h] = __ldg(reinterpret_cast<const uint16_t*>(src + 256 + 16 * h + 2 * lp));
+                const uint32_t word[4] = {code[k][h].x, code[k][h].y, code[k][h].z, code[k][h].w};
+                const uint32_t s2 = e4m3x2_to_f16x2(scale[k][h]);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const bool bad = ((scale[k][h] >> (s & 2 ? 8 : 0)) & 0x7F) == 0x7F;
+                    nan |= bad;
+                    const uint4 v = dequant8(word[s], __byte_perm(s2, s2, s & 2 ? 0x3232 : 0x1010));
+                    *reinterpret_cast<uint4*>(dst + (4 * h + s) * kStageBytes + 4096 * k) = bad ? make_uint4(0, 0, 0, 0) : v;
+                }
             }
-            if (p.rope) rope[k] = ldg_nc_v4(p.rope + row[k] * kRope + 8 * lp);
-        }
-    }
-    const int atoms = p.rope ? 9 : 8;
-    uint8_t* dst = p.image + static_cast<int64_t>(blockIdx.x) * atoms * kStageBytes + r0 * 128 + ((lp ^ (r0 & 7)) << 4);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int t = r0 + 32 * k;
-        uint32_t nan = 0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t word[4] = {code[k][h].x, code[k][h].y, code[k][h].z, code[k][h].w};
-            const uint32_t s2 = e4m3x2_to_f16x2(scale[k][h]);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const bool bad = ((scale[k][h] >> (s & 2 ? 8 : 0)) & 0x7F) == 0x7F;
-                nan |= bad;
-                const uint4 v = dequant8(word[s], __byte_perm(s2, s2, s & 2 ? 0x3232 : 0x1010));
-                *reinterpret_cast<uint4*>(dst + (4 * h + s) * kStageBytes + 4096 * k) = bad ? make_uint4(0, 0, 0, 0) : v;
+            if (p.rope) *reinterpret_cast<uint4*>(dst + 8 * kStageBytes + 4096 * k) = rope[k];
+            if (nan) atomicOr(&bits[4 + k], 1u << (t & 31));
+            if (lp == 0) {
+                if (row[k] >= 0) atomicOr(&bits[k], 1u << (t & 31));
+                else if (pos_s + t < L) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
             }
         }
-        if (p.rope) *reinterpret_cast<uint4*>(dst + 8 * kStageBytes + 4096 * k) = rope[k];
-        if (nan) atomicOr(&bits[4 + k], 1u << (t & 31));
-        if (lp == 0) {
-            if (row[k] >= 0) atomicOr(&bits[k], 1u << (t & 31));
-            else if (pos_s + t < L) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
-        }
+        __syncthreads();
+        if (tid < 8) p.image_bits[8 * static_cast<int64_t>(item) + tid] = bits[tid];
+        __syncthreads();      // (the next item's words)
     }
-    __syncthreads();
-    if (tid < 8) p.image_bits[8 * static_cast<int64_t>(blockIdx.x) + tid] = bits[tid];
 }
 
 // ------------------------------------------------------------------ attention
@@ -1125,7 +1132,8 @@ extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_
         const dim3 grid(2 * pl.pairs);
         cudaError_t e = cudaSuccess;
         if (pl.image_blocks > 0) {
-            prefill_image_kernel<<<pl.image_blocks, 256, 0, st>>>(p);
+            const int most = 8 * device_sm_count();
+            prefill_image_kernel<<<pl.image_blocks < most ? pl.image_blocks : most, 256, 0, st>>>(p);
             if ((rc = check_launch("nvfp4kv_mla_prefill image")) != NVFP4KV_OK) return rc;
             // its set-up overlaps the image kernel; all else it reads was there before that one
             e = launch_dependent(mla_prefill_kernel, grid, dim3(kThreads), kSmemBytes, st, p);

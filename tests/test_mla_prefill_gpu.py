@@ -214,3 +214,18 @@ def test_same_inputs_give_the_same_bits_and_other_streams():
     s.synchronize()
     assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
     p.check(out, lse)
+
+
+def test_a_batch_whose_images_do_not_fit_runs_in_groups():
+    """max_seq_len bounds the workspace: with a large one the batch takes several passes over it."""
+    p = Problem([3, 40, 1], [300, 90, 1000], 16, 64, True, seed=18)
+    out, lse = p.run()
+    p.check(out, lse)
+    most = 400000
+    p.tables = torch.cat([p.tables, torch.full((3, most // 64 - p.width), -1, dtype=torch.int32)], 1)
+    cu = torch.tensor([0, 3, 43, 44], dtype=torch.int32, device="cuda")
+    seq = torch.tensor(p.ctx, dtype=torch.int32, device="cuda")
+    again, lse2 = rt.mla_prefill(p.q, p.pool, None, 512, 64, p.tables.cuda(), cu, seq, 40, most, bmm1_scale=p.scale,
+                                 rope_cache=p.rope, return_lse=True)
+    assert rt.device_errors() == 0
+    p.check(again, lse2)
