@@ -602,15 +602,13 @@ def index_scores_buffer(device=None) -> torch.Tensor | None:
 # A few tokens' operators run for less time on the device than their call takes on the host, so the
 # call below uses torch's raw getters: 3 us less than the stream object and device guard.
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_err_ptrs: dict = {}
 
 
 def _call(name: str, index: int, *args) -> None:
     """The C entry ``name`` on device ``index``'s current stream, with the device error word; raises
     on a non-OK code."""
-    err = _err_ptrs.get(index)
-    if err is None:
-        err = _err_ptrs[index] = _err_word(torch.device("cuda", index)).data_ptr()
+    word = _bufs.get(("err", index))
+    err = (_err_word(torch.device("cuda", index)) if word is None else word).data_ptr()
     fn = getattr(_lib.lib(), name)
     if torch._C._cuda_getDevice() == index:
         rc = fn(*args, err, _raw_stream(index))
