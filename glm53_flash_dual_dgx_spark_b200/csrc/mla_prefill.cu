@@ -80,9 +80,9 @@ constexpr int SM_RED = SM_RING + kStages * kStageBytes;      // 2 x 4 x 64 f32: 
 constexpr int SM_LSUM = SM_RED + 2 * 4 * 64 * 4;             // 4 x 64 f32
 constexpr int SM_QS = SM_LSUM + 4 * 64 * 4;                  // 2 x 64 f32: score factor (log2 units) of a row
 constexpr int SM_FLAGS = SM_QS + 2 * 64 * 4;                 // [0] TMEM base, [1] abort
-constexpr int SM_WORK = SM_FLAGS + 16;                       // a Work per warp
+constexpr int SM_WORK = SM_FLAGS + 16;                       // a Work per warp, and one with the range's first part
 constexpr int kWorkBytes = 96;
-constexpr int SM_BARS = SM_WORK + (kThreads / 32) * kWorkBytes;
+constexpr int SM_BARS = SM_WORK + (kThreads / 32 + 1) * kWorkBytes;
 constexpr int B_FULL = 0;                      // [kStages] leader: stage landed in both CTAs
 constexpr int B_EMPTY = B_FULL + kStages;      // [kStages] both: the MMAs have read the stage
 constexpr int B_LAND = B_EMPTY + kStages;      // [kStages] own: an image copy landed
@@ -497,6 +497,78 @@ __global__ void __launch_bounds__(256) prefill_image_kernel(const __grid_constan
 }
 
 // ------------------------------------------------------------------ attention
+// Q of a unit: rows -> fp16 after a power of two per row that brings its largest |q| to [2^10, 2^11)
+// (the rope part by the same factor, in bf16).  A warp per row, 16 + 2 dims per lane, kQRows rows at
+// a time: r, r + step, ... of the CTA's 64.
+struct QRows {
+    uint4 u[kQRows][2];
+    uint32_t rope[kQRows];
+};
+__device__ __forceinline__ void load_q(const PrefillParams& p, const volatile Part& t, int cta, int r, int step, QRows& q) {
+    const int lane = threadIdx.x & 31, row0 = t.block * kUnitRows + kCtaRows * cta, rows = t.rows, first = t.first;
+#pragma unroll
+    for (int j = 0; j < kQRows; ++j) {
+        q.u[j][0] = q.u[j][1] = make_uint4(0, 0, 0, 0);
+        q.rope[j] = 0;
+        const int row = row0 + r + j * step;
+        if (row < rows && r + j * step < kCtaRows) {
+            int tok = p.heads == 1 ? row : static_cast<int>(__umulhi(row, p.heads_magic));      // row / heads, or one more
+            tok -= tok * p.heads > row;
+            const __nv_bfloat16* src = p.q + static_cast<int64_t>(first + tok) * p.q_st + static_cast<int64_t>(row - tok * p.heads) * p.q_sh;
+            q.u[j][0] = ldg_nc_v4(src + 16 * lane);
+            q.u[j][1] = ldg_nc_v4(src + 16 * lane + 8);
+            if (p.rope) q.rope[j] = __ldg(reinterpret_cast<const uint32_t*>(src + kLatent) + lane);
+        }
+    }
+}
+__device__ __forceinline__ void store_q(const PrefillParams& p, uint8_t* smem, float* qs, int r0, int step, const QRows& q) {
+    const int lane = threadIdx.x & 31;
+    uint32_t w[kQRows][8], amax[kQRows];
+#pragma unroll
+    for (int j = 0; j < kQRows; ++j) {
+        w[j][0] = q.u[j][0].x; w[j][1] = q.u[j][0].y; w[j][2] = q.u[j][0].z; w[j][3] = q.u[j][0].w;
+        w[j][4] = q.u[j][1].x; w[j][5] = q.u[j][1].y; w[j][6] = q.u[j][1].z; w[j][7] = q.u[j][1].w;
+        uint32_t hi = 0, lo = 0;      // the largest |q| of the pairs' halves: as integers, the order of |x|
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            hi = max(hi, w[j][i] & 0x7FFF0000u);
+            lo = max(lo, w[j][i] & 0x7FFFu);
+        }
+        amax[j] = max(hi, lo << 16);
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1)
+#pragma unroll
+        for (int j = 0; j < kQRows; ++j) amax[j] = max(amax[j], __shfl_xor_sync(0xFFFFFFFFu, amax[j], o));
+#pragma unroll
+    for (int j = 0; j < kQRows; ++j) {
+        const int r = r0 + j * step;
+        const int eb = static_cast<int>((amax[j] >> 23) & 0xFFu);      // 255: inf or NaN
+        const int e = eb > 0 && eb < 255 ? max(eb - 127 - 10, -100) : 0;
+        float factor = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        float mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        mul = p.scale_log2 < 0.0f ? -mul : mul;
+        if (factor == 0.0f) {          // every score 0: zero queries, and a factor that keeps a hidden score's -inf
+            factor = 1.0f;
+            mul = 0.0f;
+        }
+        uint32_t h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            h[i] = pack_half2(__uint_as_float(w[j][i] << 16) * mul, __uint_as_float(w[j][i] & 0xFFFF0000u) * mul);
+        // dims 16 lane + 8 c: half lane / 16, piece (lane / 2) % 8, chunk 2 (lane % 2) + c
+        uint8_t* dst = smem + SM_Q + ((lane >> 4) * 4 + 2 * (lane & 1)) * (kCtaRows * 128) + r * 128 + ((((lane >> 1) & 7) ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(dst + kCtaRows * 128) = make_uint4(h[4], h[5], h[6], h[7]);
+        if (p.rope) {
+            const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(q.rope[j] << 16) * mul, __uint_as_float(q.rope[j] & 0xFFFF0000u) * mul);
+            *reinterpret_cast<uint32_t*>(smem + SM_Q + 8 * (kCtaRows * 128) + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)) =
+                *reinterpret_cast<const uint32_t*>(&two);
+        }
+        if (lane == 0) qs[r] = factor;
+    }
+}
+
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -513,6 +585,14 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         if (lane == 0) {
             flags[1] = 0;
             for (int k = 0; k < kThreads / 32; ++k) reinterpret_cast<Work*>(smem + SM_WORK + k * kWorkBytes)->range = r;
+            // the range's first part with tiles, whose Q all warps load now
+            Work* w = reinterpret_cast<Work*>(smem + SM_WORK + kThreads / 32 * kWorkBytes);
+            Range r1 = r;
+            Part t1;
+            bool more = next_part_of(p, r1, t1);
+            while (more && t1.n_tiles == 0) more = next_part_of(p, r1, t1);
+            w->more = more;
+            w->part = t1;
             if (cta == 0) p.parts[2 * pair].used = p.parts[2 * pair + 1].used = 0;
         }
     }
@@ -539,6 +619,17 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
     const volatile Part& t = work->part;
     if (reinterpret_cast<volatile Work*>(work)->range.left <= 0) return;       // nothing for this pair: the whole cluster
     if (warp == kMmaWarp) pair_tmem_alloc(sbase + SM_FLAGS, kTmemCols);
+    {
+        const Work* w = reinterpret_cast<const Work*>(smem + SM_WORK + kThreads / 32 * kWorkBytes);
+        constexpr int kWarps = kThreads / 32;
+        static_assert(kWarps * kQRows == kCtaRows, "one round of rows");
+        if (w->more) {
+            QRows q;
+            load_q(p, w->part, cta, warp, kWarps, q);
+            store_q(p, smem, reinterpret_cast<float*>(smem + SM_QS), warp, kWarps, q);
+            fence_proxy_async_smem();
+        }
+    }
     tc_fence_before();
     cluster_sync();
     tc_fence_after();
@@ -566,7 +657,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 while (next_part(p, work) && !*abort_flag) {
                     const int n_tiles = t.n_tiles;
                     if (n_tiles == 0) continue;
-                    mbar_wait(bar(B_Q_FULL), parts & 1, abort_flag, p.err);
+                    if (parts > 0) mbar_wait(bar(B_Q_FULL), (parts - 1) & 1, abort_flag, p.err);
 #pragma unroll 1
                     for (int i = 0; i <= n_tiles; ++i, ++tile) {
                         if (i < n_tiles) {
@@ -679,86 +770,21 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
 #pragma unroll 1
         while (next_part(p, work)) {
             if (t.n_tiles == 0) continue;
-            // Q: 64 rows -> fp16 after a power of two per row that brings its largest |q| to [2^10, 2^11)
-            // (the rope part by the same factor, in bf16); a warp per row, 16 + 2 dims per lane, the next
-            // kQRows rows on their way meanwhile (the first ones from before the last part's QK is done)
-            const int rows = t.rows, q_row0 = t.block * kUnitRows + kCtaRows * cta + warp - kQWarp0, first = t.first;
-            float* qs = reinterpret_cast<float*>(smem + SM_QS) + 64 * (parts & 1);
-            uint4 u[kQRows][2];
-            uint32_t rw[kQRows];
-            auto load = [&](int r0) {      // rows r0, r0 + kQWarps, ... of this warp
-#pragma unroll
-                for (int j = 0; j < kQRows; ++j) {
-                    u[j][0] = u[j][1] = make_uint4(0, 0, 0, 0);
-                    rw[j] = 0;
-                    const int row = q_row0 + r0 + j * kQWarps;
-                    if (row < rows && r0 < kCtaRows) {
-                        int tok = p.heads == 1 ? row : static_cast<int>(__umulhi(row, p.heads_magic));      // row / heads, or one more
-                        tok -= tok * p.heads > row;
-                        const __nv_bfloat16* src = p.q + static_cast<int64_t>(first + tok) * p.q_st + static_cast<int64_t>(row - tok * p.heads) * p.q_sh;
-                        u[j][0] = ldg_nc_v4(src + 16 * lane);
-                        u[j][1] = ldg_nc_v4(src + 16 * lane + 8);
-                        if (p.rope) rw[j] = __ldg(reinterpret_cast<const uint32_t*>(src + kLatent) + lane);
-                    }
-                }
-            };
-            load(0);
-            if (parts > 0) wait_phase(bar(B_Q_FREE), (parts - 1) & 1, abort_flag, p.err);
+            if (parts > 0) {                     // (the first part's is there)
+                // the next rows on their way while some are converted, the first before the last part's QK is done
+                QRows q;
+                load_q(p, t, cta, warp - kQWarp0, kQWarps, q);
+                wait_phase(bar(B_Q_FREE), (parts - 1) & 1, abort_flag, p.err);
 #pragma unroll 1
-            for (int r0 = 0; r0 < kCtaRows; r0 += kQRows * kQWarps) {
-                uint32_t w[kQRows][8], rope_w[kQRows];
-                float amax[kQRows];
-#pragma unroll
-                for (int j = 0; j < kQRows; ++j) {
-                    w[j][0] = u[j][0].x; w[j][1] = u[j][0].y; w[j][2] = u[j][0].z; w[j][3] = u[j][0].w;
-                    w[j][4] = u[j][1].x; w[j][5] = u[j][1].y; w[j][6] = u[j][1].z; w[j][7] = u[j][1].w;
-                    rope_w[j] = rw[j];
-                    // |bf16 pairs| by their largest: as integers, the order of |x|
-                    uint32_t hi = 0, lo = 0;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        hi = max(hi, w[j][i] & 0x7FFF0000u);
-                        lo = max(lo, w[j][i] & 0x7FFFu);
-                    }
-                    amax[j] = __uint_as_float(max(hi, lo << 16));
+                for (int r = warp - kQWarp0; r < kCtaRows; r += kQRows * kQWarps) {
+                    const QRows now = q;
+                    load_q(p, t, cta, r + kQRows * kQWarps, kQWarps, q);
+                    store_q(p, smem, reinterpret_cast<float*>(smem + SM_QS) + 64 * (parts & 1), r, kQWarps, now);
                 }
-                load(r0 + kQRows * kQWarps);
-#pragma unroll
-                for (int o = 16; o >= 1; o >>= 1)
-#pragma unroll
-                    for (int j = 0; j < kQRows; ++j)
-                        amax[j] = __uint_as_float(max(__float_as_uint(amax[j]), __shfl_xor_sync(0xFFFFFFFFu, __float_as_uint(amax[j]), o)));
-#pragma unroll
-                for (int j = 0; j < kQRows; ++j) {
-                    const int r = warp - kQWarp0 + r0 + j * kQWarps;
-                    const int eb = static_cast<int>((__float_as_uint(amax[j]) >> 23) & 0xFFu);      // 255: inf or NaN
-                    const int e = eb > 0 && eb < 255 ? max(eb - 127 - 10, -100) : 0;
-                    float factor = fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-                    float mul = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                    mul = p.scale_log2 < 0.0f ? -mul : mul;
-                    if (factor == 0.0f) {          // every score 0: zero queries, and a factor that keeps a hidden score's -inf
-                        factor = 1.0f;
-                        mul = 0.0f;
-                    }
-                    uint32_t h[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        h[i] = pack_half2(__uint_as_float(w[j][i] << 16) * mul, __uint_as_float(w[j][i] & 0xFFFF0000u) * mul);
-                    // dims 16 lane + 8 c: half lane / 16, piece (lane / 2) % 8, chunk 2 (lane % 2) + c
-                    uint8_t* dst = smem + SM_Q + ((lane >> 4) * 4 + 2 * (lane & 1)) * (kCtaRows * 128) + r * 128 + ((((lane >> 1) & 7) ^ (r & 7)) << 4);
-                    *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4*>(dst + kCtaRows * 128) = make_uint4(h[4], h[5], h[6], h[7]);
-                    if (p.rope) {
-                        const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(rope_w[j] << 16) * mul, __uint_as_float(rope_w[j] & 0xFFFF0000u) * mul);
-                        *reinterpret_cast<uint32_t*>(smem + SM_Q + 8 * (kCtaRows * 128) + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)) =
-                            *reinterpret_cast<const uint32_t*>(&two);
-                    }
-                    if (lane == 0) qs[r] = factor;
-                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) leader_arrive(bar(B_Q_FULL));
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) leader_arrive(bar(B_Q_FULL));
             ++parts;
         }
     } else {
@@ -884,44 +910,57 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             }
             if (!whole && threadIdx.x == 0 && cta == 0)
                 p.parts[2 * pair + (first_part ? 0 : 1)] = PartInfo{1, t.head, t.tail, t.first, t.n, t.block};
-            // 64 columns a step in registers, 32-byte stores by the lanes that hold the rows (whole rows
-            // staged in shared memory and stored by warps took 9,000 cycles for barriers and latency)
+            // Two pieces a step, 16 dims of each as 32-byte stores by the lanes that hold the rows, the next two
+            // on their way from tensor memory.  Rolled up: this code runs once per part, and unrolled its
+            // instructions took longer to arrive than to run.  (Whole rows staged in shared memory and
+            // stored by warps were no faster.)
             __nv_bfloat16* out = p.out + static_cast<int64_t>(t.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh + 256 * (sp >> 1) + 16 * ch;
             float* part_o = p.part_o + part_row * kLatent + 256 * (sp >> 1) + 16 * ch;
             const bool wide = (reinterpret_cast<uintptr_t>(p.out) % 32 == 0) && p.o_st % 16 == 0 && p.o_sh % 16 == 0;
+            const uint32_t o_addr = tmem + kTO + 128 * ch + lanes;
+            uint32_t ahead_o[2][16];      // columns 8 j .. + 16 (dims a = 0 of pieces j, j + 1) and 64 + 8 j .. (a = 1)
+            if (n_tiles > 0) {
+                tmem_ld16(o_addr, ahead_o[0]);
+                tmem_ld16(o_addr + 64, ahead_o[1]);
+                tmem_wait_ld();
+            }
 #pragma unroll 1
-            for (int p0 = 0; p0 < 8; p0 += 4) {         // pieces p0 .. p0 + 3: 16 dims of each, in columns 8 p0 .. and 64 + 8 p0 ..
-                uint32_t o[2][32];
-                if (n_tiles > 0) {
-                    tmem_ld32(tmem + kTO + 128 * ch + 8 * p0 + lanes, o[0]);
-                    tmem_ld32(tmem + kTO + 128 * ch + 64 + 8 * p0 + lanes, o[1]);
-                    tmem_wait_ld();
+            for (int j = 0; j < 8; j += 2) {
+                uint32_t o[2][16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    o[0][k] = any ? __float_as_uint(__uint_as_float(ahead_o[0][k]) * mul) : 0u;
+                    o[1][k] = any ? __float_as_uint(__uint_as_float(ahead_o[1][k]) * mul) : 0u;
                 }
-                if (!real) continue;
+                if (n_tiles > 0 && j < 6) {
+                    tmem_ld16(o_addr + 8 * j + 16, ahead_o[0]);
+                    tmem_ld16(o_addr + 8 * j + 80, ahead_o[1]);
+                }
+                if (real) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t v[16];
+                    for (int h = 0; h < 2; ++h) {
+                        if (whole) {
+                            uint32_t w[8];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) v[k] = any ? __float_as_uint(__uint_as_float(o[k >> 3][8 * j + (k & 7)]) * mul) : 0u;
-                    if (whole) {
-                        uint32_t w[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
-                            w[k] = *reinterpret_cast<const uint32_t*>(&two);
+                            for (int k = 0; k < 8; ++k) {
+                                const uint32_t* src = &o[k >> 2][8 * h + 2 * (k & 3)];
+                                const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(src[0]), __uint_as_float(src[1]));
+                                w[k] = *reinterpret_cast<const uint32_t*>(&two);
+                            }
+                            __nv_bfloat16* dst = out + 32 * (j + h);
+                            if (wide) {
+                                st_global_v8(dst, w);
+                            } else {
+                                *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+                                *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                            }
+                        } else if (any) {
+                            st_global_v8(part_o + 32 * (j + h), &o[0][8 * h]);
+                            st_global_v8(part_o + 32 * (j + h) + 8, &o[1][8 * h]);
                         }
-                        __nv_bfloat16* dst = out + 32 * (p0 + j);
-                        if (wide) {
-                            st_global_v8(dst, w);
-                        } else {
-                            *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-                            *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-                        }
-                    } else if (any) {
-                        st_global_v8(part_o + 32 * (p0 + j), v);
-                        st_global_v8(part_o + 32 * (p0 + j) + 8, v + 8);
                     }
                 }
+                tmem_wait_ld();
             }
             if (n_tiles > 0) {
                 tc_fence_before();
@@ -1142,7 +1181,7 @@ extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_
         }
         if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill launch failed: %s", cudaGetErrorString(e));
         if ((rc = check_launch("nvfp4kv_mla_prefill")) != NVFP4KV_OK) return rc;
-        if (pl.pairs == 1) continue;
+        if (pl.pairs == 1 || max_seq_len <= kTile) continue;      // no unit can be cut
         e = launch_dependent(prefill_combine_kernel, dim3(pl.pairs * kUnitRows), dim3(128), 0, st, p);
         if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill combine launch failed: %s", cudaGetErrorString(e));
         if ((rc = check_launch("nvfp4kv_mla_prefill combine")) != NVFP4KV_OK) return rc;
