@@ -73,15 +73,16 @@ constexpr float kRescaleLog2 = 8.0f;
 constexpr int kMaxPairs = 128;
 constexpr int kImageTok = 128;                  // tokens of an image block
 
+constexpr int kQBytes = 9 * kCtaRows * 128;
 constexpr int SM_Q = 0;                                      // 9 dim atoms x [64 rows x 128 B]
 constexpr int SM_P = SM_Q + 9 * kCtaRows * 128;              // 4 token atoms x [64 rows x 128 B]
 constexpr int SM_RING = SM_P + 4 * kCtaRows * 128;
 constexpr int SM_RED = SM_RING + kStages * kStageBytes;      // 2 x 4 x 64 f32: row maxima of the token quarters
 constexpr int SM_LSUM = SM_RED + 2 * 4 * 64 * 4;             // 4 x 64 f32
-constexpr int SM_QS = SM_LSUM + 4 * 64 * 4;                  // 2 x 64 f32: score factor (log2 units) of a row
-constexpr int SM_FLAGS = SM_QS + 2 * 64 * 4;                 // [0] TMEM base, [1] abort
+constexpr int SM_QS = SM_LSUM + 4 * 64 * 4;                  // 4 x 64 f32: score factor (log2 units) of a row
+constexpr int SM_FLAGS = SM_QS + 4 * 64 * 4;                 // [0] TMEM base, [1] abort
 constexpr int SM_WORK = SM_FLAGS + 16;                       // a Work per warp, and one with the range's first part
-constexpr int kWorkBytes = 96;
+constexpr int kWorkBytes = 144;
 constexpr int SM_BARS = SM_WORK + (kThreads / 32 + 1) * kWorkBytes;
 constexpr int B_FULL = 0;                      // [kStages] leader: stage landed in both CTAs
 constexpr int B_EMPTY = B_FULL + kStages;      // [kStages] both: the MMAs have read the stage
@@ -92,7 +93,8 @@ constexpr int B_P_FULL = B_S_FREE + 2;         // leader: P written in both CTAs
 constexpr int B_PV_DONE = B_P_FULL + 1;        // both: O stable, P free
 constexpr int B_Q_FULL = B_PV_DONE + 1;        // leader: Q written in both CTAs
 constexpr int B_Q_FREE = B_Q_FULL + 1;         // both: the last QK of a part complete
-constexpr int B_O_FREE = B_Q_FREE + 1;         // leader: O read by both CTAs
+constexpr int B_Q_LAND = B_Q_FREE + 1;         // own: Q copied
+constexpr int B_O_FREE = B_Q_LAND + 1;         // leader: O read by both CTAs
 constexpr int B_DRAIN = B_O_FREE + 1;          // both: every MMA complete
 constexpr int kNumBars = B_DRAIN + 1;
 constexpr int kSmemBytes = SM_BARS + kNumBars * 8 + 1024;    // slack to align the base
@@ -104,8 +106,9 @@ static_assert(SM_BARS % 8 == 0 && kSmemBytes <= 232448, "shared memory budget");
 constexpr uint32_t kTS = 0, kTO = 256, kTmemCols = 512;
 
 // A part of a unit that another pair's part completes: what the combine kernel reads.
-struct PartInfo {
-    int32_t used, head, tail, first, n, block;
+struct __align__(16) PartInfo {
+    int32_t used, head, tail, pad;
+    int32_t first, n, block, pad2;
 };
 
 struct PrefillParams {
@@ -128,6 +131,7 @@ struct PrefillParams {
     PartInfo* parts;    // [pairs][2]: the range's first part of a unit, and its last one
     float* part_ml;     // [pairs][2][128][2]: maximum (log2 units), sum
     float* part_o;      // [pairs][2][128][512]
+    uint8_t* q_scratch; // [pairs][2 CTAs][kQBytes]: the next part's Q
     uint8_t* image;     // [blocks][8 or 9 atoms][128 tokens x 128 B]
     uint32_t* image_bits;   // [blocks][8]: 128 bits of tokens that exist, 128 of those that hold a NaN
     int32_t* err;
@@ -320,6 +324,7 @@ struct Part {
     int tile0, n_tiles;
     int image;              // the sequence's first image block
     int head, tail;         // it begins / ends the unit
+    int half;               // rows in the leading CTA (the unit's others are in the second)
 };
 // The next part of the range; parts without tiles are given only where they are a whole unit (one
 // that sees no token).
@@ -342,6 +347,8 @@ __device__ __forceinline__ bool next_part_of(const PrefillParams& p, Range& r, P
         t.b = r.b; t.block = r.k;
         t.first = s.first; t.n = s.n; t.L = s.L; t.rows = s.rows;
         t.image = r.image0;
+        // 64 rows or fewer (one token of 64 heads): 32 in each CTA, so that both store O
+        t.half = s.rows - r.k * kUnitRows <= kCtaRows ? kCtaRows / 2 : kCtaRows;
         t.head = t.tile0 == 0;
         t.tail = t.tile0 + t.n_tiles == tiles;
         r.left -= take;
@@ -360,20 +367,38 @@ struct Work {
     Range range;
     int more;
     Part part;
+    Part ahead;
 };
 static_assert(sizeof(Work) <= kWorkBytes, "a warp's work record");
-__device__ __forceinline__ bool next_part(const PrefillParams& p, Work* w) {
-    __syncwarp();
+// The search for a part takes a microsecond of dependent loads and divisions, so a warp may look for
+// the next one (ahead) while it waits for something else, and move on to it later (advance_part).
+__device__ __forceinline__ void look_ahead(const PrefillParams& p, Work* w) {
     if ((threadIdx.x & 31) == 0) {
         Range r = w->range;
         Part t;
         const bool more = next_part_of(p, r, t);
         w->range = r;
         w->more = more;
-        if (more) w->part = t;
+        if (more) w->ahead = t;
+    }
+}
+__device__ __forceinline__ bool advance_part(Work* w) {
+    __syncwarp();
+    const bool more = *reinterpret_cast<volatile int*>(&w->more) != 0;
+    if (more) {
+        const int* src = reinterpret_cast<const int*>(&w->ahead);
+        int* dst = reinterpret_cast<int*>(&w->part);
+        static_assert(sizeof(Part) <= 128 && sizeof(Part) % 4 == 0, "a word per lane");
+        const int lane = threadIdx.x & 31;
+        if (lane < static_cast<int>(sizeof(Part) / 4)) dst[lane] = src[lane];
     }
     __syncwarp();
-    return *reinterpret_cast<volatile int*>(&w->more) != 0;
+    return more;
+}
+__device__ __forceinline__ bool next_part(const PrefillParams& p, Work* w) {
+    __syncwarp();
+    look_ahead(p, w);
+    return advance_part(w);
 }
 
 // Pool row of position pos < end of a sequence, -1 for a missing page or past the end.
@@ -505,13 +530,13 @@ struct QRows {
     uint32_t rope[kQRows];
 };
 __device__ __forceinline__ void load_q(const PrefillParams& p, const volatile Part& t, int cta, int r, int step, QRows& q) {
-    const int lane = threadIdx.x & 31, row0 = t.block * kUnitRows + kCtaRows * cta, rows = t.rows, first = t.first;
+    const int lane = threadIdx.x & 31, half = t.half, row0 = t.block * kUnitRows + half * cta, rows = t.rows, first = t.first;
 #pragma unroll
     for (int j = 0; j < kQRows; ++j) {
         q.u[j][0] = q.u[j][1] = make_uint4(0, 0, 0, 0);
         q.rope[j] = 0;
         const int row = row0 + r + j * step;
-        if (row < rows && r + j * step < kCtaRows) {
+        if (row < rows && r + j * step < half) {
             int tok = p.heads == 1 ? row : static_cast<int>(__umulhi(row, p.heads_magic));      // row / heads, or one more
             tok -= tok * p.heads > row;
             const __nv_bfloat16* src = p.q + static_cast<int64_t>(first + tok) * p.q_st + static_cast<int64_t>(row - tok * p.heads) * p.q_sh;
@@ -521,7 +546,8 @@ __device__ __forceinline__ void load_q(const PrefillParams& p, const volatile Pa
         }
     }
 }
-__device__ __forceinline__ void store_q(const PrefillParams& p, uint8_t* smem, float* qs, int r0, int step, const QRows& q) {
+// (base: the operand's place, or its copy in the workspace)
+__device__ __forceinline__ void store_q(const PrefillParams& p, uint8_t* base, float* qs, int r0, int step, const QRows& q) {
     const int lane = threadIdx.x & 31;
     uint32_t w[kQRows][8], amax[kQRows];
 #pragma unroll
@@ -557,12 +583,12 @@ __device__ __forceinline__ void store_q(const PrefillParams& p, uint8_t* smem, f
         for (int i = 0; i < 8; ++i)
             h[i] = pack_half2(__uint_as_float(w[j][i] << 16) * mul, __uint_as_float(w[j][i] & 0xFFFF0000u) * mul);
         // dims 16 lane + 8 c: half lane / 16, piece (lane / 2) % 8, chunk 2 (lane % 2) + c
-        uint8_t* dst = smem + SM_Q + ((lane >> 4) * 4 + 2 * (lane & 1)) * (kCtaRows * 128) + r * 128 + ((((lane >> 1) & 7) ^ (r & 7)) << 4);
+        uint8_t* dst = base + ((lane >> 4) * 4 + 2 * (lane & 1)) * (kCtaRows * 128) + r * 128 + ((((lane >> 1) & 7) ^ (r & 7)) << 4);
         *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(dst + kCtaRows * 128) = make_uint4(h[4], h[5], h[6], h[7]);
         if (p.rope) {
             const __nv_bfloat162 two = __floats2bfloat162_rn(__uint_as_float(q.rope[j] << 16) * mul, __uint_as_float(q.rope[j] & 0xFFFF0000u) * mul);
-            *reinterpret_cast<uint32_t*>(smem + SM_Q + 8 * (kCtaRows * 128) + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)) =
+            *reinterpret_cast<uint32_t*>(base + 8 * (kCtaRows * 128) + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)) =
                 *reinterpret_cast<const uint32_t*>(&two);
         }
         if (lane == 0) qs[r] = factor;
@@ -608,8 +634,9 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         }
         mbar_init(bar(B_P_FULL), 2 * kSoftmaxWarps);
         mbar_init(bar(B_PV_DONE), 1);
-        mbar_init(bar(B_Q_FULL), 2 * kQWarps);
+        mbar_init(bar(B_Q_FULL), 2);
         mbar_init(bar(B_Q_FREE), 1);
+        mbar_init(bar(B_Q_LAND), 1);
         mbar_init(bar(B_O_FREE), 2 * kSoftmaxWarps);
         mbar_init(bar(B_DRAIN), 1);
         mbar_fence_init();
@@ -626,7 +653,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         if (w->more) {
             QRows q;
             load_q(p, w->part, cta, warp, kWarps, q);
-            store_q(p, smem, reinterpret_cast<float*>(smem + SM_QS), warp, kWarps, q);
+            store_q(p, smem + SM_Q, reinterpret_cast<float*>(smem + SM_QS), warp, kWarps, q);
             fence_proxy_async_smem();
         }
     }
@@ -766,24 +793,43 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
     } else if (warp >= kQWarp0) {
         set_registers<kRegsQ>();
         // ============================================================ Q of each part
+        // The factors have four places: part k's are written once the last QK of part k - 2 is complete, so
+        // (S has two buffers) S of the tile two before it has been read, a tile of part k - 4 at the
+        // earliest, whose factors the softmax warps read before.
+        float* qs = reinterpret_cast<float*>(smem + SM_QS);
         int parts = 0;
 #pragma unroll 1
         while (next_part(p, work)) {
             if (t.n_tiles == 0) continue;
             if (parts > 0) {                     // (the first part's is there)
-                // the next rows on their way while some are converted, the first before the last part's QK is done
+                // Converted into the workspace while the last part runs, and copied from there once its last QK
+                // is done: converted only then, the MMAs waited 10,000 cycles a part for it.
+                uint8_t* scratch = p.q_scratch + static_cast<int64_t>(2 * pair + cta) * kQBytes;
                 QRows q;
                 load_q(p, t, cta, warp - kQWarp0, kQWarps, q);
-                wait_phase(bar(B_Q_FREE), (parts - 1) & 1, abort_flag, p.err);
 #pragma unroll 1
                 for (int r = warp - kQWarp0; r < kCtaRows; r += kQRows * kQWarps) {
                     const QRows now = q;
                     load_q(p, t, cta, r + kQRows * kQWarps, kQWarps, q);
-                    store_q(p, smem, reinterpret_cast<float*>(smem + SM_QS) + 64 * (parts & 1), r, kQWarps, now);
+                    store_q(p, scratch, qs + 64 * (parts & 3), r, kQWarps, now);
                 }
-                fence_proxy_async_smem();
+                __threadfence();
+                asm volatile("fence.proxy.async;" ::: "memory");
+                named_bar_sync(3, 32 * kQWarps);
+                wait_phase(bar(B_Q_FREE), (parts - 1) & 1, abort_flag, p.err);
+                if (warp == kQWarp0 && __all_sync(0xFFFFFFFFu, !*abort_flag)) {
+                    if (elect_one()) {
+                        const uint32_t bytes = k_stages * kCtaRows * 128;
+                        mbar_arrive_expect_tx(bar(B_Q_LAND), bytes);
+                        bulk_copy_g2s(sbase + SM_Q, scratch, bytes, bar(B_Q_LAND));
+                    }
+                    __syncwarp();
+                    mbar_drain_wait(bar(B_Q_LAND), (parts - 1) & 1);      // whatever else fails: the CTA does not exit under it
+                } else {
+                    wait_phase(bar(B_Q_LAND), (parts - 1) & 1, abort_flag, p.err);
+                }
+                if (warp == kQWarp0 && lane == 0) leader_arrive(bar(B_Q_FULL));
                 __syncwarp();
-                if (lane == 0) leader_arrive(bar(B_Q_FULL));
             }
             ++parts;
         }
@@ -799,14 +845,15 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         float* lsum = reinterpret_cast<float*>(smem + SM_LSUM);
         int parts = 0, tile = 0;                 // parts with tiles, and tiles, so far
         bool first_part = true;
+        look_ahead(p, work);
         griddep_wait();                          // the image kernel's token bits
 #pragma unroll 1
-        while (next_part(p, work)) {
+        while (advance_part(work)) {
             const int n_tiles = t.n_tiles, tile0 = t.tile0, image = t.image;
             int lim = 0;                                                      // tokens the row sees
             {
-                const int grow = t.block * kUnitRows + kCtaRows * cta + row;  // row of the sequence
-                if (grow < t.rows) lim = min(t.L, t.L - t.n + grow / p.heads + 1);
+                const int grow = t.block * kUnitRows + t.half * cta + row;    // row of the sequence
+                if (grow < t.rows && row < t.half) lim = min(t.L, t.L - t.n + grow / p.heads + 1);
             }
             float factor = 1.0f, m_ref = -INFINITY, l = 0.0f;
             // bits of the quarter's tokens that exist, and of those that hold a NaN, loaded a tile ahead
@@ -825,7 +872,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 const int see = lim - ((tile0 + i) * kTile + 64 * q4);     // tokens of the quarter the row sees
                 wait_phase(bar(B_S_FULL + (tile & 1)), (tile >> 1) & 1, abort_flag, p.err);
                 tc_fence_after();
-                if (i == 0) factor = reinterpret_cast<const float*>(smem + SM_QS)[64 * (parts & 1) + row];
+                if (i == 0) factor = reinterpret_cast<const float*>(smem + SM_QS)[64 * (parts & 3) + row];
                 float x[64];
                 tmem_ld32(tmem + kTS + 128 * (tile & 1) + 64 * ch + lanes, reinterpret_cast<uint32_t*>(x));
                 tmem_ld32(tmem + kTS + 128 * (tile & 1) + 64 * ch + 32 + lanes, reinterpret_cast<uint32_t*>(x) + 32);
@@ -889,6 +936,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 __syncwarp();
                 if (lane == 0) leader_arrive(bar(B_P_FULL));
             }
+            look_ahead(p, work);                        // (the last PV is running)
             // ---- epilogue: sums over the row's four warps, O out of TMEM
             named_bar_sync(1 + (sp & 1), 128);          // the last part's sums are read
             lsum[64 * q4 + row] = l;
@@ -897,19 +945,19 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             if (n_tiles > 0) wait_phase(bar(B_PV_DONE), (tile - 1) & 1, abort_flag, p.err);
             tc_fence_after();
             const bool any = l > 0.0f || l != l, whole = t.head && t.tail;
-            const int grow = t.block * kUnitRows + kCtaRows * cta + row;
-            const bool real = grow < t.rows;
+            const int unit_row = t.half * cta + row, grow = t.block * kUnitRows + unit_row;
+            const bool real = grow < t.rows && row < t.half;
             const int tok = real ? grow / p.heads : 0, head = grow - tok * p.heads;
-            const int64_t part_row = (2 * pair + (first_part ? 0 : 1)) * kUnitRows + kCtaRows * cta + row;
+            const int64_t part_row = (2 * pair + (first_part ? 0 : 1)) * kUnitRows + unit_row;
             const float mul = whole ? (any ? p.out_scale / l : 0.0f) : 1.0f;
-            if (q4 == 0) {
+            if (q4 == 0 && real) {
                 if (!whole)
                     *reinterpret_cast<float2*>(p.part_ml + 2 * part_row) = make_float2(m_ref, l);
-                else if (p.lse && real)
+                else if (p.lse)
                     p.lse[static_cast<int64_t>(t.first + tok) * p.heads + head] = any ? 0.69314718055994531f * (m_ref + log2f(l)) : -INFINITY;
             }
             if (!whole && threadIdx.x == 0 && cta == 0)
-                p.parts[2 * pair + (first_part ? 0 : 1)] = PartInfo{1, t.head, t.tail, t.first, t.n, t.block};
+                p.parts[2 * pair + (first_part ? 0 : 1)] = PartInfo{1, t.head, t.tail, 0, t.first, t.n, t.block, 0};
             // Two pieces a step, 16 dims of each as 32-byte stores by the lanes that hold the rows, the next two
             // on their way from tensor memory.  Rolled up: this code runs once per part, and unrolled its
             // instructions took longer to arrive than to run.  (Whole rows staged in shared memory and
@@ -978,81 +1026,105 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
 
 // Merges the parts of the units that a range's end cut: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s -
 // M) l_s.  blockIdx.x / 128 = a pair whose last part begins a unit; the others are the first parts
-// of the pairs after it, up to the one that ends the unit.  A block per row.
+// of the pairs after it, up to the one that ends the unit.  A block per row, bound by the latency of
+// three dependent loads (the parts' records, a pair per thread; their maxima; O): rows sharing a
+// block were no faster.
 __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_constant__ PrefillParams p) {
-    __shared__ float wts[kMaxPairs + 1];
-    __shared__ float red[2][4];
-    __shared__ int last;
+    static_assert(kMaxPairs <= 128, "a pair per thread");
+    __shared__ uint32_t used_bits[4], tail_bits[4];
+    __shared__ PartInfo head;
+    __shared__ int head_part, count_s, parts[kMaxPairs + 1];
+    __shared__ float wts[kMaxPairs + 1], red[2][4];
+    const int pair = blockIdx.x / kUnitRows, r = blockIdx.x % kUnitRows, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     griddep_wait();
-    const int pair = blockIdx.x / kUnitRows, r = blockIdx.x % kUnitRows, tid = threadIdx.x, lane = tid & 31;
-    const int at = p.parts[2 * pair + 1].used ? 1 : 0;
-    const PartInfo h = p.parts[2 * pair + at];
-    if (!h.used || !h.head || h.tail) return;
-    const int row = h.block * kUnitRows + r;
-    if (row >= h.n * p.heads) return;
-    if (tid == 0) last = kMaxPairs;
-    __syncthreads();
-    // part 0: the head; part 1 + k: the first one of pair + 1 + k
-    if (pair + 1 + tid < p.pairs) {
-        const PartInfo& q = p.parts[2 * (pair + 1 + tid)];
-        if (q.used && q.tail) atomicMin(&last, tid);
+    int4 flags = make_int4(0, 0, 0, 0);      // used, head, tail of a later pair's first part
+    if (tid > pair && tid < p.pairs) flags = *reinterpret_cast<const int4*>(p.parts + 2 * tid);
+    const bool used = flags.x != 0;
+    const uint32_t ub = __ballot_sync(0xFFFFFFFFu, used), tb = __ballot_sync(0xFFFFFFFFu, used && flags.z);
+    if (lane == 0) {
+        used_bits[warp] = ub;
+        tail_bits[warp] = tb;
+    }
+    if (tid == pair) {
+        const PartInfo a = p.parts[2 * pair], b = p.parts[2 * pair + 1];
+        head = b.used ? b : a;
+        head_part = 2 * pair + (b.used ? 1 : 0);
+        count_s = 0;
     }
     __syncthreads();
-    const int count = min(last + 2, p.pairs - pair);
-    auto ml_of = [&](int k) {      // (a pair whose range is empty has no part)
-        const int64_t part = k == 0 ? 2 * pair + at : 2 * (pair + k);
-        if (!p.parts[part].used) return make_float2(-INFINITY, 0.0f);
-        return *reinterpret_cast<const float2*>(p.part_ml + 2 * (part * kUnitRows + r));
-    };
-    float m = -INFINITY;
-    for (int k = tid; k < count; k += 128) {
-        const float2 v = ml_of(k);
-        if (v.y > 0.0f || v.y != v.y) m = fmaxf(m, v.x);
+    if (!head.used || !head.head || head.tail) return;
+    const int row = head.block * kUnitRows + r;
+    if (row >= head.n * p.heads) return;
+    // part 0: the head; then the used first parts up to the first that ends the unit (a pair whose
+    // range is empty has none)
+    bool after_tail = false;
+    int rank = 1;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const uint32_t below = w < warp ? 0xFFFFFFFFu : w == warp ? (1u << lane) - 1u : 0u;
+        after_tail |= (tail_bits[w] & below) != 0;
+        rank += __popc(used_bits[w] & below);
     }
+    const bool mine = used && !after_tail;
+    if (mine) parts[rank] = 2 * tid;
+    if (mine && flags.z) count_s = rank + 1;
+    if (tid == 0) parts[0] = head_part;
+    __syncthreads();
+    // (without a tail, after a timed-out wait, all there are)
+    const int count = count_s > 0 ? count_s : 1 + __popc(used_bits[0]) + __popc(used_bits[1]) + __popc(used_bits[2]) + __popc(used_bits[3]);
+    auto ml_of = [&](int k) { return *reinterpret_cast<const float2*>(p.part_ml + 2 * (static_cast<int64_t>(parts[k]) * kUnitRows + r)); };
+    float2 ml = make_float2(-INFINITY, 0.0f), ml2 = ml;
+    if (tid < count) ml = ml_of(tid);
+    if (tid + 128 < count) ml2 = ml_of(tid + 128);
+    const bool some = ml.y > 0.0f || ml.y != ml.y, some2 = ml2.y > 0.0f || ml2.y != ml2.y;
+    float m = fmaxf(some ? ml.x : -INFINITY, some2 ? ml2.x : -INFINITY);
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    if (lane == 0) red[0][tid >> 5] = m;
+    if (lane == 0) red[0][warp] = m;
     __syncthreads();
     m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    float l = 0.0f;
-    for (int k = tid; k < count; k += 128) {
-        const float2 v = ml_of(k);
-        const float w = v.y > 0.0f || v.y != v.y ? exp2f(v.x - m) : 0.0f;
-        wts[k] = w;
-        if (w != 0.0f) l += w * v.y;
-    }
+    const float w = some ? exp2f(ml.x - m) : 0.0f, w2 = some2 ? exp2f(ml2.x - m) : 0.0f;
+    if (tid < count) wts[tid] = w;
+    if (tid + 128 < count) wts[tid + 128] = w2;
+    float l = (w != 0.0f ? w * ml.y : 0.0f) + (w2 != 0.0f ? w2 * ml2.y : 0.0f);
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
-    if (lane == 0) red[1][tid >> 5] = l;
+    if (lane == 0) red[1][warp] = l;
     __syncthreads();
     l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
     const bool any = l > 0.0f || l != l;
     const float inv = any ? p.out_scale / l : 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int k = 0; k < count; ++k) {
-        const float w = wts[k];
-        if (w != 0.0f) {      // a part that saw no token wrote no O
-            const int64_t part = k == 0 ? 2 * pair + at : 2 * (pair + k);
-            const float4 v = *reinterpret_cast<const float4*>(p.part_o + (part * kUnitRows + r) * kLatent + 4 * tid);
-            acc.x = fmaf(w, v.x, acc.x);
-            acc.y = fmaf(w, v.y, acc.y);
-            acc.z = fmaf(w, v.z, acc.z);
-            acc.w = fmaf(w, v.w, acc.w);
+    for (int k0 = 0; k0 < count; k0 += 4) {
+        float4 v[4];
+        float wk[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            wk[k] = k0 + k < count ? wts[k0 + k] : 0.0f;
+            v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (wk[k] != 0.0f)      // (a part that saw no token wrote no O)
+                v[k] = *reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(parts[k0 + k]) * kUnitRows + r) * kLatent + 4 * tid);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            acc.x = fmaf(wk[k], v[k].x, acc.x);
+            acc.y = fmaf(wk[k], v[k].y, acc.y);
+            acc.z = fmaf(wk[k], v[k].z, acc.z);
+            acc.w = fmaf(wk[k], v[k].w, acc.w);
         }
     }
     const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-    const int tok = row / p.heads, head = row - tok * p.heads;
-    *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(h.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh + 4 * tid) =
+    const int tok = row / p.heads, h = row - tok * p.heads;
+    *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(head.first + tok) * p.o_st + static_cast<int64_t>(h) * p.o_sh + 4 * tid) =
         make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
     if (p.lse && tid == 0)
-        p.lse[static_cast<int64_t>(h.first + tok) * p.heads + head] = any ? 0.69314718055994531f * (m + log2f(l)) : -INFINITY;
+        p.lse[static_cast<int64_t>(head.first + tok) * p.heads + h] = any ? 0.69314718055994531f * (m + log2f(l)) : -INFINITY;
 }
 
 struct PrefillPlan {
     int group;               // sequences per pass over the workspace
     int pairs, image_blocks;
-    size_t image_bytes, bits_bytes, o_bytes, ml_bytes, ws_bytes;
+    size_t image_bytes, bits_bytes, q_bytes, o_bytes, ml_bytes, ws_bytes;
 };
 
 // Images take at most this, or one sequence's; a larger batch runs in groups of sequences.
@@ -1081,7 +1153,8 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
     pl.bits_bytes = round256(static_cast<size_t>(blocks) * 32);
     pl.o_bytes = static_cast<size_t>(pl.pairs) * 2 * kUnitRows * kLatent * sizeof(float);
     pl.ml_bytes = static_cast<size_t>(pl.pairs) * 2 * kUnitRows * 2 * sizeof(float);
-    pl.ws_bytes = pl.image_bytes + pl.bits_bytes + pl.o_bytes + pl.ml_bytes + round256(static_cast<size_t>(pl.pairs) * 2 * sizeof(PartInfo));
+    pl.q_bytes = static_cast<size_t>(pl.pairs) * 2 * kQBytes;
+    pl.ws_bytes = pl.image_bytes + pl.bits_bytes + pl.q_bytes + pl.o_bytes + pl.ml_bytes + round256(static_cast<size_t>(pl.pairs) * 2 * sizeof(PartInfo));
     return pl;
 }
 
@@ -1157,7 +1230,8 @@ extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     p.image = ws;
     p.image_bits = reinterpret_cast<uint32_t*>(ws += pl.image_bytes);
-    p.part_o = reinterpret_cast<float*>(ws += pl.bits_bytes);
+    p.q_scratch = ws += pl.bits_bytes;
+    p.part_o = reinterpret_cast<float*>(ws += pl.q_bytes);
     p.part_ml = reinterpret_cast<float*>(ws += pl.o_bytes);
     p.parts = reinterpret_cast<PartInfo*>(ws += pl.ml_bytes);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
