@@ -123,8 +123,9 @@ constexpr int kRopeSteps = 2;
 // A unit is a 16-byte vector of a head (a rotated one of the half layout: the pair of vectors that
 // turn together).  The units of the call are dealt flat, two to a thread and 256 apart: every warp
 // moves 512 contiguous bytes, every block is full, and two loads in flight per thread are enough at
-// the occupancy that leaves (8,192 tokens x 64 heads x 576 bf16, 1.2 GB: 176 us against 203 with one
-// and 178 with four; 225 with blocks of whole heads, whose last steps are part empty).
+// the occupancy that leaves (8,192 tokens x 64 heads x 576 bf16, 1.2 GB: 188 us = 6.4 TB/s, as much
+// as a plain copy; 8 % more with one, 1 % more with four, 20 % more with blocks of whole heads, whose
+// last steps are part empty).  The gradient of 2,049 tokens x 32 heads x 128 fp32 takes 12 us.
 template <typename T, bool kInterleaved>
 __global__ void __launch_bounds__(256, kInterleaved && sizeof(T) == 2 ? 8 : 4) rope_vec_kernel(const __grid_constant__ RopeArgs p) {
     constexpr int N = Vec<T>::kN;
@@ -268,10 +269,16 @@ struct RopeAppendArgs {
     int32_t* err;
 };
 
-// 8 bf16, as one 16-byte access or element by element.
+// 8 bf16, as one 16-byte access or element by element.  The accesses are marked as streaming: a step's
+// rows pass once, while the table rows of its positions come back with every layer, and should stay
+// in L2 (32,768 tokens x 16 heads over a table of 77 MB: 28.0 us against 33.3 without the marks, and
+// 29.8 with the next blocks' table rows prefetched instead).
 template <bool kVec> __device__ __forceinline__ Vec<__nv_bfloat16> get8(const __nv_bfloat16* p) {
     if constexpr (kVec) {
-        return load_vec(p);
+        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
+        Vec<__nv_bfloat16> r;
+        memcpy(&r, &u, 16);
+        return r;
     } else {
         Vec<__nv_bfloat16> r;
 #pragma unroll
@@ -281,7 +288,9 @@ template <bool kVec> __device__ __forceinline__ Vec<__nv_bfloat16> get8(const __
 }
 template <bool kVec> __device__ __forceinline__ void put8(__nv_bfloat16* p, const Vec<__nv_bfloat16>& r) {
     if constexpr (kVec) {
-        store_vec(p, r);
+        uint4 u;
+        memcpy(&u, &r, 16);
+        __stcs(reinterpret_cast<uint4*>(p), u);
     } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) p[k] = r.v[k];
@@ -289,7 +298,9 @@ template <bool kVec> __device__ __forceinline__ void put8(__nv_bfloat16* p, cons
 }
 
 // The units (8 dims of a row, half layout: 8 and their partners) of all rows, dealt flat as in
-// rope_vec_kernel; a token's rows are its key and the heads of its query.
+// rope_vec_kernel, two a thread (37.7 us with one, 42 with four, before the streaming marks); a
+// token's rows are its key and the heads of its query.  What bounds it is the latency of a block's
+// three dependent accesses (position, table row, store) at full occupancy, then HBM.
 template <bool kInterleaved, bool kVec>
 __global__ void __launch_bounds__(256) rope_append_rotated_kernel(const __grid_constant__ RopeAppendArgs p) {
     using V = Vec<__nv_bfloat16>;
