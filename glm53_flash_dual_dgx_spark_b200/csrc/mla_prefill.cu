@@ -72,6 +72,8 @@ static_assert(256 * kRegsSoftmax + 128 * kRegsQ + 128 * kRegsCtl <= kThreads * k
 constexpr float kRescaleLog2 = 8.0f;
 constexpr int kMaxPairs = 128;
 constexpr int kImageTok = 128;                  // tokens of an image block
+constexpr int kImageRows = 1;                   // rows of a thread of the image kernel
+constexpr int kImagePieces = kImageTok / (32 * kImageRows);
 
 constexpr int kQBytes = 9 * kCtaRows * 128;
 constexpr int SM_Q = 0;                                      // 9 dim atoms x [64 rows x 128 B]
@@ -437,13 +439,14 @@ __device__ __forceinline__ uint4 dequant8(uint32_t code, uint32_t scale2) {
 // code bytes), a thread writes its 32 dims as 16 bytes to each of four atoms, a warp whole 128-byte
 // rows; all of a block's loads are in flight before the first is used.
 // The blocks of the grid take the image's in turn (their number is on the device).
-__global__ void __launch_bounds__(256) prefill_image_kernel(const __grid_constant__ PrefillParams p) {
-    __shared__ uint32_t bits[8];
+__global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_constant__ PrefillParams p) {
+    __shared__ uint32_t bits[2 * kImageRows];
     __shared__ int b_s, pos_s, total_s;
     griddep_launch_dependents();
     const int tid = threadIdx.x, lp = tid & 7, r0 = tid >> 3;
     int total = 0x7FFFFFFF;
     for (int item = blockIdx.x; item < total; item += gridDim.x) {
+        const int block = item / kImagePieces, piece = item % kImagePieces;
         if (tid < 32) {
             const int lane = tid;
             int base = 0, b = -1, pos = 0;
@@ -451,11 +454,11 @@ __global__ void __launch_bounds__(256) prefill_image_kernel(const __grid_constan
                 int blocks = 0;
                 if (b0 + lane < p.batch) blocks = image_blocks_of(load_seq(p, b0 + lane));
                 const int upto = base + warp_inclusive_sum(blocks, lane);
-                const uint32_t hit = __ballot_sync(0xFFFFFFFFu, item < upto);
+                const uint32_t hit = __ballot_sync(0xFFFFFFFFu, block < upto);
                 if (hit && b < 0) {
                     const int src = __ffs(hit) - 1;
                     b = b0 + src;
-                    pos = kImageTok * (item - __shfl_sync(0xFFFFFFFFu, upto - blocks, src));
+                    pos = kImageTok * (block - __shfl_sync(0xFFFFFFFFu, upto - blocks, src)) + 32 * kImageRows * piece;
                 }
                 base = __shfl_sync(0xFFFFFFFFu, upto, 31);
             }
@@ -464,20 +467,20 @@ __global__ void __launch_bounds__(256) prefill_image_kernel(const __grid_constan
                 pos_s = pos;
                 total_s = base;
             }
-            if (lane < 8) bits[lane] = 0;
+            if (lane < 2 * kImageRows) bits[lane] = 0;
         }
         __syncthreads();
         if (b_s < 0) return;
-        total = total_s;
+        total = total_s * kImagePieces;
         const int L = load_seq(p, b_s).L;
         const int32_t* table = p.tables + b_s * p.tables_stride;
-        int64_t row[4];
-        uint4 code[4][2], rope[4];
-        uint16_t scale[4][2];
+        int64_t row[kImageRows];
+        uint4 code[kImageRows][2], rope[kImageRows];
+        uint16_t scale[kImageRows][2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) row[k] = pool_row(p, table, pos_s + r0 + 32 * k, L);
+        for (int k = 0; k < kImageRows; ++k) row[k] = pool_row(p, table, pos_s + r0 + 32 * k, L);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < kImageRows; ++k) {
             rope[k] = code[k][0] = code[k][1] = make_uint4(0, 0, 0, 0);
             scale[k][0] = scale[k][1] = 0;
             if (row[k] >= 0) {
@@ -491,9 +494,9 @@ __global__ void __launch_bounds__(256) prefill_image_kernel(const __grid_constan
             }
         }
         const int atoms = p.rope ? 9 : 8;
-        uint8_t* dst = p.image + static_cast<int64_t>(item) * atoms * kStageBytes + r0 * 128 + ((lp ^ (r0 & 7)) << 4);
+        uint8_t* dst = p.image + static_cast<int64_t>(block) * atoms * kStageBytes + piece * (4096 * kImageRows) + r0 * 128 + ((lp ^ (r0 & 7)) << 4);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < kImageRows; ++k) {
             const int t = r0 + 32 * k;
             uint32_t nan = 0;
 #pragma unroll
@@ -509,14 +512,15 @@ __global__ void __launch_bounds__(256) prefill_image_kernel(const __grid_constan
                 }
             }
             if (p.rope) *reinterpret_cast<uint4*>(dst + 8 * kStageBytes + 4096 * k) = rope[k];
-            if (nan) atomicOr(&bits[4 + k], 1u << (t & 31));
+            if (nan) atomicOr(&bits[kImageRows + k], 1u << (t & 31));
             if (lp == 0) {
                 if (row[k] >= 0) atomicOr(&bits[k], 1u << (t & 31));
                 else if (pos_s + t < L) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
             }
         }
         __syncthreads();
-        if (tid < 8) p.image_bits[8 * static_cast<int64_t>(item) + tid] = bits[tid];
+        if (tid < 2 * kImageRows)
+            p.image_bits[8 * static_cast<int64_t>(block) + 4 * (tid / kImageRows) + kImageRows * piece + tid % kImageRows] = bits[tid];
         __syncthreads();      // (the next item's words)
     }
 }
@@ -1246,7 +1250,7 @@ extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_
         cudaError_t e = cudaSuccess;
         if (pl.image_blocks > 0) {
             const int most = 8 * device_sm_count();
-            prefill_image_kernel<<<pl.image_blocks < most ? pl.image_blocks : most, 256, 0, st>>>(p);
+            prefill_image_kernel<<<kImagePieces * pl.image_blocks < most ? kImagePieces * pl.image_blocks : most, 256, 0, st>>>(p);
             if ((rc = check_launch("nvfp4kv_mla_prefill image")) != NVFP4KV_OK) return rc;
             // its set-up overlaps the image kernel; all else it reads was there before that one
             e = launch_dependent(mla_prefill_kernel, grid, dim3(kThreads), kSmemBytes, st, p);
