@@ -132,7 +132,7 @@ struct PrefillParams {
     float* lse;
     PartInfo* parts;    // [pairs][2]: the range's first part of a unit, and its last one
     float* part_ml;     // [pairs][2][128][2]: maximum (log2 units), sum
-    float* part_o;      // [pairs][2][128][512]
+    float* part_o;      // [pairs][2][64 chunks of 8 dims][128 rows][8]
     uint8_t* q_scratch; // [pairs][2 CTAs][kQBytes]: the next part's Q
     uint8_t* image;     // [blocks][8 or 9 atoms][128 tokens x 128 B]
     uint32_t* image_bits;   // [blocks][8]: 128 bits of tokens that exist, 128 of those that hold a NaN
@@ -274,7 +274,14 @@ __device__ __forceinline__ Range find_range(const PrefillParams& p, int pair) {
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
-    const int64_t lo = total * pair / p.pairs, hi = total * (pair + 1) / p.pairs;
+    int64_t lo, hi;
+    if (total <= 0xFFFFFFFFll / kMaxPairs) {      // (64-bit divisions take hundreds of cycles)
+        lo = static_cast<uint32_t>(total) * pair / p.pairs;
+        hi = static_cast<uint32_t>(total) * (pair + 1) / p.pairs;
+    } else {
+        lo = total * pair / p.pairs;
+        hi = total * (pair + 1) / p.pairs;
+    }
     Range r{hi - lo, 0, 0, 0, 0};
     if (hi <= lo) return r;
     int64_t before = 0;
@@ -614,15 +621,19 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         const Range r = find_range(p, pair);
         if (lane == 0) {
             flags[1] = 0;
-            for (int k = 0; k < kThreads / 32; ++k) reinterpret_cast<Work*>(smem + SM_WORK + k * kWorkBytes)->range = r;
-            // the range's first part with tiles, whose Q all warps load now
+            // the range's first part, for every warp, and in `part` the first one with tiles: its Q and
+            // its first stages are fetched before the roles begin
             Work* w = reinterpret_cast<Work*>(smem + SM_WORK + kThreads / 32 * kWorkBytes);
-            Range r1 = r;
-            Part t1;
-            bool more = next_part_of(p, r1, t1);
-            while (more && t1.n_tiles == 0) more = next_part_of(p, r1, t1);
+            Range r0 = r;
+            Part t0;
+            const bool more = next_part_of(p, r0, t0);
+            w->range = r0;
             w->more = more;
-            w->part = t1;
+            if (more) w->ahead = t0;
+            bool tiles = more && t0.n_tiles > 0;
+            while (more && !tiles && next_part_of(p, r0, t0)) tiles = t0.n_tiles > 0;
+            if (!tiles) t0.n_tiles = 0;
+            w->part = t0;
             if (cta == 0) p.parts[2 * pair].used = p.parts[2 * pair + 1].used = 0;
         }
     }
@@ -648,24 +659,60 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
     __syncthreads();
     Work* work = reinterpret_cast<Work*>(smem + SM_WORK + warp * kWorkBytes);
     const volatile Part& t = work->part;
-    if (reinterpret_cast<volatile Work*>(work)->range.left <= 0) return;       // nothing for this pair: the whole cluster
-    if (warp == kMmaWarp) pair_tmem_alloc(sbase + SM_FLAGS, kTmemCols);
+    const Work* first = reinterpret_cast<const Work*>(smem + SM_WORK + kThreads / 32 * kWorkBytes);
+    if (!first->more) {               // nothing for this pair: the whole cluster
+        griddep_wait();               // (this grid ends after the image kernel)
+        return;
+    }
     {
-        const Work* w = reinterpret_cast<const Work*>(smem + SM_WORK + kThreads / 32 * kWorkBytes);
+        static_assert(sizeof(Work) % 4 == 0 && sizeof(Work) <= 256, "two words per lane");
+        for (int k = lane; k < static_cast<int>(sizeof(Work) / 4); k += 32)
+            reinterpret_cast<int*>(work)[k] = reinterpret_cast<const int*>(first)[k];
+    }
+    if (warp == kMmaWarp) pair_tmem_alloc(sbase + SM_FLAGS, kTmemCols);
+    const int k_stages = p.rope ? 9 : 8;
+    // A stage of a part's ring: K stage c.s of tile c.i, or V stage c.s - k_stages of tile c.i - 1.
+    const int64_t image_bytes = static_cast<int64_t>(k_stages) * kStageBytes;
+    auto copy_stage = [&](const Cursor& c, int image, int last, int tile0, int slot) {
+        const uint32_t dst = sbase + SM_RING + slot * kStageBytes, landed = bar(B_LAND + slot);
+        if (elect_one()) {
+            mbar_arrive_expect_tx(landed, kStageBytes);
+            if (c.s < k_stages) {
+                const int blk = min(image + 2 * (tile0 + c.i) + cta, last);
+                bulk_copy_g2s(dst, p.image + blk * image_bytes + c.s * kStageBytes, kStageBytes, landed);
+            } else {
+                const int v = c.s - k_stages;      // tokens 64 (v / 2) .., dim atoms 4 c + 2 (v % 2), + 1
+                const int blk = min(image + 2 * (tile0 + c.i - 1) + (v >> 2), last);
+                const uint8_t* src = p.image + blk * image_bytes + (4 * cta + 2 * (v & 1)) * kStageBytes + ((v >> 1) & 1) * 8192;
+                bulk_copy_g2s(dst, src, 8192, landed);
+                bulk_copy_g2s(dst + 8192, src + kStageBytes, 8192, landed);
+            }
+        }
+        __syncwarp();
+    };
+    auto last_block = [&](int image, int L) { return image + (L + kImageTok - 1) / kImageTok - 1; };      // (tokens past it are masked)
+    int early = 0;                    // stages copied before the roles begin
+    if (first->part.n_tiles > 0) {
+        const Part& t1 = first->part;
+        QRows q;
         constexpr int kWarps = kThreads / 32;
         static_assert(kWarps * kQRows == kCtaRows, "one round of rows");
-        if (w->more) {
-            QRows q;
-            load_q(p, w->part, cta, warp, kWarps, q);
-            store_q(p, smem + SM_Q, reinterpret_cast<float*>(smem + SM_QS), warp, kWarps, q);
-            fence_proxy_async_smem();
+        load_q(p, t1, cta, warp, kWarps, q);
+        if (warp == kCopyWarp0 || warp == kCopyWarp0 + 1) {
+            griddep_wait();           // the image kernel's writes
+            early = kStages;          // (a tile has more)
+            static_assert(kStages < 8 + kVStages, "stages of one tile");
+            Cursor c{0, 0, 0};
+            for (int u = 0; u < kStages; ++u, advance(c, k_stages, t1.n_tiles))
+                if ((u & 1) == warp - kCopyWarp0) copy_stage(c, t1.image, last_block(t1.image, t1.L), t1.tile0, u);
         }
+        store_q(p, smem + SM_Q, reinterpret_cast<float*>(smem + SM_QS), warp, kWarps, q);
+        fence_proxy_async_smem();
     }
     tc_fence_before();
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem = static_cast<uint32_t>(flags[0]);
-    const int k_stages = p.rope ? 9 : 8;
 
     if (warp >= kMmaWarp) {
         set_registers<kRegsCtl>();
@@ -685,7 +732,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                     }
                 };
 #pragma unroll 1
-                while (next_part(p, work) && !*abort_flag) {
+                for (bool more = advance_part(work); more && !*abort_flag; more = next_part(p, work)) {
                     const int n_tiles = t.n_tiles;
                     if (n_tiles == 0) continue;
                     if (parts > 0) mbar_wait(bar(B_Q_FULL), (parts - 1) & 1, abort_flag, p.err);
@@ -744,7 +791,6 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         } else {
             // ======================================================== image copies and their relay
             // Two warps take the stages in turn, a third hands each landed stage to the leader.
-            const int64_t image_bytes = static_cast<int64_t>(k_stages) * kStageBytes;
             const bool relay = warp == kRelayWarp;
             const int mine = warp - kCopyWarp0;
             int u = 0, slot = 0;                  // stage number and its ring slot
@@ -752,9 +798,9 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             bool ok = true;
             griddep_wait();                       // the image kernel's writes
 #pragma unroll 1
-            while (ok && next_part(p, work)) {
+            for (bool more = advance_part(work); ok && more; more = next_part(p, work)) {
                 const int n_tiles = t.n_tiles, total = n_tiles * (k_stages + kVStages), image = t.image, tile0 = t.tile0;
-                const int last = image + (t.L + kImageTok - 1) / kImageTok - 1;      // (tokens past it are masked)
+                const int last = last_block(image, t.L);
                 Cursor c{0, 0, 0};
 #pragma unroll 1
                 for (; c.u < total; advance(c, k_stages, n_tiles)) {
@@ -762,25 +808,11 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                         if (!(ok = mbar_wait(bar(B_LAND + slot), phase, abort_flag, p.err))) break;
                         if (lane == 0) leader_arrive(bar(B_FULL + slot));
                         __syncwarp();
-                    } else if ((u & 1) == mine) {
+                    } else if ((u & 1) == mine && u >= early) {
                         // (a release waited for by the other warp in between is earlier than this one's: no
                         // phase is skipped unseen)
                         if (u >= kStages && !(ok = mbar_wait(bar(B_EMPTY + slot), phase ^ 1, abort_flag, p.err))) break;
-                        const uint32_t dst = sbase + SM_RING + slot * kStageBytes, landed = bar(B_LAND + slot);
-                        if (elect_one()) {
-                            mbar_arrive_expect_tx(landed, kStageBytes);
-                            if (c.s < k_stages) {
-                                const int blk = min(image + 2 * (tile0 + c.i) + cta, last);
-                                bulk_copy_g2s(dst, p.image + blk * image_bytes + c.s * kStageBytes, kStageBytes, landed);
-                            } else {
-                                const int v = c.s - k_stages;      // tokens 64 (v / 2) .., dim atoms 4 c + 2 (v % 2), + 1
-                                const int blk = min(image + 2 * (tile0 + c.i - 1) + (v >> 2), last);
-                                const uint8_t* src = p.image + blk * image_bytes + (4 * cta + 2 * (v & 1)) * kStageBytes + ((v >> 1) & 1) * 8192;
-                                bulk_copy_g2s(dst, src, 8192, landed);
-                                bulk_copy_g2s(dst + 8192, src + kStageBytes, 8192, landed);
-                            }
-                        }
-                        __syncwarp();
+                        copy_stage(c, image, last, tile0, slot);
                     }
                     ++u;
                     if (++slot == kStages) {
@@ -792,7 +824,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             // Every copy has landed once the MMAs that read it are done; after a timed-out wait the ones in
             // flight (the stages before u) are awaited here, so that the CTA does not exit under them.
             if (!relay && *abort_flag)
-                for (int k = max(0, u - kStages); k < u; ++k) mbar_drain_wait(bar(B_LAND + k % kStages), (k / kStages) & 1);
+                for (int k = max(0, max(u, early) - kStages); k < max(u, early); ++k) mbar_drain_wait(bar(B_LAND + k % kStages), (k / kStages) & 1);
         }
     } else if (warp >= kQWarp0) {
         set_registers<kRegsQ>();
@@ -803,7 +835,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         float* qs = reinterpret_cast<float*>(smem + SM_QS);
         int parts = 0;
 #pragma unroll 1
-        while (next_part(p, work)) {
+        for (bool more = advance_part(work); more; more = next_part(p, work)) {
             if (t.n_tiles == 0) continue;
             if (parts > 0) {                     // (the first part's is there)
                 // Converted into the workspace while the last part runs, and copied from there once its last QK
@@ -849,7 +881,6 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         float* lsum = reinterpret_cast<float*>(smem + SM_LSUM);
         int parts = 0, tile = 0;                 // parts with tiles, and tiles, so far
         bool first_part = true;
-        look_ahead(p, work);
         griddep_wait();                          // the image kernel's token bits
 #pragma unroll 1
         while (advance_part(work)) {
@@ -967,7 +998,8 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             // instructions took longer to arrive than to run.  (Whole rows staged in shared memory and
             // stored by warps were no faster.)
             __nv_bfloat16* out = p.out + static_cast<int64_t>(t.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh + 256 * (sp >> 1) + 16 * ch;
-            float* part_o = p.part_o + part_row * kLatent + 256 * (sp >> 1) + 16 * ch;
+            // (chunk 8 (dim / 8) by chunk: a warp's 32 rows are 1 KB together; as rows they took 7 K cycles)
+            float* part_o = p.part_o + (static_cast<int64_t>(2 * pair + (first_part ? 0 : 1)) * 64 + 32 * (sp >> 1) + 2 * ch) * (8 * kUnitRows) + 8 * unit_row;
             const bool wide = (reinterpret_cast<uintptr_t>(p.out) % 32 == 0) && p.o_st % 16 == 0 && p.o_sh % 16 == 0;
             const uint32_t o_addr = tmem + kTO + 128 * ch + lanes;
             uint32_t ahead_o[2][16];      // columns 8 j .. + 16 (dims a = 0 of pieces j, j + 1) and 64 + 8 j .. (a = 1)
@@ -1007,8 +1039,8 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                                 *reinterpret_cast<uint4*>(dst + 8) = make_uint4(w[4], w[5], w[6], w[7]);
                             }
                         } else if (any) {
-                            st_global_v8(part_o + 32 * (j + h), &o[0][8 * h]);
-                            st_global_v8(part_o + 32 * (j + h) + 8, &o[1][8 * h]);
+                            st_global_v8(part_o + 4 * (j + h) * (8 * kUnitRows), &o[0][8 * h]);
+                            st_global_v8(part_o + (4 * (j + h) + 1) * (8 * kUnitRows), &o[1][8 * h]);
                         }
                     }
                 }
@@ -1029,17 +1061,21 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
 }
 
 // Merges the parts of the units that a range's end cut: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s -
-// M) l_s.  blockIdx.x / 128 = a pair whose last part begins a unit; the others are the first parts
-// of the pairs after it, up to the one that ends the unit.  A block per row, bound by the latency of
-// three dependent loads (the parts' records, a pair per thread; their maxima; O): rows sharing a
-// block were no faster.
+// M) l_s.  A pair whose last part begins a unit has 32 row groups x 4 / kQ blocks here; the unit's
+// other parts are the first ones of the pairs after it, up to the one that ends it.  A block takes 4
+// rows x 128 kQ dims, so that the chunks it reads are whole 128-byte lines; it is bound by the latency
+// of three dependent loads (the parts' records, a pair per thread; their maxima, a row per warp; O).
+// kQ = 4 where there are many pairs (8 chunks of new tokens, 74 pairs: 11.5 us against 18.5), kQ = 1
+// where four times the blocks find idle SMs (12 pairs: 4.1 against 5.4).
+template <int kQ>
 __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_constant__ PrefillParams p) {
     static_assert(kMaxPairs <= 128, "a pair per thread");
     __shared__ uint32_t used_bits[4], tail_bits[4];
     __shared__ PartInfo head;
     __shared__ int head_part, count_s, parts[kMaxPairs + 1];
-    __shared__ float wts[kMaxPairs + 1], red[2][4];
-    const int pair = blockIdx.x / kUnitRows, r = blockIdx.x % kUnitRows, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ float wts[kMaxPairs + 1][4], invs[4];
+    const int pair = blockIdx.x / (kUnitRows / kQ), row0 = blockIdx.x % (kUnitRows / kQ) / (4 / kQ) * 4, dim0 = blockIdx.x % (4 / kQ) * 128 * kQ;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     griddep_wait();
     int4 flags = make_int4(0, 0, 0, 0);      // used, head, tail of a later pair's first part
     if (tid > pair && tid < p.pairs) flags = *reinterpret_cast<const int4*>(p.parts + 2 * tid);
@@ -1057,8 +1093,8 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_const
     }
     __syncthreads();
     if (!head.used || !head.head || head.tail) return;
-    const int row = head.block * kUnitRows + r;
-    if (row >= head.n * p.heads) return;
+    const int unit_row = head.block * kUnitRows + row0, rows = head.n * p.heads;
+    if (unit_row >= rows) return;
     // part 0: the head; then the used first parts up to the first that ends the unit (a pair whose
     // range is empty has none)
     bool after_tail = false;
@@ -1076,53 +1112,78 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_const
     __syncthreads();
     // (without a tail, after a timed-out wait, all there are)
     const int count = count_s > 0 ? count_s : 1 + __popc(used_bits[0]) + __popc(used_bits[1]) + __popc(used_bits[2]) + __popc(used_bits[3]);
-    auto ml_of = [&](int k) { return *reinterpret_cast<const float2*>(p.part_ml + 2 * (static_cast<int64_t>(parts[k]) * kUnitRows + r)); };
-    float2 ml = make_float2(-INFINITY, 0.0f), ml2 = ml;
-    if (tid < count) ml = ml_of(tid);
-    if (tid + 128 < count) ml2 = ml_of(tid + 128);
-    const bool some = ml.y > 0.0f || ml.y != ml.y, some2 = ml2.y > 0.0f || ml2.y != ml2.y;
-    float m = fmaxf(some ? ml.x : -INFINITY, some2 ? ml2.x : -INFINITY);
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    if (lane == 0) red[0][warp] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    const float w = some ? exp2f(ml.x - m) : 0.0f, w2 = some2 ? exp2f(ml2.x - m) : 0.0f;
-    if (tid < count) wts[tid] = w;
-    if (tid + 128 < count) wts[tid + 128] = w2;
-    float l = (w != 0.0f ? w * ml.y : 0.0f) + (w2 != 0.0f ? w2 * ml2.y : 0.0f);
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
-    if (lane == 0) red[1][warp] = l;
-    __syncthreads();
-    l = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-    const bool any = l > 0.0f || l != l;
-    const float inv = any ? p.out_scale / l : 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k0 = 0; k0 < count; k0 += 4) {
-        float4 v[4];
-        float wk[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            wk[k] = k0 + k < count ? wts[k0 + k] : 0.0f;
-            v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (wk[k] != 0.0f)      // (a part that saw no token wrote no O)
-                v[k] = *reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(parts[k0 + k]) * kUnitRows + r) * kLatent + 4 * tid);
+    {
+        // a row per warp: its weights, and what divides it
+        const int row = unit_row + warp;
+        const int n = row < rows ? count : 0;
+        auto ml_of = [&](int i) { return *reinterpret_cast<const float2*>(p.part_ml + 2 * (static_cast<int64_t>(parts[i]) * kUnitRows + row0 + warp)); };
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
+        for (int i = lane; i < n; i += 32) {
+            const float2 ml = ml_of(i);
+            if (ml.y > 0.0f || ml.y != ml.y) m = fmaxf(m, ml.x);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            acc.x = fmaf(wk[k], v[k].x, acc.x);
-            acc.y = fmaf(wk[k], v[k].y, acc.y);
-            acc.z = fmaf(wk[k], v[k].z, acc.z);
-            acc.w = fmaf(wk[k], v[k].w, acc.w);
+        for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+#pragma unroll 1
+        for (int i = lane; i < count; i += 32) {
+            float w = 0.0f;
+            if (i < n) {
+                const float2 ml = ml_of(i);
+                if (ml.y > 0.0f || ml.y != ml.y) w = exp2f(ml.x - m);
+                if (w != 0.0f) l += w * ml.y;
+            }
+            wts[i][warp] = w;
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+        if (lane == 0) {
+            const bool any = l > 0.0f || l != l;
+            invs[warp] = any ? p.out_scale / l : 0.0f;
+            if (p.lse && dim0 == 0 && row < rows)      // (row = token x heads + head)
+                p.lse[static_cast<int64_t>(head.first) * p.heads + row] = any ? 0.69314718055994531f * (m + log2f(l)) : -INFINITY;
         }
     }
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+    __syncthreads();
+    const int j = (tid >> 1) & 3, row = unit_row + j, dim = dim0 + 8 * (tid >> 3) + 4 * (tid & 1);      // and dim + 128 q
+    const int64_t at = static_cast<int64_t>(dim >> 3) * (8 * kUnitRows) + 8 * (row0 + j) + (dim & 7);
+    float4 acc[kQ];
+#pragma unroll
+    for (int q = 0; q < kQ; ++q) acc[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    constexpr int kParts = kQ == 1 ? 4 : 2;      // in flight
+    for (int k0 = 0; k0 < count; k0 += kParts) {
+        float4 v[kParts][kQ];
+        float wk[kParts];
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+            wk[k] = k0 + k < count ? wts[k0 + k][j] : 0.0f;
+#pragma unroll
+            for (int q = 0; q < kQ; ++q) v[k][q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (wk[k] != 0.0f) {      // (a part that saw no token wrote no O)
+                const float* src = p.part_o + static_cast<int64_t>(parts[k0 + k]) * (kUnitRows * kLatent) + at;
+#pragma unroll
+                for (int q = 0; q < kQ; ++q) v[k][q] = *reinterpret_cast<const float4*>(src + q * (16 * 8 * kUnitRows));
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kParts; ++k)
+#pragma unroll
+            for (int q = 0; q < kQ; ++q) {
+                acc[q].x = fmaf(wk[k], v[k][q].x, acc[q].x);
+                acc[q].y = fmaf(wk[k], v[k][q].y, acc[q].y);
+                acc[q].z = fmaf(wk[k], v[k][q].z, acc[q].z);
+                acc[q].w = fmaf(wk[k], v[k][q].w, acc[q].w);
+            }
+    }
+    if (row >= rows) return;
+    const float inv = invs[j];
     const int tok = row / p.heads, h = row - tok * p.heads;
-    *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(head.first + tok) * p.o_st + static_cast<int64_t>(h) * p.o_sh + 4 * tid) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-    if (p.lse && tid == 0)
-        p.lse[static_cast<int64_t>(head.first + tok) * p.heads + h] = any ? 0.69314718055994531f * (m + log2f(l)) : -INFINITY;
+    __nv_bfloat16* dst = p.out + static_cast<int64_t>(head.first + tok) * p.o_st + static_cast<int64_t>(h) * p.o_sh + dim;
+#pragma unroll
+    for (int q = 0; q < kQ; ++q) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(acc[q].x * inv, acc[q].y * inv), hi = __floats2bfloat162_rn(acc[q].z * inv, acc[q].w * inv);
+        *reinterpret_cast<uint2*>(dst + 128 * q) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
 }
 
 struct PrefillPlan {
@@ -1260,7 +1321,8 @@ extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_
         if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill launch failed: %s", cudaGetErrorString(e));
         if ((rc = check_launch("nvfp4kv_mla_prefill")) != NVFP4KV_OK) return rc;
         if (pl.pairs == 1 || max_seq_len <= kTile) continue;      // no unit can be cut
-        e = launch_dependent(prefill_combine_kernel, dim3(pl.pairs * kUnitRows), dim3(128), 0, st, p);
+        if (8 * pl.pairs <= device_sm_count()) e = launch_dependent(prefill_combine_kernel<1>, dim3(pl.pairs * kUnitRows), dim3(128), 0, st, p);
+        else e = launch_dependent(prefill_combine_kernel<4>, dim3(pl.pairs * (kUnitRows / 4)), dim3(128), 0, st, p);
         if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill combine launch failed: %s", cudaGetErrorString(e));
         if ((rc = check_launch("nvfp4kv_mla_prefill combine")) != NVFP4KV_OK) return rc;
     }

@@ -812,6 +812,8 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
                 _lib.check(_lib.lib().nvfp4kv_mla_prefill_workspace_size(B, T, H, int(max_q_len), int(max_seq_len),
                                                                          ctypes.byref(n)),
                            "nvfp4kv_mla_prefill_workspace_size")
+            if len(_ws_sizes) >= 4096:      # a serving loop meets ever new shapes
+                _ws_sizes.clear()
             need = _ws_sizes[key] = int(n.value)
         ws = workspace_buffer
         if ws is None or not ws.is_cuda or not ws.is_contiguous() or ws.data_ptr() % 256 \
