@@ -100,10 +100,10 @@ CASES = [
     ([130], [130], 3, 16, True), ([64], [1000], 20, 128, True), ([2, 0, 33, 1], [2, 50, 520, 0], 5, 16, True),
     ([9], [700], 128, 64, True), ([1, 1, 1, 1, 1], [1, 255, 256, 257, 2000], 64, 64, True), ([40], [300], 7, 1, False),
     ([257], [513], 64, 64, True), ([100, 3], [100, 4097], 32, 256, True),
-    # few rows per sequence (no image) with every page size
+    # few rows per sequence, with every page size
     ([1], [300], 8, 1, True), ([2], [530], 4, 2, False), ([1, 1], [301, 65], 16, 4, True), ([3], [700], 16, 8, True),
     ([2], [900], 32, 32, False), ([1], [1300], 64, 4096, True), ([1, 4], [2050, 770], 16, 256, True),
-    # more units than CTA pairs: several to a pair, cut anywhere, with and without images in turn
+    # more units than CTA pairs: several to a pair, cut anywhere
     ([150], [1500], 128, 64, True), ([1, 9, 2, 33, 1, 0, 17, 4] * 12, [300, 9, 700, 40, 1, 5, 260, 513] * 12, 32, 16, True),
     ([3] * 200, list(range(3, 203)), 64, 64, False),
 ]
@@ -229,3 +229,26 @@ def test_a_batch_whose_images_do_not_fit_runs_in_groups():
                                  rope_cache=p.rope, return_lse=True)
     assert rt.device_errors() == 0
     p.check(again, lse2)
+
+
+@pytest.mark.parametrize("new,H", [(1, 64), (1, 33), (3, 20), (4, 20), (1, 1), (2, 65)])
+def test_many_short_units(new, H):
+    """Hundreds of units of one or two tiles, several to a CTA pair: 64 rows and fewer lie in both CTAs."""
+    ctx = [new + (37 * i) % 460 for i in range(330)]
+    p = Problem([new] * len(ctx), ctx, H, 16, True, seed=H)
+    out, lse = p.run()
+    assert rt.device_errors() == 0
+    p.check(out, lse)
+    again = p.run(return_lse=False)
+    assert torch.equal(out, again)
+
+
+def test_device_errors_after_the_buffers_are_cleared():
+    p = Problem([2], [70], 16, 16, False, seed=3)
+    p.run()
+    torch.cuda.synchronize()
+    rt._bufs.clear()
+    p.tables[0, 1] = -1
+    out, lse = p.run()
+    assert rt.device_errors() == _lib.DEVERR_BAD_PAGE
+    p.check(out, lse)
