@@ -90,9 +90,9 @@ copy_pages_kernel(const __grid_constant__ Caches c, int64_t num_pages, const int
 }
 
 // The same with bulk copies through shared memory: a block is one warp that keeps kCopyStages pieces
-// in flight, loads ahead of stores, and no data passes registers (256 threads with four 16-byte
-// loads each moved 3.6 TB/s).  A page is cut into equal pieces of at most kCopyBytes; the blocks take
-// the pieces of all pairs in turn.
+// in flight, loads ahead of stores, and no data passes registers.  A page is cut into equal pieces of
+// at most kCopyBytes; the blocks take the pieces of all pairs in turn.  Compacting a 1.1 GB pool moves
+// 0.63 GB (read and written) in 97.5 us, 6.45 TB/s: as much as a plain copy.
 constexpr int kCopyStages = 8, kCopyBytes = 9216;
 struct CopyPieces {
     int first[NVFP4KV_MAX_CACHES + 1];      // a pair's first piece in each cache
@@ -167,7 +167,7 @@ bulk_copy_pages_kernel(const __grid_constant__ Caches c, const __grid_constant__
 }
 
 // ------------------------------------------------------------------ freeing
-// Block = slot.  A table entry is taken with an exchange, so that a slot named twice gives its
+// Block = slot (32 samples of 16,000 tokens: 3 us).  A table entry is taken with an exchange, so that a slot named twice gives its
 // pages back once; a decrement that finds no reference is undone and reported.
 __global__ void __launch_bounds__(256)
 free_pages_kernel(int32_t* tables, int64_t stride, int width, int64_t num_slots, int32_t* seq_lens,
@@ -226,7 +226,8 @@ __device__ __forceinline__ bool fork_partial(const ForkArgs& p, int src, int len
 }
 
 // One block: which forks count, how many free pages they need, the lowest free pages, and one of
-// them for each fork in order.
+// them for each fork in order.  Bound by the latency of its passes: 5.5 us for 28 forks over 1,024
+// pages, 7 us for 480 over 42,405 (16 counts a thread and step; it stops at the last page it needs).
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_constant__ ForkArgs p) {
     __shared__ int sums[2][32];
     const int tid = threadIdx.x;
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_co
 }
 
 // blockIdx.x = fork; y = 0: its table, counts and length, y = 1 + c: the filled rows of its last
-// page in cache c.
+// page in cache c.  480 forks of 16,000 tokens: 6 us, 17 MB of it last pages and tables.
 __global__ void __launch_bounds__(256) fork_apply_kernel(const __grid_constant__ ForkArgs p, const __grid_constant__ Caches c) {
     griddep_wait();
     const int k = blockIdx.x;
@@ -392,7 +393,8 @@ __global__ void __launch_bounds__(kPlanThreads) compact_count_kernel(const __gri
 // With n = live pages in all: the k-th live page past n goes to the k-th hole before it.  A page's
 // number among the live ones is the live pages of the blocks before its own plus a scan; that of a
 // hole before n is its index less that; that of a live page past n is that less the live pages
-// before n, which every block counts for itself.  (In place, only counts of free pages and of
+// before n, which every block counts for itself (42,405 pages: counting 2.6 us, this 7.4, the tables
+// 4.2; one block alone took 70).  (In place, only counts of free pages and of
 // pages past n change, which no other block's counting depends on.)
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid_constant__ CompactArgs p) {
     __shared__ int sums[3][32];

@@ -22,10 +22,15 @@
 // attention dequantises every token once, into the very bytes of the stages (1,152 a token).  A pair
 // needs every latent byte twice (K and V lie in different CTAs), and 64 heads make a unit of every
 // two new tokens, so dequantising in the attention kernel repeats the work once per unit and twice
-// in it: producer warps that did so held a tile to 13,000 cycles (issue slots) where the copies take
-// 6,400, and already a batch of single tokens gains nothing by them.  Copies from L2 reach 70 bytes a
-// cycle and SM with two warps issuing (46 with one); what bounds a tile then is shared memory: 40 KB
-// written and read per stage, 320 of the 256 cycles its MMAs take.
+// in it: producer warps that did so held a tile to 13,000 cycles (issue slots), and a batch of single
+// tokens gained nothing by them.  Copies from L2 reach 70 bytes a cycle and SM with two warps issuing
+// (46 with one).
+//
+// What bounds it: a tile's 17 stages are 4,352 cycles of MMAs and, at 40 KB written and read each,
+// 5,440 cycles of shared memory; it measures 6,500.  2,048 new tokens x 64 heads over 16,384: 3.26 ms
+// as a single call (1.34 PFLOP/s), 3.6 ms back to back, where the GPU is at its power limit (1.22
+// PFLOP/s; a large library product sustains 1.39 there).  A part's first tile and its epilogue add
+// about 8,000 cycles, most of it under the next part's first two QK.
 //
 // The work of a call, all (unit, tile) pairs in order and one more per unit for its set-up, is cut
 // into one equal range per CTA pair, so that no pair waits for another's longer sequence; a unit cut
@@ -72,8 +77,7 @@ static_assert(256 * kRegsSoftmax + 128 * kRegsQ + 128 * kRegsCtl <= kThreads * k
 constexpr float kRescaleLog2 = 8.0f;
 constexpr int kMaxPairs = 128;
 constexpr int kImageTok = 128;                  // tokens of an image block
-constexpr int kImageRows = 1;                   // rows of a thread of the image kernel
-constexpr int kImagePieces = kImageTok / (32 * kImageRows);
+constexpr int kImagePieces = kImageTok / 32;    // a block of the image kernel does 32 at a time
 
 constexpr int kQBytes = 9 * kCtaRows * 128;
 constexpr int SM_Q = 0;                                      // 9 dim atoms x [64 rows x 128 B]
@@ -444,10 +448,11 @@ __device__ __forceinline__ uint4 dequant8(uint32_t code, uint32_t scale2) {
 // swizzled, zeros for tokens that do not exist and for blocks with a NaN scale (the token's bit says
 // so instead: a NaN in V would reach rows that do not see it).  Eight lanes read a row's half (128
 // code bytes), a thread writes its 32 dims as 16 bytes to each of four atoms, a warp whole 128-byte
-// rows; all of a block's loads are in flight before the first is used.
-// The blocks of the grid take the image's in turn (their number is on the device).
+// rows.  The blocks of the grid take pieces of 32 tokens in turn (their number is on the device), a
+// row per thread, six blocks on an SM: 24.2 us for 91K tokens (143 MB read and written, 5.9 TB/s;
+// with four rows a thread and two blocks 26.6, and 5.4 against 3.4 for 2.4K tokens).
 __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_constant__ PrefillParams p) {
-    __shared__ uint32_t bits[2 * kImageRows];
+    __shared__ uint32_t bits[2];      // of the piece's tokens: those that exist, those that hold a NaN
     __shared__ int b_s, pos_s, total_s;
     griddep_launch_dependents();
     const int tid = threadIdx.x, lp = tid & 7, r0 = tid >> 3;
@@ -465,7 +470,7 @@ __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_cons
                 if (hit && b < 0) {
                     const int src = __ffs(hit) - 1;
                     b = b0 + src;
-                    pos = kImageTok * (block - __shfl_sync(0xFFFFFFFFu, upto - blocks, src)) + 32 * kImageRows * piece;
+                    pos = kImageTok * (block - __shfl_sync(0xFFFFFFFFu, upto - blocks, src)) + 32 * piece;
                 }
                 base = __shfl_sync(0xFFFFFFFFu, upto, 31);
             }
@@ -474,60 +479,48 @@ __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_cons
                 pos_s = pos;
                 total_s = base;
             }
-            if (lane < 2 * kImageRows) bits[lane] = 0;
+            if (lane < 2) bits[lane] = 0;
         }
         __syncthreads();
         if (b_s < 0) return;
         total = total_s * kImagePieces;
-        const int L = load_seq(p, b_s).L;
-        const int32_t* table = p.tables + b_s * p.tables_stride;
-        int64_t row[kImageRows];
-        uint4 code[kImageRows][2], rope[kImageRows];
-        uint16_t scale[kImageRows][2];
-#pragma unroll
-        for (int k = 0; k < kImageRows; ++k) row[k] = pool_row(p, table, pos_s + r0 + 32 * k, L);
-#pragma unroll
-        for (int k = 0; k < kImageRows; ++k) {
-            rope[k] = code[k][0] = code[k][1] = make_uint4(0, 0, 0, 0);
-            scale[k][0] = scale[k][1] = 0;
-            if (row[k] >= 0) {
-                const uint8_t* src = p.pool + row[k] * kRowBytes;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    code[k][h] = ldg_nc_v4(src + 128 * h + 16 * lp);
-                    scale[k][h] = __ldg(reinterpret_cast<const uint16_t*>(src + 256 + 16 * h + 2 * lp));
-                }
-                if (p.rope) rope[k] = ldg_nc_v4(p.rope + row[k] * kRope + 8 * lp);
-            }
-        }
-        const int atoms = p.rope ? 9 : 8;
-        uint8_t* dst = p.image + static_cast<int64_t>(block) * atoms * kStageBytes + piece * (4096 * kImageRows) + r0 * 128 + ((lp ^ (r0 & 7)) << 4);
-#pragma unroll
-        for (int k = 0; k < kImageRows; ++k) {
-            const int t = r0 + 32 * k;
-            uint32_t nan = 0;
+        const int L = load_seq(p, b_s).L, t = pos_s + r0;
+        const int64_t row = pool_row(p, p.tables + b_s * p.tables_stride, t, L);
+        uint4 code[2], rope = make_uint4(0, 0, 0, 0);
+        uint16_t scale[2] = {0, 0};
+        code[0] = code[1] = rope;
+        if (row >= 0) {
+            const uint8_t* src = p.pool + row * kRowBytes;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t word[4] = {code[k][h].x, code[k][h].y, code[k][h].z, code[k][h].w};
-                const uint32_t s2 = e4m3x2_to_f16x2(scale[k][h]);
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const bool bad = ((scale[k][h] >> (s & 2 ? 8 : 0)) & 0x7F) == 0x7F;
-                    nan |= bad;
-                    const uint4 v = dequant8(word[s], __byte_perm(s2, s2, s & 2 ? 0x3232 : 0x1010));
-                    *reinterpret_cast<uint4*>(dst + (4 * h + s) * kStageBytes + 4096 * k) = bad ? make_uint4(0, 0, 0, 0) : v;
-                }
+                code[h] = ldg_nc_v4(src + 128 * h + 16 * lp);
+                scale[h] = __ldg(reinterpret_cast<const uint16_t*>(src + 256 + 16 * h + 2 * lp));
             }
-            if (p.rope) *reinterpret_cast<uint4*>(dst + 8 * kStageBytes + 4096 * k) = rope[k];
-            if (nan) atomicOr(&bits[kImageRows + k], 1u << (t & 31));
-            if (lp == 0) {
-                if (row[k] >= 0) atomicOr(&bits[k], 1u << (t & 31));
-                else if (pos_s + t < L) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
+            if (p.rope) rope = ldg_nc_v4(p.rope + row * kRope + 8 * lp);
+        }
+        const int atoms = p.rope ? 9 : 8;
+        uint8_t* dst = p.image + static_cast<int64_t>(block) * atoms * kStageBytes + piece * 4096 + r0 * 128 + ((lp ^ (r0 & 7)) << 4);
+        bool nan = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t word[4] = {code[h].x, code[h].y, code[h].z, code[h].w};
+            const uint32_t s2 = e4m3x2_to_f16x2(scale[h]);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const bool bad = ((scale[h] >> (s & 2 ? 8 : 0)) & 0x7F) == 0x7F;
+                nan |= bad;
+                const uint4 v = dequant8(word[s], __byte_perm(s2, s2, s & 2 ? 0x3232 : 0x1010));
+                *reinterpret_cast<uint4*>(dst + (4 * h + s) * kStageBytes) = bad ? make_uint4(0, 0, 0, 0) : v;
             }
         }
+        if (p.rope) *reinterpret_cast<uint4*>(dst + 8 * kStageBytes) = rope;
+        if (nan) atomicOr(&bits[1], 1u << r0);
+        if (lp == 0) {
+            if (row >= 0) atomicOr(&bits[0], 1u << r0);
+            else if (t < L) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
+        }
         __syncthreads();
-        if (tid < 2 * kImageRows)
-            p.image_bits[8 * static_cast<int64_t>(block) + 4 * (tid / kImageRows) + kImageRows * piece + tid % kImageRows] = bits[tid];
+        if (tid < 2) p.image_bits[8 * static_cast<int64_t>(block) + 4 * tid + piece] = bits[tid];
         __syncthreads();      // (the next item's words)
     }
 }
@@ -839,7 +832,8 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             if (t.n_tiles == 0) continue;
             if (parts > 0) {                     // (the first part's is there)
                 // Converted into the workspace while the last part runs, and copied from there once its last QK
-                // is done: converted only then, the MMAs waited 10,000 cycles a part for it.
+                // is done: converted only then, the MMAs waited 10,000 cycles a part for it (8 chunks of 777
+                // tokens: 425 us against 401).
                 uint8_t* scratch = p.q_scratch + static_cast<int64_t>(2 * pair + cta) * kQBytes;
                 QRows q;
                 load_q(p, t, cta, warp - kQWarp0, kQWarps, q);
@@ -995,10 +989,10 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 p.parts[2 * pair + (first_part ? 0 : 1)] = PartInfo{1, t.head, t.tail, 0, t.first, t.n, t.block, 0};
             // Two pieces a step, 16 dims of each as 32-byte stores by the lanes that hold the rows, the next two
             // on their way from tensor memory.  Rolled up: this code runs once per part, and unrolled its
-            // instructions took longer to arrive than to run.  (Whole rows staged in shared memory and
-            // stored by warps were no faster.)
+            // instructions took longer to arrive than to run.  (Whole rows of the output staged in shared
+            // memory and stored by warps were no faster.)
             __nv_bfloat16* out = p.out + static_cast<int64_t>(t.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh + 256 * (sp >> 1) + 16 * ch;
-            // (chunk 8 (dim / 8) by chunk: a warp's 32 rows are 1 KB together; as rows they took 7 K cycles)
+            // (chunks of 8 dims, each of all rows: a warp's store is 1 KB in one piece; 4,400 cycles, as rows 6,800)
             float* part_o = p.part_o + (static_cast<int64_t>(2 * pair + (first_part ? 0 : 1)) * 64 + 32 * (sp >> 1) + 2 * ch) * (8 * kUnitRows) + 8 * unit_row;
             const bool wide = (reinterpret_cast<uintptr_t>(p.out) % 32 == 0) && p.o_st % 16 == 0 && p.o_sh % 16 == 0;
             const uint32_t o_addr = tmem + kTO + 128 * ch + lanes;
