@@ -861,7 +861,11 @@ def _check_int32(**tensors):
 
 
 def _stream_buffer(index: int, name: str, n: int, dtype: torch.dtype) -> torch.Tensor:
-    """A persistent buffer of the current stream, so that calls on two streams never share one."""
+    """A persistent buffer of the current stream, so that calls on two streams never share one.  A
+    call that is being captured gets one from the graph's own pool: a persistent one may be
+    replaced by a larger one while the graph lives."""
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return torch.empty(n, dtype=dtype, device=torch.device("cuda", index))
     key = (name, index, _raw_stream(index))
     ws = _bufs.get(key)
     if ws is None or ws.numel() < n:

@@ -71,7 +71,12 @@ int nvfp4kv_append_rope_rotated(const void* k_pe, int64_t num_tokens, int64_t k_
  *    exp(bmm1_scale * q.k), -inf for such a row.
  * Tokens on a missing page (id outside the pool) are masked and set NVFP4KV_DEVERR_BAD_PAGE.
  * A hidden token never reaches a row, whatever its bytes hold.
- * workspace: nvfp4kv_mla_prefill_workspace_size() bytes, 256-byte aligned.
+ * cu_seqlens_q[batch] rows of out and lse are written, all of them if it is total_q.
+ * pool_rows is a multiple of page_size below 2^31, page_size a power of two up to 4096.
+ * workspace: nvfp4kv_mla_prefill_workspace_size() bytes, 256-byte aligned: a dequantised image
+ *    of the contexts (1,152 bytes a token, max_seq_len for each sequence, at most 1 GiB or one
+ *    sequence's; a larger batch runs in groups of sequences) and partial results.  Give the
+ *    batch's own max_q_len and max_seq_len: they size both the workspace and the grid.
  */
 int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* pool,
                         int64_t pool_rows, const void* rope_pool, const int32_t* tables,

@@ -68,3 +68,66 @@ def test_prefill_in_a_cuda_graph_follows_the_lengths_on_the_device():
         assert torch.equal(got[: starts[-1]], out[: starts[-1]])
         assert bool((got[starts[-1]:] == 7.0).all())
     assert rt.device_errors() == 0
+
+
+def test_every_operator_in_one_graph():
+    """Rotate, write, attend, fork, free and compact as one captured graph: a replay gives what the
+    calls give, also after larger calls on the same stream have grown the buffers there."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    pages, page, H = 64, 16, 16
+    randn = lambda *n: torch.randn(*n, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    latent = torch.zeros(pages, page, 288, dtype=torch.uint8, device="cuda")
+    rt.write_nvfp4(randn(pages * page, 512), latent, torch.arange(pages * page, device="cuda"))
+    rope = randn(pages, page, 64)
+    tables = torch.full((8, 16), -1, dtype=torch.int32, device="cuda")
+    tables[0, :7] = torch.arange(20, 27, dtype=torch.int32)
+    tables[1, :3] = torch.arange(50, 53, dtype=torch.int32)
+    seq = torch.tensor([101, 37, 0, 0, 0, 0, 0, 0], dtype=torch.int32, device="cuda")
+    refs = torch.zeros(pages, dtype=torch.int32, device="cuda")
+    refs[20:27], refs[50:53] = 1, 1
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    src, dst, ended, cu = ints(0, 1, 0), ints(2, 3, 4), ints(1), ints(0, 3, 4)
+    cos_sin = rt.rope_cos_sin(256).cuda()
+    positions = torch.tensor([98, 99, 100, 36], device="cuda")
+    slots = torch.tensor([26 * 16 + 2, 26 * 16 + 3, 26 * 16 + 4, 52 * 16 + 4], device="cuda")
+    q, k_pe, x = randn(4, H, 576), randn(4, 64), randn(4, 2, 128)
+    state = [latent, rope, tables, seq, refs, q]
+    start = [t.clone() for t in state]
+    out = torch.empty(4, H, 512, dtype=torch.bfloat16, device="cuda")
+    turned = torch.empty_like(x)
+
+    def calls():
+        rt.apply_rope(x, positions, cos_sin, out=turned)
+        rt.write_nvfp4_rope_rotated(k_pe, rope, slots, positions, cos_sin, q_pe=q[..., 512:])
+        rt.mla_prefill(q, latent, None, 512, 64, tables[:2], cu, seq[:2], 3, 256, out=out, rope_cache=rope, bmm1_scale=1 / 24)
+        rt.fork_pages([latent, rope], tables, seq, src, dst, refs)
+        rt.free_pages(tables, seq, ended, refs)
+        return rt.compact_pages([latent, rope], tables, refs)
+
+    def reset():
+        for t, t0 in zip(state, start):
+            t.copy_(t0)
+        out.zero_()
+        turned.zero_()
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        live = int(calls())
+        want = [t.clone() for t in state + [out, turned]]
+        reset()
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            count = calls()
+        rt.mla_prefill(randn(900, H, 576), latent, None, 512, 64, tables[:1], ints(0, 900), ints(100), 900, 256)
+        rt.compact_pages([torch.zeros(9000, 16, 288, dtype=torch.uint8, device="cuda")], ints(3).view(1, 1),
+                         torch.zeros(9000, dtype=torch.int32, device="cuda").index_fill(0, torch.tensor([3], device="cuda"), 1))
+        for _ in range(2):
+            reset()
+            graph.replay()
+            s.synchronize()
+            assert int(count) == live == 12      # 7 + 1 + 1 of the first prompt, 3 of the fork of the second
+            for a, b in zip(state + [out, turned], want):
+                assert torch.equal(a, b)
+    assert rt.device_errors() == 0
