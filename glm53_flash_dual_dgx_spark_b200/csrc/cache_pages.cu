@@ -393,36 +393,40 @@ __global__ void __launch_bounds__(kPlanThreads) compact_count_kernel(const __gri
 // With n = live pages in all: the k-th live page past n goes to the k-th hole before it.  A page's
 // number among the live ones is the live pages of the blocks before its own plus a scan; that of a
 // hole before n is its index less that; that of a live page past n is that less the live pages
-// before n, which every block counts for itself (42,405 pages: counting 2.6 us, this 7.4, the tables
+// before n, which every block counts for itself.  A pool of one block needs no counting kernel (42,405 pages: counting 2.6 us, this 7.4, the tables
 // 4.2; one block alone took 70).  (In place, only counts of free pages and of
 // pages past n change, which no other block's counting depends on.)
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid_constant__ CompactArgs p) {
     __shared__ int sums[3][32];
     const int tid = threadIdx.x, blocks = gridDim.x;
     griddep_wait();
-    int mine[2] = {0, 0}, n, before;
-    for (int b = tid; b < blocks; b += kPlanThreads) {
-        const int c = p.counts[b];
-        mine[0] += c;
-        if (b < static_cast<int>(blockIdx.x)) mine[1] += c;
-    }
-    block_exclusive_scan(mine[0], sums[0], &n);
-    block_exclusive_scan(mine[1], sums[1], &before);
-    // live pages before page n: whole blocks, and the part of n's own
-    const int nb = n / kBlockPages;
-    int part = 0, live_low;
-    for (int b = tid; b < nb; b += kPlanThreads) part += p.counts[b];
-    int r[kPer];
-    const int64_t at = static_cast<int64_t>(nb) * kBlockPages + tid * kPer;
-    load_counts(p.refs, at, n, r);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) part += r[j] > 0;
-    block_exclusive_scan(part, sums[2], &live_low);
     const int64_t i0 = static_cast<int64_t>(blockIdx.x) * kBlockPages + tid * kPer;
+    int r[kPer], live = 0, total, n, before = 0, part = 0, live_low;
     load_counts(p.refs, i0, p.num_pages, r);
-    int live = 0, total;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) live += r[j] > 0;
+    if (blocks == 1) {                                      // (nothing was counted before)
+        block_exclusive_scan(live, sums[0], &n);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) part += r[j] > 0 && i0 + j < n;
+    } else {
+        int all = 0, below = 0;
+        for (int b = tid; b < blocks; b += kPlanThreads) {
+            const int c = p.counts[b];
+            all += c;
+            if (b < static_cast<int>(blockIdx.x)) below += c;
+        }
+        block_exclusive_scan(all, sums[0], &n);
+        block_exclusive_scan(below, sums[1], &before);
+        // live pages before page n: whole blocks, and the part of n's own
+        const int nb = n / kBlockPages;
+        for (int b = tid; b < nb; b += kPlanThreads) part += p.counts[b];
+        int low[kPer];
+        load_counts(p.refs, static_cast<int64_t>(nb) * kBlockPages + tid * kPer, n, low);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) part += low[j] > 0;
+    }
+    block_exclusive_scan(part, sums[2], &live_low);
     __syncthreads();
     int rank = before + block_exclusive_scan(live, sums[0], &total);      // live pages before the thread's first
 #pragma unroll
@@ -517,7 +521,13 @@ int launch_copy(const Caches& c, int64_t num_pages, const int32_t* src, const in
     cudaError_t e;
     if (align % 16 == 0) {      // what a bulk copy can move
         static_assert(kCopyStages * kCopyBytes * 3 <= 227 * 1024, "three blocks on an SM");
-        e = cudaFuncSetAttribute(bulk_copy_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCopyStages * kCopyBytes);
+        static int done[64] = {0};      // (a device's limit, set once)
+        int dev = 0;
+        e = cudaGetDevice(&dev);
+        if (e == cudaSuccess && (dev >= 64 || !done[dev])) {
+            e = cudaFuncSetAttribute(bulk_copy_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCopyStages * kCopyBytes);
+            if (e == cudaSuccess && dev < 64) done[dev] = 1;
+        }
         int64_t blocks = 3 * device_sm_count();
         blocks = blocks < most_pairs * pieces.first[c.num] ? blocks : most_pairs * pieces.first[c.num];
         if (e == cudaSuccess)
@@ -626,9 +636,10 @@ extern "C" int nvfp4kv_compact_pages(const void* const* caches, const int64_t* p
     a.tables = block_tables; a.stride = tables_stride; a.width = table_width; a.num_slots = num_slots;
     a.out_tables = out_tables; a.out_stride = out_tables_stride; a.err = err_flag;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    compact_count_kernel<<<blocks, kPlanThreads, 0, st>>>(a);
-    rc = check_launch("nvfp4kv_compact_pages count");
-    if (rc != NVFP4KV_OK) return rc;
+    if (blocks > 1) {
+        compact_count_kernel<<<blocks, kPlanThreads, 0, st>>>(a);
+        if ((rc = check_launch("nvfp4kv_compact_pages count")) != NVFP4KV_OK) return rc;
+    }
     const int64_t want = (num_slots * table_width + 255) / 256, most = 8 * device_sm_count();
     cudaError_t e = launch_dependent(compact_plan_kernel, dim3(blocks), dim3(kPlanThreads), 0, st, a);
     if (e == cudaSuccess)

@@ -1236,7 +1236,7 @@ extern "C" int nvfp4kv_mla_prefill_workspace_size(int batch, int total_q, int nu
     using namespace nvfp4kv;
     if (!bytes) return fail(NVFP4KV_EINVAL, "mla_prefill_workspace_size: null output");
     if (batch < 0 || total_q < 0 || num_heads < 1 || max_q_len < 0 || max_seq_len < 0)
-        return fail(NVFP4KV_EINVAL, "mla_prefill_workspace_size: bad shape");
+        return fail(NVFP4KV_EINVAL, "mla_prefill_workspace_size: batch, total_q, max_q_len and max_seq_len must be >= 0, num_heads >= 1");
     *bytes = batch == 0 || total_q == 0 ? 0 : make_prefill_plan(batch, total_q, num_heads, max_q_len, max_seq_len).ws_bytes;
     return NVFP4KV_OK;
 }

@@ -604,12 +604,17 @@ def index_scores_buffer(device=None) -> torch.Tensor | None:
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
+_entries: dict = {}    # C entries by name
+
+
 def _call(name: str, index: int, *args) -> None:
     """The C entry ``name`` on device ``index``'s current stream, with the device error word; raises
     on a non-OK code."""
     word = _bufs.get(("err", index))
     err = (_err_word(torch.device("cuda", index)) if word is None else word).data_ptr()
-    fn = getattr(_lib.lib(), name)
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.lib(), name)
     if torch._C._cuda_getDevice() == index:
         rc = fn(*args, err, _raw_stream(index))
     else:
@@ -713,14 +718,15 @@ def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_
     q_pe [T, H, 64] bf16 rotated into q_out (default: in place).  Returns q_out."""
     _require_cuda(k_pe, "k_pe")
     _require_cuda(rope_cache, "rope_cache")
-    ks = k_pe.stride()
-    if k_pe.dtype != torch.bfloat16 or len(ks) != 2 or k_pe.shape[1] < ROPE or ks[1] != 1:
+    ks, (T, width) = k_pe.stride(), k_pe.shape if k_pe.dim() == 2 else (0, 0)
+    if width < ROPE or k_pe.dtype is not torch.bfloat16 or ks[1] != 1:
         raise ValueError("k_pe must be bf16 [T, >=64] with a contiguous last dimension")
-    if rope_cache.dtype != torch.bfloat16:
+    if rope_cache.dtype is not torch.bfloat16:
         raise TypeError("rope_cache must be bf16")
-    if not rope_cache.is_contiguous() or rope_cache.numel() % ROPE:
+    rows, rest = divmod(rope_cache.numel(), ROPE)
+    if rest or not rope_cache.is_contiguous():
         raise ValueError("rope_cache must be contiguous rows of 64")
-    T = k_pe.shape[0]
+    _require_cuda(slot_mapping, "slot_mapping")
     slot = _vector(slot_mapping)
     if slot.shape[0] != T:
         raise ValueError(f"slot_mapping has {slot.shape[0]} entries for {T} tokens")
@@ -730,14 +736,17 @@ def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_
     pos, pdt = _check_angles(cos_sin, positions, T, ROPE)
     H, qs, qos, q_ptr, qo_ptr = 0, (0, 0), (0, 0), None, None
     if q_pe is not None:
-        q_out = q_pe if q_out is None else q_out
         _require_cuda(q_pe, "q_pe")
-        _require_cuda(q_out, "q_out")
-        shape, qs, qos = q_pe.shape, q_pe.stride(), q_out.stride()
-        if len(shape) != 3 or shape[0] != T or shape[2] != ROPE or qs[2] != 1 or q_pe.dtype != torch.bfloat16:
+        shape, qs = q_pe.shape, q_pe.stride()
+        if len(shape) != 3 or shape[0] != T or shape[2] != ROPE or qs[2] != 1 or q_pe.dtype is not torch.bfloat16:
             raise ValueError("q_pe must be bf16 [T, H, 64] with a contiguous last dimension")
-        if q_out.shape != shape or qos[2] != 1 or q_out.dtype != torch.bfloat16:
-            raise ValueError("q_out must be bf16 of q_pe's shape with a contiguous last dimension")
+        if q_out is None or q_out is q_pe:
+            q_out, qos = q_pe, qs
+        else:
+            _require_cuda(q_out, "q_out")
+            qos = q_out.stride()
+            if q_out.shape != shape or qos[2] != 1 or q_out.dtype is not torch.bfloat16:
+                raise ValueError("q_out must be bf16 of q_pe's shape with a contiguous last dimension")
         H = shape[1]
         if H:
             q_ptr, qo_ptr = q_pe.data_ptr(), q_out.data_ptr()
@@ -746,7 +755,7 @@ def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_
     if T == 0:
         return q_out
     _call("nvfp4kv_append_rope_rotated", k_pe.get_device(), k_pe.data_ptr(), T, ks[0], rope_cache.data_ptr(),
-          rope_cache.numel() // ROPE, slot.data_ptr(), sdt, pos.data_ptr(), pdt, cos_sin.data_ptr(),
+          rows, slot.data_ptr(), sdt, pos.data_ptr(), pdt, cos_sin.data_ptr(),
           cos_sin.shape[0], int(interleaved), q_ptr, H, qs[0], qs[1], qo_ptr, qos[0], qos[1])
     return q_out
 
@@ -766,42 +775,51 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
     mla_decode (dense).  max_q_len and max_seq_len bound the device-side lengths; nothing
     synchronises the host.  Returns out [T, H, kv_lora_rank] bf16, with ``return_lse`` also
     lse [T, H] float32 (natural log; -inf for a row that sees no token, whose out is zeros)."""
-    _require_cuda(query, "query")
-    _require_cuda(kv_cache, "kv_cache")
+    try:      # (the whole host side of a call is about as long as a short batch on the device)
+        on_device = query.is_cuda and kv_cache.is_cuda and block_tables.is_cuda and cu_seqlens_q.is_cuda \
+            and seq_lens.is_cuda and (rope_cache is None or rope_cache.is_cuda)
+    except AttributeError:
+        on_device = False
+    if not on_device:
+        for name, t in (("query", query), ("kv_cache", kv_cache), ("block_tables", block_tables),
+                        ("cu_seqlens_q", cu_seqlens_q), ("seq_lens", seq_lens), ("rope_cache", rope_cache)):
+            _require_cuda(t, name)
     if isinstance(bmm1_scale, torch.Tensor) or isinstance(bmm2_scale, torch.Tensor):
         raise TypeError("bmm1_scale / bmm2_scale must be Python floats (a device scalar would need a sync)")
-    if query.dtype != torch.bfloat16 or query.dim() != 3 or query.stride(2) != 1:
+    qs = query.stride()
+    if query.dtype is not torch.bfloat16 or len(qs) != 3 or qs[2] != 1:
         raise ValueError("query must be bf16 [T, H, D] with a contiguous last dimension")
     T, H, D = query.shape
     if kv_lora_rank != LATENT or D != kv_lora_rank + qk_rope_head_dim:
         raise ValueError(f"query dim {D} must equal kv_lora_rank (512) + qk_rope_head_dim")
-    if kv_cache.shape[-1] != NV_BYTES or not kv_cache.is_contiguous():
+    pool = kv_cache.shape
+    if pool[-1] != NV_BYTES or not kv_cache.is_contiguous():
         raise ValueError("kv_cache must be a contiguous pool of 288-byte rows")
     rows = kv_cache.numel() // NV_BYTES
-    page_size = kv_cache.shape[-2] if kv_cache.dim() >= 3 else 64
-    for name, t in (("block_tables", block_tables), ("cu_seqlens_q", cu_seqlens_q), ("seq_lens", seq_lens)):
-        _require_cuda(t, name)
-        if t.dtype != torch.int32:
-            raise TypeError(f"{name} must be int32")
+    page_size = pool[-2] if len(pool) >= 3 else 64
+    if not (block_tables.dtype is cu_seqlens_q.dtype is seq_lens.dtype is torch.int32):
+        raise TypeError("block_tables, cu_seqlens_q and seq_lens must be int32")
     cu, sl = _vector(cu_seqlens_q), _vector(seq_lens)
-    B, ts = sl.shape[0], block_tables.stride()
-    if block_tables.dim() != 2 or block_tables.shape[0] != B or (block_tables.shape[1] > 1 and ts[1] != 1):
+    B, tables, ts = sl.shape[0], block_tables.shape, block_tables.stride()
+    if len(tables) != 2 or tables[0] != B or (tables[1] > 1 and ts[1] != 1):
         raise ValueError("block_tables must be [B, width] with a contiguous last dimension")
     if cu.shape[0] != B + 1:
         raise ValueError("cu_seqlens_q must have one entry more than seq_lens")
-    if block_tables.shape[1] * page_size < max_seq_len:
+    if tables[1] * page_size < max_seq_len:
         raise ValueError("block_tables too narrow for max_seq_len")
     if out is None:
-        out = torch.empty(T, H, LATENT, dtype=torch.bfloat16, device=query.device)
-    elif out.shape != (T, H, LATENT) or out.dtype != torch.bfloat16 or out.stride(2) != 1:
-        raise ValueError("out must be bf16 [T, H, 512] with a contiguous last dimension")
+        out = query.new_empty((T, H, LATENT))
+        os = (H * LATENT, LATENT)
+    else:
+        os = out.stride()
+        if not out.is_cuda or out.shape != (T, H, LATENT) or out.dtype is not torch.bfloat16 or os[2] != 1:
+            raise ValueError("out must be bf16 [T, H, 512] on the device with a contiguous last dimension")
     rope = None
     if rope_cache is not None:
-        _require_cuda(rope_cache, "rope_cache")
-        if rope_cache.dtype != torch.bfloat16 or rope_cache.numel() != rows * ROPE or not rope_cache.is_contiguous():
+        if rope_cache.dtype is not torch.bfloat16 or rope_cache.numel() != rows * ROPE or not rope_cache.is_contiguous():
             raise ValueError("rope_cache must be a contiguous bf16 [pool rows, 64] side-pool")
         rope = rope_cache.data_ptr()
-    lse = torch.empty(T, H, dtype=torch.float32, device=query.device) if return_lse else None
+    lse = query.new_empty((T, H), dtype=torch.float32) if return_lse else None
     if T > 0 and B > 0:
         index = query.get_device()
         key = ("prefill", B, T, H, max_q_len, max_seq_len, index)
@@ -819,7 +837,6 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
         if ws is None or not ws.is_cuda or not ws.is_contiguous() or ws.data_ptr() % 256 \
                 or ws.numel() * ws.element_size() < need:
             ws = _stream_buffer(index, "prefill_ws", need, torch.uint8)
-        qs, os = query.stride(), out.stride()
         _call("nvfp4kv_mla_prefill", index, query.data_ptr(), qs[0], qs[1], kv_cache.data_ptr(), rows, rope,
               block_tables.data_ptr(), ts[0], cu.data_ptr(), sl.data_ptr(), B, T, H, D, kv_lora_rank, page_size,
               int(max_q_len), int(max_seq_len), bmm1_scale, bmm2_scale, out.data_ptr(), os[0], os[1],
@@ -828,13 +845,19 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
 
 
 # ------------------------------------------------------------------ page upkeep
+_MAX_CACHES = 8        # NVFP4KV_MAX_CACHES
+_POINTERS, _SIZES = ctypes.c_void_p * _MAX_CACHES, ctypes.c_int64 * _MAX_CACHES
+
+
 def _cache_list(caches):
     """(device pointers, bytes per page, pages, page size) of pools [num_pages, page_size, ...]."""
     if not caches:
         raise ValueError("caches must name at least one pool")
     pages, size = caches[0].shape[:2]
     n = len(caches)
-    ptrs, sizes = (ctypes.c_void_p * n)(), (ctypes.c_int64 * n)()
+    if n > _MAX_CACHES:
+        raise ValueError(f"at most {_MAX_CACHES} caches in one call")
+    ptrs, sizes = _POINTERS(), _SIZES()
     for k, c in enumerate(caches):
         _require_cuda(c, "caches")
         shape = c.shape
@@ -927,14 +950,19 @@ def compact_pages(caches, block_tables: torch.Tensor, ref_counts: torch.Tensor, 
     ptrs, sizes, n, pages, _ = _cache_list(caches)
     out_tables = block_tables if out_tables is None else out_tables
     out_ref_counts = ref_counts if out_ref_counts is None else out_ref_counts
-    _check_int32(block_tables=block_tables, ref_counts=ref_counts, out_tables=out_tables, out_ref_counts=out_ref_counts)
+    _check_int32(block_tables=block_tables, ref_counts=ref_counts)
+    if out_tables is not block_tables or out_ref_counts is not ref_counts:
+        _check_int32(out_tables=out_tables, out_ref_counts=out_ref_counts)
     if ref_counts.numel() != pages or out_ref_counts.numel() != pages or out_tables.shape != block_tables.shape:
         raise ValueError("ref_counts must have one entry per page, out_tables block_tables' shape")
     index = block_tables.get_device()
-    live = torch.empty((), dtype=torch.int32, device=block_tables.device)
-    need = ctypes.c_int64(0)
-    _lib.check(_lib.lib().nvfp4kv_compact_workspace_ints(pages, ctypes.byref(need)), "nvfp4kv_compact_workspace_ints")
-    ws = _stream_buffer(index, "compact_ws", need.value, torch.int32)
+    live = block_tables.new_empty(())
+    need = _ws_sizes.get(("compact", pages))
+    if need is None:
+        n64 = ctypes.c_int64(0)
+        _lib.check(_lib.lib().nvfp4kv_compact_workspace_ints(pages, ctypes.byref(n64)), "nvfp4kv_compact_workspace_ints")
+        need = _ws_sizes["compact", pages] = int(n64.value)
+    ws = _stream_buffer(index, "compact_ws", need, torch.int32)
     S, width = block_tables.shape
     _call("nvfp4kv_compact_pages", index, ptrs, sizes, n, block_tables.data_ptr(), block_tables.stride(0), width, S,
           ref_counts.data_ptr(), pages, out_tables.data_ptr(), out_tables.stride(0), out_ref_counts.data_ptr(),
