@@ -169,6 +169,14 @@ __device__ __forceinline__ bool try_wait_asleep(uint32_t bar, uint32_t parity) {
                  "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
     return ok != 0;
 }
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool test_phase(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
     if (try_wait_asleep(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
@@ -716,64 +724,62 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 const uint64_t dp = smem_desc_sw128(sbase + SM_P, 16, 1024);
                 const uint64_t dk = smem_desc_sw128(sbase + SM_RING, 16, 1024);
                 const uint64_t dv = smem_desc_sw128(sbase + SM_RING, 8192, 1024);
-                int slot = 0, parts = 0, tile = 0;      // ring slot; parts and tiles so far
-                uint32_t phase = 0;
-                auto next = [&] {
-                    if (++slot == kStages) {
-                        slot = 0;
-                        phase ^= 1;
-                    }
-                };
+                int stages = 0, parts = 0, tile = 0;      // so far
 #pragma unroll 1
                 for (bool more = advance_part(work); more && !*abort_flag; more = next_part(p, work)) {
                     const int n_tiles = t.n_tiles;
                     if (n_tiles == 0) continue;
                     if (parts > 0) mbar_wait(bar(B_Q_FULL), (parts - 1) & 1, abort_flag, p.err);
-#pragma unroll 1
-                    for (int i = 0; i <= n_tiles; ++i, ++tile) {
-                        if (i < n_tiles) {
-                            const uint32_t d = tmem + kTS + 128 * (tile & 1);
-                            if (tile >= 2) mbar_wait(bar(B_S_FREE + (tile & 1)), ((tile >> 1) - 1) & 1, abort_flag, p.err);
-#pragma unroll 1
-                            for (int j = 0; j < k_stages; ++j) {
-                                mbar_wait(bar(B_FULL + slot), phase, abort_flag, p.err);
-                                tc_fence_after();
-                                const uint64_t a = dq + ((j * kCtaRows * 128) >> 4), b = dk + ((slot * kStageBytes) >> 4);
-                                const uint32_t id = j == 8 ? kIdescRope : kIdescQk;
-                                if (elect_one()) {
-#pragma unroll
-                                    for (int k = 0; k < 4; ++k) pair_mma_f16(d, a + 2 * k, b + 2 * k, id, (j | k) != 0);
-                                    pair_commit(bar(B_EMPTY + slot));
-                                    if (j == k_stages - 1) {
-                                        pair_commit(bar(B_S_FULL + (tile & 1)));
-                                        if (i == n_tiles - 1) pair_commit(bar(B_Q_FREE));
-                                    }
-                                }
-                                __syncwarp();
-                                next();
+                    // One thread runs the part.  Only about one MMA is queued behind the running one, so all that
+                    // comes between two MMAs has 64 cycles to hide in: the next stage's barrier is looked at in
+                    // the middle of a stage.  (A wait per stage by the whole warp: 375 cycles a stage where the
+                    // MMAs take 256.)
+                    if (elect_one()) {
+                        int slot = stages % kStages;
+                        uint32_t phase = (stages / kStages) & 1;
+                        bool landed = false;
+                        auto stage = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t step, uint32_t id, bool first) {
+                            if (!landed) mbar_wait(bar(B_FULL + slot), phase, abort_flag, p.err);
+                            const uint32_t done = bar(B_EMPTY + slot);
+                            if (++slot == kStages) {
+                                slot = 0;
+                                phase ^= 1;
                             }
-                        }
-                        if (i > 0) {
-                            mbar_wait(bar(B_P_FULL), (tile - 1) & 1, abort_flag, p.err);
-                            if (i == 1 && parts > 0) mbar_wait(bar(B_O_FREE), (parts - 1) & 1, abort_flag, p.err);
+                            pair_mma_f16(d, a, b, id, !first);
+                            pair_mma_f16(d, a + 2, b + step, id, 1);
+                            landed = test_phase(bar(B_FULL + slot), phase);
+                            pair_mma_f16(d, a + 4, b + 2 * step, id, 1);
+                            pair_mma_f16(d, a + 6, b + 3 * step, id, 1);
+                            pair_commit(done);
+                        };
 #pragma unroll 1
-                            for (int s = 0; s < kVStages; ++s) {
-                                mbar_wait(bar(B_FULL + slot), phase, abort_flag, p.err);
+                        for (int i = 0; i <= n_tiles; ++i) {
+                            if (i < n_tiles) {
+                                const int at = tile + i;
+                                const uint32_t d = tmem + kTS + 128 * (at & 1);
+                                if (at >= 2) mbar_wait(bar(B_S_FREE + (at & 1)), ((at >> 1) - 1) & 1, abort_flag, p.err);
                                 tc_fence_after();
-                                const uint64_t a = dp + (((s >> 1) * kCtaRows * 128) >> 4), b = dv + ((slot * kStageBytes) >> 4);
-                                const uint32_t d = tmem + kTO + 128 * (s & 1);
-                                if (elect_one()) {
-#pragma unroll
-                                    for (int k = 0; k < 4; ++k) pair_mma_f16(d, a + 2 * k, b + 128 * k, kIdescPv, ((i - 1) | (s >> 1) | k) != 0);
-                                    pair_commit(bar(B_EMPTY + slot));
-                                    if (s == kVStages - 1) pair_commit(bar(B_PV_DONE));
-                                }
-                                __syncwarp();
-                                next();
+#pragma unroll 1
+                                for (int j = 0; j < k_stages; ++j)
+                                    stage(d, dq + ((j * kCtaRows * 128) >> 4), dk + ((slot * kStageBytes) >> 4), 2, j == 8 ? kIdescRope : kIdescQk, j == 0);
+                                pair_commit(bar(B_S_FULL + (at & 1)));
+                                if (i == n_tiles - 1) pair_commit(bar(B_Q_FREE));
+                            }
+                            if (i > 0) {
+                                mbar_wait(bar(B_P_FULL), (tile + i - 1) & 1, abort_flag, p.err);
+                                if (i == 1 && parts > 0) mbar_wait(bar(B_O_FREE), (parts - 1) & 1, abort_flag, p.err);
+                                tc_fence_after();
+#pragma unroll 1
+                                for (int s = 0; s < kVStages; ++s)
+                                    stage(tmem + kTO + 128 * (s & 1), dp + (((s >> 1) * kCtaRows * 128) >> 4), dv + ((slot * kStageBytes) >> 4), 128, kIdescPv,
+                                          i == 1 && s < 2);
+                                pair_commit(bar(B_PV_DONE));
                             }
                         }
                     }
-                    --tile;      // the last pass has no tile of its own
+                    __syncwarp();
+                    stages += n_tiles * (k_stages + kVStages);
+                    tile += n_tiles;
                     ++parts;
                 }
                 if (elect_one()) pair_commit(bar(B_DRAIN));

@@ -54,6 +54,7 @@ def simulate(parts, k_stages, places, seed):
             while not full[u % SLOTS].passed(u // SLOTS):
                 yield
             assert ring[u % SLOTS] == u
+            full[(u + 1) % SLOTS].passed((u + 1) // SLOTS)      # the look at the next stage's barrier
             yield
             assert ring[u % SLOTS] == u
             empty[u % SLOTS].arrive()
