@@ -202,6 +202,32 @@ __device__ __forceinline__ void st_global_v8(void* dst, const uint32_t* w) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
                  ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
+// Pairs of fp32: one instruction for two.
+__device__ __forceinline__ uint64_t pair_of(float2 v) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+    return r;
+}
+__device__ __forceinline__ float2 of_pair(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair_of(a)), "l"(pair_of(b)), "l"(pair_of(c)));
+    return of_pair(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair_of(a)), "l"(pair_of(b)));
+    return of_pair(r);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // Instruction descriptors: fp32 accumulators, M = 128 (a pair's rows), N = 256.
 constexpr uint32_t kIdescQk = idesc_f16_f32(128, 256, false, false);
 constexpr uint32_t kIdescRope = kIdescQk | (1u << 7) | (1u << 10);      // both operands bf16
@@ -924,7 +950,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < 64; ++k) mx[k & 3] = fmaxf(mx[k & 3], x[k]);
+                for (int k = 0; k < 32; ++k) mx[k & 3] = max3(mx[k & 3], x[2 * k], x[2 * k + 1]);
                 float* slot = red + (tile & 1) * 256;
                 slot[64 * q4 + row] = factor * fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 named_bar_sync(1 + (sp & 1), 128);
@@ -937,15 +963,17 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 }
                 const float base = m_ref == -INFINITY ? 0.0f : m_ref;
                 uint32_t pk[32];
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                const float2 factor2 = make_float2(factor, factor), base2 = make_float2(-base, -base);
 #pragma unroll
                 for (int k = 0; k < 32; ++k) {
-                    const float a = ex2_approx(fmaf(x[2 * k], factor, -base)), b = ex2_approx(fmaf(x[2 * k + 1], factor, -base));
-                    sum[k & 1] += a;
-                    sum[2 + (k & 1)] += b;
-                    pk[k] = pack_half2(a, b);
+                    const float2 e = fma2(make_float2(x[2 * k], x[2 * k + 1]), factor2, base2);
+                    const float2 w = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                    sum[k & 1] = add2(sum[k & 1], w);
+                    pk[k] = pack_half2(w.x, w.y);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                sum[0] = add2(sum[0], sum[1]);
+                l += sum[0].x + sum[0].y;
                 if (i > 0) {
                     wait_phase(bar(B_PV_DONE), (tile - 1) & 1, abort_flag, p.err);
                     if (__any_sync(0xFFFFFFFFu, alpha != 1.0f)) {          // the row's O: this warp's lanes, block ch
