@@ -27,13 +27,13 @@
 // (46 with one).
 //
 // What bounds it: a tile's 17 stages are 4,352 cycles of MMAs and, at 40 KB written and read each,
-// 5,440 cycles of shared memory; it measures 6,500.  2,048 new tokens x 64 heads over 16,384: 3.26 ms
-// as a single call (1.34 PFLOP/s), 3.6 ms back to back, where the GPU is at its power limit (1.22
+// 5,440 cycles of shared memory; it measures 5,800.  2,048 new tokens x 64 heads over 16,384: 3.2 ms
+// in a short run (1.37 PFLOP/s), 3.46 ms back to back, where the GPU is at its power limit (1.27
 // PFLOP/s; a large library product sustains 1.39 there).  A part's first tile and its epilogue add
-// about 8,000 cycles, most of it under the next part's first two QK.
+// about 8,700 cycles.
 //
-// The work of a call, all (unit, tile) pairs in order and one more per unit for its set-up, is cut
-// into one equal range per CTA pair, so that no pair waits for another's longer sequence; a unit cut
+// The work of a call, all (unit, tile) pairs in order and one and a half more per unit, is cut into
+// one equal range per CTA pair, so that no pair waits for another's longer sequence; a unit cut
 // by a range's end leaves its parts in the workspace for the combine kernel.  The ranges come from
 // the device-side lengths in closed form, in every CTA.
 //
@@ -268,18 +268,22 @@ __device__ __forceinline__ int unit_end(const PrefillParams& p, const Seq& s, in
 __device__ __forceinline__ int unit_tiles(const PrefillParams& p, const Seq& s, int k) {
     return (unit_end(p, s, k) + kTile - 1) / kTile;
 }
-// Weight of the sequence's first K units: their tiles and one each.  A unit's tiles do not fall with
-// k, so the sum goes over tile counts (at most n / 256 + 2 of them), not over units.
+// Weights of the work: a tile, and what a unit adds (its first tile's and its epilogue's latency, about
+// 8,700 cycles of a tile's 5,700).  With one tile's weight for a unit, pairs with short units took 9 %
+// longer than the mean in a batch of chunks, now 6.
+constexpr int kTileWeight = 2, kUnitWeight = 3;
+// Weight of the sequence's first K units.  A unit's tiles do not fall with k, so the sum goes over
+// tile counts (at most n / 256 + 2 of them), not over units.
 __device__ __forceinline__ int64_t weight_before(const PrefillParams& p, const Seq& s, int K) {
     if (K <= 0) return 0;
     const int t0 = unit_tiles(p, s, 0), t1 = unit_tiles(p, s, s.units - 1);
-    int64_t w = static_cast<int64_t>(K) * (t0 + 1);
+    int64_t w = static_cast<int64_t>(K) * (kTileWeight * t0 + kUnitWeight);
     for (int t = t0; t < t1; ++t) {
         // units of at most t tiles: those whose last row's token is at most y
         const int64_t y1 = static_cast<int64_t>(t) * kTile - (s.L - s.n);      // y + 1
         const int64_t rows = y1 * p.heads;
         int64_t c = y1 <= 0 ? 0 : rows >= s.rows ? s.units : rows / kUnitRows;
-        w += K - (c < K ? c : K);
+        w += kTileWeight * (K - (c < K ? c : K));
     }
     return w;
 }
@@ -373,6 +377,8 @@ struct Part {
     int head, tail;         // it begins / ends the unit
     int half;               // rows in the leading CTA (the unit's others are in the second)
 };
+// Tiles in a unit's first `weight`.
+__device__ __forceinline__ int tiles_in(int weight) { return max(weight - kUnitWeight, 0) / kTileWeight; }
 // The next part of the range; parts without tiles are given only where they are a whole unit (one
 // that sees no token).
 __device__ __forceinline__ bool next_part_of(const PrefillParams& p, Range& r, Part& t) {
@@ -388,9 +394,10 @@ __device__ __forceinline__ bool next_part_of(const PrefillParams& p, Range& r, P
         }
         t.end = unit_end(p, s, r.k);
         const int tiles = (t.end + kTile - 1) / kTile;
-        const int take = static_cast<int>(r.left < tiles + 1 - r.offset ? r.left : tiles + 1 - r.offset);
-        t.tile0 = max(r.offset - 1, 0);
-        t.n_tiles = r.offset + take - 1 - t.tile0;
+        const int weight = kTileWeight * tiles + kUnitWeight, begin = r.offset;
+        const int take = static_cast<int>(r.left < weight - begin ? r.left : weight - begin);
+        t.tile0 = tiles_in(begin);
+        t.n_tiles = tiles_in(begin + take) - t.tile0;
         t.b = r.b; t.block = r.k;
         t.first = s.first; t.n = s.n; t.L = s.L; t.rows = s.rows;
         t.image = r.image0;
@@ -400,11 +407,11 @@ __device__ __forceinline__ bool next_part_of(const PrefillParams& p, Range& r, P
         t.tail = t.tile0 + t.n_tiles == tiles;
         r.left -= take;
         r.offset += take;
-        if (r.offset == tiles + 1) {
+        if (r.offset == weight) {
             ++r.k;
             r.offset = 0;
         }
-        if (t.n_tiles > 0 || tiles == 0) return true;
+        if (t.n_tiles > 0 || (tiles == 0 && begin == 0)) return true;
     }
     return false;
 }
@@ -865,7 +872,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             if (parts > 0) {                     // (the first part's is there)
                 // Converted into the workspace while the last part runs, and copied from there once its last QK
                 // is done: converted only then, the MMAs waited 10,000 cycles a part for it (8 chunks of 777
-                // tokens: 425 us against 401).
+                // tokens took 6 % longer).
                 uint8_t* scratch = p.q_scratch + static_cast<int64_t>(2 * pair + cta) * kQBytes;
                 QRows q;
                 load_q(p, t, cta, warp - kQWarp0, kQWarps, q);
@@ -1231,14 +1238,15 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
     const int64_t cap = static_cast<int64_t>(kImageCap / (9 * kStageBytes));
     const int64_t fit = one > 0 ? cap / one : batch;
     pl.group = static_cast<int>(fit < 1 ? 1 : (fit < batch ? fit : batch));
-    // no more pairs than tiles there can be in a group
+    // no more pairs than leave each less than a tile's weight: what a group can have
     const int64_t longest = max_q_len < total_q ? max_q_len : total_q;
     const int64_t by_seq = (longest * num_heads + kUnitRows - 1) / kUnitRows * pl.group;
     const int64_t by_rows = (static_cast<int64_t>(total_q) * num_heads + static_cast<int64_t>(pl.group) * (kUnitRows - 1)) / kUnitRows;
-    const int64_t tiles = (by_seq < by_rows ? by_seq : by_rows) * ((static_cast<int64_t>(max_seq_len) + kTile - 1) / kTile);
+    const int64_t units = by_seq < by_rows ? by_seq : by_rows;
+    const int64_t most = units * (kUnitWeight + kTileWeight * ((static_cast<int64_t>(max_seq_len) + kTile - 1) / kTile)) / kTileWeight + 1;
     int64_t pairs = device_sm_count() / 2;
     pairs = pairs > kMaxPairs ? kMaxPairs : pairs;
-    pairs = pairs > tiles ? tiles : pairs;
+    pairs = pairs > most ? most : pairs;
     pl.pairs = static_cast<int>(pairs < 1 ? 1 : pairs);
     const int64_t blocks = one * pl.group;
     pl.image_blocks = static_cast<int>(blocks);
