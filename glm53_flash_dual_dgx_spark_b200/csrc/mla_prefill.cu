@@ -28,7 +28,7 @@
 //
 // What bounds it: a tile's 17 stages are 4,352 cycles of MMAs and, at 40 KB written and read each,
 // 5,440 cycles of shared memory; it measures 5,800.  2,048 new tokens x 64 heads over 16,384: 3.2 ms
-// in a short run (1.37 PFLOP/s), 3.46 ms back to back, where the GPU is at its power limit (1.27
+// in a short run (1.37 PFLOP/s), 3.5 ms back to back, where the GPU is at its power limit (1.25
 // PFLOP/s; a large library product sustains 1.39 there).  A part's first tile and its epilogue add
 // about 8,700 cycles.
 //
