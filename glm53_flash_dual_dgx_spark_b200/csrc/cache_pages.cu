@@ -172,6 +172,7 @@ bulk_copy_pages_kernel(const __grid_constant__ Caches c, const __grid_constant__
 __global__ void __launch_bounds__(256)
 free_pages_kernel(int32_t* tables, int64_t stride, int width, int64_t num_slots, int32_t* seq_lens,
                   const int32_t* __restrict__ slots, int32_t* refs, int64_t num_pages, int32_t* err) {
+    griddep_wait();
     const int slot = __ldg(slots + blockIdx.x);
     if (slot < 0 || slot >= num_slots) {
         if (threadIdx.x == 0) set_error(err, NVFP4KV_DEVERR_BAD_SLOT);
@@ -382,6 +383,7 @@ __device__ __forceinline__ void load_counts(const int32_t* refs, int64_t i0, int
 __global__ void __launch_bounds__(kPlanThreads) compact_count_kernel(const __grid_constant__ CompactArgs p) {
     __shared__ int sums[32];
     int r[kPer], live = 0, total;
+    griddep_wait();
     load_counts(p.refs, static_cast<int64_t>(blockIdx.x) * kBlockPages + threadIdx.x * kPer, p.num_pages, r);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) live += r[j] > 0;
@@ -568,8 +570,9 @@ extern "C" int nvfp4kv_free_pages(int32_t* block_tables, int64_t tables_stride, 
     if (!slots || !seq_lens) return fail(NVFP4KV_EINVAL, "nvfp4kv_free_pages: null pointer");
     int rc = check_tables("nvfp4kv_free_pages", block_tables, tables_stride, table_width, num_slots, ref_counts, num_pages);
     if (rc != NVFP4KV_OK) return rc;
-    free_pages_kernel<<<num, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-        block_tables, tables_stride, table_width, num_slots, seq_lens, slots, ref_counts, num_pages, err_flag);
+    const cudaError_t e = launch_dependent(free_pages_kernel, dim3(num), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), block_tables,
+                                           tables_stride, table_width, num_slots, seq_lens, slots, ref_counts, num_pages, err_flag);
+    if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_free_pages launch failed: %s", cudaGetErrorString(e));
     return check_launch("nvfp4kv_free_pages");
 }
 
@@ -636,12 +639,10 @@ extern "C" int nvfp4kv_compact_pages(const void* const* caches, const int64_t* p
     a.tables = block_tables; a.stride = tables_stride; a.width = table_width; a.num_slots = num_slots;
     a.out_tables = out_tables; a.out_stride = out_tables_stride; a.err = err_flag;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (blocks > 1) {
-        compact_count_kernel<<<blocks, kPlanThreads, 0, st>>>(a);
-        if ((rc = check_launch("nvfp4kv_compact_pages count")) != NVFP4KV_OK) return rc;
-    }
     const int64_t want = (num_slots * table_width + 255) / 256, most = 8 * device_sm_count();
-    cudaError_t e = launch_dependent(compact_plan_kernel, dim3(blocks), dim3(kPlanThreads), 0, st, a);
+    cudaError_t e = cudaSuccess;
+    if (blocks > 1) e = launch_dependent(compact_count_kernel, dim3(blocks), dim3(kPlanThreads), 0, st, a);
+    if (e == cudaSuccess) e = launch_dependent(compact_plan_kernel, dim3(blocks), dim3(kPlanThreads), 0, st, a);
     if (e == cudaSuccess)
         e = launch_dependent(compact_tables_kernel, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(256), 0, st, a);
     if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_compact_pages launch failed: %s", cudaGetErrorString(e));

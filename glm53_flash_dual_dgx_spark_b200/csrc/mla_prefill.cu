@@ -495,6 +495,7 @@ __device__ __forceinline__ uint4 dequant8(uint32_t code, uint32_t scale2) {
 __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_constant__ PrefillParams p) {
     __shared__ uint32_t bits[2];      // of the piece's tokens: those that exist, those that hold a NaN
     __shared__ int b_s, pos_s, total_s;
+    griddep_wait();                   // first: what starts now counts on all before this grid being done
     griddep_launch_dependents();
     const int tid = threadIdx.x, lp = tid & 7, r0 = tid >> 3;
     int total = 0x7FFFFFFF;
@@ -1347,8 +1348,9 @@ extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_
         cudaError_t e = cudaSuccess;
         if (pl.image_blocks > 0) {
             const int most = 8 * device_sm_count();
-            prefill_image_kernel<<<kImagePieces * pl.image_blocks < most ? kImagePieces * pl.image_blocks : most, 256, 0, st>>>(p);
-            if ((rc = check_launch("nvfp4kv_mla_prefill image")) != NVFP4KV_OK) return rc;
+            const int blocks = kImagePieces * pl.image_blocks;
+            e = launch_dependent(prefill_image_kernel, dim3(blocks < most ? blocks : most), dim3(256), 0, st, p);
+            if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill image launch failed: %s", cudaGetErrorString(e));
             // its set-up overlaps the image kernel; all else it reads was there before that one
             e = launch_dependent(mla_prefill_kernel, grid, dim3(kThreads), kSmemBytes, st, p);
         } else {

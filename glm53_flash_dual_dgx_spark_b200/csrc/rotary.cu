@@ -9,6 +9,7 @@
 #include "../../include/nvfp4kv_serving.h"
 #include "abi_common.h"
 #include "common.cuh"
+#include "decode_shared.h"
 
 namespace nvfp4kv {
 namespace {
@@ -140,6 +141,7 @@ __global__ void __launch_bounds__(256, kInterleaved && sizeof(T) == 2 ? 8 : 4) r
     }
     const uint32_t j0 = static_cast<uint32_t>(u0 - row0 * p.units.d), h0 = static_cast<uint32_t>(row0 - t0 * p.by_heads.d);
     const int half = p.rotary / 2;
+    griddep_wait();
     Vec<T> a[kRopeSteps], b[kRopeSteps];
     int64_t t[kRopeSteps], at[kRopeSteps];
     int r[kRopeSteps];      // dim within the rotated part, -1 for a copy, -2 past the end
@@ -235,8 +237,8 @@ int launch_rope(RopeArgs a, int64_t tokens, bool interleaved, cudaStream_t st) {
         a.total = tokens * heads * units;
         blocks = (a.total + 256 * kRopeSteps - 1) / (256 * kRopeSteps);
         if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: too many rows for one call");
-        if (interleaved) rope_vec_kernel<T, true><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
-        else rope_vec_kernel<T, false><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+        const cudaError_t e = launch_dependent(interleaved ? rope_vec_kernel<T, true> : rope_vec_kernel<T, false>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a);
+        if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_rope launch failed: %s", cudaGetErrorString(e));
     } else {
         int hb = 1024 / a.dim;
         hb = hb < 1 ? 1 : (hb > a.heads ? a.heads : hb);
@@ -309,6 +311,7 @@ __global__ void __launch_bounds__(256) rope_append_rotated_kernel(const __grid_c
     const int64_t t0 = row0 < (1ll << 32) ? static_cast<int64_t>(static_cast<uint32_t>(row0) / p.rows_of_token.d) : row0 / p.rows_of_token.d;
     const uint32_t first = static_cast<uint32_t>(row0 - t0 * p.rows_of_token.d);
     const int u = threadIdx.x % kU;
+    griddep_wait();
     V a[kSteps], b[kSteps];
     int64_t t[kSteps];
     int h[kSteps];          // head, -1 for the key
@@ -432,12 +435,9 @@ extern "C" int nvfp4kv_append_rope_rotated(const void* k_pe, int64_t num_tokens,
     if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: too many rows for one call");
     const dim3 grid(static_cast<unsigned>(blocks));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (interleaved) {
-        if (vec) rope_append_rotated_kernel<true, true><<<grid, 256, 0, st>>>(a);
-        else rope_append_rotated_kernel<true, false><<<grid, 256, 0, st>>>(a);
-    } else {
-        if (vec) rope_append_rotated_kernel<false, true><<<grid, 256, 0, st>>>(a);
-        else rope_append_rotated_kernel<false, false><<<grid, 256, 0, st>>>(a);
-    }
+    void (*kernel)(RopeAppendArgs) = interleaved ? (vec ? rope_append_rotated_kernel<true, true> : rope_append_rotated_kernel<true, false>)
+                                                 : (vec ? rope_append_rotated_kernel<false, true> : rope_append_rotated_kernel<false, false>);
+    const cudaError_t e = launch_dependent(kernel, grid, dim3(256), 0, st, a);
+    if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_append_rope_rotated launch failed: %s", cudaGetErrorString(e));
     return check_launch("nvfp4kv_append_rope_rotated");
 }
