@@ -624,6 +624,13 @@ def _call(name: str, index: int, *args) -> None:
         _lib.check(rc, name)
 
 
+def _require_on(index: int, t: torch.Tensor, name: str) -> None:
+    """t is on CUDA device ``index``: a kernel that reads another device's memory may fault."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != index:
+        _require_cuda(t, name)
+        raise ValueError(f"{name} must be on cuda:{index} like the others")
+
+
 def _vector(t: torch.Tensor) -> torch.Tensor:
     return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
 
@@ -662,9 +669,9 @@ def rope_cos_sin(max_positions: int, rotary_dim: int = ROPE, base: float = 10000
     return (torch.cat([angle.cos(), angle.sin()], 1) * gain).float()
 
 
-def _check_angles(cos_sin: torch.Tensor, positions: torch.Tensor, T: int, rotary_dim: int):
-    _require_cuda(cos_sin, "cos_sin")
-    _require_cuda(positions, "positions")
+def _check_angles(index: int, cos_sin: torch.Tensor, positions: torch.Tensor, T: int, rotary_dim: int):
+    _require_on(index, cos_sin, "cos_sin")
+    _require_on(index, positions, "positions")
     if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != rotary_dim \
             or not cos_sin.is_contiguous():
         raise ValueError(f"cos_sin must be a contiguous float32 [positions, {rotary_dim}] table")
@@ -694,17 +701,18 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, 
         raise ValueError("x must be [T, H, D] or [T, D] with a contiguous last dimension")
     if out is None:
         out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    _require_cuda(out, "out")
+    index = x.get_device()
+    _require_on(index, out, "out")
     ost = out.stride()
     if out.shape != shape or out.dtype != x.dtype or ost[-1] != 1:
         raise ValueError("out must have x's shape and dtype and a contiguous last dimension")
     T, D = shape[0], shape[-1]
     H, sh, osh = (shape[1], st[1], ost[1]) if len(shape) == 3 else (1, D, D)
     P, r = cos_sin.shape
-    pos, pdt = _check_angles(cos_sin, positions, T, r)
+    pos, pdt = _check_angles(index, cos_sin, positions, T, r)
     if T == 0 or H == 0:
         return out
-    _call("nvfp4kv_rope", x.get_device(), x.data_ptr(), dtype, T, H, D, st[0], sh, pos.data_ptr(), pdt,
+    _call("nvfp4kv_rope", index, x.data_ptr(), dtype, T, H, D, st[0], sh, pos.data_ptr(), pdt,
           cos_sin.data_ptr(), P, r, D - r if rope_offset is None else int(rope_offset), int(interleaved),
           int(inverse), out.data_ptr(), ost[0], osh)
     return out
@@ -717,7 +725,8 @@ def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_
     into the rope side-pool at slot_mapping (as write_nvfp4_rope), and the queries' rope dims
     q_pe [T, H, 64] bf16 rotated into q_out (default: in place).  Returns q_out."""
     _require_cuda(k_pe, "k_pe")
-    _require_cuda(rope_cache, "rope_cache")
+    index = k_pe.get_device()
+    _require_on(index, rope_cache, "rope_cache")
     ks, (T, width) = k_pe.stride(), k_pe.shape if k_pe.dim() == 2 else (0, 0)
     if width < ROPE or k_pe.dtype is not torch.bfloat16 or ks[1] != 1:
         raise ValueError("k_pe must be bf16 [T, >=64] with a contiguous last dimension")
@@ -726,24 +735,24 @@ def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_
     rows, rest = divmod(rope_cache.numel(), ROPE)
     if rest or not rope_cache.is_contiguous():
         raise ValueError("rope_cache must be contiguous rows of 64")
-    _require_cuda(slot_mapping, "slot_mapping")
+    _require_on(index, slot_mapping, "slot_mapping")
     slot = _vector(slot_mapping)
     if slot.shape[0] != T:
         raise ValueError(f"slot_mapping has {slot.shape[0]} entries for {T} tokens")
     sdt = _INDEX_DTYPES.get(slot.dtype)
     if sdt is None:
         raise TypeError("slot_mapping must be int64 or int32")
-    pos, pdt = _check_angles(cos_sin, positions, T, ROPE)
+    pos, pdt = _check_angles(index, cos_sin, positions, T, ROPE)
     H, qs, qos, q_ptr, qo_ptr = 0, (0, 0), (0, 0), None, None
     if q_pe is not None:
-        _require_cuda(q_pe, "q_pe")
+        _require_on(index, q_pe, "q_pe")
         shape, qs = q_pe.shape, q_pe.stride()
         if len(shape) != 3 or shape[0] != T or shape[2] != ROPE or qs[2] != 1 or q_pe.dtype is not torch.bfloat16:
             raise ValueError("q_pe must be bf16 [T, H, 64] with a contiguous last dimension")
         if q_out is None or q_out is q_pe:
             q_out, qos = q_pe, qs
         else:
-            _require_cuda(q_out, "q_out")
+            _require_on(index, q_out, "q_out")
             qos = q_out.stride()
             if q_out.shape != shape or qos[2] != 1 or q_out.dtype is not torch.bfloat16:
                 raise ValueError("q_out must be bf16 of q_pe's shape with a contiguous last dimension")
@@ -754,7 +763,7 @@ def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_
         raise ValueError("q_out without q_pe")
     if T == 0:
         return q_out
-    _call("nvfp4kv_append_rope_rotated", k_pe.get_device(), k_pe.data_ptr(), T, ks[0], rope_cache.data_ptr(),
+    _call("nvfp4kv_append_rope_rotated", index, k_pe.data_ptr(), T, ks[0], rope_cache.data_ptr(),
           rows, slot.data_ptr(), sdt, pos.data_ptr(), pdt, cos_sin.data_ptr(),
           cos_sin.shape[0], int(interleaved), q_ptr, H, qs[0], qs[1], qo_ptr, qos[0], qos[1])
     return q_out
@@ -776,14 +785,16 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
     synchronises the host.  Returns out [T, H, kv_lora_rank] bf16, with ``return_lse`` also
     lse [T, H] float32 (natural log; -inf for a row that sees no token, whose out is zeros)."""
     try:      # (the whole host side of a call is about as long as a short batch on the device)
-        on_device = query.is_cuda and kv_cache.is_cuda and block_tables.is_cuda and cu_seqlens_q.is_cuda \
-            and seq_lens.is_cuda and (rope_cache is None or rope_cache.is_cuda)
+        index = query.get_device()
+        together = index >= 0 and kv_cache.get_device() == block_tables.get_device() == cu_seqlens_q.get_device() \
+            == seq_lens.get_device() == index and (rope_cache is None or rope_cache.get_device() == index)
     except AttributeError:
-        on_device = False
-    if not on_device:
-        for name, t in (("query", query), ("kv_cache", kv_cache), ("block_tables", block_tables),
-                        ("cu_seqlens_q", cu_seqlens_q), ("seq_lens", seq_lens), ("rope_cache", rope_cache)):
-            _require_cuda(t, name)
+        together = False
+    if not together:
+        _require_cuda(query, "query")
+        for name, t in (("kv_cache", kv_cache), ("block_tables", block_tables), ("cu_seqlens_q", cu_seqlens_q),
+                        ("seq_lens", seq_lens), ("rope_cache", rope_cache)):
+            _require_on(query.get_device(), t, name)
     if isinstance(bmm1_scale, torch.Tensor) or isinstance(bmm2_scale, torch.Tensor):
         raise TypeError("bmm1_scale / bmm2_scale must be Python floats (a device scalar would need a sync)")
     qs = query.stride()
@@ -812,7 +823,7 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
         os = (H * LATENT, LATENT)
     else:
         os = out.stride()
-        if not out.is_cuda or out.shape != (T, H, LATENT) or out.dtype is not torch.bfloat16 or os[2] != 1:
+        if out.get_device() != index or out.shape != (T, H, LATENT) or out.dtype is not torch.bfloat16 or os[2] != 1:
             raise ValueError("out must be bf16 [T, H, 512] on the device with a contiguous last dimension")
     rope = None
     if rope_cache is not None:
@@ -821,7 +832,6 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
         rope = rope_cache.data_ptr()
     lse = query.new_empty((T, H), dtype=torch.float32) if return_lse else None
     if T > 0 and B > 0:
-        index = query.get_device()
         key = ("prefill", B, T, H, max_q_len, max_seq_len, index)
         need = _ws_sizes.get(key)
         if need is None:
@@ -834,7 +844,7 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
                 _ws_sizes.clear()
             need = _ws_sizes[key] = int(n.value)
         ws = workspace_buffer
-        if ws is None or not ws.is_cuda or not ws.is_contiguous() or ws.data_ptr() % 256 \
+        if ws is None or ws.get_device() != index or not ws.is_contiguous() or ws.data_ptr() % 256 \
                 or ws.numel() * ws.element_size() < need:
             ws = _stream_buffer(index, "prefill_ws", need, torch.uint8)
         _call("nvfp4kv_mla_prefill", index, query.data_ptr(), qs[0], qs[1], kv_cache.data_ptr(), rows, rope,
@@ -853,13 +863,15 @@ def _cache_list(caches):
     """(device pointers, bytes per page, pages, page size) of pools [num_pages, page_size, ...]."""
     if not caches:
         raise ValueError("caches must name at least one pool")
+    _require_cuda(caches[0], "caches")
+    index = caches[0].get_device()
     pages, size = caches[0].shape[:2]
     n = len(caches)
     if n > _MAX_CACHES:
         raise ValueError(f"at most {_MAX_CACHES} caches in one call")
     ptrs, sizes = _POINTERS(), _SIZES()
     for k, c in enumerate(caches):
-        _require_cuda(c, "caches")
+        _require_on(index, c, "caches")
         shape = c.shape
         if len(shape) < 3 or shape[0] != pages or shape[1] != size or not c.is_contiguous():
             raise ValueError("caches must be contiguous [num_pages, page_size, ...] pools of one geometry")
@@ -868,12 +880,13 @@ def _cache_list(caches):
     return ptrs, sizes, n, pages, size
 
 
-def _check_int32(**tensors):
+def _check_int32(index: int, **tensors):
     for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor) or t.get_device() != index:
+            _require_on(index, t, name)
         st = t.stride()
-        if t.dtype is torch.int32 and t.is_cuda and st[-1] == 1 and len(st) == (2 if name.endswith("tables") else 1):
+        if t.dtype is torch.int32 and len(st) == (2 if name.endswith("tables") else 1) and st[-1] == 1:
             continue
-        _require_cuda(t, name)
         if t.dtype != torch.int32:
             raise TypeError(f"{name} must be int32")
         if name.endswith("tables"):
@@ -901,10 +914,11 @@ def copy_pages(caches, src: torch.Tensor, dst: torch.Tensor) -> None:
     latent rows, rope rows, indexer rows).  Negative ids skip the pair.  A page may not be a
     source and a destination, nor a destination twice."""
     ptrs, sizes, n, pages, _ = _cache_list(caches)
-    _check_int32(src=src, dst=dst)
+    index = caches[0].get_device()
+    _check_int32(index, src=src, dst=dst)
     if src.numel() != dst.numel():
         raise ValueError("src and dst must have the same length")
-    _call("nvfp4kv_copy_pages", caches[0].get_device(), ptrs, sizes, n, pages, src.data_ptr(), dst.data_ptr(),
+    _call("nvfp4kv_copy_pages", index, ptrs, sizes, n, pages, src.data_ptr(), dst.data_ptr(),
           src.shape[0])
 
 
@@ -912,11 +926,13 @@ def free_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, slots: torch.
                ref_counts: torch.Tensor) -> None:
     """Empties the sequences in ``slots``: their pages lose one reference each (0 = free), their
     rows of block_tables [num_slots, width] become -1 and their seq_lens 0, in place."""
-    _check_int32(block_tables=block_tables, seq_lens=seq_lens, slots=slots, ref_counts=ref_counts)
+    _require_cuda(block_tables, "block_tables")
+    index = block_tables.get_device()
+    _check_int32(index, block_tables=block_tables, seq_lens=seq_lens, slots=slots, ref_counts=ref_counts)
     if seq_lens.numel() != block_tables.shape[0]:
         raise ValueError("seq_lens must have one entry per row of block_tables")
     S, width = block_tables.shape
-    _call("nvfp4kv_free_pages", block_tables.get_device(), block_tables.data_ptr(), block_tables.stride(0), width, S,
+    _call("nvfp4kv_free_pages", index, block_tables.data_ptr(), block_tables.stride(0), width, S,
           seq_lens.data_ptr(), slots.data_ptr(), slots.shape[0], ref_counts.data_ptr(), ref_counts.shape[0])
 
 
@@ -927,12 +943,12 @@ def fork_pages(caches, block_tables: torch.Tensor, seq_lens: torch.Tensor, src: 
     page are copied in every pool of ``caches`` into the lowest free page (ref_counts == 0), in
     order of k.  Beams and samples that share a prompt; see free_pages for the way back."""
     ptrs, sizes, n, pages, size = _cache_list(caches)
-    _check_int32(block_tables=block_tables, seq_lens=seq_lens, src=src, dst=dst, ref_counts=ref_counts)
-    if src.numel() != dst.numel():
+    index, num = caches[0].get_device(), src.numel()
+    _check_int32(index, block_tables=block_tables, seq_lens=seq_lens, src=src, dst=dst, ref_counts=ref_counts)
+    if num != dst.numel():
         raise ValueError("src and dst must have the same length")
     if seq_lens.numel() != block_tables.shape[0] or ref_counts.numel() != pages:
         raise ValueError("seq_lens must have one entry per row of block_tables, ref_counts one per page")
-    index, num = block_tables.get_device(), src.shape[0]
     ws = _stream_buffer(index, "fork_ws", max(3 * num, 1024), torch.int32)
     S, width = block_tables.shape
     _call("nvfp4kv_fork_pages", index, ptrs, sizes, n, size, block_tables.data_ptr(), block_tables.stride(0), width, S,
@@ -950,12 +966,12 @@ def compact_pages(caches, block_tables: torch.Tensor, ref_counts: torch.Tensor, 
     ptrs, sizes, n, pages, _ = _cache_list(caches)
     out_tables = block_tables if out_tables is None else out_tables
     out_ref_counts = ref_counts if out_ref_counts is None else out_ref_counts
-    _check_int32(block_tables=block_tables, ref_counts=ref_counts)
+    index = caches[0].get_device()
+    _check_int32(index, block_tables=block_tables, ref_counts=ref_counts)
     if out_tables is not block_tables or out_ref_counts is not ref_counts:
-        _check_int32(out_tables=out_tables, out_ref_counts=out_ref_counts)
+        _check_int32(index, out_tables=out_tables, out_ref_counts=out_ref_counts)
     if ref_counts.numel() != pages or out_ref_counts.numel() != pages or out_tables.shape != block_tables.shape:
         raise ValueError("ref_counts must have one entry per page, out_tables block_tables' shape")
-    index = block_tables.get_device()
     live = block_tables.new_empty(())
     need = _ws_sizes.get(("compact", pages))
     if need is None:

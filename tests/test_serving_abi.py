@@ -129,3 +129,21 @@ def test_python_entries_refuse_cpu_tensors_and_bad_tables():
         rt.copy_pages([], None, None)
     with pytest.raises(ValueError, match="rotary_dim"):
         rt.rope_cos_sin(8, 63)
+
+
+def test_tensors_of_another_device_are_refused():
+    class Elsewhere(torch.Tensor):
+        """A CPU tensor that says it is on the second GPU."""
+        is_cuda = True
+
+        def get_device(self):
+            return 1
+
+    t = torch.zeros(4).as_subclass(Elsewhere)
+    rt._require_on(1, t, "t")
+    with pytest.raises(ValueError, match="t must be on cuda:0"):
+        rt._require_on(0, t, "t")
+    with pytest.raises(ValueError, match="must be a CUDA tensor"):
+        rt._require_on(0, torch.zeros(4), "t")
+    with pytest.raises(ValueError, match="must be a CUDA tensor"):
+        rt._require_on(0, None, "t")
