@@ -856,11 +856,12 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
 
 # ------------------------------------------------------------------ page upkeep
 _MAX_CACHES = 8        # NVFP4KV_MAX_CACHES
+_INT32 = torch.int32
 _POINTERS, _SIZES = ctypes.c_void_p * _MAX_CACHES, ctypes.c_int64 * _MAX_CACHES
 
 
 def _cache_list(caches):
-    """(device pointers, bytes per page, pages, page size) of pools [num_pages, page_size, ...]."""
+    """(device pointers, bytes per page, their number, pages, page size, device) of pools [num_pages, page_size, ...]."""
     if not caches:
         raise ValueError("caches must name at least one pool")
     _require_cuda(caches[0], "caches")
@@ -871,22 +872,34 @@ def _cache_list(caches):
         raise ValueError(f"at most {_MAX_CACHES} caches in one call")
     ptrs, sizes = _POINTERS(), _SIZES()
     for k, c in enumerate(caches):
-        _require_on(index, c, "caches")
+        if k:
+            _require_on(index, c, "caches")
         shape = c.shape
         if len(shape) < 3 or shape[0] != pages or shape[1] != size or not c.is_contiguous():
             raise ValueError("caches must be contiguous [num_pages, page_size, ...] pools of one geometry")
         ptrs[k] = c.data_ptr()
         sizes[k] = c.nbytes // pages if pages else size
-    return ptrs, sizes, n, pages, size
+    return ptrs, sizes, n, pages, size, index
+
+
+def _ints(index: int, *vectors) -> bool:
+    """Whether all are contiguous int32 vectors on the device."""
+    for t in vectors:
+        if not isinstance(t, torch.Tensor) or t.dtype is not _INT32 or t.get_device() != index or t.dim() != 1 or not t.is_contiguous():
+            return False
+    return True
+
+
+def _tables(index: int, tables: torch.Tensor, strides, *vectors) -> bool:
+    """Whether ``tables`` is an int32 [slots, width] on the device with contiguous rows and the others
+    are _ints."""
+    return tables.dtype is _INT32 and len(strides) == 2 and strides[1] == 1 and _ints(index, *vectors)
 
 
 def _check_int32(index: int, **tensors):
+    """Says which of a call's tensors is not what it has to be."""
     for name, t in tensors.items():
-        if not isinstance(t, torch.Tensor) or t.get_device() != index:
-            _require_on(index, t, name)
-        st = t.stride()
-        if t.dtype is torch.int32 and len(st) == (2 if name.endswith("tables") else 1) and st[-1] == 1:
-            continue
+        _require_on(index, t, name)
         if t.dtype != torch.int32:
             raise TypeError(f"{name} must be int32")
         if name.endswith("tables"):
@@ -913,9 +926,9 @@ def copy_pages(caches, src: torch.Tensor, dst: torch.Tensor) -> None:
     """Pages src[k] -> dst[k] (int32) of every pool in ``caches`` ([num_pages, page_size, ...] each:
     latent rows, rope rows, indexer rows).  Negative ids skip the pair.  A page may not be a
     source and a destination, nor a destination twice."""
-    ptrs, sizes, n, pages, _ = _cache_list(caches)
-    index = caches[0].get_device()
-    _check_int32(index, src=src, dst=dst)
+    ptrs, sizes, n, pages, _, index = _cache_list(caches)
+    if not _ints(index, src, dst):
+        _check_int32(index, src=src, dst=dst)
     if src.numel() != dst.numel():
         raise ValueError("src and dst must have the same length")
     _call("nvfp4kv_copy_pages", index, ptrs, sizes, n, pages, src.data_ptr(), dst.data_ptr(),
@@ -927,13 +940,14 @@ def free_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, slots: torch.
     """Empties the sequences in ``slots``: their pages lose one reference each (0 = free), their
     rows of block_tables [num_slots, width] become -1 and their seq_lens 0, in place."""
     _require_cuda(block_tables, "block_tables")
-    index = block_tables.get_device()
-    _check_int32(index, block_tables=block_tables, seq_lens=seq_lens, slots=slots, ref_counts=ref_counts)
-    if seq_lens.numel() != block_tables.shape[0]:
-        raise ValueError("seq_lens must have one entry per row of block_tables")
+    index, st = block_tables.get_device(), block_tables.stride()
+    if not _tables(index, block_tables, st, seq_lens, slots, ref_counts):
+        _check_int32(index, block_tables=block_tables, seq_lens=seq_lens, slots=slots, ref_counts=ref_counts)
     S, width = block_tables.shape
-    _call("nvfp4kv_free_pages", index, block_tables.data_ptr(), block_tables.stride(0), width, S,
-          seq_lens.data_ptr(), slots.data_ptr(), slots.shape[0], ref_counts.data_ptr(), ref_counts.shape[0])
+    if seq_lens.numel() != S:
+        raise ValueError("seq_lens must have one entry per row of block_tables")
+    _call("nvfp4kv_free_pages", index, block_tables.data_ptr(), st[0], width, S, seq_lens.data_ptr(), slots.data_ptr(),
+          slots.numel(), ref_counts.data_ptr(), ref_counts.numel())
 
 
 def fork_pages(caches, block_tables: torch.Tensor, seq_lens: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
@@ -942,18 +956,21 @@ def fork_pages(caches, block_tables: torch.Tensor, seq_lens: torch.Tensor, src: 
     full pages are shared (one reference more each), the filled rows of a partly filled last
     page are copied in every pool of ``caches`` into the lowest free page (ref_counts == 0), in
     order of k.  Beams and samples that share a prompt; see free_pages for the way back."""
-    ptrs, sizes, n, pages, size = _cache_list(caches)
-    index, num = caches[0].get_device(), src.numel()
-    _check_int32(index, block_tables=block_tables, seq_lens=seq_lens, src=src, dst=dst, ref_counts=ref_counts)
+    ptrs, sizes, n, pages, size, index = _cache_list(caches)
+    _require_on(index, block_tables, "block_tables")
+    st = block_tables.stride()
+    if not _tables(index, block_tables, st, seq_lens, src, dst, ref_counts):
+        _check_int32(index, block_tables=block_tables, seq_lens=seq_lens, src=src, dst=dst, ref_counts=ref_counts)
+    num = src.numel()
     if num != dst.numel():
         raise ValueError("src and dst must have the same length")
-    if seq_lens.numel() != block_tables.shape[0] or ref_counts.numel() != pages:
-        raise ValueError("seq_lens must have one entry per row of block_tables, ref_counts one per page")
-    ws = _stream_buffer(index, "fork_ws", max(3 * num, 1024), torch.int32)
     S, width = block_tables.shape
-    _call("nvfp4kv_fork_pages", index, ptrs, sizes, n, size, block_tables.data_ptr(), block_tables.stride(0), width, S,
+    if seq_lens.numel() != S or ref_counts.numel() != pages:
+        raise ValueError("seq_lens must have one entry per row of block_tables, ref_counts one per page")
+    ws = _stream_buffer(index, "fork_ws", max(3 * num, 1024), _INT32)
+    _call("nvfp4kv_fork_pages", index, ptrs, sizes, n, size, block_tables.data_ptr(), st[0], width, S,
           seq_lens.data_ptr(), src.data_ptr(), dst.data_ptr(), num, ref_counts.data_ptr(), pages, ws.data_ptr(),
-          ws.shape[0])
+          ws.numel())
 
 
 def compact_pages(caches, block_tables: torch.Tensor, ref_counts: torch.Tensor, out_tables: torch.Tensor | None = None,
@@ -963,13 +980,20 @@ def compact_pages(caches, block_tables: torch.Tensor, ref_counts: torch.Tensor, 
     with it are written to out_tables / out_ref_counts (default: in place; an engine whose
     running step still reads the old tables gives others).  Returns the number of pages in use,
     int32 [] on the device."""
-    ptrs, sizes, n, pages, _ = _cache_list(caches)
-    out_tables = block_tables if out_tables is None else out_tables
-    out_ref_counts = ref_counts if out_ref_counts is None else out_ref_counts
-    index = caches[0].get_device()
-    _check_int32(index, block_tables=block_tables, ref_counts=ref_counts)
-    if out_tables is not block_tables or out_ref_counts is not ref_counts:
-        _check_int32(index, out_tables=out_tables, out_ref_counts=out_ref_counts)
+    ptrs, sizes, n, pages, _, index = _cache_list(caches)
+    _require_on(index, block_tables, "block_tables")
+    ost = st = block_tables.stride()
+    if not _tables(index, block_tables, st, ref_counts):
+        _check_int32(index, block_tables=block_tables, ref_counts=ref_counts)
+    if out_tables is None:
+        out_tables = block_tables
+    else:
+        _check_int32(index, out_tables=out_tables)
+        ost = out_tables.stride()
+    if out_ref_counts is None:
+        out_ref_counts = ref_counts
+    else:
+        _check_int32(index, out_ref_counts=out_ref_counts)
     if ref_counts.numel() != pages or out_ref_counts.numel() != pages or out_tables.shape != block_tables.shape:
         raise ValueError("ref_counts must have one entry per page, out_tables block_tables' shape")
     live = block_tables.new_empty(())
@@ -980,7 +1004,7 @@ def compact_pages(caches, block_tables: torch.Tensor, ref_counts: torch.Tensor, 
         need = _ws_sizes["compact", pages] = int(n64.value)
     ws = _stream_buffer(index, "compact_ws", need, torch.int32)
     S, width = block_tables.shape
-    _call("nvfp4kv_compact_pages", index, ptrs, sizes, n, block_tables.data_ptr(), block_tables.stride(0), width, S,
-          ref_counts.data_ptr(), pages, out_tables.data_ptr(), out_tables.stride(0), out_ref_counts.data_ptr(),
-          live.data_ptr(), ws.data_ptr(), ws.shape[0])
+    _call("nvfp4kv_compact_pages", index, ptrs, sizes, n, block_tables.data_ptr(), st[0], width, S,
+          ref_counts.data_ptr(), pages, out_tables.data_ptr(), ost[0], out_ref_counts.data_ptr(), live.data_ptr(),
+          ws.data_ptr(), ws.numel())
     return live
