@@ -1157,7 +1157,7 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_const
 #pragma unroll 1
         for (int i = lane; i < n; i += 32) {
             const float2 ml = ml_of(i);
-            if (ml.y > 0.0f || ml.y != ml.y) m = fmaxf(m, ml.x);
+            if (ml.y > 0.0f) m = fmaxf(m, ml.x);
         }
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
@@ -1166,7 +1166,8 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_const
             float w = 0.0f;
             if (i < n) {
                 const float2 ml = ml_of(i);
-                if (ml.y > 0.0f || ml.y != ml.y) w = exp2f(ml.x - m);
+                if (ml.y > 0.0f) w = exp2f(ml.x - m);
+                if (ml.y != ml.y) w = ml.y;      // a NaN counts whatever its part's maximum, which no NaN raises
                 if (w != 0.0f) l += w * ml.y;
             }
             wts[i][warp] = w;
