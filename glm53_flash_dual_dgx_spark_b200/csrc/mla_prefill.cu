@@ -44,8 +44,11 @@
 // Numbers: a code times its e4m3 scale is exact in fp16, q is scaled per row by a power of two and
 // then exact in fp16 (but for parts below 2^-35 of the row's largest), the rope part stays bf16;
 // products accumulate in fp32.  Probabilities are fp16 (11 bits; bf16 would add as much error as
-// the output's own rounding), their sums fp32 and of the unrounded values.  A row's maximum moves
-// only when a tile exceeds it by 2^8, so O is rarely rescaled and P stays far from fp16's largest.
+// the output's own rounding), their sums fp32 and of the unrounded values.  A row's reference is
+// 2^7 below its maximum and moves only when a tile exceeds that by 2^8, so O is rarely rescaled, P
+// stays at or below 2^15 (fp16's largest is 65504), and a long flat tail under one high score keeps
+// its mass: what fp16 rounds away of a probability is at most 2^-32 of the largest (with P = 1 at the
+// maximum it is 2^-25, and 131,072 tokens at exp(-18) of one score lost all of theirs).
 //
 // Warps: 0-7 softmax (a row's 256 scores over four of them) and epilogue, 8-11 Q, 12 issues the
 // MMAs (in the leading CTA), 13-14 image copies, 15 hands landed copies to the leader.  Every wait is
@@ -74,7 +77,8 @@ constexpr uint32_t kRegsLaunch = 128, kRegsSoftmax = 160, kRegsQ = 128, kRegsCtl
 constexpr int kQRows = 4;                       // rows of Q a warp converts at a time
 static_assert(256 * kRegsSoftmax + 128 * kRegsQ + 128 * kRegsCtl <= kThreads * kRegsLaunch,
               "the register split stays within what the block is launched with");
-constexpr float kRescaleLog2 = 8.0f;
+constexpr float kRescaleLog2 = 8.0f;             // how far scores may pass the maximum that set the reference,
+constexpr float kTopLog2 = 7.0f;                // and log2 of P there
 constexpr int kMaxPairs = 128;
 constexpr int kImageTok = 128;                  // tokens of an image block
 constexpr int kImagePieces = kImageTok / 32;    // a block of the image kernel does 32 at a time
@@ -135,7 +139,7 @@ struct PrefillParams {
     int64_t o_st, o_sh;
     float* lse;
     PartInfo* parts;    // [pairs][2]: the range's first part of a unit, and its last one
-    float* part_ml;     // [pairs][2][128][2]: maximum (log2 units), sum
+    float* part_ml;     // [pairs][2][128][2]: reference (log2 units), sum
     float* part_o;      // [pairs][2][64 chunks of 8 dims][128 rows][8]
     uint8_t* q_scratch; // [pairs][2 CTAs][kQBytes]: the next part's Q
     uint8_t* image;     // [blocks][8 or 9 atoms][128 tokens x 128 B]
@@ -964,10 +968,12 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 named_bar_sync(1 + (sp & 1), 128);
                 const float m = fmaxf(fmaxf(slot[row], slot[64 + row]), fmaxf(slot[128 + row], slot[192 + row]));
                 float alpha = 1.0f;
-                if (m > m_ref + kRescaleLog2 || (m_ref == -INFINITY && m > -INFINITY)) {
-                    alpha = m_ref == -INFINITY ? 0.0f : ex2_approx(m_ref - m);
+                // (a difference: exact near the limit, true of a row's first score, false of equal infinities)
+                if (m - m_ref > kRescaleLog2 + kTopLog2) {
+                    const float next = m - kTopLog2;
+                    alpha = m_ref == -INFINITY ? 0.0f : ex2_approx(m_ref - next);
                     l *= alpha;
-                    m_ref = m;
+                    m_ref = next;
                 }
                 const float base = m_ref == -INFINITY ? 0.0f : m_ref;
                 uint32_t pk[32];
