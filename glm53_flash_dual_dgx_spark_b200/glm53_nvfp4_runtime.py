@@ -648,8 +648,8 @@ def rope_cos_sin(max_positions: int, rotary_dim: int = ROPE, base: float = 10000
     (position interpolation), or, with ``original_positions`` (the trained length), by the YaRN
     rule: dims that turn more than ``beta_fast`` times over the trained length keep their
     frequency, those that turn less than ``beta_slow`` times are divided by ``factor``, the ones
-    between are blended linearly, and cos and sin carry ``attention_factor`` (default
-    0.1 ln(factor) + 1)."""
+    between (their range rounded outwards to whole dims) are blended linearly, and cos and sin
+    carry ``attention_factor`` (default 0.1 ln(factor) + 1)."""
     if rotary_dim < 2 or rotary_dim % 2 or max_positions < 1:
         raise ValueError("rotary_dim must be even and >= 2, max_positions >= 1")
     half = rotary_dim // 2
@@ -661,7 +661,8 @@ def rope_cos_sin(max_positions: int, rotary_dim: int = ROPE, base: float = 10000
         def dim_of(turns):      # the dim that turns `turns` times over the trained length
             return half * math.log(original_positions / (turns * 2 * math.pi)) / math.log(base)
 
-        lo, hi = max(math.floor(dim_of(beta_fast)), 0), min(math.ceil(dim_of(beta_slow)), half - 1)
+        # (hi may lie past the last dim: a long trained length leaves the ramp unfinished there)
+        lo, hi = max(math.floor(dim_of(beta_fast)), 0), min(math.ceil(dim_of(beta_slow)), rotary_dim - 1)
         blend = ((torch.arange(half, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
         inv = inv * (1 - blend) + inv / factor * blend
         gain = 0.1 * math.log(factor) + 1.0 if attention_factor is None else attention_factor
