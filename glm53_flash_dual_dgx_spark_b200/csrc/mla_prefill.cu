@@ -118,7 +118,7 @@ constexpr uint32_t kTS = 0, kTO = 256, kTmemCols = 512;
 // A part of a unit that another pair's part completes: what the combine kernel reads.
 struct __align__(16) PartInfo {
     int32_t used, head, tail, pad;
-    int32_t first, n, block, pad2;
+    int32_t first, rows, block, pad2;
 };
 
 struct PrefillParams {
@@ -246,18 +246,18 @@ __device__ __forceinline__ void set_registers() {
 
 // ------------------------------------------------------------------ the work and its ranges
 struct Seq {
-    int first, n, L;        // first new token in q, their number, tokens of the sequence (all clamped)
-    int rows, units;
+    int first, n, L;        // first new token in q, their number, tokens of the sequence (clamped to max_seq_len)
+    int rows, units;        // of its first max_q_len new tokens
 };
 __device__ __forceinline__ Seq load_seq(const PrefillParams& p, int b) {
     Seq s;
     const int lo = max(0, min(__ldg(p.cu + b), p.total_q)), hi = max(lo, min(__ldg(p.cu + b + 1), p.total_q));
     const int len = __ldg(p.seq_lens + b);
     s.first = lo;
-    s.n = min(hi - lo, p.max_q_len);
+    s.n = hi - lo;
     s.L = max(0, min(len, p.max_seq_len));
     if (hi - lo > p.max_q_len || len > p.max_seq_len) set_error(p.err, NVFP4KV_DEVERR_SEQ_LEN);
-    s.rows = s.n * p.heads;
+    s.rows = min(s.n, p.max_q_len) * p.heads;
     s.units = (s.rows + kUnitRows - 1) / kUnitRows;
     return s;
 }
@@ -1034,7 +1034,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                     p.lse[static_cast<int64_t>(t.first + tok) * p.heads + head] = any ? 0.69314718055994531f * (m_ref + log2f(l)) : -INFINITY;
             }
             if (!whole && threadIdx.x == 0 && cta == 0)
-                p.parts[2 * pair + (first_part ? 0 : 1)] = PartInfo{1, t.head, t.tail, 0, t.first, t.n, t.block, 0};
+                p.parts[2 * pair + (first_part ? 0 : 1)] = PartInfo{1, t.head, t.tail, 0, t.first, t.rows, t.block, 0};
             // Two pieces a step, 16 dims of each as 32-byte stores by the lanes that hold the rows, the next two
             // on their way from tensor memory.  Rolled up: this code runs once per part, and unrolled its
             // instructions took longer to arrive than to run.  (Whole rows of the output staged in shared
@@ -1135,7 +1135,7 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_const
     }
     __syncthreads();
     if (!head.used || !head.head || head.tail) return;
-    const int unit_row = head.block * kUnitRows + row0, rows = head.n * p.heads;
+    const int unit_row = head.block * kUnitRows + row0, rows = head.rows;
     if (unit_row >= rows) return;
     // part 0: the head; then the used first parts up to the first that ends the unit (a pair whose
     // range is empty has none)

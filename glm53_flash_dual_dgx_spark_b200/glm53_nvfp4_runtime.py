@@ -782,9 +782,13 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
     query [T, H, kv_lora_rank + qk_rope_head_dim] bf16: the new tokens of sequence b are
     cu_seqlens_q[b] .. cu_seqlens_q[b + 1], the last of its seq_lens[b] tokens; each sees the
     tokens up to itself.  kv_cache, block_tables, rope_cache and workspace_buffer as in
-    mla_decode (dense).  max_q_len and max_seq_len bound the device-side lengths; nothing
-    synchronises the host.  Returns out [T, H, kv_lora_rank] bf16, with ``return_lse`` also
-    lse [T, H] float32 (natural log; -inf for a row that sees no token, whose out is zeros)."""
+    mla_decode (dense).  max_q_len and max_seq_len bound the device-side lengths (a sequence past
+    either is flagged in the device error word: it ends at max_seq_len tokens, and only its first
+    max_q_len new tokens are computed); nothing synchronises the host.  Returns out
+    [T, H, kv_lora_rank] bf16, with ``return_lse`` also lse [T, H] float32 (natural log; -inf for
+    a row that sees no token, whose out is zeros).  Rows of new tokens past max_q_len, and rows
+    from cu_seqlens_q[-1] on (the padding of a captured batch), are not written: they hold what
+    was in ``out`` before, and anything where the call allocates it."""
     try:      # (the whole host side of a call is about as long as a short batch on the device)
         index = query.get_device()
         together = index >= 0 and kv_cache.get_device() == block_tables.get_device() == cu_seqlens_q.get_device() \

@@ -63,15 +63,17 @@ int nvfp4kv_append_rope_rotated(const void* k_pe, int64_t num_tokens, int64_t k_
  *    multiples of 8, 16-byte aligned.  The first 512 dims meet the latent rows; with rope_pool
  *    (the rope side-pool, may be NULL) dims [512, 576) meet its rows.
  * tables [batch, >= ceil(max_seq_len / page_size)] page ids (row stride tables_stride).
- *    seq_lens and cu_seqlens_q stay on the device; max_q_len and max_seq_len bound them
- *    (longer ones are clamped and set NVFP4KV_DEVERR_SEQ_LEN).
+ *    seq_lens and cu_seqlens_q stay on the device; max_q_len and max_seq_len bound them.  What
+ *    goes past them sets NVFP4KV_DEVERR_SEQ_LEN: a sequence ends at max_seq_len tokens, and of
+ *    more than max_q_len new tokens only the first max_q_len get their rows of out and lse.
  * out: bf16 [total_q, num_heads, 512] with strides (out_stride_t, out_stride_h), multiples of
  *    8, 16-byte aligned: softmax(bmm1_scale * q.k) . v * bmm2_scale.  A row that sees no token
  *    is zeros.  lse (may be NULL): fp32 [total_q, num_heads], the natural log of the sum of
  *    exp(bmm1_scale * q.k), -inf for such a row.
  * Tokens on a missing page (id outside the pool) are masked and set NVFP4KV_DEVERR_BAD_PAGE.
  * A hidden token never reaches a row, whatever its bytes hold.
- * cu_seqlens_q[batch] rows of out and lse are written, all of them if it is total_q.
+ * Rows of out and lse that belong to no sequence (those from cu_seqlens_q[batch] on) or to a new
+ * token past max_q_len are not written; every other row is.
  * pool_rows is a multiple of page_size below 2^31, page_size a power of two up to 4096.
  * workspace: nvfp4kv_mla_prefill_workspace_size() bytes, 256-byte aligned: a dequantised image
  *    of the contexts (1,152 bytes a token, max_seq_len for each sequence, at most 1 GiB or one
