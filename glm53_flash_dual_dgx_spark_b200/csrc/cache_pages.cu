@@ -147,6 +147,7 @@ bulk_copy_pages_kernel(const __grid_constant__ Caches c, const __grid_constant__
 #pragma unroll
     for (int st = 0; st < kAhead; ++st) load(st, st);
     uint32_t phase = 0;
+    int64_t done = 0;      // pieces whose load has landed
     for (int64_t i0 = 0; i0 < mine; i0 += kCopyStages, phase ^= 1) {
 #pragma unroll
         for (int st = 0; st < kCopyStages; ++st) {
@@ -156,14 +157,15 @@ bulk_copy_pages_kernel(const __grid_constant__ Caches c, const __grid_constant__
             bulk_commit_group();
             asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kCopyStages - kAhead) : "memory");
             load(i0 + st + kAhead, (st + kAhead) % kCopyStages);
+            ++done;
         }
         if (abort_flag) break;
     }
     bulk_wait_group_read0();
-    // (after a timed-out wait: the loads in flight land before the block's shared memory goes)
+    // (after a timed-out wait: the loads in flight, each in its own round's phase, land before the
+    // block's shared memory goes; those before have landed and begin no other phase)
     if (abort_flag)
-        for (int st = 0; st < kCopyStages; ++st)
-            if (bytes[st]) mbar_drain_wait(smem_u32(&bars[st]), phase);
+        for (int64_t i = done; i < done + kAhead && i < mine; ++i) mbar_drain_wait(smem_u32(&bars[i % kCopyStages]), (i / kCopyStages) & 1);
 }
 
 // ------------------------------------------------------------------ freeing
