@@ -79,6 +79,29 @@ class Long:
             at += n
 
 
+@pytest.mark.parametrize("new,ctx,H", [([1], [131072], 4), ([2], [131073], 64), ([1, 5, 64], [200001, 131072, 300000], 3)])
+def test_long_contexts(new, ctx, H):
+    p = Long(new, ctx, H, seed=H)
+    out, lse = p.run()
+    assert rt.device_errors() == 0
+    p.check(out, lse)
+
+
+def test_chunk_over_a_long_context():
+    p = Long([2048], [300000], 8, seed=1)
+    out, lse = p.run()
+    assert rt.device_errors() == 0
+    p.check(out, lse, rows=[(0, 0), (1, 7), (777, 3), (1023, 5), (1024, 0), (2046, 6), (2047, 7)])
+
+
+def test_real_images_of_more_than_the_cap_run_in_groups():
+    """Nine contexts whose images take 1.3 GB: the batch runs in two groups."""
+    p = Long([1, 3, 1, 1, 2, 1, 1, 1, 4], [131072] * 8 + [100001], 3, seed=2)
+    out, lse = p.run()
+    assert rt.device_errors() == 0
+    p.check(out, lse)
+
+
 @pytest.mark.parametrize("below", [15.0, 18.0, 20.0])
 @pytest.mark.parametrize("new,H,sink", [(1, 2, 0), (1, 2, 131070), (2048, 8, 0), (2048, 8, 77777)])
 def test_a_sink_over_a_long_flat_tail(new, H, sink, below):
