@@ -91,8 +91,9 @@ copy_pages_kernel(const __grid_constant__ Caches c, int64_t num_pages, const int
 
 // The same with bulk copies through shared memory: a block is one warp that keeps kCopyStages pieces
 // in flight, loads ahead of stores, and no data passes registers.  A page is cut into equal pieces of
-// at most kCopyBytes; the blocks take the pieces of all pairs in turn.  Compacting a 1.1 GB pool moves
-// 0.63 GB (read and written) in 97.5 us, 6.45 TB/s: as much as a plain copy.
+// at most kCopyBytes; the blocks take the pieces of all pairs in turn.  Compacting 42,405 pages of three
+// caches (1.32 GB, 35 % in use) moves 0.60 GB, read and written, in 97.5 us: 6.1 TB/s, 95 % of a plain
+// copy's rate.
 constexpr int kCopyStages = 8, kCopyBytes = 9216;
 struct CopyPieces {
     int first[NVFP4KV_MAX_CACHES + 1];      // a pair's first piece in each cache

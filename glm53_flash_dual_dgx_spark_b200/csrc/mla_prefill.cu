@@ -273,7 +273,7 @@ __device__ __forceinline__ int unit_tiles(const PrefillParams& p, const Seq& s, 
     return (unit_end(p, s, k) + kTile - 1) / kTile;
 }
 // Weights of the work: a tile, and what a unit adds (its first tile's and its epilogue's latency, about
-// 8,700 cycles of a tile's 5,700).  With one tile's weight for a unit, pairs with short units took 9 %
+// 8,700 cycles of a tile's 5,800).  With one tile's weight for a unit, pairs with short units took 9 %
 // longer than the mean in a batch of chunks, now 6.
 constexpr int kTileWeight = 2, kUnitWeight = 3;
 // Weight of the sequence's first K units.  A unit's tiles do not fall with k, so the sum goes over
