@@ -43,9 +43,10 @@
 //
 // Numbers: a code times its e4m3 scale is exact in fp16, q is scaled per row by a power of two and
 // then exact in fp16 (but for parts below 2^-35 of the row's largest), the rope part stays bf16;
-// products accumulate in fp32.  Probabilities are fp16 (11 bits; bf16 would add as much error as
-// the output's own rounding), their sums fp32 and of the unrounded values.  A row's reference is
-// 2^7 below its maximum and moves only when a tile exceeds that by 2^8, so O is rarely rescaled, P
+// products accumulate in fp32 (beside a rope part 2^50 times larger, the latent part keeps what is
+// above 2^-85 of it).  Probabilities are fp16 (11 bits; bf16 would add as much error as the output's
+// own rounding), their sums fp32 and of the unrounded values.  A row's reference is 2^7 below its
+// maximum and moves only when a tile exceeds that by 2^8, so O is rarely rescaled, P
 // stays at or below 2^15 (fp16's largest is 65504), and a long flat tail under one high score keeps
 // its mass: what fp16 rounds away of a probability is at most 2^-32 of the largest (with P = 1 at the
 // maximum it is 2^-25, and 131,072 tokens at exp(-18) of one score lost all of theirs).
@@ -573,8 +574,11 @@ __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_cons
 
 // ------------------------------------------------------------------ attention
 // Q of a unit: rows -> fp16 after a power of two per row that brings its largest |q| to [2^10, 2^11)
-// (the rope part by the same factor, in bf16).  A warp per row, 16 + 2 dims per lane, kQRows rows at
-// a time: r, r + step, ... of the CTA's 64.
+// (the rope part by the same factor, in bf16).  A rope part far larger than the rest sets the power
+// itself, kRopeLog2 above what the latent part would: with 2^100 for a tiny latent part its products
+// passed fp32's range.  A warp per row, 16 + 2 dims per lane, kQRows rows at a time: r, r + step, ...
+// of the CTA's 64.
+constexpr uint32_t kRopeLog2 = 50;
 struct QRows {
     uint4 u[kQRows][2];
     uint32_t rope[kQRows];
@@ -610,7 +614,8 @@ __device__ __forceinline__ void store_q(const PrefillParams& p, uint8_t* base, f
             hi = max(hi, w[j][i] & 0x7FFF0000u);
             lo = max(lo, w[j][i] & 0x7FFFu);
         }
-        amax[j] = max(hi, lo << 16);
+        const int rope = static_cast<int>(max(q.rope[j] & 0x7FFF0000u, (q.rope[j] & 0x7FFFu) << 16));
+        amax[j] = max(max(hi, lo << 16), static_cast<uint32_t>(max(rope - static_cast<int>(kRopeLog2 << 23), 0)));
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1)
