@@ -18,6 +18,7 @@ LIB_PATH = os.environ.get("NVFP4KV_LIB", os.path.join(HERE, "libnvfp4kv.so"))
 OK, EINVAL, EWORKSPACE, ECUDA = 0, 1, 2, 3
 DEVERR_TIMEOUT, DEVERR_BAD_SLOT, DEVERR_BAD_INDEX, DEVERR_BAD_PAGE, DEVERR_SEQ_LEN = 1, 2, 4, 8, 16
 DEVERR_CAPACITY = 32
+PAGE_TRIMMED, MAX_AXES, MAX_AXES_DIM = -2, 4, 256
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
 DIV_IEEE, DIV_TRITON = 0, 1
 INDEX_I64, INDEX_I32 = 0, 1
@@ -81,6 +82,12 @@ SERVING_SIGNATURES = {
                                          _P, _I, _P, _I64, _I,                 # positions, cos_sin, interleaved
                                          _P, _I, _I64, _I64, _P, _I64, _I64,   # q_pe, heads, strides, q_out, strides
                                          _P, _P]),
+    "nvfp4kv_rope_axes": (_I, [_P, _I, _I64, _I, _I, _I64, _I64,
+                               _P, _I, _I64, _I, _P, _P, _I64,   # positions, axis stride, axes, pair_axes, cos_sin
+                               _I, _I, _I, _I, _P, _I64, _I64, _P, _P]),
+    "nvfp4kv_append_rope_rotated_axes": (_I, [_P, _I64, _I64, _P, _I64, _P, _I,
+                                              _P, _I, _I64, _I, _P, _P, _I64, _I,
+                                              _P, _I, _I64, _I64, _P, _I64, _I64, _P, _P]),
     "nvfp4kv_mla_prefill": (_I, [_P, _I64, _I64, _P, _I64, _P,   # q + strides, pool, rows, rope
                                  _P, _I64, _P, _P,               # tables, cu_seqlens_q, seq_lens
                                  _I, _I, _I, _I, _I,             # batch, total_q, heads, dim_qk, rank
@@ -88,9 +95,19 @@ SERVING_SIGNATURES = {
                                  _P, _I64, _I64, _P,             # out + strides, lse
                                  _P, _SZ, _P, _P]),
     "nvfp4kv_mla_prefill_workspace_size": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(_SZ)]),
+    "nvfp4kv_mla_prefill_window": (_I, [_P, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _P,
+                                        _I, _I, _I, _I, _I, _I, _I, _I,
+                                        _I, _I,                  # window, sinks
+                                        _F, _F, _P, _I64, _I64, _P, _P, _SZ, _P, _P]),
+    "nvfp4kv_mla_prefill_window_workspace_size": (_I, [_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_SZ)]),
     "nvfp4kv_copy_pages": (_I, [_P, _P, _I, _I64, _P, _P, _I64, _P, _P]),
     "nvfp4kv_free_pages": (_I, [_P, _I64, _I, _I64, _P, _P, _I, _P, _I64, _P, _P]),
     "nvfp4kv_fork_pages": (_I, [_P, _P, _I, _I, _P, _I64, _I, _I64, _P, _P, _P, _I, _P, _I64, _P, _I64, _P, _P]),
+    "nvfp4kv_extend_pages": (_I, [_P, _I64, _I, _I64, _P, _P, _P, _P, _I, _I,    # tables .. seq_lens, slots, new, lens, num, page
+                                  _P, _I64, _I64,                                # ref_counts, pages, tokens
+                                  _P, _P, _P, _P, _P, _P, _I64, _P, _P]),
+    "nvfp4kv_extend_workspace_ints": (_I, [_I, _I64, _I64, ctypes.POINTER(_I64)]),
+    "nvfp4kv_trim_pages": (_I, [_P, _I64, _I, _I64, _P, _P, _I, _I, _I, _I, _P, _I64, _P, _P]),
     "nvfp4kv_compact_pages": (_I, [_P, _P, _I, _P, _I64, _I, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _P]),
     "nvfp4kv_compact_workspace_ints": (_I, [_I64, ctypes.POINTER(_I64)]),
 }

@@ -1,5 +1,6 @@
-// Upkeep of a paged cache whose pools share page ids: copying, forking, compacting and freeing
-// pages, all on the device and in stream order (no count comes back to the host).
+// Upkeep of a paged cache whose pools share page ids: extending, trimming, copying, forking,
+// compacting and freeing pages, all on the device and in stream order (no count comes back to the
+// host).
 //
 // The results are those of the sequential definition whatever order blocks run in: counts change
 // by integer atomics, which commute, and every choice (which free page, which fork of a twice
@@ -14,6 +15,7 @@ namespace nvfp4kv {
 namespace {
 
 constexpr int kPlanThreads = 1024;
+constexpr int kTrimmed = NVFP4KV_PAGE_TRIMMED;
 
 struct Caches {
     uint8_t* base[NVFP4KV_MAX_CACHES];
@@ -169,6 +171,16 @@ bulk_copy_pages_kernel(const __grid_constant__ Caches c, const __grid_constant__
         for (int64_t i = done; i < done + kAhead && i < mine; ++i) mbar_drain_wait(smem_u32(&bars[i % kCopyStages]), (i / kCopyStages) & 1);
 }
 
+// A page loses the reference of a table entry; one that has none left is left alone and reported.
+__device__ __forceinline__ void release_page(int32_t* refs, int64_t num_pages, int p, int32_t* err) {
+    if (p >= num_pages) {
+        set_error(err, NVFP4KV_DEVERR_BAD_PAGE);
+    } else if (atomicSub(refs + p, 1) <= 0) {
+        atomicAdd(refs + p, 1);
+        set_error(err, NVFP4KV_DEVERR_BAD_PAGE);
+    }
+}
+
 // ------------------------------------------------------------------ freeing
 // Block = slot (32 samples of 16,000 tokens: 3 us).  A table entry is taken with an exchange, so that a slot named twice gives its
 // pages back once; a decrement that finds no reference is undone and reported.
@@ -184,15 +196,259 @@ free_pages_kernel(int32_t* tables, int64_t stride, int width, int64_t num_slots,
     int32_t* row = tables + slot * stride;
     for (int j = threadIdx.x; j < width; j += blockDim.x) {
         const int p = atomicExch(row + j, -1);
-        if (p < 0) continue;
-        if (p >= num_pages) {
-            set_error(err, NVFP4KV_DEVERR_BAD_PAGE);
-        } else if (atomicSub(refs + p, 1) <= 0) {
-            atomicAdd(refs + p, 1);
-            set_error(err, NVFP4KV_DEVERR_BAD_PAGE);
-        }
+        if (p >= 0) release_page(refs, num_pages, p, err);
     }
     if (threadIdx.x == 0) seq_lens[slot] = 0;
+}
+
+// ------------------------------------------------------------------ trimming
+// Block = slot: the pages behind the window of the next token, at position len, and those past the
+// end.  An entry is taken with a compare-and-swap, so that a slot named twice gives its pages back once.
+__global__ void __launch_bounds__(256)
+trim_pages_kernel(int32_t* tables, int64_t stride, int width, int64_t num_slots, const int32_t* seq_lens,
+                  const int32_t* __restrict__ slots, int page, int window, int sinks, int32_t* refs, int64_t num_pages,
+                  int32_t* err) {
+    griddep_wait();
+    const int slot = __ldg(slots + blockIdx.x);
+    if (slot < 0 || slot >= num_slots) {
+        if (threadIdx.x == 0) set_error(err, NVFP4KV_DEVERR_BAD_SLOT);
+        return;
+    }
+    int32_t* row = tables + slot * stride;
+    const int len = max(0, seq_lens[slot]);
+    const int end = len / page + (len % page != 0);                            // pages of the sequence
+    // pages [lo, hi): all of their tokens are sinks' successors and older than the window
+    const int lo = sinks / page + (sinks % page != 0), hi = window > 0 && len >= window ? (len - window + 1) / page : 0;
+    auto take = [&](int j, int mark) {
+        const int p = row[j];
+        if (p >= 0 && atomicCAS(row + j, p, mark) == p) release_page(refs, num_pages, p, err);
+    };
+    for (int j = lo + threadIdx.x; j < min(hi, width); j += blockDim.x) take(j, kTrimmed);
+    for (int j = end + threadIdx.x; j < width; j += blockDim.x) take(j, -1);
+}
+
+// ------------------------------------------------------------------ extending
+struct ExtendArgs {
+    int32_t* tables;
+    int64_t stride;
+    int width, page_size;
+    int64_t num_slots;
+    int32_t* seq_lens;
+    const int32_t* slots;
+    const int32_t* new_lens;
+    const int32_t* lens;
+    int num;
+    int32_t* refs;
+    int64_t num_pages, num_tokens;
+    int64_t* slot_mapping;
+    int32_t* positions;
+    int32_t* cu;
+    int32_t* out_lens;
+    int32_t* out_tables;
+    int32_t* start;      // [num]: the length before the step, -1 for a request that is skipped
+    int32_t* rank;       // [num]: number of its first page in free_list
+    int32_t* claim;      // [num_slots]: the first request that names the slot
+    int32_t* free_list;  // [num_pages]
+    int32_t* err;
+};
+__device__ __forceinline__ int pages_of(int len, int page) { return len / page + (len % page != 0); }
+
+// Exclusive prefix sum over the block of values whose sum fits 63 bits.
+__device__ __forceinline__ int64_t block_exclusive_scan64(int64_t v, int64_t* warp_sums, int64_t* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    int64_t w = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xFFFFFFFFu, w, o);
+        if (lane >= o) w += y;
+    }
+    *total = __shfl_sync(0xFFFFFFFFu, w, 31);
+    const int64_t before = __shfl_sync(0xFFFFFFFFu, w, warp > 0 ? warp - 1 : 0);
+    return x - v + (warp > 0 ? before : 0);
+}
+
+// One block: which requests count, what they take back, the pages they need, the lowest free pages.
+__global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(const __grid_constant__ ExtendArgs p) {
+    __shared__ int64_t sums64[3][32];
+    __shared__ int sums[32];
+    const int tid = threadIdx.x;
+    griddep_wait();
+    for (int k = tid; k < p.num; k += kPlanThreads) {
+        const int s = p.slots[k];
+        if (s >= 0 && s < p.num_slots) p.claim[s] = 0x7FFFFFFF;
+    }
+    __syncthreads();
+    for (int k = tid; k < p.num; k += kPlanThreads) {
+        const int s = p.slots[k];
+        if (s >= 0 && s < p.num_slots) atomicMin(p.claim + s, k);
+    }
+    __syncthreads();
+    // the checks, on lengths, tables and counts as they were before the call
+    const int64_t most = static_cast<int64_t>(p.width) * p.page_size;
+    for (int k = tid; k < p.num; k += kPlanThreads) {
+        const int s = p.slots[k], n = p.new_lens[k];
+        int start = -1, err = 0;
+        if (s < 0 || s >= p.num_slots || __ldcg(p.claim + s) != k) {
+            err = NVFP4KV_DEVERR_BAD_SLOT;
+        } else {
+            const int have = p.seq_lens[s], len = p.lens ? p.lens[k] : have;
+            if (n < 0 || len < 0 || len > have) {
+                err = NVFP4KV_DEVERR_SEQ_LEN;
+            } else if (static_cast<int64_t>(len) + n > most) {
+                err = NVFP4KV_DEVERR_CAPACITY;
+            } else {
+                start = len;
+                if (n > 0 && len % p.page_size != 0) {      // the new tokens begin in a page that others may read
+                    const int pg = p.tables[s * p.stride + len / p.page_size];
+                    if (pg < 0 || pg >= p.num_pages || __ldcg(p.refs + pg) != 1) {
+                        err = NVFP4KV_DEVERR_BAD_PAGE;
+                        start = -1;
+                    }
+                }
+            }
+        }
+        if (err) set_error(p.err, err);
+        p.start[k] = start;
+    }
+    __syncthreads();
+    // pages of tokens that are taken back
+    if (p.lens) {
+        for (int k = tid; k < p.num; k += kPlanThreads) {
+            const int start = p.start[k];
+            if (start < 0) continue;
+            const int s = p.slots[k], have = p.seq_lens[s];
+            int32_t* row = p.tables + s * p.stride;
+            const int end = min(pages_of(have, p.page_size), p.width);
+            for (int j = pages_of(start, p.page_size); j < end; ++j) {
+                const int pg = row[j];
+                row[j] = -1;
+                if (pg >= 0) release_page(p.refs, p.num_pages, pg, p.err);
+            }
+        }
+        __syncthreads();
+    }
+    // running sums of tokens and pages
+    int64_t tokens = 0, pages = 0;
+    for (int k0 = 0; k0 < p.num; k0 += kPlanThreads) {
+        const int k = k0 + tid, start = k < p.num ? p.start[k] : -1, n = start >= 0 ? p.new_lens[k] : 0;
+        const int need = start >= 0 ? pages_of(start + n, p.page_size) - pages_of(start, p.page_size) : 0;
+        int64_t sum_n, sum_p;
+        const int64_t at_n = tokens + block_exclusive_scan64(n, sums64[0], &sum_n);
+        const int64_t at_p = pages + block_exclusive_scan64(need, sums64[1], &sum_p);
+        if (k < p.num) {
+            // (-2: taken back, but not extended)
+            if (start >= 0 && n > 0 && at_n + n > p.num_tokens) p.rank[k] = -2;
+            else p.rank[k] = need == 0 ? -1 : static_cast<int>(at_p + need <= p.num_pages ? at_p : p.num_pages);
+        }
+        tokens += sum_n;
+        pages += sum_p;
+        __syncthreads();
+    }
+    // the lowest free pages, 16 counts a thread and step
+    constexpr int kPer = 16;
+    const int want = static_cast<int>(pages < p.num_pages ? pages : p.num_pages);
+    int found = 0;
+    for (int64_t b0 = 0; b0 < p.num_pages && found < want; b0 += kPlanThreads * kPer) {
+        const int64_t i0 = b0 + tid * kPer;
+        uint32_t zero = 0;
+        if (i0 + kPer <= p.num_pages && reinterpret_cast<uintptr_t>(p.refs) % 16 == 0) {
+            int4 v[kPer / 4];
+#pragma unroll
+            for (int j = 0; j < kPer / 4; ++j) v[j] = __ldcg(reinterpret_cast<const int4*>(p.refs + i0) + j);
+#pragma unroll
+            for (int j = 0; j < kPer / 4; ++j)
+                zero |= static_cast<uint32_t>((v[j].x == 0) | (v[j].y == 0) << 1 | (v[j].z == 0) << 2 | (v[j].w == 0) << 3) << (4 * j);
+        } else {
+            for (int j = 0; j < kPer; ++j)
+                if (i0 + j < p.num_pages && __ldcg(p.refs + i0 + j) == 0) zero |= 1u << j;
+        }
+        int total;
+        int at = found + block_exclusive_scan(__popc(zero), sums, &total);
+        for (; zero && at < want; zero &= zero - 1, ++at) p.free_list[at] = static_cast<int>(i0) + __ffs(zero) - 1;
+        found += total;
+        __syncthreads();
+    }
+    // who gets them, and where their tokens begin
+    int64_t done = 0;
+    for (int k0 = 0; k0 < p.num; k0 += kPlanThreads) {
+        const int k = k0 + tid;
+        int start = -1, n = 0;
+        bool ok = false;
+        if (k < p.num && (start = p.start[k]) >= 0) {
+            n = p.new_lens[k];
+            const int need = pages_of(start + n, p.page_size) - pages_of(start, p.page_size), rank = p.rank[k];
+            ok = rank != -2 && (need == 0 || static_cast<int64_t>(rank) + need <= found);
+            if (!ok) set_error(p.err, NVFP4KV_DEVERR_CAPACITY);
+        }
+        int64_t sum;
+        const int64_t at = done + block_exclusive_scan64(ok ? n : 0, sums64[2], &sum);
+        if (k < p.num) {
+            p.cu[k] = static_cast<int>(at);
+            p.out_lens[k] = ok ? start + n : 0;
+            if (start >= 0) p.seq_lens[p.slots[k]] = ok ? start + n : start;
+            if (!ok) p.start[k] = -1;
+        }
+        done += sum;
+        __syncthreads();
+    }
+    if (tid == 0) p.cu[p.num] = static_cast<int>(done);
+    griddep_launch_dependents();
+}
+
+// The first row_blocks blocks: the tables of a request, 1,024 entries each; the others: tokens.
+constexpr int kRowEntries = 1024, kTokensPerBlock = 256;
+__global__ void __launch_bounds__(256) extend_apply_kernel(const __grid_constant__ ExtendArgs p, int chunks, int64_t row_blocks) {
+    griddep_wait();
+    if (blockIdx.x < row_blocks) {
+        const int k = static_cast<int>(blockIdx.x / chunks), j0 = static_cast<int>(blockIdx.x % chunks) * kRowEntries;
+        const int start = p.start[k];
+        int32_t* to = p.out_tables + static_cast<int64_t>(k) * p.width;
+        if (start < 0) {
+            for (int j = j0 + threadIdx.x; j < min(j0 + kRowEntries, p.width); j += blockDim.x) to[j] = -1;
+            return;
+        }
+        int32_t* row = p.tables + p.slots[k] * p.stride;
+        const int first = pages_of(start, p.page_size), last = pages_of(p.out_lens[k], p.page_size), rank = p.rank[k];
+        for (int j = j0 + threadIdx.x; j < min(j0 + kRowEntries, p.width); j += blockDim.x) {
+            int pg;
+            if (j >= first && j < last) {
+                pg = p.free_list[rank + j - first];
+                row[j] = pg;
+                p.refs[pg] = 1;
+            } else {
+                pg = row[j];
+            }
+            to[j] = pg;
+        }
+        return;
+    }
+    const int64_t t = (blockIdx.x - row_blocks) * kTokensPerBlock + threadIdx.x;
+    if (t >= p.num_tokens) return;
+    int64_t slot = -1;
+    int pos = 0;
+    if (t < p.cu[p.num]) {
+        int lo = 0, hi = p.num - 1;      // the last request that begins at or before t (empty ones end before it)
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (__ldg(p.cu + mid) <= t) lo = mid;
+            else hi = mid - 1;
+        }
+        const int start = p.start[lo];
+        pos = start + static_cast<int>(t) - p.cu[lo];
+        const int j = pos / p.page_size, first = pages_of(start, p.page_size);
+        const int pg = j < first ? p.tables[p.slots[lo] * p.stride + j] : p.free_list[p.rank[lo] + j - first];
+        slot = static_cast<int64_t>(pg) * p.page_size + pos % p.page_size;
+    }
+    p.slot_mapping[t] = slot;
+    p.positions[t] = pos;
 }
 
 // ------------------------------------------------------------------ forking
@@ -330,7 +586,9 @@ __global__ void __launch_bounds__(256) fork_apply_kernel(const __grid_constant__
             int pg = -1;
             if (j < used) {
                 pg = from[j];
-                if (pg < 0 || pg >= p.num_pages) {
+                if (pg == kTrimmed) {
+                    // (a window left it behind: as for the parent)
+                } else if (pg < 0 || pg >= p.num_pages) {
                     pg = -1;
                     set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
                 } else if (j < full) {
@@ -471,7 +729,7 @@ __global__ void __launch_bounds__(256) compact_tables_kernel(const __grid_consta
     for (int64_t i = first; i < n; i += step) {
         const int64_t s = i / p.width, j = i - s * p.width;
         const int pg = p.tables[s * p.stride + j];
-        int q = -1;
+        int q = pg == kTrimmed ? kTrimmed : -1;
         if (pg >= 0) {
             if (pg < p.num_pages) q = p.remap[pg];
             if (q <= -2) q = p.dst[-2 - q];
@@ -607,6 +865,71 @@ extern "C" int nvfp4kv_fork_pages(const void* const* caches, const int64_t* page
     if (e == cudaSuccess) e = launch_dependent(fork_apply_kernel, dim3(num, 1 + num_caches), dim3(256), 0, st, a, c);
     if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_fork_pages launch failed: %s", cudaGetErrorString(e));
     return check_launch("nvfp4kv_fork_pages");
+}
+
+extern "C" int nvfp4kv_extend_workspace_ints(int num, int64_t num_slots, int64_t num_pages, int64_t* ints) {
+    using namespace nvfp4kv;
+    if (!ints) return fail(NVFP4KV_EINVAL, "nvfp4kv_extend_workspace_ints: null output");
+    if (num < 0 || num_slots < 1 || num_pages < 1) return fail(NVFP4KV_EINVAL, "nvfp4kv_extend_workspace_ints: bad sizes");
+    *ints = 2ll * num + num_slots + num_pages;
+    return NVFP4KV_OK;
+}
+
+extern "C" int nvfp4kv_extend_pages(int32_t* block_tables, int64_t tables_stride, int table_width, int64_t num_slots,
+                                    int32_t* seq_lens, const int32_t* slots, const int32_t* new_lens,
+                                    const int32_t* lens, int num, int page_size, int32_t* ref_counts,
+                                    int64_t num_pages, int64_t num_tokens, int64_t* slot_mapping, int32_t* positions,
+                                    int32_t* cu_seqlens_q, int32_t* out_lens, int32_t* out_tables,
+                                    int32_t* workspace, int64_t workspace_ints, int32_t* err_flag,
+                                    nvfp4kv_stream_t stream) {
+    using namespace nvfp4kv;
+    if (num < 0 || num_tokens < 0) return fail(NVFP4KV_EINVAL, "nvfp4kv_extend_pages: num or num_tokens < 0");
+    if (page_size < 1) return fail(NVFP4KV_EINVAL, "nvfp4kv_extend_pages: page_size must be >= 1");
+    int rc = check_tables("nvfp4kv_extend_pages", block_tables, tables_stride, table_width, num_slots, ref_counts, num_pages);
+    if (rc != NVFP4KV_OK) return rc;
+    if (static_cast<int64_t>(table_width) * page_size > 0x7FFFFFFFll || num_tokens > 0x7FFFFFFFll)
+        return fail(NVFP4KV_EINVAL, "nvfp4kv_extend_pages: sequences and steps of at most 2^31 - 1 tokens");
+    if (!cu_seqlens_q || (num_tokens > 0 && (!slot_mapping || !positions)) ||
+        (num > 0 && (!seq_lens || !slots || !new_lens || !out_lens || !out_tables)))
+        return fail(NVFP4KV_EINVAL, "nvfp4kv_extend_pages: null pointer");
+    if (!workspace || workspace_ints < 2ll * num + num_slots + num_pages)
+        return fail(NVFP4KV_EWORKSPACE, "nvfp4kv_extend_pages: workspace %lld ints < %lld required",
+                    (long long)workspace_ints, (long long)(2ll * num + num_slots + num_pages));
+    ExtendArgs a{};
+    a.tables = block_tables; a.stride = tables_stride; a.width = table_width; a.page_size = page_size;
+    a.num_slots = num_slots; a.seq_lens = seq_lens; a.slots = slots; a.new_lens = new_lens; a.lens = lens; a.num = num;
+    a.refs = ref_counts; a.num_pages = num_pages; a.num_tokens = num_tokens; a.slot_mapping = slot_mapping;
+    a.positions = positions; a.cu = cu_seqlens_q; a.out_lens = out_lens; a.out_tables = out_tables;
+    a.start = workspace; a.rank = a.start + num; a.claim = a.rank + num; a.free_list = a.claim + num_slots; a.err = err_flag;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const int chunks = (table_width + kRowEntries - 1) / kRowEntries;
+    const int64_t row_blocks = static_cast<int64_t>(num) * chunks;
+    const int64_t blocks = row_blocks + (num_tokens + kTokensPerBlock - 1) / kTokensPerBlock;
+    if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "nvfp4kv_extend_pages: too many requests for one call");
+    cudaError_t e = launch_dependent(extend_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
+    if (e == cudaSuccess && blocks > 0)
+        e = launch_dependent(extend_apply_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a, chunks, row_blocks);
+    if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_extend_pages launch failed: %s", cudaGetErrorString(e));
+    return check_launch("nvfp4kv_extend_pages");
+}
+
+extern "C" int nvfp4kv_trim_pages(int32_t* block_tables, int64_t tables_stride, int table_width, int64_t num_slots,
+                                  const int32_t* seq_lens, const int32_t* slots, int num, int page_size, int window,
+                                  int sinks, int32_t* ref_counts, int64_t num_pages, int32_t* err_flag,
+                                  nvfp4kv_stream_t stream) {
+    using namespace nvfp4kv;
+    if (num < 0) return fail(NVFP4KV_EINVAL, "nvfp4kv_trim_pages: num < 0");
+    if (page_size < 1 || window < 0 || sinks < 0)
+        return fail(NVFP4KV_EINVAL, "nvfp4kv_trim_pages: page_size must be >= 1, window and sinks >= 0");
+    if (num == 0) return NVFP4KV_OK;
+    if (!slots || !seq_lens) return fail(NVFP4KV_EINVAL, "nvfp4kv_trim_pages: null pointer");
+    int rc = check_tables("nvfp4kv_trim_pages", block_tables, tables_stride, table_width, num_slots, ref_counts, num_pages);
+    if (rc != NVFP4KV_OK) return rc;
+    const cudaError_t e = launch_dependent(trim_pages_kernel, dim3(num), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), block_tables,
+                                           tables_stride, table_width, num_slots, seq_lens, slots, page_size, window, sinks, ref_counts,
+                                           num_pages, err_flag);
+    if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_trim_pages launch failed: %s", cudaGetErrorString(e));
+    return check_launch("nvfp4kv_trim_pages");
 }
 
 extern "C" int nvfp4kv_compact_workspace_ints(int64_t num_pages, int64_t* ints) {

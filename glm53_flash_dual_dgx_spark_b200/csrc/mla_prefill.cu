@@ -133,6 +133,7 @@ struct PrefillParams {
     const int32_t* cu;
     const int32_t* seq_lens;
     int batch, total_q, heads, page_shift, max_q_len, max_seq_len;
+    int window, sinks;         // position p sees t > p - window and t < sinks (window 0: every t <= p)
     uint32_t heads_magic;      // ceil(2^32 / heads)
     int pairs;
     float scale_log2, out_scale;
@@ -497,6 +498,7 @@ __device__ __forceinline__ uint4 dequant8(uint32_t code, uint32_t scale2) {
 // rows.  The blocks of the grid take pieces of 32 tokens in turn (their number is on the device), a
 // row per thread, six blocks on an SM: 24.2 us for 91K tokens (143 MB read and written, 5.9 TB/s;
 // with four rows a thread and two blocks 26.6, and 5.4 against 3.4 for 2.4K tokens).
+template <bool kWindow>
 __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_constant__ PrefillParams p) {
     __shared__ uint32_t bits[2];      // of the piece's tokens: those that exist, those that hold a NaN
     __shared__ int b_s, pos_s, total_s;
@@ -531,8 +533,11 @@ __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_cons
         __syncthreads();
         if (b_s < 0) return;
         total = total_s * kImagePieces;
-        const int L = load_seq(p, b_s).L, t = pos_s + r0;
-        const int64_t row = pool_row(p, p.tables + b_s * p.tables_stride, t, L);
+        const Seq seq = load_seq(p, b_s);
+        const int L = seq.L, t = pos_s + r0;
+        // (a token that no row sees is not read: its page may be gone)
+        const bool seen = !kWindow || t < p.sinks || t > L - seq.n - p.window;
+        const int64_t row = seen ? pool_row(p, p.tables + b_s * p.tables_stride, t, L) : -1;
         uint4 code[2], rope = make_uint4(0, 0, 0, 0);
         uint16_t scale[2] = {0, 0};
         code[0] = code[1] = rope;
@@ -564,7 +569,7 @@ __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_cons
         if (nan) atomicOr(&bits[1], 1u << r0);
         if (lp == 0) {
             if (row >= 0) atomicOr(&bits[0], 1u << r0);
-            else if (t < L) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
+            else if (seen && t < L) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
         }
         __syncthreads();
         if (tid < 2) p.image_bits[8 * static_cast<int64_t>(block) + 4 * tid + piece] = bits[tid];
@@ -650,6 +655,10 @@ __device__ __forceinline__ void store_q(const PrefillParams& p, uint8_t* base, f
     }
 }
 
+// The first n bits of a word.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+template <bool kWindow>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -945,9 +954,16 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             if (n_tiles > 0) load_bits(0, ahead);
 #pragma unroll 1
             for (int i = 0; i < n_tiles; ++i, ++tile) {
-                const uint2 have = ahead[0], nan = ahead[1];
+                uint2 have = ahead[0];
+                const uint2 nan = ahead[1];
                 if (i + 1 < n_tiles) load_bits(i + 1, ahead);
-                const int see = lim - ((tile0 + i) * kTile + 64 * q4);     // tokens of the quarter the row sees
+                int see = lim - ((tile0 + i) * kTile + 64 * q4);     // tokens of the quarter the row sees
+                if constexpr (kWindow) {
+                    const int skip = see - p.window, keep = min(see, p.sinks - (lim - see));      // (lim - see: the quarter's first)
+                    have.x &= (bits_below(see) & ~bits_below(skip)) | bits_below(keep);
+                    have.y &= (bits_below(see - 32) & ~bits_below(skip - 32)) | bits_below(keep - 32);
+                    see = 64;      // (all in the bits)
+                }
                 wait_phase(bar(B_S_FULL + (tile & 1)), (tile >> 1) & 1, abort_flag, p.err);
                 tc_fence_after();
                 if (i == 0) factor = reinterpret_cast<const float*>(smem + SM_QS)[64 * (parts & 3) + row];
@@ -1245,7 +1261,7 @@ constexpr size_t kImageCap = size_t(1) << 30;
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
-PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_len, int max_seq_len) {
+PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_len, int max_seq_len, int window, int sinks) {
     PrefillPlan pl{};
     const int64_t one = (static_cast<int64_t>(max_seq_len) + kImageTok - 1) / kImageTok;
     const int64_t cap = static_cast<int64_t>(kImageCap / (9 * kStageBytes));
@@ -1272,39 +1288,67 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
     return pl;
 }
 
+template <bool kWindow>
 int set_smem_limit() {
     static int done[64] = {0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return fail(NVFP4KV_ECUDA, "cudaGetDevice failed");
     if (dev >= 0 && dev < 64 && done[dev]) return NVFP4KV_OK;
-    const cudaError_t e = cudaFuncSetAttribute(mla_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    const cudaError_t e = cudaFuncSetAttribute(mla_prefill_kernel<kWindow>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "mla_prefill: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) done[dev] = 1;
     return NVFP4KV_OK;
 }
 
-}  // namespace
-}  // namespace nvfp4kv
-
-extern "C" int nvfp4kv_mla_prefill_workspace_size(int batch, int total_q, int num_heads, int max_q_len,
-                                                  int max_seq_len, size_t* bytes) {
-    using namespace nvfp4kv;
-    if (!bytes) return fail(NVFP4KV_EINVAL, "mla_prefill_workspace_size: null output");
-    if (batch < 0 || total_q < 0 || num_heads < 1 || max_q_len < 0 || max_seq_len < 0)
-        return fail(NVFP4KV_EINVAL, "mla_prefill_workspace_size: batch, total_q, max_q_len and max_seq_len must be >= 0, num_heads >= 1");
-    *bytes = batch == 0 || total_q == 0 ? 0 : make_prefill_plan(batch, total_q, num_heads, max_q_len, max_seq_len).ws_bytes;
+// The launches of a call, a group of sequences at a time.
+template <bool kWindow>
+int launch_prefill(const PrefillParams& all, const PrefillPlan& pl, cudaStream_t st) {
+    int rc = set_smem_limit<kWindow>();
+    if (rc != NVFP4KV_OK) return rc;
+    for (int b0 = 0; b0 < all.batch; b0 += pl.group) {
+        PrefillParams p = all;
+        p.batch = all.batch - b0 < pl.group ? all.batch - b0 : pl.group;
+        p.tables = all.tables + b0 * all.tables_stride;
+        p.cu = all.cu + b0;
+        p.seq_lens = all.seq_lens + b0;
+        const dim3 grid(2 * pl.pairs);
+        cudaError_t e = cudaSuccess;
+        if (pl.image_blocks > 0) {
+            const int most = 8 * device_sm_count();
+            const int blocks = kImagePieces * pl.image_blocks;
+            e = launch_dependent(prefill_image_kernel<kWindow>, dim3(blocks < most ? blocks : most), dim3(256), 0, st, p);
+            if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill image launch failed: %s", cudaGetErrorString(e));
+            // its set-up overlaps the image kernel; all else it reads was there before that one
+            e = launch_dependent(mla_prefill_kernel<kWindow>, grid, dim3(kThreads), kSmemBytes, st, p);
+        } else {
+            mla_prefill_kernel<kWindow><<<grid, kThreads, kSmemBytes, st>>>(p);
+        }
+        if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill launch failed: %s", cudaGetErrorString(e));
+        if ((rc = check_launch("nvfp4kv_mla_prefill")) != NVFP4KV_OK) return rc;
+        if (pl.pairs == 1 || p.max_seq_len <= kTile) continue;      // no unit can be cut
+        if (8 * pl.pairs <= device_sm_count()) e = launch_dependent(prefill_combine_kernel<1>, dim3(pl.pairs * kUnitRows), dim3(128), 0, st, p);
+        else e = launch_dependent(prefill_combine_kernel<4>, dim3(pl.pairs * (kUnitRows / 4)), dim3(128), 0, st, p);
+        if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill combine launch failed: %s", cudaGetErrorString(e));
+        if ((rc = check_launch("nvfp4kv_mla_prefill combine")) != NVFP4KV_OK) return rc;
+    }
     return NVFP4KV_OK;
 }
 
-extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* pool,
-                                   int64_t pool_rows, const void* rope_pool, const int32_t* tables,
-                                   int64_t tables_stride, const int32_t* cu_seqlens_q, const int32_t* seq_lens,
-                                   int batch, int total_q, int num_heads, int head_dim_qk, int kv_lora_rank,
-                                   int page_size, int max_q_len, int max_seq_len, float bmm1_scale,
-                                   float bmm2_scale, void* out, int64_t out_stride_t, int64_t out_stride_h,
-                                   float* lse, void* workspace, size_t workspace_bytes, int32_t* err_flag,
-                                   nvfp4kv_stream_t stream) {
-    using namespace nvfp4kv;
+int workspace_call(int batch, int total_q, int num_heads, int max_q_len, int max_seq_len, int window, int sinks, size_t* bytes) {
+    if (!bytes) return fail(NVFP4KV_EINVAL, "mla_prefill_workspace_size: null output");
+    if (batch < 0 || total_q < 0 || num_heads < 1 || max_q_len < 0 || max_seq_len < 0)
+        return fail(NVFP4KV_EINVAL, "mla_prefill_workspace_size: batch, total_q, max_q_len and max_seq_len must be >= 0, num_heads >= 1");
+    *bytes = batch == 0 || total_q == 0 ? 0 : make_prefill_plan(batch, total_q, num_heads, max_q_len, max_seq_len, window, sinks).ws_bytes;
+    return NVFP4KV_OK;
+}
+
+// nvfp4kv_mla_prefill (window 0) and nvfp4kv_mla_prefill_window
+int prefill_call(const void* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* pool, int64_t pool_rows,
+                 const void* rope_pool, const int32_t* tables, int64_t tables_stride, const int32_t* cu_seqlens_q,
+                 const int32_t* seq_lens, int batch, int total_q, int num_heads, int head_dim_qk, int kv_lora_rank,
+                 int page_size, int max_q_len, int max_seq_len, int window, int sinks, float bmm1_scale,
+                 float bmm2_scale, void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse, void* workspace,
+                 size_t workspace_bytes, int32_t* err_flag, nvfp4kv_stream_t stream) {
     if (batch < 0 || total_q < 0) return fail(NVFP4KV_EINVAL, "mla_prefill: batch or total_q < 0");
     if (num_heads < 1 || max_q_len < 0 || max_seq_len < 0)
         return fail(NVFP4KV_EINVAL, "mla_prefill: num_heads must be >= 1, max_q_len and max_seq_len >= 0");
@@ -1325,7 +1369,7 @@ extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_
         return fail(NVFP4KV_EINVAL, "mla_prefill: pools and q must be 16-byte aligned and q strides multiples of 8");
     if (reinterpret_cast<uintptr_t>(out) % 16 || out_stride_t % 8 || out_stride_h % 8)
         return fail(NVFP4KV_EINVAL, "mla_prefill: out must be 16-byte aligned and its strides multiples of 8");
-    const PrefillPlan pl = make_prefill_plan(batch, total_q, num_heads, max_q_len, max_seq_len);
+    const PrefillPlan pl = make_prefill_plan(batch, total_q, num_heads, max_q_len, max_seq_len, window, sinks);
     const size_t need = pl.ws_bytes;
     if (need && (!workspace || workspace_bytes < need))
         return fail(NVFP4KV_EWORKSPACE, "mla_prefill: workspace %zu bytes < %zu required", workspace_bytes, need);
@@ -1348,33 +1392,58 @@ extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_
     p.part_o = reinterpret_cast<float*>(ws += pl.q_bytes);
     p.part_ml = reinterpret_cast<float*>(ws += pl.o_bytes);
     p.parts = reinterpret_cast<PartInfo*>(ws += pl.ml_bytes);
+    p.window = window; p.sinks = sinks;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    int rc = set_smem_limit();
-    if (rc != NVFP4KV_OK) return rc;
-    for (int b0 = 0; b0 < batch; b0 += pl.group) {
-        p.batch = batch - b0 < pl.group ? batch - b0 : pl.group;
-        p.tables = tables + b0 * tables_stride;
-        p.cu = cu_seqlens_q + b0;
-        p.seq_lens = seq_lens + b0;
-        const dim3 grid(2 * pl.pairs);
-        cudaError_t e = cudaSuccess;
-        if (pl.image_blocks > 0) {
-            const int most = 8 * device_sm_count();
-            const int blocks = kImagePieces * pl.image_blocks;
-            e = launch_dependent(prefill_image_kernel, dim3(blocks < most ? blocks : most), dim3(256), 0, st, p);
-            if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill image launch failed: %s", cudaGetErrorString(e));
-            // its set-up overlaps the image kernel; all else it reads was there before that one
-            e = launch_dependent(mla_prefill_kernel, grid, dim3(kThreads), kSmemBytes, st, p);
-        } else {
-            mla_prefill_kernel<<<grid, kThreads, kSmemBytes, st>>>(p);
-        }
-        if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill launch failed: %s", cudaGetErrorString(e));
-        if ((rc = check_launch("nvfp4kv_mla_prefill")) != NVFP4KV_OK) return rc;
-        if (pl.pairs == 1 || max_seq_len <= kTile) continue;      // no unit can be cut
-        if (8 * pl.pairs <= device_sm_count()) e = launch_dependent(prefill_combine_kernel<1>, dim3(pl.pairs * kUnitRows), dim3(128), 0, st, p);
-        else e = launch_dependent(prefill_combine_kernel<4>, dim3(pl.pairs * (kUnitRows / 4)), dim3(128), 0, st, p);
-        if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill combine launch failed: %s", cudaGetErrorString(e));
-        if ((rc = check_launch("nvfp4kv_mla_prefill combine")) != NVFP4KV_OK) return rc;
-    }
+    return window > 0 ? launch_prefill<true>(p, pl, st) : launch_prefill<false>(p, pl, st);
+}
+
+// A window that hides nothing is none; otherwise it and the sinks lie within max_seq_len.
+int check_window(const char* what, int max_seq_len, int* window, int* sinks) {
+    if (*window < 1 || *sinks < 0) return fail(NVFP4KV_EINVAL, "%s: window must be >= 1 and sinks >= 0", what);
+    if (max_seq_len >= 0 && static_cast<int64_t>(*window) + *sinks >= max_seq_len) *window = *sinks = 0;
     return NVFP4KV_OK;
+}
+
+}  // namespace
+}  // namespace nvfp4kv
+
+extern "C" int nvfp4kv_mla_prefill_workspace_size(int batch, int total_q, int num_heads, int max_q_len,
+                                                  int max_seq_len, size_t* bytes) {
+    return nvfp4kv::workspace_call(batch, total_q, num_heads, max_q_len, max_seq_len, 0, 0, bytes);
+}
+
+extern "C" int nvfp4kv_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* pool,
+                                   int64_t pool_rows, const void* rope_pool, const int32_t* tables,
+                                   int64_t tables_stride, const int32_t* cu_seqlens_q, const int32_t* seq_lens,
+                                   int batch, int total_q, int num_heads, int head_dim_qk, int kv_lora_rank,
+                                   int page_size, int max_q_len, int max_seq_len, float bmm1_scale,
+                                   float bmm2_scale, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                                   float* lse, void* workspace, size_t workspace_bytes, int32_t* err_flag,
+                                   nvfp4kv_stream_t stream) {
+    return nvfp4kv::prefill_call(q, q_stride_t, q_stride_h, pool, pool_rows, rope_pool, tables, tables_stride, cu_seqlens_q, seq_lens, batch,
+                                 total_q, num_heads, head_dim_qk, kv_lora_rank, page_size, max_q_len, max_seq_len, 0, 0,
+                                 bmm1_scale, bmm2_scale, out, out_stride_t, out_stride_h, lse, workspace, workspace_bytes, err_flag,
+                                 stream);
+}
+
+extern "C" int nvfp4kv_mla_prefill_window_workspace_size(int batch, int total_q, int num_heads, int max_q_len,
+                                                         int max_seq_len, int window, int sinks, size_t* bytes) {
+    const int rc = nvfp4kv::check_window("mla_prefill_window_workspace_size", max_seq_len, &window, &sinks);
+    return rc != NVFP4KV_OK ? rc : nvfp4kv::workspace_call(batch, total_q, num_heads, max_q_len, max_seq_len, window, sinks, bytes);
+}
+
+extern "C" int nvfp4kv_mla_prefill_window(const void* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* pool,
+                                          int64_t pool_rows, const void* rope_pool, const int32_t* tables,
+                                          int64_t tables_stride, const int32_t* cu_seqlens_q, const int32_t* seq_lens,
+                                          int batch, int total_q, int num_heads, int head_dim_qk, int kv_lora_rank,
+                                          int page_size, int max_q_len, int max_seq_len, int window, int sinks, float bmm1_scale,
+                                          float bmm2_scale, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                                          float* lse, void* workspace, size_t workspace_bytes, int32_t* err_flag,
+                                          nvfp4kv_stream_t stream) {
+    const int rc = nvfp4kv::check_window("mla_prefill_window", max_seq_len, &window, &sinks);
+    if (rc != NVFP4KV_OK) return rc;
+    return nvfp4kv::prefill_call(q, q_stride_t, q_stride_h, pool, pool_rows, rope_pool, tables, tables_stride, cu_seqlens_q, seq_lens, batch,
+                                 total_q, num_heads, head_dim_qk, kv_lora_rank, page_size, max_q_len, max_seq_len, window, sinks,
+                                 bmm1_scale, bmm2_scale, out, out_stride_t, out_stride_h, lse, workspace, workspace_bytes, err_flag,
+                                 stream);
 }

@@ -1,5 +1,6 @@
 // Rotary positions: nvfp4kv_rope (whole heads, any layout) and nvfp4kv_append_rope_rotated (the
-// rope part of a step: rotated keys into the paged side-pool, queries rotated beside them).
+// rope part of a step: rotated keys into the paged side-pool, queries rotated beside them), and
+// both with positions on several axes (nvfp4kv_rope_axes, nvfp4kv_append_rope_rotated_axes).
 //
 // A pair (a, b) of a head turns by its token's angle: (a c - b s, b c + a s), in fp32, rounded
 // once.  cos and sin come from the caller's table, so that scaled frequencies cost nothing here
@@ -64,13 +65,65 @@ template <int N> __device__ __forceinline__ void load_angles(const float* p, flo
     }
 }
 
-// One 16-byte vector of an interleaved rotation: pairs inside the vector.  cs -> cos of its first pair.
-template <typename T>
-__device__ __forceinline__ Vec<T> rotate_pairs(const Vec<T>& x, const float* cs, int half, float sign) {
+// Positions on several axes: the axis of each pair, two bits each, 32 pairs a word.
+struct Axes {
+    uint64_t pair_axes[NVFP4KV_MAX_AXES_DIM / 64];
+    int64_t stride;      // between the axes of positions
+    int num;
+};
+// Where the angles of a token come from: one row of the table, or with several axes a row for each.
+struct Angles {
+    const float* row;                            // one axis
+    int64_t at[NVFP4KV_MAX_AXES];                // several: the rows' offsets in the table
+    bool turn;                                   // every position is in the table
+};
+template <bool kAxes>
+__device__ __forceinline__ Angles find_angles(const void* positions, bool i64, int64_t t, const Axes& axes, const float* table,
+                                              int64_t max_positions, int rotary) {
+    Angles r;
+    if constexpr (kAxes) {
+        r.turn = true;
+#pragma unroll
+        for (int a = 0; a < NVFP4KV_MAX_AXES; ++a) {
+            const int64_t pos = a < axes.num ? load_index(positions, i64, a * axes.stride + t) : 0;
+            const bool in = pos >= 0 && pos < max_positions;
+            r.turn &= in;
+            r.at[a] = in ? pos * rotary : 0;
+        }
+        r.row = table;
+    } else {
+        const int64_t pos = load_index(positions, i64, t);
+        r.turn = pos >= 0 && pos < max_positions;
+        r.row = table + (r.turn ? pos : 0) * rotary;
+    }
+    return r;
+}
+__device__ __forceinline__ const float* axis_row(const Angles& a, uint32_t axis) {
+    return a.row + (axis & 2 ? (axis & 1 ? a.at[3] : a.at[2]) : (axis & 1 ? a.at[1] : a.at[0]));
+}
+// cos and sin of N pairs from pair i on (i a multiple of N, N a power of two up to 8).
+template <int N, bool kAxes>
+__device__ __forceinline__ void load_pairs(const Angles& a, const Axes& axes, int i, int half, float (&c)[N], float (&s)[N]) {
+    if constexpr (kAxes) {
+        const uint32_t of = static_cast<uint32_t>(axes.pair_axes[i >> 5] >> (2 * (i & 31)));
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const float* p = axis_row(a, of >> (2 * k)) + i + k;
+            c[k] = __ldg(p);
+            s[k] = __ldg(p + half);
+        }
+    } else {
+        load_angles<N>(a.row + i, c);
+        load_angles<N>(a.row + i + half, s);
+    }
+}
+
+// One 16-byte vector of an interleaved rotation: pairs inside the vector, from pair i on.
+template <typename T, bool kAxes>
+__device__ __forceinline__ Vec<T> rotate_pairs(const Vec<T>& x, const Angles& a, const Axes& axes, int i, int half, float sign) {
     constexpr int N = Vec<T>::kN;
     float c[N / 2], s[N / 2];
-    load_angles<N / 2>(cs, c);
-    load_angles<N / 2>(cs + half, s);
+    load_pairs<N / 2, kAxes>(a, axes, i, half, c, s);
     Vec<T> y;
 #pragma unroll
     for (int k = 0; k < N / 2; ++k) {
@@ -83,12 +136,11 @@ __device__ __forceinline__ Vec<T> rotate_pairs(const Vec<T>& x, const float* cs,
 }
 
 // The two vectors of a half-layout rotation: dims i.. and i + half.. .
-template <typename T>
-__device__ __forceinline__ void rotate_halves(Vec<T>& xa, Vec<T>& xb, const float* cs, int half, float sign) {
+template <typename T, bool kAxes>
+__device__ __forceinline__ void rotate_halves(Vec<T>& xa, Vec<T>& xb, const Angles& a, const Axes& axes, int i, int half, float sign) {
     constexpr int N = Vec<T>::kN;
     float c[N], s[N];
-    load_angles<N>(cs, c);
-    load_angles<N>(cs + half, s);
+    load_pairs<N, kAxes>(a, axes, i, half, c, s);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         float u, v;
@@ -118,6 +170,7 @@ struct RopeArgs {
     SmallDiv units, by_heads;
     int pos_i64, inverse, in_place;
     int32_t* err;
+    Axes axes;
 };
 constexpr int kRopeSteps = 2;
 
@@ -127,8 +180,8 @@ constexpr int kRopeSteps = 2;
 // the occupancy that leaves (8,192 tokens x 64 heads x 576 bf16, 1.2 GB: 188 us = 6.4 TB/s, as much
 // as a plain copy; 8 % more with one, 1 % more with four, 20 % more with blocks of whole heads, whose
 // last steps are part empty).  The gradient of 2,049 tokens x 32 heads x 128 fp32 takes 12 us.
-template <typename T, bool kInterleaved>
-__global__ void __launch_bounds__(256, kInterleaved && sizeof(T) == 2 ? 8 : 4) rope_vec_kernel(const __grid_constant__ RopeArgs p) {
+template <typename T, bool kInterleaved, bool kAxes>
+__global__ void __launch_bounds__(256, kInterleaved && sizeof(T) == 2 && !kAxes ? 8 : 4) rope_vec_kernel(const __grid_constant__ RopeArgs p) {
     constexpr int N = Vec<T>::kN;
     const int64_t u0 = static_cast<int64_t>(blockIdx.x) * (256 * kRopeSteps);
     int64_t row0, t0;       // the block's first head row, its token
@@ -168,15 +221,13 @@ __global__ void __launch_bounds__(256, kInterleaved && sizeof(T) == 2 ? 8 : 4) r
         if (r[k] == -2) break;
         T* op = static_cast<T*>(p.out) + at[k];
         if (r[k] >= 0) {
-            const int64_t pos = load_index(p.positions, p.pos_i64, t[k]);
-            const bool turn = pos >= 0 && pos < p.max_positions;
-            if (!turn) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
-            const float* cs = p.cos_sin + (turn ? pos : 0) * p.rotary + (kInterleaved ? r[k] / 2 : r[k]);
+            const Angles g = find_angles<kAxes>(p.positions, p.pos_i64, t[k], p.axes, p.cos_sin, p.max_positions, p.rotary);
+            if (!g.turn) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
             const float sign = p.inverse ? -1.0f : 1.0f;
             if (kInterleaved) {
-                if (turn) a[k] = rotate_pairs(a[k], cs, half, sign);
+                if (g.turn) a[k] = rotate_pairs<T, kAxes>(a[k], g, p.axes, r[k] / 2, half, sign);
             } else {
-                if (turn) rotate_halves(a[k], b[k], cs, half, sign);
+                if (g.turn) rotate_halves<T, kAxes>(a[k], b[k], g, p.axes, r[k], half, sign);
                 store_vec(op + half, b[k]);
             }
         }
@@ -188,15 +239,13 @@ __global__ void __launch_bounds__(256, kInterleaved && sizeof(T) == 2 ? 8 : 4) r
 // that no 16-byte access can take (views at an odd offset, heads of odd sizes).  It is bound by its
 // 2- or 4-byte accesses and a division per element: 8,192 tokens x 64 heads x 192 bf16, shifted by 3,
 // take 388 us where the bytes take 62 (1.0 TB/s; fp32 2.1).  A caller that can align its rows should.
-template <typename T, bool kInterleaved>
+template <typename T, bool kInterleaved, bool kAxes>
 __global__ void __launch_bounds__(256) rope_elem_kernel(const __grid_constant__ RopeArgs p, int head_blocks, int heads_per_block) {
     const int64_t t = blockIdx.x / head_blocks;
     const int h0 = static_cast<int>(blockIdx.x % head_blocks) * heads_per_block;
     const int heads = min(heads_per_block, p.heads - h0);
-    const int64_t pos = load_index(p.positions, p.pos_i64, t);
-    const bool turn = pos >= 0 && pos < p.max_positions;
-    if (!turn && threadIdx.x == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
-    const float* cs = p.cos_sin + (turn ? pos : 0) * p.rotary;
+    const Angles g = find_angles<kAxes>(p.positions, p.pos_i64, t, p.axes, p.cos_sin, p.max_positions, p.rotary);
+    if (!g.turn && threadIdx.x == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
     const int half = p.rotary / 2;
     const float sign = p.inverse ? -1.0f : 1.0f;
     const T* x = static_cast<const T*>(p.x) + t * p.x_st + h0 * p.x_sh;
@@ -206,13 +255,14 @@ __global__ void __launch_bounds__(256) rope_elem_kernel(const __grid_constant__ 
         const T* xp = x + h * p.x_sh;
         T* op = o + h * p.o_sh;
         const int r = d - p.offset;
-        if (r < 0 || r >= p.rotary || !turn) {
+        if (r < 0 || r >= p.rotary || !g.turn) {
             op[d] = xp[d];
             continue;
         }
         const int i = kInterleaved ? r / 2 : r;
         if (kInterleaved ? (r & 1) : r >= half) continue;      // done with its partner
         const int db = kInterleaved ? d + 1 : d + half;
+        const float* cs = kAxes ? axis_row(g, static_cast<uint32_t>(p.axes.pair_axes[i >> 5] >> (2 * (i & 31)))) : g.row;
         float u0, v0;
         rotate(load_f32(xp + d), load_f32(xp + db), __ldg(cs + i), sign * __ldg(cs + half + i), u0, v0);
         op[d] = from_f32<T>(u0);
@@ -220,7 +270,7 @@ __global__ void __launch_bounds__(256) rope_elem_kernel(const __grid_constant__ 
     }
 }
 
-template <typename T>
+template <typename T, bool kAxes>
 int launch_rope(RopeArgs a, int64_t tokens, bool interleaved, cudaStream_t st) {
     constexpr int N = Vec<T>::kN;
     const uintptr_t bases = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.out);
@@ -240,7 +290,7 @@ int launch_rope(RopeArgs a, int64_t tokens, bool interleaved, cudaStream_t st) {
         a.total = tokens * heads * units;
         blocks = (a.total + 256 * kRopeSteps - 1) / (256 * kRopeSteps);
         if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: too many rows for one call");
-        const cudaError_t e = launch_dependent(interleaved ? rope_vec_kernel<T, true> : rope_vec_kernel<T, false>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a);
+        const cudaError_t e = launch_dependent(interleaved ? rope_vec_kernel<T, true, kAxes> : rope_vec_kernel<T, false, kAxes>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a);
         if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_rope launch failed: %s", cudaGetErrorString(e));
     } else {
         int hb = 1024 / a.dim;
@@ -248,8 +298,8 @@ int launch_rope(RopeArgs a, int64_t tokens, bool interleaved, cudaStream_t st) {
         const int head_blocks = (a.heads + hb - 1) / hb, per_block = (a.heads + head_blocks - 1) / head_blocks;
         blocks = tokens * head_blocks;
         if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: too many rows for one call");
-        if (interleaved) rope_elem_kernel<T, true><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, head_blocks, per_block);
-        else rope_elem_kernel<T, false><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, head_blocks, per_block);
+        if (interleaved) rope_elem_kernel<T, true, kAxes><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, head_blocks, per_block);
+        else rope_elem_kernel<T, false, kAxes><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, head_blocks, per_block);
     }
     return check_launch("nvfp4kv_rope");
 }
@@ -272,6 +322,7 @@ struct RopeAppendArgs {
     SmallDiv rows_of_token;    // heads + 1
     int slot_i64, pos_i64;
     int32_t* err;
+    Axes axes;
 };
 
 // 8 bf16, as one 16-byte access or element by element.  The accesses are marked as streaming: a step's
@@ -306,7 +357,7 @@ template <bool kVec> __device__ __forceinline__ void put8(__nv_bfloat16* p, cons
 // rope_vec_kernel, two a thread (37.7 us with one, 42 with four, before the streaming marks); a
 // token's rows are its key and the heads of its query.  What bounds it is the latency of a block's
 // three dependent accesses (position, table row, store) at full occupancy, then HBM.
-template <bool kInterleaved, bool kVec>
+template <bool kInterleaved, bool kVec, bool kAxes>
 __global__ void __launch_bounds__(256) rope_append_rotated_kernel(const __grid_constant__ RopeAppendArgs p) {
     using V = Vec<__nv_bfloat16>;
     constexpr int kU = kInterleaved ? 8 : 4, kSteps = kAppendSteps, kRows = 256 / kU;      // rows of a block and step
@@ -331,12 +382,10 @@ __global__ void __launch_bounds__(256) rope_append_rotated_kernel(const __grid_c
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
         if (t[k] >= p.tokens) break;
-        const int64_t pos = load_index(p.positions, p.pos_i64, t[k]);
-        const bool turn = pos >= 0 && pos < p.max_positions;
-        const float* cs = p.cos_sin + (turn ? pos : 0) * NVFP4KV_ROPE;
+        const Angles g = find_angles<kAxes>(p.positions, p.pos_i64, t[k], p.axes, p.cos_sin, p.max_positions, NVFP4KV_ROPE);
         __nv_bfloat16* dst;
         if (h[k] < 0) {
-            if (!turn && u == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
+            if (!g.turn && u == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
             const int64_t slot = load_index(p.slots, p.slot_i64, t[k]);
             if (slot < 0) continue;
             if (slot >= p.rows) {
@@ -348,13 +397,137 @@ __global__ void __launch_bounds__(256) rope_append_rotated_kernel(const __grid_c
             dst = p.qo + t[k] * p.qo_st + h[k] * p.qo_sh;
         }
         if (kInterleaved) {
-            if (turn) a[k] = rotate_pairs(a[k], cs + 4 * u, 32, 1.0f);
+            if (g.turn) a[k] = rotate_pairs<__nv_bfloat16, kAxes>(a[k], g, p.axes, 4 * u, 32, 1.0f);
         } else {
-            if (turn) rotate_halves(a[k], b[k], cs + 8 * u, 32, 1.0f);
+            if (g.turn) rotate_halves<__nv_bfloat16, kAxes>(a[k], b[k], g, p.axes, 8 * u, 32, 1.0f);
             put8<kVec>(dst + 32 + 8 * u, b[k]);
         }
         put8<kVec>(dst + 8 * u, a[k]);
     }
+}
+
+// The axes of a call (num 0: one, as nvfp4kv_rope).
+int check_axes(const char* what, int64_t stride, int num, const uint8_t* pair_axes, int rotary_dim, Axes* out) {
+    if (num < 1 || num > NVFP4KV_MAX_AXES) return fail(NVFP4KV_EINVAL, "%s: num_axes %d not in [1, %d]", what, num, NVFP4KV_MAX_AXES);
+    if (!pair_axes) return fail(NVFP4KV_EINVAL, "%s: null pointer", what);
+    if (rotary_dim > NVFP4KV_MAX_AXES_DIM)
+        return fail(NVFP4KV_EINVAL, "%s: rotary_dim %d with several axes (at most %d)", what, rotary_dim, NVFP4KV_MAX_AXES_DIM);
+    *out = Axes{};
+    out->stride = stride;
+    out->num = num;
+    for (int i = 0; i < rotary_dim / 2; ++i) {
+        if (pair_axes[i] >= num) return fail(NVFP4KV_EINVAL, "%s: pair %d has axis %d of %d", what, i, pair_axes[i], num);
+        out->pair_axes[i >> 5] |= static_cast<uint64_t>(pair_axes[i]) << (2 * (i & 31));
+    }
+    return NVFP4KV_OK;
+}
+
+// nvfp4kv_rope (num_axes 0) and nvfp4kv_rope_axes
+int rope_call(const char* what, const void* x, int dtype, int64_t num_tokens, int num_heads, int head_dim,
+                            int64_t x_stride_t, int64_t x_stride_h, const void* positions, int pos_dtype,
+                            int64_t positions_stride, int num_axes, const uint8_t* pair_axes,
+                            const float* cos_sin, int64_t max_positions, int rotary_dim, int rope_offset,
+                            int interleaved, int inverse, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                            int32_t* err_flag, nvfp4kv_stream_t stream) {
+    if (num_tokens < 0) return fail(NVFP4KV_EINVAL, "%s: num_tokens < 0", what);
+    if (dtype != NVFP4KV_DTYPE_BF16 && dtype != NVFP4KV_DTYPE_F16 && dtype != NVFP4KV_DTYPE_F32)
+        return fail(NVFP4KV_EINVAL, "%s: dtype must be bf16, fp16 or fp32", what);
+    if (pos_dtype != NVFP4KV_INDEX_I64 && pos_dtype != NVFP4KV_INDEX_I32)
+        return fail(NVFP4KV_EINVAL, "%s: position dtype must be int64 or int32", what);
+    if (num_heads < 1 || head_dim < 1) return fail(NVFP4KV_EINVAL, "%s: num_heads and head_dim must be >= 1", what);
+    if (rotary_dim < 2 || rotary_dim % 2 || rope_offset < 0 || rope_offset > head_dim - rotary_dim)
+        return fail(NVFP4KV_EINVAL, "%s: rotary_dim %d at offset %d does not fit head_dim %d (even, >= 2)", what,
+                    rotary_dim, rope_offset, head_dim);
+    if (max_positions < 1) return fail(NVFP4KV_EINVAL, "%s: empty cos_sin table", what);
+    Axes axes{};
+    if (num_axes != 0) {
+        const int rc = check_axes(what, positions_stride, num_axes, pair_axes, rotary_dim, &axes);
+        if (rc != NVFP4KV_OK) return rc;
+    }
+    if (num_tokens == 0) return NVFP4KV_OK;
+    if (!x || !positions || !cos_sin || !out) return fail(NVFP4KV_EINVAL, "%s: null pointer", what);
+    const uintptr_t size = dtype == NVFP4KV_DTYPE_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(x) % size || reinterpret_cast<uintptr_t>(out) % size ||
+        reinterpret_cast<uintptr_t>(cos_sin) % 4)
+        return fail(NVFP4KV_EINVAL, "%s: x, out and cos_sin must be aligned to their elements", what);
+    if (x == out && (x_stride_t != out_stride_t || x_stride_h != out_stride_h))
+        return fail(NVFP4KV_EINVAL, "%s: in place needs equal strides", what);
+    RopeArgs a{};
+    a.x = x; a.out = out; a.x_st = x_stride_t; a.x_sh = x_stride_h; a.o_st = out_stride_t; a.o_sh = out_stride_h;
+    a.positions = positions; a.cos_sin = cos_sin; a.max_positions = max_positions;
+    a.heads = num_heads; a.dim = head_dim; a.rotary = rotary_dim; a.offset = rope_offset;
+    a.pos_i64 = pos_dtype == NVFP4KV_INDEX_I64; a.inverse = inverse != 0; a.in_place = x == out; a.err = err_flag;
+    a.axes = axes;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const bool il = interleaved != 0;
+    if (num_axes == 0) {
+        if (dtype == NVFP4KV_DTYPE_BF16) return launch_rope<__nv_bfloat16, false>(a, num_tokens, il, st);
+        if (dtype == NVFP4KV_DTYPE_F16) return launch_rope<__half, false>(a, num_tokens, il, st);
+        return launch_rope<float, false>(a, num_tokens, il, st);
+    }
+    if (dtype == NVFP4KV_DTYPE_BF16) return launch_rope<__nv_bfloat16, true>(a, num_tokens, il, st);
+    if (dtype == NVFP4KV_DTYPE_F16) return launch_rope<__half, true>(a, num_tokens, il, st);
+    return launch_rope<float, true>(a, num_tokens, il, st);
+}
+
+
+// nvfp4kv_append_rope_rotated (num_axes 0) and nvfp4kv_append_rope_rotated_axes
+int append_rotated_call(const char* what, const void* k_pe, int64_t num_tokens, int64_t k_stride, void* rope_pool,
+                        int64_t pool_rows, const void* slot_mapping, int slot_dtype, const void* positions,
+                        int pos_dtype, int64_t positions_stride, int num_axes, const uint8_t* pair_axes,
+                        const float* cos_sin, int64_t max_positions, int interleaved, const void* q_pe,
+                        int num_heads, int64_t q_stride_t, int64_t q_stride_h, void* q_out, int64_t qo_stride_t,
+                        int64_t qo_stride_h, int32_t* err_flag, nvfp4kv_stream_t stream) {
+    if (num_tokens < 0) return fail(NVFP4KV_EINVAL, "%s: num_tokens < 0", what);
+    if ((slot_dtype != NVFP4KV_INDEX_I64 && slot_dtype != NVFP4KV_INDEX_I32) ||
+        (pos_dtype != NVFP4KV_INDEX_I64 && pos_dtype != NVFP4KV_INDEX_I32))
+        return fail(NVFP4KV_EINVAL, "%s: slots and positions must be int64 or int32", what);
+    Axes axes{};
+    if (num_axes != 0) {
+        const int rc = check_axes(what, positions_stride, num_axes, pair_axes, NVFP4KV_ROPE, &axes);
+        if (rc != NVFP4KV_OK) return rc;
+    }
+    if (num_tokens == 0) return NVFP4KV_OK;
+    if (!k_pe || !rope_pool || !slot_mapping || !positions || !cos_sin || (q_pe && !q_out))
+        return fail(NVFP4KV_EINVAL, "%s: null pointer", what);
+    if (k_stride < NVFP4KV_ROPE)
+        return fail(NVFP4KV_EINVAL, "%s: k_stride %lld < 64", what, (long long)k_stride);
+    if (pool_rows <= 0 || max_positions < 1)
+        return fail(NVFP4KV_EINVAL, "%s: empty rope pool or cos_sin table", what);
+    if (q_pe && (num_heads < 1 || num_heads >= kMostDivisor))
+        return fail(NVFP4KV_EINVAL, "%s: num_heads %d not in [1, %d)", what, num_heads, kMostDivisor);
+    if (reinterpret_cast<uintptr_t>(rope_pool) % 16 || reinterpret_cast<uintptr_t>(cos_sin) % 16 ||
+        (reinterpret_cast<uintptr_t>(k_pe) | reinterpret_cast<uintptr_t>(q_pe) | reinterpret_cast<uintptr_t>(q_out)) % 2)
+        return fail(NVFP4KV_EINVAL, "%s: rope pool and cos_sin must be 16-byte aligned", what);
+    if (q_pe && q_pe == q_out && (q_stride_t != qo_stride_t || q_stride_h != qo_stride_h))
+        return fail(NVFP4KV_EINVAL, "%s: in place needs equal strides", what);
+    RopeAppendArgs a{};
+    a.k = static_cast<const __nv_bfloat16*>(k_pe); a.k_st = k_stride; a.tokens = num_tokens;
+    a.pool = static_cast<__nv_bfloat16*>(rope_pool); a.rows = pool_rows;
+    a.slots = slot_mapping; a.slot_i64 = slot_dtype == NVFP4KV_INDEX_I64;
+    a.positions = positions; a.pos_i64 = pos_dtype == NVFP4KV_INDEX_I64;
+    a.cos_sin = cos_sin; a.max_positions = max_positions; a.err = err_flag; a.axes = axes;
+    a.q = static_cast<const __nv_bfloat16*>(q_pe); a.qo = static_cast<__nv_bfloat16*>(q_out);
+    a.heads = q_pe ? num_heads : 0;
+    a.q_st = q_stride_t; a.q_sh = q_stride_h; a.qo_st = qo_stride_t; a.qo_sh = qo_stride_h;
+    const bool vec = reinterpret_cast<uintptr_t>(k_pe) % 16 == 0 && k_stride % 8 == 0 &&
+                     (!q_pe || ((reinterpret_cast<uintptr_t>(q_pe) | reinterpret_cast<uintptr_t>(q_out)) % 16 == 0 &&
+                                (q_stride_t | q_stride_h | qo_stride_t | qo_stride_h) % 8 == 0));
+    const uint32_t per_token = a.heads + 1;
+    a.rows_of_token = {per_token, static_cast<uint32_t>(((1ull << 32) + per_token - 1) / per_token)};
+    const int64_t per_block = kAppendSteps * 256 / (interleaved ? 8 : 4), blocks = (num_tokens * per_token + per_block - 1) / per_block;
+    if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "%s: too many rows for one call", what);
+    const dim3 grid(static_cast<unsigned>(blocks));
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    constexpr void (*kKernels[2][2][2])(RopeAppendArgs) = {
+        {{rope_append_rotated_kernel<false, false, false>, rope_append_rotated_kernel<false, false, true>},
+         {rope_append_rotated_kernel<false, true, false>, rope_append_rotated_kernel<false, true, true>}},
+        {{rope_append_rotated_kernel<true, false, false>, rope_append_rotated_kernel<true, false, true>},
+         {rope_append_rotated_kernel<true, true, false>, rope_append_rotated_kernel<true, true, true>}}};
+    void (*kernel)(RopeAppendArgs) = kKernels[interleaved != 0][vec][num_axes != 0];
+    const cudaError_t e = launch_dependent(kernel, grid, dim3(256), 0, st, a);
+    if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
+    return check_launch(what);
 }
 
 }  // namespace
@@ -365,34 +538,21 @@ extern "C" int nvfp4kv_rope(const void* x, int dtype, int64_t num_tokens, int nu
                             const float* cos_sin, int64_t max_positions, int rotary_dim, int rope_offset,
                             int interleaved, int inverse, void* out, int64_t out_stride_t, int64_t out_stride_h,
                             int32_t* err_flag, nvfp4kv_stream_t stream) {
-    using namespace nvfp4kv;
-    if (num_tokens < 0) return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: num_tokens < 0");
-    if (dtype != NVFP4KV_DTYPE_BF16 && dtype != NVFP4KV_DTYPE_F16 && dtype != NVFP4KV_DTYPE_F32)
-        return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: dtype must be bf16, fp16 or fp32");
-    if (pos_dtype != NVFP4KV_INDEX_I64 && pos_dtype != NVFP4KV_INDEX_I32)
-        return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: position dtype must be int64 or int32");
-    if (num_heads < 1 || head_dim < 1) return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: num_heads and head_dim must be >= 1");
-    if (rotary_dim < 2 || rotary_dim % 2 || rope_offset < 0 || rope_offset > head_dim - rotary_dim)
-        return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: rotary_dim %d at offset %d does not fit head_dim %d (even, >= 2)",
-                    rotary_dim, rope_offset, head_dim);
-    if (max_positions < 1) return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: empty cos_sin table");
-    if (num_tokens == 0) return NVFP4KV_OK;
-    if (!x || !positions || !cos_sin || !out) return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: null pointer");
-    const uintptr_t size = dtype == NVFP4KV_DTYPE_F32 ? 4 : 2;
-    if (reinterpret_cast<uintptr_t>(x) % size || reinterpret_cast<uintptr_t>(out) % size ||
-        reinterpret_cast<uintptr_t>(cos_sin) % 4)
-        return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: x, out and cos_sin must be aligned to their elements");
-    if (x == out && (x_stride_t != out_stride_t || x_stride_h != out_stride_h))
-        return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: in place needs equal strides");
-    RopeArgs a{};
-    a.x = x; a.out = out; a.x_st = x_stride_t; a.x_sh = x_stride_h; a.o_st = out_stride_t; a.o_sh = out_stride_h;
-    a.positions = positions; a.cos_sin = cos_sin; a.max_positions = max_positions;
-    a.heads = num_heads; a.dim = head_dim; a.rotary = rotary_dim; a.offset = rope_offset;
-    a.pos_i64 = pos_dtype == NVFP4KV_INDEX_I64; a.inverse = inverse != 0; a.in_place = x == out; a.err = err_flag;
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (dtype == NVFP4KV_DTYPE_BF16) return launch_rope<__nv_bfloat16>(a, num_tokens, interleaved != 0, st);
-    if (dtype == NVFP4KV_DTYPE_F16) return launch_rope<__half>(a, num_tokens, interleaved != 0, st);
-    return launch_rope<float>(a, num_tokens, interleaved != 0, st);
+    return nvfp4kv::rope_call("nvfp4kv_rope", x, dtype, num_tokens, num_heads, head_dim, x_stride_t, x_stride_h, positions,
+                              pos_dtype, 0, 0, nullptr, cos_sin, max_positions, rotary_dim, rope_offset, interleaved, inverse,
+                              out, out_stride_t, out_stride_h, err_flag, stream);
+}
+
+extern "C" int nvfp4kv_rope_axes(const void* x, int dtype, int64_t num_tokens, int num_heads, int head_dim,
+                                 int64_t x_stride_t, int64_t x_stride_h, const void* positions, int pos_dtype,
+                                 int64_t positions_stride, int num_axes, const uint8_t* pair_axes,
+                                 const float* cos_sin, int64_t max_positions, int rotary_dim, int rope_offset,
+                                 int interleaved, int inverse, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                                 int32_t* err_flag, nvfp4kv_stream_t stream) {
+    // (0 axes are refused here, where nvfp4kv_rope means one)
+    return nvfp4kv::rope_call("nvfp4kv_rope_axes", x, dtype, num_tokens, num_heads, head_dim, x_stride_t, x_stride_h, positions,
+                              pos_dtype, positions_stride, num_axes == 0 ? -1 : num_axes, pair_axes, cos_sin, max_positions,
+                              rotary_dim, rope_offset, interleaved, inverse, out, out_stride_t, out_stride_h, err_flag, stream);
 }
 
 extern "C" int nvfp4kv_append_rope_rotated(const void* k_pe, int64_t num_tokens, int64_t k_stride, void* rope_pool,
@@ -401,46 +561,21 @@ extern "C" int nvfp4kv_append_rope_rotated(const void* k_pe, int64_t num_tokens,
                                            int64_t max_positions, int interleaved, const void* q_pe, int num_heads,
                                            int64_t q_stride_t, int64_t q_stride_h, void* q_out, int64_t qo_stride_t,
                                            int64_t qo_stride_h, int32_t* err_flag, nvfp4kv_stream_t stream) {
-    using namespace nvfp4kv;
-    if (num_tokens < 0) return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: num_tokens < 0");
-    if ((slot_dtype != NVFP4KV_INDEX_I64 && slot_dtype != NVFP4KV_INDEX_I32) ||
-        (pos_dtype != NVFP4KV_INDEX_I64 && pos_dtype != NVFP4KV_INDEX_I32))
-        return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: slots and positions must be int64 or int32");
-    if (num_tokens == 0) return NVFP4KV_OK;
-    if (!k_pe || !rope_pool || !slot_mapping || !positions || !cos_sin || (q_pe && !q_out))
-        return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: null pointer");
-    if (k_stride < NVFP4KV_ROPE)
-        return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: k_stride %lld < 64", (long long)k_stride);
-    if (pool_rows <= 0 || max_positions < 1)
-        return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: empty rope pool or cos_sin table");
-    if (q_pe && (num_heads < 1 || num_heads >= kMostDivisor))
-        return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: num_heads %d not in [1, %d)", num_heads, kMostDivisor);
-    if (reinterpret_cast<uintptr_t>(rope_pool) % 16 || reinterpret_cast<uintptr_t>(cos_sin) % 16 ||
-        (reinterpret_cast<uintptr_t>(k_pe) | reinterpret_cast<uintptr_t>(q_pe) | reinterpret_cast<uintptr_t>(q_out)) % 2)
-        return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: rope pool and cos_sin must be 16-byte aligned");
-    if (q_pe && q_pe == q_out && (q_stride_t != qo_stride_t || q_stride_h != qo_stride_h))
-        return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: in place needs equal strides");
-    RopeAppendArgs a{};
-    a.k = static_cast<const __nv_bfloat16*>(k_pe); a.k_st = k_stride; a.tokens = num_tokens;
-    a.pool = static_cast<__nv_bfloat16*>(rope_pool); a.rows = pool_rows;
-    a.slots = slot_mapping; a.slot_i64 = slot_dtype == NVFP4KV_INDEX_I64;
-    a.positions = positions; a.pos_i64 = pos_dtype == NVFP4KV_INDEX_I64;
-    a.cos_sin = cos_sin; a.max_positions = max_positions; a.err = err_flag;
-    a.q = static_cast<const __nv_bfloat16*>(q_pe); a.qo = static_cast<__nv_bfloat16*>(q_out);
-    a.heads = q_pe ? num_heads : 0;
-    a.q_st = q_stride_t; a.q_sh = q_stride_h; a.qo_st = qo_stride_t; a.qo_sh = qo_stride_h;
-    const bool vec = reinterpret_cast<uintptr_t>(k_pe) % 16 == 0 && k_stride % 8 == 0 &&
-                     (!q_pe || ((reinterpret_cast<uintptr_t>(q_pe) | reinterpret_cast<uintptr_t>(q_out)) % 16 == 0 &&
-                                (q_stride_t | q_stride_h | qo_stride_t | qo_stride_h) % 8 == 0));
-    const uint32_t per_token = a.heads + 1;
-    a.rows_of_token = {per_token, static_cast<uint32_t>(((1ull << 32) + per_token - 1) / per_token)};
-    const int64_t per_block = kAppendSteps * 256 / (interleaved ? 8 : 4), blocks = (num_tokens * per_token + per_block - 1) / per_block;
-    if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "nvfp4kv_append_rope_rotated: too many rows for one call");
-    const dim3 grid(static_cast<unsigned>(blocks));
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    void (*kernel)(RopeAppendArgs) = interleaved ? (vec ? rope_append_rotated_kernel<true, true> : rope_append_rotated_kernel<true, false>)
-                                                 : (vec ? rope_append_rotated_kernel<false, true> : rope_append_rotated_kernel<false, false>);
-    const cudaError_t e = launch_dependent(kernel, grid, dim3(256), 0, st, a);
-    if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_append_rope_rotated launch failed: %s", cudaGetErrorString(e));
-    return check_launch("nvfp4kv_append_rope_rotated");
+    return nvfp4kv::append_rotated_call("nvfp4kv_append_rope_rotated", k_pe, num_tokens, k_stride, rope_pool, pool_rows,
+                                        slot_mapping, slot_dtype, positions, pos_dtype, 0, 0, nullptr, cos_sin, max_positions,
+                                        interleaved, q_pe, num_heads, q_stride_t, q_stride_h, q_out, qo_stride_t, qo_stride_h,
+                                        err_flag, stream);
+}
+
+extern "C" int nvfp4kv_append_rope_rotated_axes(const void* k_pe, int64_t num_tokens, int64_t k_stride, void* rope_pool,
+                                                int64_t pool_rows, const void* slot_mapping, int slot_dtype,
+                                                const void* positions, int pos_dtype, int64_t positions_stride,
+                                                int num_axes, const uint8_t* pair_axes, const float* cos_sin,
+                                                int64_t max_positions, int interleaved, const void* q_pe, int num_heads,
+                                                int64_t q_stride_t, int64_t q_stride_h, void* q_out, int64_t qo_stride_t,
+                                                int64_t qo_stride_h, int32_t* err_flag, nvfp4kv_stream_t stream) {
+    return nvfp4kv::append_rotated_call("nvfp4kv_append_rope_rotated_axes", k_pe, num_tokens, k_stride, rope_pool, pool_rows,
+                                        slot_mapping, slot_dtype, positions, pos_dtype, positions_stride,
+                                        num_axes == 0 ? -1 : num_axes, pair_axes, cos_sin, max_positions, interleaved, q_pe,
+                                        num_heads, q_stride_t, q_stride_h, q_out, qo_stride_t, qo_stride_h, err_flag, stream);
 }

@@ -25,6 +25,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -670,6 +671,55 @@ def rope_cos_sin(max_positions: int, rotary_dim: int = ROPE, base: float = 10000
     return (torch.cat([angle.cos(), angle.sin()], 1) * gain).float()
 
 
+def rope_axes(sections, rotary_dim: int = ROPE, dealt: bool = False) -> tuple[int, ...]:
+    """The axis of each of the rotary_dim / 2 pairs, for ``axes`` of the rotary operators: sections[a]
+    pairs turn by axis a (time, height, width ...; at most 4), in sections one after the other, or
+    ``dealt``: a pair to each axis in turn that has some left."""
+    left = [int(n) for n in sections]
+    if not 1 <= len(left) <= _lib.MAX_AXES or min(left) < 0 or 2 * sum(left) != rotary_dim:
+        raise ValueError(f"sections must be 1 to {_lib.MAX_AXES} numbers of pairs that add up to rotary_dim / 2")
+    if not dealt:
+        return tuple(a for a, n in enumerate(left) for _ in range(n))
+    out = []
+    while len(out) < rotary_dim // 2:
+        for a, n in enumerate(left):
+            if n:
+                out.append(a)
+                left[a] = n - 1
+    return tuple(out)
+
+
+_pair_axes: dict = {}      # the C entries' pair_axes, by the tuple of axes
+
+
+def _axes(axes, num: int, rotary_dim: int):
+    """The host array of a call's pair axes."""
+    array = _pair_axes.get((axes, num, rotary_dim)) if type(axes) is tuple else None
+    if array is None:
+        axes = tuple(int(a) for a in axes)
+        if len(axes) != rotary_dim // 2 or not all(0 <= a < num for a in axes):
+            raise ValueError(f"axes must be {rotary_dim // 2} numbers in [0, {num}), one for each rotated pair")
+        if len(_pair_axes) >= 256:
+            _pair_axes.clear()
+        array = _pair_axes[axes, num, rotary_dim] = (ctypes.c_uint8 * len(axes))(*axes)
+    return array
+
+
+def _check_axes(index: int, cos_sin: torch.Tensor, positions: torch.Tensor, T: int, rotary_dim: int, axes):
+    """_check_angles for positions [axes, T]: also their stride, their number and the pairs' axes."""
+    if axes is None:
+        raise ValueError("positions of several axes need axes, the axis of each pair (see rope_axes)")
+    shape = positions.shape
+    if len(shape) != 2 or not 1 <= shape[0] <= _lib.MAX_AXES or shape[1] != T:
+        raise ValueError(f"positions must be [axes, {T}] with at most {_lib.MAX_AXES} axes")
+    if rotary_dim > _lib.MAX_AXES_DIM:
+        raise ValueError(f"several axes rotate at most {_lib.MAX_AXES_DIM} dims")
+    if T > 1 and positions.stride(1) != 1:
+        positions = positions.contiguous()
+    _, dtype = _check_angles(index, cos_sin, positions[0], T, rotary_dim)
+    return positions, dtype, positions.stride(0), shape[0], _axes(axes, shape[0], rotary_dim)
+
+
 def _check_angles(index: int, cos_sin: torch.Tensor, positions: torch.Tensor, T: int, rotary_dim: int):
     _require_on(index, cos_sin, "cos_sin")
     _require_on(index, positions, "positions")
@@ -686,13 +736,17 @@ def _check_angles(index: int, cos_sin: torch.Tensor, positions: torch.Tensor, T:
 
 
 def apply_rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, rope_offset: int | None = None,
-               interleaved: bool = True, inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+               interleaved: bool = True, inverse: bool = False, out: torch.Tensor | None = None,
+               axes=None) -> torch.Tensor:
     """Rotary positions: x [T, H, D] or [T, D] (bf16, fp16 or fp32, last dim contiguous), dims
     [rope_offset, rope_offset + cos_sin.shape[1]) of every head rotated by its token's angles
     (default: the last dims), the others copied.  ``interleaved`` pairs dims (2i, 2i + 1), else
     (i, i + half).  ``inverse`` rotates back: the gradient with respect to x.  ``out`` may be x;
     a position outside the table leaves its token as it is and is flagged in the device error
-    word.  cos_sin: see rope_cos_sin."""
+    word.  cos_sin: see rope_cos_sin.
+
+    With ``axes`` (the axis of each of the cos_sin.shape[1] / 2 pairs, see rope_axes) positions is
+    [axes, T]: pair i of token t turns by positions[axes[i], t]."""
     _require_cuda(x, "x")
     dtype = _ROPE_DTYPES.get(x.dtype)
     if dtype is None:
@@ -710,6 +764,13 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, 
     T, D = shape[0], shape[-1]
     H, sh, osh = (shape[1], st[1], ost[1]) if len(shape) == 3 else (1, D, D)
     P, r = cos_sin.shape
+    if axes is not None:
+        pos, pdt, ps, A, pairs = _check_axes(index, cos_sin, positions, T, r, axes)
+        if T and H:
+            _call("nvfp4kv_rope_axes", index, x.data_ptr(), dtype, T, H, D, st[0], sh, pos.data_ptr(), pdt, ps, A, pairs,
+                  cos_sin.data_ptr(), P, r, D - r if rope_offset is None else int(rope_offset), int(interleaved),
+                  int(inverse), out.data_ptr(), ost[0], osh)
+        return out
     pos, pdt = _check_angles(index, cos_sin, positions, T, r)
     if T == 0 or H == 0:
         return out
@@ -721,10 +782,12 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, 
 
 def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_mapping: torch.Tensor,
                              positions: torch.Tensor, cos_sin: torch.Tensor, q_pe: torch.Tensor | None = None,
-                             q_out: torch.Tensor | None = None, interleaved: bool = True) -> torch.Tensor | None:
+                             q_out: torch.Tensor | None = None, interleaved: bool = True,
+                             axes=None) -> torch.Tensor | None:
     """The rope part of a step in one launch: k_pe [T, 64] bf16, rotated by its tokens' angles,
     into the rope side-pool at slot_mapping (as write_nvfp4_rope), and the queries' rope dims
-    q_pe [T, H, 64] bf16 rotated into q_out (default: in place).  Returns q_out."""
+    q_pe [T, H, 64] bf16 rotated into q_out (default: in place).  Returns q_out.  ``axes``: positions
+    [axes, T], as in apply_rope."""
     _require_cuda(k_pe, "k_pe")
     index = k_pe.get_device()
     _require_on(index, rope_cache, "rope_cache")
@@ -743,7 +806,10 @@ def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_
     sdt = _INDEX_DTYPES.get(slot.dtype)
     if sdt is None:
         raise TypeError("slot_mapping must be int64 or int32")
-    pos, pdt = _check_angles(index, cos_sin, positions, T, ROPE)
+    if axes is None:
+        pos, pdt = _check_angles(index, cos_sin, positions, T, ROPE)
+    else:
+        pos, pdt, ps, A, pairs = _check_axes(index, cos_sin, positions, T, ROPE, axes)
     H, qs, qos, q_ptr, qo_ptr = 0, (0, 0), (0, 0), None, None
     if q_pe is not None:
         _require_on(index, q_pe, "q_pe")
@@ -764,6 +830,11 @@ def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_
         raise ValueError("q_out without q_pe")
     if T == 0:
         return q_out
+    if axes is not None:
+        _call("nvfp4kv_append_rope_rotated_axes", index, k_pe.data_ptr(), T, ks[0], rope_cache.data_ptr(),
+              rows, slot.data_ptr(), sdt, pos.data_ptr(), pdt, ps, A, pairs, cos_sin.data_ptr(),
+              cos_sin.shape[0], int(interleaved), q_ptr, H, qs[0], qs[1], qo_ptr, qos[0], qos[1])
+        return q_out
     _call("nvfp4kv_append_rope_rotated", index, k_pe.data_ptr(), T, ks[0], rope_cache.data_ptr(),
           rows, slot.data_ptr(), sdt, pos.data_ptr(), pdt, cos_sin.data_ptr(),
           cos_sin.shape[0], int(interleaved), q_ptr, H, qs[0], qs[1], qo_ptr, qos[0], qos[1])
@@ -775,7 +846,7 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
                 kv_lora_rank: int, qk_rope_head_dim: int, block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor,
                 seq_lens: torch.Tensor, max_q_len: int, max_seq_len: int, out: torch.Tensor | None = None,
                 bmm1_scale: float = 1.0, bmm2_scale: float = 1.0, rope_cache: torch.Tensor | None = None,
-                return_lse: bool = False):
+                return_lse: bool = False, window: int = 0, sinks: int = 0):
     """Causal MLA attention of a ragged batch of new tokens over the paged pool, whose rows
     already hold them: chunked prefill, speculative steps and single tokens in one call.
 
@@ -788,7 +859,10 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
     [T, H, kv_lora_rank] bf16, with ``return_lse`` also lse [T, H] float32 (natural log; -inf for
     a row that sees no token, whose out is zeros).  Rows of new tokens past max_q_len, and rows
     from cu_seqlens_q[-1] on (the padding of a captured batch), are not written: they hold what
-    was in ``out`` before, and anything where the call allocates it."""
+    was in ``out`` before, and anything where the call allocates it.
+
+    ``window`` > 0: the query at position p sees only tokens t > p - window, and the first ``sinks``
+    of its sequence.  What no new token sees is not read, and its pages may be gone (trim_pages)."""
     try:      # (the whole host side of a call is about as long as a short batch on the device)
         index = query.get_device()
         together = index >= 0 and kv_cache.get_device() == block_tables.get_device() == cu_seqlens_q.get_device() \
@@ -802,6 +876,8 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
             _require_on(query.get_device(), t, name)
     if isinstance(bmm1_scale, torch.Tensor) or isinstance(bmm2_scale, torch.Tensor):
         raise TypeError("bmm1_scale / bmm2_scale must be Python floats (a device scalar would need a sync)")
+    if window < 0 or sinks < 0 or (sinks and not window):
+        raise ValueError("window and sinks must be >= 0, and sinks need a window")
     qs = query.stride()
     if query.dtype is not torch.bfloat16 or len(qs) != 3 or qs[2] != 1:
         raise ValueError("query must be bf16 [T, H, D] with a contiguous last dimension")
@@ -837,14 +913,21 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
         rope = rope_cache.data_ptr()
     lse = query.new_empty((T, H), dtype=torch.float32) if return_lse else None
     if T > 0 and B > 0:
-        key = ("prefill", B, T, H, max_q_len, max_seq_len, index)
+        if window:      # (as C ints: what is longer than a sequence hides nothing)
+            window, sinks = min(int(window), 0x7FFFFFFF), min(int(sinks), 0x7FFFFFFF)
+        key = ("prefill", B, T, H, max_q_len, max_seq_len, window, sinks, index)
         need = _ws_sizes.get(key)
         if need is None:
             n = ctypes.c_size_t(0)
             with _on_device(query.device):
-                _lib.check(_lib.lib().nvfp4kv_mla_prefill_workspace_size(B, T, H, int(max_q_len), int(max_seq_len),
-                                                                         ctypes.byref(n)),
-                           "nvfp4kv_mla_prefill_workspace_size")
+                if window:
+                    _lib.check(_lib.lib().nvfp4kv_mla_prefill_window_workspace_size(
+                        B, T, H, int(max_q_len), int(max_seq_len), window, sinks, ctypes.byref(n)),
+                        "nvfp4kv_mla_prefill_window_workspace_size")
+                else:
+                    _lib.check(_lib.lib().nvfp4kv_mla_prefill_workspace_size(B, T, H, int(max_q_len), int(max_seq_len),
+                                                                             ctypes.byref(n)),
+                               "nvfp4kv_mla_prefill_workspace_size")
             if len(_ws_sizes) >= 4096:      # a serving loop meets ever new shapes
                 _ws_sizes.clear()
             need = _ws_sizes[key] = int(n.value)
@@ -852,10 +935,10 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
         if ws is None or ws.get_device() != index or not ws.is_contiguous() or ws.data_ptr() % 256 \
                 or ws.numel() * ws.element_size() < need:
             ws = _stream_buffer(index, "prefill_ws", need, torch.uint8)
-        _call("nvfp4kv_mla_prefill", index, query.data_ptr(), qs[0], qs[1], kv_cache.data_ptr(), rows, rope,
-              block_tables.data_ptr(), ts[0], cu.data_ptr(), sl.data_ptr(), B, T, H, D, kv_lora_rank, page_size,
-              int(max_q_len), int(max_seq_len), bmm1_scale, bmm2_scale, out.data_ptr(), os[0], os[1],
-              None if lse is None else lse.data_ptr(), ws.data_ptr(), need)
+        _call("nvfp4kv_mla_prefill_window" if window else "nvfp4kv_mla_prefill", index, query.data_ptr(), qs[0], qs[1],
+              kv_cache.data_ptr(), rows, rope, block_tables.data_ptr(), ts[0], cu.data_ptr(), sl.data_ptr(), B, T, H, D,
+              kv_lora_rank, page_size, int(max_q_len), int(max_seq_len), *((window, sinks) if window else ()), bmm1_scale,
+              bmm2_scale, out.data_ptr(), os[0], os[1], None if lse is None else lse.data_ptr(), ws.data_ptr(), need)
     return (out, lse) if return_lse else out
 
 
@@ -925,6 +1008,72 @@ def _stream_buffer(index: int, name: str, n: int, dtype: torch.dtype) -> torch.T
     if ws is None or ws.numel() < n:
         ws = _bufs[key] = torch.empty(n, dtype=dtype, device=torch.device("cuda", index))
     return ws
+
+
+class StepTables(NamedTuple):
+    """What the kernels of a step take (extend_pages), for its n requests and num_tokens rows."""
+    slot_mapping: torch.Tensor     # [num_tokens] int64: pool slot of each new token, -1 for padding
+    positions: torch.Tensor        # [num_tokens] int32: its position, 0 for padding
+    cu_seqlens_q: torch.Tensor     # [n + 1] int32: where each request's tokens begin
+    seq_lens: torch.Tensor         # [n] int32: its length with them
+    block_tables: torch.Tensor     # [n, width] int32: its table
+
+
+def extend_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, slots: torch.Tensor, new_lens: torch.Tensor,
+                 ref_counts: torch.Tensor, page_size: int, num_tokens: int,
+                 lens: torch.Tensor | None = None) -> StepTables:
+    """The tables of a step, built on the device: request k appends new_lens[k] tokens to the sequence
+    in slots[k] of block_tables [num_slots, width] and seq_lens.  Every page that begins in them is
+    the lowest free one (ref_counts 0 -> 1), in order of k; tables, lengths and counts change in
+    place.  ``lens`` [n]: the sequences' lengths before the step where they are shorter than seq_lens
+    (drafts that were not accepted are taken back, and their pages given back first).
+
+    num_tokens: the step's rows, at least the new tokens; the rest is padding.  A request that cannot
+    be extended is skipped, with no tokens, length 0 and an empty table, and flagged in the device
+    error word: a bad or twice named slot, a bad length, more than the table's width, the free pages
+    or num_tokens hold in order of k, or a first page that is missing or shared."""
+    _require_cuda(block_tables, "block_tables")
+    index, st = block_tables.get_device(), block_tables.stride()
+    if not _tables(index, block_tables, st, seq_lens, slots, new_lens, ref_counts) or (lens is not None and not _ints(index, lens)):
+        _check_int32(index, block_tables=block_tables, seq_lens=seq_lens, slots=slots, new_lens=new_lens, ref_counts=ref_counts,
+                     **({} if lens is None else {"lens": lens}))
+    n, (S, width), pages = slots.shape[0], block_tables.shape, ref_counts.shape[0]
+    if seq_lens.shape[0] != S:
+        raise ValueError("seq_lens must have one entry per row of block_tables")
+    if new_lens.shape[0] != n or (lens is not None and lens.shape[0] != n):
+        raise ValueError("new_lens and lens must have one entry per slot")
+    if num_tokens < 0:
+        raise ValueError("num_tokens must be >= 0")
+    dev = block_tables.device
+    slot_mapping = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    tables, positions, out_lens, cu = torch.empty(n * width + num_tokens + 2 * n + 1, dtype=_INT32, device=dev).split(
+        (n * width, num_tokens, n, n + 1))
+    need = 2 * n + S + pages       # nvfp4kv_extend_workspace_ints
+    ws = _stream_buffer(index, "extend_ws", need, _INT32)
+    _call("nvfp4kv_extend_pages", index, block_tables.data_ptr(), st[0], width, S, seq_lens.data_ptr(), slots.data_ptr(),
+          new_lens.data_ptr(), None if lens is None else lens.data_ptr(), n, page_size, ref_counts.data_ptr(), pages,
+          num_tokens, slot_mapping.data_ptr(), positions.data_ptr(), cu.data_ptr(), out_lens.data_ptr(), tables.data_ptr(),
+          ws.data_ptr(), ws.numel())
+    return StepTables(slot_mapping, positions, cu, out_lens, tables.view(n, width))
+
+
+def trim_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, slots: torch.Tensor, ref_counts: torch.Tensor,
+               page_size: int, window: int = 0, sinks: int = 0) -> None:
+    """Gives back pages of the sequences in ``slots`` that no later step reads, in place: with
+    ``window`` those behind the window of the next token, but for the first ``sinks`` tokens (their
+    entries become -2), and those past the sequence's end (-1)."""
+    _require_cuda(block_tables, "block_tables")
+    index, st = block_tables.get_device(), block_tables.stride()
+    if not _tables(index, block_tables, st, seq_lens, slots, ref_counts):
+        _check_int32(index, block_tables=block_tables, seq_lens=seq_lens, slots=slots, ref_counts=ref_counts)
+    S, width = block_tables.shape
+    if seq_lens.numel() != S:
+        raise ValueError("seq_lens must have one entry per row of block_tables")
+    if window < 0 or sinks < 0 or (sinks and not window):
+        raise ValueError("window and sinks must be >= 0, and sinks need a window")
+    _call("nvfp4kv_trim_pages", index, block_tables.data_ptr(), st[0], width, S, seq_lens.data_ptr(), slots.data_ptr(),
+          slots.numel(), page_size, min(int(window), 0x7FFFFFFF), min(int(sinks), 0x7FFFFFFF), ref_counts.data_ptr(),
+          ref_counts.numel())
 
 
 def copy_pages(caches, src: torch.Tensor, dst: torch.Tensor) -> None:
