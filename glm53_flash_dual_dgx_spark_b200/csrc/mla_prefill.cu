@@ -93,7 +93,7 @@ constexpr int SM_LSUM = SM_RED + 2 * 4 * 64 * 4;             // 4 x 64 f32
 constexpr int SM_QS = SM_LSUM + 4 * 64 * 4;                  // 4 x 64 f32: score factor (log2 units) of a row
 constexpr int SM_FLAGS = SM_QS + 4 * 64 * 4;                 // [0] TMEM base, [1] abort
 constexpr int SM_WORK = SM_FLAGS + 16;                       // a Work per warp, and one with the range's first part
-constexpr int kWorkBytes = 144;
+constexpr int kWorkBytes = 160;
 constexpr int SM_BARS = SM_WORK + (kThreads / 32 + 1) * kWorkBytes;
 constexpr int B_FULL = 0;                      // [kStages] leader: stage landed in both CTAs
 constexpr int B_EMPTY = B_FULL + kStages;      // [kStages] both: the MMAs have read the stage
@@ -134,6 +134,7 @@ struct PrefillParams {
     const int32_t* seq_lens;
     int batch, total_q, heads, page_shift, max_q_len, max_seq_len;
     int window, sinks;         // position p sees t > p - window and t < sinks (window 0: every t <= p)
+    int sink_rows, max_tiles;  // sinks rounded up to 64; tiles of a unit far into its sequence
     uint32_t heads_magic;      // ceil(2^32 / heads)
     int pairs;
     float scale_log2, out_scale;
@@ -263,16 +264,35 @@ __device__ __forceinline__ Seq load_seq(const PrefillParams& p, int b) {
     s.units = (s.rows + kUnitRows - 1) / kUnitRows;
     return s;
 }
-__device__ __forceinline__ int image_blocks_of(const Seq& s) {
-    return s.units > 0 ? (s.L + kImageTok - 1) / kImageTok : 0;
-}
 // Tokens that unit k of the sequence sees: those of its last row.
 __device__ __forceinline__ int unit_end(const PrefillParams& p, const Seq& s, int k) {
     const int last = min(s.rows, (k + 1) * kUnitRows) - 1;
     return max(0, min(s.L, s.L - s.n + last / p.heads + 1));
 }
+template <bool kWindow>
+__device__ __forceinline__ int tiles_to(const PrefillParams& p, int end) {
+    const int tiles = (end + kTile - 1) / kTile;
+    return kWindow ? min(tiles, p.max_tiles) : tiles;
+}
+template <bool kWindow>
 __device__ __forceinline__ int unit_tiles(const PrefillParams& p, const Seq& s, int k) {
-    return (unit_end(p, s, k) + kTile - 1) / kTile;
+    return tiles_to<kWindow>(p, unit_end(p, s, k));
+}
+// A window's unit covers, in max_tiles tiles, the first sink_rows tokens and the last ones up to its
+// end (rounded up to 64); positions it leaves out in between.  0 for a unit that covers everything.
+__device__ __forceinline__ int unit_gap(const PrefillParams& p, int end) {
+    return end > p.max_tiles * kTile ? (end + 63) / 64 * 64 - p.max_tiles * kTile : 0;
+}
+// Rows of the sequence's image: its tokens, or with a window those that its units cover (without the gap
+// of the first one, which is the smallest).
+template <bool kWindow>
+__device__ __forceinline__ int image_rows_of(const PrefillParams& p, const Seq& s) {
+    if (s.units == 0) return 0;
+    return kWindow ? unit_end(p, s, s.units - 1) - unit_gap(p, unit_end(p, s, 0)) : s.L;
+}
+template <bool kWindow>
+__device__ __forceinline__ int image_blocks_of(const PrefillParams& p, const Seq& s) {
+    return (image_rows_of<kWindow>(p, s) + kImageTok - 1) / kImageTok;
 }
 // Weights of the work: a tile, and what a unit adds (its first tile's and its epilogue's latency, about
 // 8,700 cycles of a tile's 5,800).  With one tile's weight for a unit, pairs with short units took 9 %
@@ -280,9 +300,10 @@ __device__ __forceinline__ int unit_tiles(const PrefillParams& p, const Seq& s, 
 constexpr int kTileWeight = 2, kUnitWeight = 3;
 // Weight of the sequence's first K units.  A unit's tiles do not fall with k, so the sum goes over
 // tile counts (at most n / 256 + 2 of them), not over units.
+template <bool kWindow>
 __device__ __forceinline__ int64_t weight_before(const PrefillParams& p, const Seq& s, int K) {
     if (K <= 0) return 0;
-    const int t0 = unit_tiles(p, s, 0), t1 = unit_tiles(p, s, s.units - 1);
+    const int t0 = unit_tiles<kWindow>(p, s, 0), t1 = unit_tiles<kWindow>(p, s, s.units - 1);
     int64_t w = static_cast<int64_t>(K) * (kTileWeight * t0 + kUnitWeight);
     for (int t = t0; t < t1; ++t) {
         // units of at most t tiles: those whose last row's token is at most y
@@ -311,13 +332,14 @@ struct Range {
     int image0;         // image blocks of the sequences before b
 };
 // Where pair `pair` of p.pairs begins.  Run by one warp, a sequence per lane (and pass, past 32).
+template <bool kWindow>
 __device__ __forceinline__ Range find_range(const PrefillParams& p, int pair) {
     const int lane = threadIdx.x & 31;
     Seq s{};
     int64_t w = 0, total = 0;
     for (int b = lane; b < p.batch; b += 32) {
         s = load_seq(p, b);
-        w = weight_before(p, s, s.units);
+        w = weight_before<kWindow>(p, s, s.units);
         total += w;
     }
 #pragma unroll
@@ -337,9 +359,9 @@ __device__ __forceinline__ Range find_range(const PrefillParams& p, int pair) {
         if (p.batch > 32) {       // (else the first pass left them here)
             s = Seq{};
             if (b0 + lane < p.batch) s = load_seq(p, b0 + lane);
-            w = weight_before(p, s, s.units);
+            w = weight_before<kWindow>(p, s, s.units);
         }
-        const int blocks = image_blocks_of(s);
+        const int blocks = image_blocks_of<kWindow>(p, s);
         const int64_t upto = before + warp_inclusive_sum(w, lane);
         const int img = r.image0 + warp_inclusive_sum(blocks, lane);
         const uint32_t hit = __ballot_sync(0xFFFFFFFFu, lo < upto);
@@ -357,13 +379,13 @@ __device__ __forceinline__ Range find_range(const PrefillParams& p, int pair) {
             int k = 0, len = t.units;
             while (len > 1) {                          // the last unit that begins at or before x, 32 candidates a step
                 const int step = (len + 31) / 32, cand = k + lane * step;
-                const uint32_t ok = __ballot_sync(0xFFFFFFFFu, cand < k + len && weight_before(p, t, cand) <= x);
+                const uint32_t ok = __ballot_sync(0xFFFFFFFFu, cand < k + len && weight_before<kWindow>(p, t, cand) <= x);
                 const int at = 31 - __clz(ok);
                 len = min(step, k + len - (k + at * step));
                 k += at * step;
             }
             r.k = k;
-            r.offset = static_cast<int>(x - weight_before(p, t, k));
+            r.offset = static_cast<int>(x - weight_before<kWindow>(p, t, k));
             return r;
         }
         before = __shfl_sync(0xFFFFFFFFu, upto, 31);
@@ -382,24 +404,31 @@ struct Part {
     int image;              // the sequence's first image block
     int head, tail;         // it begins / ends the unit
     int half;               // rows in the leading CTA (the unit's others are in the second)
+    int image_rows;         // of the sequence
+    int gap, lift;          // with a window: positions, and image rows, left out after sink_rows
 };
 // Tiles in a unit's first `weight`.
 __device__ __forceinline__ int tiles_in(int weight) { return max(weight - kUnitWeight, 0) / kTileWeight; }
 // The next part of the range; parts without tiles are given only where they are a whole unit (one
 // that sees no token).
+template <bool kWindow>
 __device__ __forceinline__ bool next_part_of(const PrefillParams& p, Range& r, Part& t) {
     while (r.left > 0) {
         const Seq s = load_seq(p, r.b);
-        const int blocks = image_blocks_of(s);
+        t.image_rows = image_rows_of<kWindow>(p, s);
         if (r.k >= s.units) {
             ++r.b;
             r.k = 0;
             r.offset = 0;
-            r.image0 += blocks;
+            r.image0 += (t.image_rows + kImageTok - 1) / kImageTok;
             continue;
         }
         t.end = unit_end(p, s, r.k);
-        const int tiles = (t.end + kTile - 1) / kTile;
+        const int tiles = tiles_to<kWindow>(p, t.end);
+        if (kWindow) {
+            t.gap = unit_gap(p, t.end);
+            t.lift = t.gap - unit_gap(p, unit_end(p, s, 0));
+        }
         const int weight = kTileWeight * tiles + kUnitWeight, begin = r.offset;
         const int take = static_cast<int>(r.left < weight - begin ? r.left : weight - begin);
         t.tile0 = tiles_in(begin);
@@ -432,11 +461,12 @@ struct Work {
 static_assert(sizeof(Work) <= kWorkBytes, "a warp's work record");
 // The search for a part takes a microsecond of dependent loads and divisions, so a warp may look for
 // the next one (ahead) while it waits for something else, and move on to it later (advance_part).
+template <bool kWindow>
 __device__ __forceinline__ void look_ahead(const PrefillParams& p, Work* w) {
     if ((threadIdx.x & 31) == 0) {
         Range r = w->range;
         Part t;
-        const bool more = next_part_of(p, r, t);
+        const bool more = next_part_of<kWindow>(p, r, t);
         w->range = r;
         w->more = more;
         if (more) w->ahead = t;
@@ -455,9 +485,10 @@ __device__ __forceinline__ bool advance_part(Work* w) {
     __syncwarp();
     return more;
 }
+template <bool kWindow>
 __device__ __forceinline__ bool next_part(const PrefillParams& p, Work* w) {
     __syncwarp();
-    look_ahead(p, w);
+    look_ahead<kWindow>(p, w);
     return advance_part(w);
 }
 
@@ -513,7 +544,7 @@ __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_cons
             int base = 0, b = -1, pos = 0;
             for (int b0 = 0; b0 < p.batch; b0 += 32) {
                 int blocks = 0;
-                if (b0 + lane < p.batch) blocks = image_blocks_of(load_seq(p, b0 + lane));
+                if (b0 + lane < p.batch) blocks = image_blocks_of<kWindow>(p, load_seq(p, b0 + lane));
                 const int upto = base + warp_inclusive_sum(blocks, lane);
                 const uint32_t hit = __ballot_sync(0xFFFFFFFFu, block < upto);
                 if (hit && b < 0) {
@@ -534,9 +565,13 @@ __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_cons
         if (b_s < 0) return;
         total = total_s * kImagePieces;
         const Seq seq = load_seq(p, b_s);
-        const int L = seq.L, t = pos_s + r0;
-        // (a token that no row sees is not read: its page may be gone)
-        const bool seen = !kWindow || t < p.sinks || t > L - seq.n - p.window;
+        int L = seq.L, t = pos_s + r0;
+        bool seen = true;
+        if (kWindow) {      // (a token that no row sees is not read: its page may be gone)
+            L = unit_end(p, seq, seq.units - 1);
+            if (t >= p.sink_rows) t += unit_gap(p, unit_end(p, seq, 0));
+            seen = t < p.sinks || t > seq.L - seq.n - p.window;
+        }
         const int64_t row = seen ? pool_row(p, p.tables + b_s * p.tables_stride, t, L) : -1;
         uint4 code[2], rope = make_uint4(0, 0, 0, 0);
         uint16_t scale[2] = {0, 0};
@@ -671,7 +706,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
     auto bar = [&](int i) -> uint32_t { return sbase + SM_BARS + 8 * i; };
 
     if (warp == 0) {
-        const Range r = find_range(p, pair);
+        const Range r = find_range<kWindow>(p, pair);
         if (lane == 0) {
             flags[1] = 0;
             // the range's first part, for every warp, and in `part` the first one with tiles: its Q and
@@ -679,12 +714,12 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             Work* w = reinterpret_cast<Work*>(smem + SM_WORK + kThreads / 32 * kWorkBytes);
             Range r0 = r;
             Part t0;
-            const bool more = next_part_of(p, r0, t0);
+            const bool more = next_part_of<kWindow>(p, r0, t0);
             w->range = r0;
             w->more = more;
             if (more) w->ahead = t0;
             bool tiles = more && t0.n_tiles > 0;
-            while (more && !tiles && next_part_of(p, r0, t0)) tiles = t0.n_tiles > 0;
+            while (more && !tiles && next_part_of<kWindow>(p, r0, t0)) tiles = t0.n_tiles > 0;
             if (!tiles) t0.n_tiles = 0;
             w->part = t0;
             if (cta == 0) p.parts[2 * pair].used = p.parts[2 * pair + 1].used = 0;
@@ -726,11 +761,28 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
     const int k_stages = p.rope ? 9 : 8;
     // A stage of a part's ring: K stage c.s of tile c.i, or V stage c.s - k_stages of tile c.i - 1.
     const int64_t image_bytes = static_cast<int64_t>(k_stages) * kStageBytes;
-    auto copy_stage = [&](const Cursor& c, int image, int last, int tile0, int slot) {
+    // (with a window, `last` is the sequence's last run of 64 image rows, `lift` in such runs)
+    auto copy_stage = [&](const Cursor& c, int image, int last, int tile0, int lift, int slot) {
         const uint32_t dst = sbase + SM_RING + slot * kStageBytes, landed = bar(B_LAND + slot);
         if (elect_one()) {
             mbar_arrive_expect_tx(landed, kStageBytes);
-            if (c.s < k_stages) {
+            if constexpr (kWindow) {
+                auto run = [&](int g) {      // 64 tokens of the unit: where their rows of atom 0 lie
+                    if (64 * g >= p.sink_rows) g += lift;
+                    g = min(g, last);
+                    return p.image + (image + (g >> 1)) * image_bytes + (g & 1) * 8192;
+                };
+                if (c.s < k_stages) {
+                    const int g = 4 * (tile0 + c.i) + 2 * cta;
+                    bulk_copy_g2s(dst, run(g) + c.s * kStageBytes, 8192, landed);
+                    bulk_copy_g2s(dst + 8192, run(g + 1) + c.s * kStageBytes, 8192, landed);
+                } else {
+                    const int v = c.s - k_stages;
+                    const uint8_t* src = run(4 * (tile0 + c.i - 1) + (v >> 1)) + (4 * cta + 2 * (v & 1)) * kStageBytes;
+                    bulk_copy_g2s(dst, src, 8192, landed);
+                    bulk_copy_g2s(dst + 8192, src + kStageBytes, 8192, landed);
+                }
+            } else if (c.s < k_stages) {
                 const int blk = min(image + 2 * (tile0 + c.i) + cta, last);
                 bulk_copy_g2s(dst, p.image + blk * image_bytes + c.s * kStageBytes, kStageBytes, landed);
             } else {
@@ -743,7 +795,10 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         }
         __syncwarp();
     };
-    auto last_block = [&](int image, int L) { return image + (L + kImageTok - 1) / kImageTok - 1; };      // (tokens past it are masked)
+    auto last_block = [&](int image, int rows) {      // (tokens past it are masked)
+        const int blocks = (rows + kImageTok - 1) / kImageTok;
+        return kWindow ? 2 * blocks - 1 : image + blocks - 1;
+    };
     int early = 0;                    // stages copied before the roles begin
     if (first->part.n_tiles > 0) {
         const Part& t1 = first->part;
@@ -757,7 +812,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             static_assert(kStages < 8 + kVStages, "stages of one tile");
             Cursor c{0, 0, 0};
             for (int u = 0; u < kStages; ++u, advance(c, k_stages, t1.n_tiles))
-                if ((u & 1) == warp - kCopyWarp0) copy_stage(c, t1.image, last_block(t1.image, t1.L), t1.tile0, u);
+                if ((u & 1) == warp - kCopyWarp0) copy_stage(c, t1.image, last_block(t1.image, t1.image_rows), t1.tile0, t1.lift / 64, u);
         }
         store_q(p, smem + SM_Q, reinterpret_cast<float*>(smem + SM_QS), warp, kWarps, q);
         fence_proxy_async_smem();
@@ -778,7 +833,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 const uint64_t dv = smem_desc_sw128(sbase + SM_RING, 8192, 1024);
                 int stages = 0, parts = 0, tile = 0;      // so far
 #pragma unroll 1
-                for (bool more = advance_part(work); more && !*abort_flag; more = next_part(p, work)) {
+                for (bool more = advance_part(work); more && !*abort_flag; more = next_part<kWindow>(p, work)) {
                     const int n_tiles = t.n_tiles;
                     if (n_tiles == 0) continue;
                     if (parts > 0) mbar_wait(bar(B_Q_FULL), (parts - 1) & 1, abort_flag, p.err);
@@ -849,9 +904,9 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             bool ok = true;
             griddep_wait();                       // the image kernel's writes
 #pragma unroll 1
-            for (bool more = advance_part(work); ok && more; more = next_part(p, work)) {
+            for (bool more = advance_part(work); ok && more; more = next_part<kWindow>(p, work)) {
                 const int n_tiles = t.n_tiles, total = n_tiles * (k_stages + kVStages), image = t.image, tile0 = t.tile0;
-                const int last = last_block(image, t.L);
+                const int last = last_block(image, t.image_rows), lift = kWindow ? t.lift / 64 : 0;
                 Cursor c{0, 0, 0};
 #pragma unroll 1
                 for (; c.u < total; advance(c, k_stages, n_tiles)) {
@@ -863,7 +918,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                         // (a release waited for by the other warp in between is earlier than this one's: no
                         // phase is skipped unseen)
                         if (u >= kStages && !(ok = mbar_wait(bar(B_EMPTY + slot), phase ^ 1, abort_flag, p.err))) break;
-                        copy_stage(c, image, last, tile0, slot);
+                        copy_stage(c, image, last, tile0, lift, slot);
                     }
                     ++u;
                     if (++slot == kStages) {
@@ -886,7 +941,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         float* qs = reinterpret_cast<float*>(smem + SM_QS);
         int parts = 0;
 #pragma unroll 1
-        for (bool more = advance_part(work); more; more = next_part(p, work)) {
+        for (bool more = advance_part(work); more; more = next_part<kWindow>(p, work)) {
             if (t.n_tiles == 0) continue;
             if (parts > 0) {                     // (the first part's is there)
                 // Converted into the workspace while the last part runs, and copied from there once its last QK
@@ -936,7 +991,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         griddep_wait();                          // the image kernel's token bits
 #pragma unroll 1
         while (advance_part(work)) {
-            const int n_tiles = t.n_tiles, tile0 = t.tile0, image = t.image;
+            const int n_tiles = t.n_tiles, tile0 = t.tile0, image = t.image, gap = kWindow ? t.gap : 0, lift = kWindow ? t.lift : 0;
             int lim = 0;                                                      // tokens the row sees
             {
                 const int grow = t.block * kUnitRows + t.half * cta + row;    // row of the sequence
@@ -946,6 +1001,13 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             // bits of the quarter's tokens that exist, and of those that hold a NaN, loaded a tile ahead
             auto load_bits = [&](int i, uint2 (&w)[2]) {
                 const int tok0 = (tile0 + i) * kTile + 64 * q4;
+                if constexpr (kWindow) {
+                    const int row0 = min(tok0 < p.sink_rows ? tok0 : tok0 + lift, t.image_rows - 1);
+                    const uint32_t* src = p.image_bits + 8 * static_cast<int64_t>(image + row0 / kImageTok) + (row0 & 64) / 32;
+                    w[0] = *reinterpret_cast<const uint2*>(src);
+                    w[1] = *reinterpret_cast<const uint2*>(src + 4);
+                    return;
+                }
                 const uint32_t* src = p.image_bits + 8 * static_cast<int64_t>(image + min(tok0, t.L - 1) / kImageTok) + ((tok0 & (kImageTok - 1)) >> 5);
                 w[0] = *reinterpret_cast<const uint2*>(src);
                 w[1] = *reinterpret_cast<const uint2*>(src + 4);
@@ -959,6 +1021,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 if (i + 1 < n_tiles) load_bits(i + 1, ahead);
                 int see = lim - ((tile0 + i) * kTile + 64 * q4);     // tokens of the quarter the row sees
                 if constexpr (kWindow) {
+                    if (lim - see >= p.sink_rows) see -= gap;
                     const int skip = see - p.window, keep = min(see, p.sinks - (lim - see));      // (lim - see: the quarter's first)
                     have.x &= (bits_below(see) & ~bits_below(skip)) | bits_below(keep);
                     have.y &= (bits_below(see - 32) & ~bits_below(skip - 32)) | bits_below(keep - 32);
@@ -1034,7 +1097,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 __syncwarp();
                 if (lane == 0) leader_arrive(bar(B_P_FULL));
             }
-            look_ahead(p, work);                        // (the last PV is running)
+            look_ahead<kWindow>(p, work);                        // (the last PV is running)
             // ---- epilogue: sums over the row's four warps, O out of TMEM
             named_bar_sync(1 + (sp & 1), 128);          // the last part's sums are read
             lsum[64 * q4 + row] = l;
@@ -1253,6 +1316,7 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_const
 struct PrefillPlan {
     int group;               // sequences per pass over the workspace
     int pairs, image_blocks;
+    int sink_rows, max_tiles;
     size_t image_bytes, bits_bytes, q_bytes, o_bytes, ml_bytes, ws_bytes;
 };
 
@@ -1263,16 +1327,27 @@ size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
 PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_len, int max_seq_len, int window, int sinks) {
     PrefillPlan pl{};
-    const int64_t one = (static_cast<int64_t>(max_seq_len) + kImageTok - 1) / kImageTok;
+    const int64_t longest = max_q_len < total_q ? max_q_len : total_q;
+    int64_t tiles = (static_cast<int64_t>(max_seq_len) + kTile - 1) / kTile, image_rows = max_seq_len;
+    if (window > 0) {
+        // a unit's rows belong to at most `span` tokens, and see no more than the sinks and the window - 1 +
+        // span last tokens up to its end, which is rounded up to a multiple of 64
+        const int64_t by_rows = (num_heads + kUnitRows - 2) / num_heads + 1, span = by_rows < longest ? by_rows : longest;
+        pl.sink_rows = (sinks + 63) / 64 * 64;
+        const int64_t most = (pl.sink_rows + static_cast<int64_t>(window) - 1 + span + 63 + kTile - 1) / kTile;
+        tiles = most < tiles ? most : tiles;
+        image_rows = kTile * most + longest < image_rows ? kTile * most + longest : image_rows;
+    }
+    pl.max_tiles = static_cast<int>(tiles);
+    const int64_t one = (image_rows + kImageTok - 1) / kImageTok;
     const int64_t cap = static_cast<int64_t>(kImageCap / (9 * kStageBytes));
     const int64_t fit = one > 0 ? cap / one : batch;
     pl.group = static_cast<int>(fit < 1 ? 1 : (fit < batch ? fit : batch));
     // no more pairs than leave each less than a tile's weight: what a group can have
-    const int64_t longest = max_q_len < total_q ? max_q_len : total_q;
     const int64_t by_seq = (longest * num_heads + kUnitRows - 1) / kUnitRows * pl.group;
     const int64_t by_rows = (static_cast<int64_t>(total_q) * num_heads + static_cast<int64_t>(pl.group) * (kUnitRows - 1)) / kUnitRows;
     const int64_t units = by_seq < by_rows ? by_seq : by_rows;
-    const int64_t most = units * (kUnitWeight + kTileWeight * ((static_cast<int64_t>(max_seq_len) + kTile - 1) / kTile)) / kTileWeight + 1;
+    const int64_t most = units * (kUnitWeight + kTileWeight * tiles) / kTileWeight + 1;
     int64_t pairs = device_sm_count() / 2;
     pairs = pairs > kMaxPairs ? kMaxPairs : pairs;
     pairs = pairs > most ? most : pairs;
@@ -1325,7 +1400,7 @@ int launch_prefill(const PrefillParams& all, const PrefillPlan& pl, cudaStream_t
         }
         if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill launch failed: %s", cudaGetErrorString(e));
         if ((rc = check_launch("nvfp4kv_mla_prefill")) != NVFP4KV_OK) return rc;
-        if (pl.pairs == 1 || p.max_seq_len <= kTile) continue;      // no unit can be cut
+        if (pl.pairs == 1 || pl.max_tiles <= 1) continue;      // no unit can be cut
         if (8 * pl.pairs <= device_sm_count()) e = launch_dependent(prefill_combine_kernel<1>, dim3(pl.pairs * kUnitRows), dim3(128), 0, st, p);
         else e = launch_dependent(prefill_combine_kernel<4>, dim3(pl.pairs * (kUnitRows / 4)), dim3(128), 0, st, p);
         if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill combine launch failed: %s", cudaGetErrorString(e));
@@ -1392,7 +1467,7 @@ int prefill_call(const void* q, int64_t q_stride_t, int64_t q_stride_h, const ui
     p.part_o = reinterpret_cast<float*>(ws += pl.q_bytes);
     p.part_ml = reinterpret_cast<float*>(ws += pl.o_bytes);
     p.parts = reinterpret_cast<PartInfo*>(ws += pl.ml_bytes);
-    p.window = window; p.sinks = sinks;
+    p.window = window; p.sinks = sinks; p.sink_rows = pl.sink_rows; p.max_tiles = pl.max_tiles;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return window > 0 ? launch_prefill<true>(p, pl, st) : launch_prefill<false>(p, pl, st);
 }
