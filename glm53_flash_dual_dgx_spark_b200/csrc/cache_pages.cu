@@ -276,61 +276,75 @@ __device__ __forceinline__ int64_t block_exclusive_scan64(int64_t v, int64_t* wa
 }
 
 // One block: which requests count, what they take back, the pages they need, the lowest free pages.
+// It is bound by the latency of its dependent accesses, so the claims on slots and the requests' state
+// are kept in shared memory where they fit.
+constexpr int kSharedSlots = 6144, kSharedRequests = 2048;
 __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(const __grid_constant__ ExtendArgs p) {
     __shared__ int64_t sums64[3][32];
     __shared__ int sums[32];
-    const int tid = threadIdx.x;
+    __shared__ int claim_s[kSharedSlots], start_s[kSharedRequests], rank_s[kSharedRequests];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int* claim = p.num_slots <= kSharedSlots ? claim_s : p.claim;
+    int* starts = p.num <= kSharedRequests ? start_s : p.start;
+    int* ranks = p.num <= kSharedRequests ? rank_s : p.rank;
     griddep_wait();
     for (int k = tid; k < p.num; k += kPlanThreads) {
         const int s = p.slots[k];
-        if (s >= 0 && s < p.num_slots) p.claim[s] = 0x7FFFFFFF;
+        if (s >= 0 && s < p.num_slots) claim[s] = 0x7FFFFFFF;
     }
     __syncthreads();
     for (int k = tid; k < p.num; k += kPlanThreads) {
         const int s = p.slots[k];
-        if (s >= 0 && s < p.num_slots) atomicMin(p.claim + s, k);
+        if (s >= 0 && s < p.num_slots) atomicMin(claim + s, k);
     }
     __syncthreads();
     // the checks, on lengths, tables and counts as they were before the call
     const int64_t most = static_cast<int64_t>(p.width) * p.page_size;
     for (int k = tid; k < p.num; k += kPlanThreads) {
         const int s = p.slots[k], n = p.new_lens[k];
+        const bool in = s >= 0 && s < p.num_slots;
+        const int have = in ? p.seq_lens[s] : 0, len = p.lens ? p.lens[k] : have;
+        const int first = in ? *static_cast<volatile int*>(claim + s) : -1;
         int start = -1, err = 0;
-        if (s < 0 || s >= p.num_slots || __ldcg(p.claim + s) != k) {
+        if (first != k) {
             err = NVFP4KV_DEVERR_BAD_SLOT;
+        } else if (n < 0 || len < 0 || len > have) {
+            err = NVFP4KV_DEVERR_SEQ_LEN;
+        } else if (static_cast<int64_t>(len) + n > most) {
+            err = NVFP4KV_DEVERR_CAPACITY;
         } else {
-            const int have = p.seq_lens[s], len = p.lens ? p.lens[k] : have;
-            if (n < 0 || len < 0 || len > have) {
-                err = NVFP4KV_DEVERR_SEQ_LEN;
-            } else if (static_cast<int64_t>(len) + n > most) {
-                err = NVFP4KV_DEVERR_CAPACITY;
-            } else {
-                start = len;
-                if (n > 0 && len % p.page_size != 0) {      // the new tokens begin in a page that others may read
-                    const int pg = p.tables[s * p.stride + len / p.page_size];
-                    if (pg < 0 || pg >= p.num_pages || __ldcg(p.refs + pg) != 1) {
-                        err = NVFP4KV_DEVERR_BAD_PAGE;
-                        start = -1;
-                    }
+            start = len;
+            if (n > 0 && len % p.page_size != 0) {      // the new tokens begin in a page that others may read
+                const int pg = p.tables[s * p.stride + len / p.page_size];
+                if (pg < 0 || pg >= p.num_pages || __ldcg(p.refs + pg) != 1) {
+                    err = NVFP4KV_DEVERR_BAD_PAGE;
+                    start = -1;
                 }
             }
         }
         if (err) set_error(p.err, err);
-        p.start[k] = start;
+        starts[k] = start;
     }
     __syncthreads();
-    // pages of tokens that are taken back
+    // pages of tokens that are taken back: a request per warp
     if (p.lens) {
-        for (int k = tid; k < p.num; k += kPlanThreads) {
-            const int start = p.start[k];
-            if (start < 0) continue;
-            const int s = p.slots[k], have = p.seq_lens[s];
-            int32_t* row = p.tables + s * p.stride;
-            const int end = min(pages_of(have, p.page_size), p.width);
-            for (int j = pages_of(start, p.page_size); j < end; ++j) {
-                const int pg = row[j];
-                row[j] = -1;
-                if (pg >= 0) release_page(p.refs, p.num_pages, pg, p.err);
+        for (int k0 = 0; k0 < p.num; k0 += kPlanThreads) {
+            const int k = k0 + 32 * lane + warp, start = k < p.num ? starts[k] : -1;
+            int s = 0, j0 = 0, j1 = 0;
+            if (start >= 0) {
+                s = p.slots[k];
+                j0 = pages_of(start, p.page_size);
+                j1 = min(pages_of(p.seq_lens[s], p.page_size), p.width);
+            }
+            for (uint32_t todo = __ballot_sync(0xFFFFFFFFu, j0 < j1); todo; todo &= todo - 1) {
+                const int l = __ffs(todo) - 1;
+                int32_t* row = p.tables + __shfl_sync(0xFFFFFFFFu, s, l) * p.stride;
+                const int end = __shfl_sync(0xFFFFFFFFu, j1, l);
+                for (int j = __shfl_sync(0xFFFFFFFFu, j0, l) + lane; j < end; j += 32) {
+                    const int pg = row[j];
+                    row[j] = -1;
+                    if (pg >= 0) release_page(p.refs, p.num_pages, pg, p.err);
+                }
             }
         }
         __syncthreads();
@@ -338,15 +352,15 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(const __grid_
     // running sums of tokens and pages
     int64_t tokens = 0, pages = 0;
     for (int k0 = 0; k0 < p.num; k0 += kPlanThreads) {
-        const int k = k0 + tid, start = k < p.num ? p.start[k] : -1, n = start >= 0 ? p.new_lens[k] : 0;
+        const int k = k0 + tid, start = k < p.num ? starts[k] : -1, n = start >= 0 ? p.new_lens[k] : 0;
         const int need = start >= 0 ? pages_of(start + n, p.page_size) - pages_of(start, p.page_size) : 0;
         int64_t sum_n, sum_p;
         const int64_t at_n = tokens + block_exclusive_scan64(n, sums64[0], &sum_n);
         const int64_t at_p = pages + block_exclusive_scan64(need, sums64[1], &sum_p);
         if (k < p.num) {
             // (-2: taken back, but not extended)
-            if (start >= 0 && n > 0 && at_n + n > p.num_tokens) p.rank[k] = -2;
-            else p.rank[k] = need == 0 ? -1 : static_cast<int>(at_p + need <= p.num_pages ? at_p : p.num_pages);
+            if (start >= 0 && n > 0 && at_n + n > p.num_tokens) ranks[k] = -2;
+            else ranks[k] = need == 0 ? -1 : static_cast<int>(at_p + need <= p.num_pages ? at_p : p.num_pages);
         }
         tokens += sum_n;
         pages += sum_p;
@@ -380,11 +394,12 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(const __grid_
     int64_t done = 0;
     for (int k0 = 0; k0 < p.num; k0 += kPlanThreads) {
         const int k = k0 + tid;
-        int start = -1, n = 0;
+        int start = -1, n = 0, rank = -1;
         bool ok = false;
-        if (k < p.num && (start = p.start[k]) >= 0) {
+        if (k < p.num && (start = starts[k]) >= 0) {
             n = p.new_lens[k];
-            const int need = pages_of(start + n, p.page_size) - pages_of(start, p.page_size), rank = p.rank[k];
+            rank = ranks[k];
+            const int need = pages_of(start + n, p.page_size) - pages_of(start, p.page_size);
             ok = rank != -2 && (need == 0 || static_cast<int64_t>(rank) + need <= found);
             if (!ok) set_error(p.err, NVFP4KV_DEVERR_CAPACITY);
         }
@@ -394,7 +409,8 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(const __grid_
             p.cu[k] = static_cast<int>(at);
             p.out_lens[k] = ok ? start + n : 0;
             if (start >= 0) p.seq_lens[p.slots[k]] = ok ? start + n : start;
-            if (!ok) p.start[k] = -1;
+            p.start[k] = ok ? start : -1;
+            p.rank[k] = rank;
         }
         done += sum;
         __syncthreads();
@@ -404,7 +420,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(const __grid_
 }
 
 // The first row_blocks blocks: the tables of a request, 1,024 entries each; the others: tokens.
-constexpr int kRowEntries = 1024, kTokensPerBlock = 256;
+constexpr int kRowEntries = 1024, kTokensPerBlock = 1024;
 __global__ void __launch_bounds__(256) extend_apply_kernel(const __grid_constant__ ExtendArgs p, int chunks, int64_t row_blocks) {
     griddep_wait();
     if (blockIdx.x < row_blocks) {
@@ -430,25 +446,34 @@ __global__ void __launch_bounds__(256) extend_apply_kernel(const __grid_constant
         }
         return;
     }
-    const int64_t t = (blockIdx.x - row_blocks) * kTokensPerBlock + threadIdx.x;
-    if (t >= p.num_tokens) return;
-    int64_t slot = -1;
-    int pos = 0;
-    if (t < p.cu[p.num]) {
-        int lo = 0, hi = p.num - 1;      // the last request that begins at or before t (empty ones end before it)
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (__ldg(p.cu + mid) <= t) lo = mid;
-            else hi = mid - 1;
-        }
-        const int start = p.start[lo];
-        pos = start + static_cast<int>(t) - p.cu[lo];
-        const int j = pos / p.page_size, first = pages_of(start, p.page_size);
-        const int pg = j < first ? p.tables[p.slots[lo] * p.stride + j] : p.free_list[p.rank[lo] + j - first];
-        slot = static_cast<int64_t>(pg) * p.page_size + pos % p.page_size;
+    const int64_t t0 = (blockIdx.x - row_blocks) * kTokensPerBlock;
+    __shared__ int cu_s[kSharedRequests + 1];
+    const int* cu = p.cu;
+    if (p.num <= kSharedRequests) {      // (a search of dependent steps, on the chip)
+        for (int k = threadIdx.x; k <= p.num; k += blockDim.x) cu_s[k] = p.cu[k];
+        __syncthreads();
+        cu = cu_s;
     }
-    p.slot_mapping[t] = slot;
-    p.positions[t] = pos;
+    const int live = cu[p.num];
+    for (int64_t t = t0 + threadIdx.x; t < min(t0 + kTokensPerBlock, p.num_tokens); t += blockDim.x) {
+        int64_t slot = -1;
+        int pos = 0;
+        if (t < live) {
+            int lo = 0, hi = p.num - 1;      // the last request that begins at or before t (empty ones end before it)
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (cu[mid] <= t) lo = mid;
+                else hi = mid - 1;
+            }
+            const int start = p.start[lo];
+            pos = start + static_cast<int>(t) - cu[lo];
+            const int j = pos / p.page_size, first = pages_of(start, p.page_size);
+            const int pg = j < first ? p.tables[p.slots[lo] * p.stride + j] : p.free_list[p.rank[lo] + j - first];
+            slot = static_cast<int64_t>(pg) * p.page_size + pos % p.page_size;
+        }
+        p.slot_mapping[t] = slot;
+        p.positions[t] = pos;
+    }
 }
 
 // ------------------------------------------------------------------ forking

@@ -48,18 +48,20 @@ __device__ __forceinline__ void rotate(float a, float b, float c, float s, float
     v = b * c + a * s;
 }
 
-// N consecutive cos (or sin) values, N a multiple of 4 or 2, 8-byte aligned.
-template <int N> __device__ __forceinline__ void load_angles(const float* p, float (&r)[N]) {
+// N consecutive cos (or sin) values, N a multiple of 4 or 2, 8-byte aligned, of the table or in shared memory.
+template <int N, bool kShared> __device__ __forceinline__ void load_angles(const float* p, float (&r)[N]) {
     if constexpr (N % 4 == 0) {
 #pragma unroll
         for (int k = 0; k < N / 4; ++k) {
-            const float4 f = __ldg(reinterpret_cast<const float4*>(p) + k);
+            const float4* src = reinterpret_cast<const float4*>(p) + k;
+            const float4 f = kShared ? *src : __ldg(src);
             r[4 * k] = f.x; r[4 * k + 1] = f.y; r[4 * k + 2] = f.z; r[4 * k + 3] = f.w;
         }
     } else {
 #pragma unroll
         for (int k = 0; k < N / 2; ++k) {
-            const float2 f = __ldg(reinterpret_cast<const float2*>(p) + k);
+            const float2* src = reinterpret_cast<const float2*>(p) + k;
+            const float2 f = kShared ? *src : __ldg(src);
             r[2 * k] = f.x; r[2 * k + 1] = f.y;
         }
     }
@@ -71,59 +73,37 @@ struct Axes {
     int64_t stride;      // between the axes of positions
     int num;
 };
-// Where the angles of a token come from: one row of the table, or with several axes a row for each.
+// The angles of a token: a row of cos | sin, from the table or gathered from the rows of its axes, and
+// whether its positions are in the table.
 struct Angles {
-    const float* row;                            // one axis
-    int64_t at[NVFP4KV_MAX_AXES];                // several: the rows' offsets in the table
-    bool turn;                                   // every position is in the table
+    const float* row;
+    bool turn;
 };
-template <bool kAxes>
-__device__ __forceinline__ Angles find_angles(const void* positions, bool i64, int64_t t, const Axes& axes, const float* table,
-                                              int64_t max_positions, int rotary) {
-    Angles r;
-    if constexpr (kAxes) {
-        r.turn = true;
-#pragma unroll
-        for (int a = 0; a < NVFP4KV_MAX_AXES; ++a) {
-            const int64_t pos = a < axes.num ? load_index(positions, i64, a * axes.stride + t) : 0;
-            const bool in = pos >= 0 && pos < max_positions;
-            r.turn &= in;
-            r.at[a] = in ? pos * rotary : 0;
-        }
-        r.row = table;
-    } else {
-        const int64_t pos = load_index(positions, i64, t);
-        r.turn = pos >= 0 && pos < max_positions;
-        r.row = table + (r.turn ? pos : 0) * rotary;
-    }
-    return r;
+__device__ __forceinline__ Angles find_angles(const void* positions, bool i64, int64_t t, const float* table, int64_t max_positions, int rotary) {
+    const int64_t pos = load_index(positions, i64, t);
+    const bool turn = pos >= 0 && pos < max_positions;
+    return {table + (turn ? pos : 0) * rotary, turn};
 }
-__device__ __forceinline__ const float* axis_row(const Angles& a, uint32_t axis) {
-    return a.row + (axis & 2 ? (axis & 1 ? a.at[3] : a.at[2]) : (axis & 1 ? a.at[1] : a.at[0]));
+__device__ __forceinline__ uint32_t axis_of(const Axes& axes, int pair) {
+    return static_cast<uint32_t>(axes.pair_axes[pair >> 5] >> (2 * (pair & 31))) & 3u;
 }
-// cos and sin of N pairs from pair i on (i a multiple of N, N a power of two up to 8).
-template <int N, bool kAxes>
-__device__ __forceinline__ void load_pairs(const Angles& a, const Axes& axes, int i, int half, float (&c)[N], float (&s)[N]) {
-    if constexpr (kAxes) {
-        const uint32_t of = static_cast<uint32_t>(axes.pair_axes[i >> 5] >> (2 * (i & 31)));
+__device__ __forceinline__ bool all_in_table(const void* positions, bool i64, int64_t t, const Axes& axes, int64_t max_positions) {
+    bool in = true;
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const float* p = axis_row(a, of >> (2 * k)) + i + k;
-            c[k] = __ldg(p);
-            s[k] = __ldg(p + half);
-        }
-    } else {
-        load_angles<N>(a.row + i, c);
-        load_angles<N>(a.row + i + half, s);
+    for (int a = 0; a < NVFP4KV_MAX_AXES; ++a) {
+        const int64_t pos = a < axes.num ? load_index(positions, i64, a * axes.stride + t) : 0;
+        in &= pos >= 0 && pos < max_positions;
     }
+    return in;
 }
 
-// One 16-byte vector of an interleaved rotation: pairs inside the vector, from pair i on.
-template <typename T, bool kAxes>
-__device__ __forceinline__ Vec<T> rotate_pairs(const Vec<T>& x, const Angles& a, const Axes& axes, int i, int half, float sign) {
+// One 16-byte vector of an interleaved rotation: pairs inside the vector.  cs -> cos of its first pair.
+template <typename T, bool kShared>
+__device__ __forceinline__ Vec<T> rotate_pairs(const Vec<T>& x, const float* cs, int half, float sign) {
     constexpr int N = Vec<T>::kN;
     float c[N / 2], s[N / 2];
-    load_pairs<N / 2, kAxes>(a, axes, i, half, c, s);
+    load_angles<N / 2, kShared>(cs, c);
+    load_angles<N / 2, kShared>(cs + half, s);
     Vec<T> y;
 #pragma unroll
     for (int k = 0; k < N / 2; ++k) {
@@ -136,11 +116,12 @@ __device__ __forceinline__ Vec<T> rotate_pairs(const Vec<T>& x, const Angles& a,
 }
 
 // The two vectors of a half-layout rotation: dims i.. and i + half.. .
-template <typename T, bool kAxes>
-__device__ __forceinline__ void rotate_halves(Vec<T>& xa, Vec<T>& xb, const Angles& a, const Axes& axes, int i, int half, float sign) {
+template <typename T, bool kShared>
+__device__ __forceinline__ void rotate_halves(Vec<T>& xa, Vec<T>& xb, const float* cs, int half, float sign) {
     constexpr int N = Vec<T>::kN;
     float c[N], s[N];
-    load_pairs<N, kAxes>(a, axes, i, half, c, s);
+    load_angles<N, kShared>(cs, c);
+    load_angles<N, kShared>(cs + half, s);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         float u, v;
@@ -158,6 +139,30 @@ struct SmallDiv {
 };
 __device__ __forceinline__ uint32_t quotient(uint32_t n, const SmallDiv& v) { return v.d == 1 ? n : __umulhi(n, v.magic); }
 
+// With several axes, a block gathers the cos | sin rows of its `num` tokens from t0 on in shared memory
+// once, so that its units read them as 16-byte vectors like a row of the table, whichever way the
+// axes are spread over the pairs (loaded pair by pair in every unit they took as many load slots as the
+// values themselves: 8,192 tokens x 32 heads x 128 bf16 42 us, now 28.3, with one axis 29.1).  It comes
+// before the units' own loads: behind them their addresses stay in registers, and fewer blocks fit
+// (31.6 us; the gradient of 2,049 x 20 x 192 fp32 13.1 us against 11.3).  rows [num][rotary], turns [num].
+__device__ __forceinline__ void gather_rows(float* rows, uint8_t* turns, int num, int64_t t0, int64_t tokens, const void* positions,
+                                            bool i64, const Axes& axes, const SmallDiv& half, const float* table, int64_t max_positions) {
+    const int h = static_cast<int>(half.d);
+    for (int l = threadIdx.x; l < num * h; l += blockDim.x) {
+        const int k = static_cast<int>(quotient(l, half)), i = l - k * h;
+        const int64_t t = t0 + k;
+        if (t >= tokens) break;
+        const int64_t pos = load_index(positions, i64, axis_of(axes, i) * axes.stride + t);
+        const float* src = table + (pos >= 0 && pos < max_positions ? pos : 0) * (2 * h) + i;
+        rows[2 * h * k + i] = __ldg(src);
+        rows[2 * h * k + h + i] = __ldg(src + h);
+        if (i == 0) turns[k] = all_in_table(positions, i64, t, axes, max_positions);
+    }
+    __syncthreads();
+}
+
+inline SmallDiv small_div(uint32_t d) { return {d, static_cast<uint32_t>(((1ull << 32) + d - 1) / d)}; }
+
 struct RopeArgs {
     const void* x;
     void* out;
@@ -171,6 +176,8 @@ struct RopeArgs {
     int pos_i64, inverse, in_place;
     int32_t* err;
     Axes axes;
+    SmallDiv half;          // with several axes: rotary / 2, the tokens of a block at most
+    int block_tokens;
 };
 constexpr int kRopeSteps = 2;
 
@@ -181,7 +188,7 @@ constexpr int kRopeSteps = 2;
 // as a plain copy; 8 % more with one, 1 % more with four, 20 % more with blocks of whole heads, whose
 // last steps are part empty).  The gradient of 2,049 tokens x 32 heads x 128 fp32 takes 12 us.
 template <typename T, bool kInterleaved, bool kAxes>
-__global__ void __launch_bounds__(256, kInterleaved && sizeof(T) == 2 && !kAxes ? 8 : 4) rope_vec_kernel(const __grid_constant__ RopeArgs p) {
+__global__ void __launch_bounds__(256, kAxes ? (kInterleaved ? 7 : 5) : (kInterleaved && sizeof(T) == 2 ? 8 : 4)) rope_vec_kernel(const __grid_constant__ RopeArgs p) {
     constexpr int N = Vec<T>::kN;
     const int64_t u0 = static_cast<int64_t>(blockIdx.x) * (256 * kRopeSteps);
     int64_t row0, t0;       // the block's first head row, its token
@@ -195,6 +202,10 @@ __global__ void __launch_bounds__(256, kInterleaved && sizeof(T) == 2 && !kAxes 
     const uint32_t j0 = static_cast<uint32_t>(u0 - row0 * p.units.d), h0 = static_cast<uint32_t>(row0 - t0 * p.by_heads.d);
     const int half = p.rotary / 2;
     griddep_wait();
+    extern __shared__ __align__(16) float block_rows[];
+    uint8_t* turns = reinterpret_cast<uint8_t*>(block_rows + p.block_tokens * p.rotary);
+    if constexpr (kAxes)
+        gather_rows(block_rows, turns, p.block_tokens, t0, p.tokens, p.positions, p.pos_i64, p.axes, p.half, p.cos_sin, p.max_positions);
     Vec<T> a[kRopeSteps], b[kRopeSteps];
     int64_t t[kRopeSteps], at[kRopeSteps];
     int r[kRopeSteps];      // dim within the rotated part, -1 for a copy, -2 past the end
@@ -221,13 +232,16 @@ __global__ void __launch_bounds__(256, kInterleaved && sizeof(T) == 2 && !kAxes 
         if (r[k] == -2) break;
         T* op = static_cast<T*>(p.out) + at[k];
         if (r[k] >= 0) {
-            const Angles g = find_angles<kAxes>(p.positions, p.pos_i64, t[k], p.axes, p.cos_sin, p.max_positions, p.rotary);
+            const int l = static_cast<int>(t[k] - t0);
+            const Angles g = kAxes ? Angles{block_rows + l * p.rotary, turns[l] != 0}
+                                   : find_angles(p.positions, p.pos_i64, t[k], p.cos_sin, p.max_positions, p.rotary);
             if (!g.turn) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
+            const float* cs = g.row + (kInterleaved ? r[k] / 2 : r[k]);
             const float sign = p.inverse ? -1.0f : 1.0f;
             if (kInterleaved) {
-                if (g.turn) a[k] = rotate_pairs<T, kAxes>(a[k], g, p.axes, r[k] / 2, half, sign);
+                if (g.turn) a[k] = rotate_pairs<T, kAxes>(a[k], cs, half, sign);
             } else {
-                if (g.turn) rotate_halves<T, kAxes>(a[k], b[k], g, p.axes, r[k], half, sign);
+                if (g.turn) rotate_halves<T, kAxes>(a[k], b[k], cs, half, sign);
                 store_vec(op + half, b[k]);
             }
         }
@@ -244,7 +258,8 @@ __global__ void __launch_bounds__(256) rope_elem_kernel(const __grid_constant__ 
     const int64_t t = blockIdx.x / head_blocks;
     const int h0 = static_cast<int>(blockIdx.x % head_blocks) * heads_per_block;
     const int heads = min(heads_per_block, p.heads - h0);
-    const Angles g = find_angles<kAxes>(p.positions, p.pos_i64, t, p.axes, p.cos_sin, p.max_positions, p.rotary);
+    Angles g = kAxes ? Angles{p.cos_sin, all_in_table(p.positions, p.pos_i64, t, p.axes, p.max_positions)}
+                     : find_angles(p.positions, p.pos_i64, t, p.cos_sin, p.max_positions, p.rotary);
     if (!g.turn && threadIdx.x == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
     const int half = p.rotary / 2;
     const float sign = p.inverse ? -1.0f : 1.0f;
@@ -262,7 +277,8 @@ __global__ void __launch_bounds__(256) rope_elem_kernel(const __grid_constant__ 
         const int i = kInterleaved ? r / 2 : r;
         if (kInterleaved ? (r & 1) : r >= half) continue;      // done with its partner
         const int db = kInterleaved ? d + 1 : d + half;
-        const float* cs = kAxes ? axis_row(g, static_cast<uint32_t>(p.axes.pair_axes[i >> 5] >> (2 * (i & 31)))) : g.row;
+        if (kAxes) g.row = p.cos_sin + load_index(p.positions, p.pos_i64, axis_of(p.axes, i) * p.axes.stride + t) * p.rotary;
+        const float* cs = g.row;
         float u0, v0;
         rotate(load_f32(xp + d), load_f32(xp + db), __ldg(cs + i), sign * __ldg(cs + half + i), u0, v0);
         op[d] = from_f32<T>(u0);
@@ -285,12 +301,21 @@ int launch_rope(RopeArgs a, int64_t tokens, bool interleaved, cudaStream_t st) {
         a.rotated = a.rotary / (interleaved ? N : 2 * N);
         a.before = a.in_place ? 0 : a.offset / N;
         const uint32_t units = a.rotated + (a.in_place ? 0 : (a.dim - a.rotary) / N), heads = a.heads;
-        a.units = {units, static_cast<uint32_t>(((1ull << 32) + units - 1) / units)};
-        a.by_heads = {heads, static_cast<uint32_t>(((1ull << 32) + heads - 1) / heads)};
+        a.units = small_div(units);
+        a.by_heads = small_div(heads);
         a.total = tokens * heads * units;
         blocks = (a.total + 256 * kRopeSteps - 1) / (256 * kRopeSteps);
+        size_t smem = 0;
+        if (kAxes) {
+            // a block's units begin anywhere in a token's; they touch at most 16 KB of rows (32 KB in the
+            // half layout, whose units are two vectors) and two rows more
+            const int64_t per_token = static_cast<int64_t>(heads) * units, most = (256 * kRopeSteps + per_token - 2) / per_token + 1;
+            a.block_tokens = static_cast<int>(most < tokens ? most : tokens);
+            a.half = small_div(a.rotary / 2);
+            smem = a.block_tokens * (a.rotary * sizeof(float) + 1);
+        }
         if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "nvfp4kv_rope: too many rows for one call");
-        const cudaError_t e = launch_dependent(interleaved ? rope_vec_kernel<T, true, kAxes> : rope_vec_kernel<T, false, kAxes>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a);
+        const cudaError_t e = launch_dependent(interleaved ? rope_vec_kernel<T, true, kAxes> : rope_vec_kernel<T, false, kAxes>, dim3(static_cast<unsigned>(blocks)), dim3(256), smem, st, a);
         if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_rope launch failed: %s", cudaGetErrorString(e));
     } else {
         int hb = 1024 / a.dim;
@@ -323,6 +348,7 @@ struct RopeAppendArgs {
     int slot_i64, pos_i64;
     int32_t* err;
     Axes axes;
+    int block_tokens;          // with several axes: the tokens of a block at most
 };
 
 // 8 bf16, as one 16-byte access or element by element.  The accesses are marked as streaming: a step's
@@ -358,7 +384,7 @@ template <bool kVec> __device__ __forceinline__ void put8(__nv_bfloat16* p, cons
 // token's rows are its key and the heads of its query.  What bounds it is the latency of a block's
 // three dependent accesses (position, table row, store) at full occupancy, then HBM.
 template <bool kInterleaved, bool kVec, bool kAxes>
-__global__ void __launch_bounds__(256) rope_append_rotated_kernel(const __grid_constant__ RopeAppendArgs p) {
+__device__ __forceinline__ void rope_append_rotated(const RopeAppendArgs& p) {
     using V = Vec<__nv_bfloat16>;
     constexpr int kU = kInterleaved ? 8 : 4, kSteps = kAppendSteps, kRows = 256 / kU;      // rows of a block and step
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kRows * kSteps);
@@ -366,6 +392,11 @@ __global__ void __launch_bounds__(256) rope_append_rotated_kernel(const __grid_c
     const uint32_t first = static_cast<uint32_t>(row0 - t0 * p.rows_of_token.d);
     const int u = threadIdx.x % kU;
     griddep_wait();
+    extern __shared__ __align__(16) float block_rows[];
+    uint8_t* turns = reinterpret_cast<uint8_t*>(block_rows + p.block_tokens * NVFP4KV_ROPE);
+    if constexpr (kAxes)
+        gather_rows(block_rows, turns, p.block_tokens, t0, p.tokens, p.positions, p.pos_i64, p.axes,
+                    SmallDiv{NVFP4KV_ROPE / 2, 1u << (32 - 5)}, p.cos_sin, p.max_positions);
     V a[kSteps], b[kSteps];
     int64_t t[kSteps];
     int h[kSteps];          // head, -1 for the key
@@ -382,7 +413,9 @@ __global__ void __launch_bounds__(256) rope_append_rotated_kernel(const __grid_c
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
         if (t[k] >= p.tokens) break;
-        const Angles g = find_angles<kAxes>(p.positions, p.pos_i64, t[k], p.axes, p.cos_sin, p.max_positions, NVFP4KV_ROPE);
+        const int l = static_cast<int>(t[k] - t0);
+        const Angles g = kAxes ? Angles{block_rows + l * NVFP4KV_ROPE, turns[l] != 0}
+                               : find_angles(p.positions, p.pos_i64, t[k], p.cos_sin, p.max_positions, NVFP4KV_ROPE);
         __nv_bfloat16* dst;
         if (h[k] < 0) {
             if (!g.turn && u == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_INDEX);
@@ -397,13 +430,24 @@ __global__ void __launch_bounds__(256) rope_append_rotated_kernel(const __grid_c
             dst = p.qo + t[k] * p.qo_st + h[k] * p.qo_sh;
         }
         if (kInterleaved) {
-            if (g.turn) a[k] = rotate_pairs<__nv_bfloat16, kAxes>(a[k], g, p.axes, 4 * u, 32, 1.0f);
+            if (g.turn) a[k] = rotate_pairs<__nv_bfloat16, kAxes>(a[k], g.row + 4 * u, 32, 1.0f);
         } else {
-            if (g.turn) rotate_halves<__nv_bfloat16, kAxes>(a[k], b[k], g, p.axes, 8 * u, 32, 1.0f);
+            if (g.turn) rotate_halves<__nv_bfloat16, kAxes>(a[k], b[k], g.row + 8 * u, 32, 1.0f);
             put8<kVec>(dst + 32 + 8 * u, b[k]);
         }
         put8<kVec>(dst + 8 * u, a[k]);
     }
+}
+
+template <bool kInterleaved, bool kVec>
+__global__ void __launch_bounds__(256) rope_append_rotated_kernel(const __grid_constant__ RopeAppendArgs p) {
+    rope_append_rotated<kInterleaved, kVec, false>(p);
+}
+// (more blocks on an SM hide the gathering: 43 us with the angles loaded pair by pair, 36 gathered
+// beside the rows' loads with 5 blocks, 31.6 gathered before them with 8, the table's own rows 26)
+template <bool kInterleaved, bool kVec>
+__global__ void __launch_bounds__(256, kInterleaved && kVec ? 8 : kVec ? 5 : 4) rope_append_axes_kernel(const __grid_constant__ RopeAppendArgs p) {
+    rope_append_rotated<kInterleaved, kVec, true>(p);
 }
 
 // The axes of a call (num 0: one, as nvfp4kv_rope).
@@ -454,7 +498,7 @@ int rope_call(const char* what, const void* x, int dtype, int64_t num_tokens, in
         return fail(NVFP4KV_EINVAL, "%s: in place needs equal strides", what);
     RopeArgs a{};
     a.x = x; a.out = out; a.x_st = x_stride_t; a.x_sh = x_stride_h; a.o_st = out_stride_t; a.o_sh = out_stride_h;
-    a.positions = positions; a.cos_sin = cos_sin; a.max_positions = max_positions;
+    a.positions = positions; a.cos_sin = cos_sin; a.max_positions = max_positions; a.tokens = num_tokens;
     a.heads = num_heads; a.dim = head_dim; a.rotary = rotary_dim; a.offset = rope_offset;
     a.pos_i64 = pos_dtype == NVFP4KV_INDEX_I64; a.inverse = inverse != 0; a.in_place = x == out; a.err = err_flag;
     a.axes = axes;
@@ -514,18 +558,24 @@ int append_rotated_call(const char* what, const void* k_pe, int64_t num_tokens, 
                      (!q_pe || ((reinterpret_cast<uintptr_t>(q_pe) | reinterpret_cast<uintptr_t>(q_out)) % 16 == 0 &&
                                 (q_stride_t | q_stride_h | qo_stride_t | qo_stride_h) % 8 == 0));
     const uint32_t per_token = a.heads + 1;
-    a.rows_of_token = {per_token, static_cast<uint32_t>(((1ull << 32) + per_token - 1) / per_token)};
+    a.rows_of_token = small_div(per_token);
     const int64_t per_block = kAppendSteps * 256 / (interleaved ? 8 : 4), blocks = (num_tokens * per_token + per_block - 1) / per_block;
     if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "%s: too many rows for one call", what);
     const dim3 grid(static_cast<unsigned>(blocks));
+    size_t smem = 0;
+    if (num_axes != 0) {
+        const int64_t most = (per_block + per_token - 2) / per_token + 1;
+        a.block_tokens = static_cast<int>(most < num_tokens ? most : num_tokens);
+        smem = a.block_tokens * (NVFP4KV_ROPE * sizeof(float) + 1);      // (up to 129 tokens)
+    }
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     constexpr void (*kKernels[2][2][2])(RopeAppendArgs) = {
-        {{rope_append_rotated_kernel<false, false, false>, rope_append_rotated_kernel<false, false, true>},
-         {rope_append_rotated_kernel<false, true, false>, rope_append_rotated_kernel<false, true, true>}},
-        {{rope_append_rotated_kernel<true, false, false>, rope_append_rotated_kernel<true, false, true>},
-         {rope_append_rotated_kernel<true, true, false>, rope_append_rotated_kernel<true, true, true>}}};
+        {{rope_append_rotated_kernel<false, false>, rope_append_axes_kernel<false, false>},
+         {rope_append_rotated_kernel<false, true>, rope_append_axes_kernel<false, true>}},
+        {{rope_append_rotated_kernel<true, false>, rope_append_axes_kernel<true, false>},
+         {rope_append_rotated_kernel<true, true>, rope_append_axes_kernel<true, true>}}};
     void (*kernel)(RopeAppendArgs) = kKernels[interleaved != 0][vec][num_axes != 0];
-    const cudaError_t e = launch_dependent(kernel, grid, dim3(256), 0, st, a);
+    const cudaError_t e = launch_dependent(kernel, grid, dim3(256), smem, st, a);
     if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
     return check_launch(what);
 }

@@ -707,17 +707,20 @@ def _axes(axes, num: int, rotary_dim: int):
 
 def _check_axes(index: int, cos_sin: torch.Tensor, positions: torch.Tensor, T: int, rotary_dim: int, axes):
     """_check_angles for positions [axes, T]: also their stride, their number and the pairs' axes."""
-    if axes is None:
-        raise ValueError("positions of several axes need axes, the axis of each pair (see rope_axes)")
-    shape = positions.shape
+    if not (isinstance(positions, torch.Tensor) and positions.get_device() == index == cos_sin.get_device()
+            and cos_sin.dtype is torch.float32 and cos_sin.is_contiguous()):
+        _check_angles(index, cos_sin, positions, T, rotary_dim)
+    shape, st, dtype = positions.shape, positions.stride(), _INDEX_DTYPES.get(positions.dtype)
     if len(shape) != 2 or not 1 <= shape[0] <= _lib.MAX_AXES or shape[1] != T:
         raise ValueError(f"positions must be [axes, {T}] with at most {_lib.MAX_AXES} axes")
-    if rotary_dim > _lib.MAX_AXES_DIM:
-        raise ValueError(f"several axes rotate at most {_lib.MAX_AXES_DIM} dims")
-    if T > 1 and positions.stride(1) != 1:
+    if rotary_dim != cos_sin.shape[1] or rotary_dim > _lib.MAX_AXES_DIM:
+        raise ValueError(f"cos_sin must be [positions, {rotary_dim}], with several axes at most {_lib.MAX_AXES_DIM} wide")
+    if dtype is None:
+        raise TypeError("positions must be int64 or int32")
+    if st[1] != 1 and T > 1:
         positions = positions.contiguous()
-    _, dtype = _check_angles(index, cos_sin, positions[0], T, rotary_dim)
-    return positions, dtype, positions.stride(0), shape[0], _axes(axes, shape[0], rotary_dim)
+        st = positions.stride()
+    return positions, dtype, st[0], shape[0], _axes(axes, shape[0], rotary_dim)
 
 
 def _check_angles(index: int, cos_sin: torch.Tensor, positions: torch.Tensor, T: int, rotary_dim: int):
