@@ -275,96 +275,181 @@ __device__ __forceinline__ int64_t block_exclusive_scan64(int64_t v, int64_t* wa
     return x - v + (warp > 0 ? before : 0);
 }
 
+// Entries [j0, j1) of request k's table, by the threads tid, tid + nt, ... : into the sequence's and out.
+// Eight in flight a thread.
+__device__ __forceinline__ void write_rows(const ExtendArgs& p, int k, int j0, int j1, int tid, int nt, int start, int rank) {
+    int32_t* to = p.out_tables + static_cast<int64_t>(k) * p.width;
+    if (start < 0) {
+        for (int j = j0 + tid; j < j1; j += nt) to[j] = -1;
+        return;
+    }
+    int32_t* row = p.tables + p.slots[k] * p.stride;
+    const int first = pages_of(start, p.page_size), last = pages_of(p.out_lens[k], p.page_size);
+    for (int j = j0 + tid; j < j1; j += 8 * nt) {
+        int pg[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = j + i * nt;
+            if (e < j1) pg[i] = e >= first && e < last ? p.free_list[rank + e - first] : row[e];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = j + i * nt;
+            if (e >= j1) break;
+            if (e >= first && e < last) {
+                row[e] = pg[i];
+                p.refs[pg[i]] = 1;
+            }
+            to[e] = pg[i];
+        }
+    }
+}
+// Rows [t0, t1) of the step.
+__device__ __forceinline__ void write_tokens(const ExtendArgs& p, int64_t t0, int64_t t1, const int* cu, const int* starts, const int* ranks) {
+    const int live = cu[p.num];
+    for (int64_t t = t0 + threadIdx.x; t < t1; t += blockDim.x) {
+        int64_t slot = -1;
+        int pos = 0;
+        if (t < live) {
+            int lo = 0, hi = p.num - 1;      // the last request that begins at or before t (empty ones end before it)
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (cu[mid] <= t) lo = mid;
+                else hi = mid - 1;
+            }
+            const int start = starts[lo];
+            pos = start + static_cast<int>(t) - cu[lo];
+            const int j = pos / p.page_size, first = pages_of(start, p.page_size);
+            const int pg = j < first ? p.tables[p.slots[lo] * p.stride + j] : p.free_list[ranks[lo] + j - first];
+            slot = static_cast<int64_t>(pg) * p.page_size + pos % p.page_size;
+        }
+        p.slot_mapping[t] = slot;
+        p.positions[t] = pos;
+    }
+}
+
 // One block: which requests count, what they take back, the pages they need, the lowest free pages.
-// It is bound by the latency of its dependent accesses, so the claims on slots and the requests' state
-// are kept in shared memory where they fit.
-constexpr int kSharedSlots = 6144, kSharedRequests = 2048;
-__global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(const __grid_constant__ ExtendArgs p) {
-    __shared__ int64_t sums64[3][32];
-    __shared__ int sums[32];
-    __shared__ int claim_s[kSharedSlots], start_s[kSharedRequests], rank_s[kSharedRequests];
+// It is bound by the latency of its dependent accesses, so a thread keeps its request in registers where
+// there is one a thread at most (kOne; more are read again in each pass), and the claims on slots are
+// in shared memory where they fit.
+constexpr int kSharedSlots = 4096;
+template <bool kOne>
+__device__ __forceinline__ void extend_plan(const ExtendArgs& p) {
+    __shared__ int64_t sums64[2][32];
+    __shared__ int sums[2][32], many;
+    __shared__ int claim_s[kSharedSlots], list[kPlanThreads];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int* claim = p.num_slots <= kSharedSlots ? claim_s : p.claim;
-    int* starts = p.num <= kSharedRequests ? start_s : p.start;
-    int* ranks = p.num <= kSharedRequests ? rank_s : p.rank;
-    griddep_wait();
-    for (int k = tid; k < p.num; k += kPlanThreads) {
-        const int s = p.slots[k];
-        if (s >= 0 && s < p.num_slots) claim[s] = 0x7FFFFFFF;
+    struct Request {
+        int s, n, len, start, rank;      // slot (-1: bad), new tokens, length to begin at, what the checks leave of it, first page
+    };
+    auto read = [&](int k) {
+        Request r{-1, 0, 0, -1, -1};
+        if (k < p.num) {
+            r.s = p.slots[k];
+            r.n = p.new_lens[k];
+            if (p.lens) r.len = p.lens[k];
+            if (r.s < 0 || r.s >= p.num_slots) r.s = -1;
+            else if (!p.lens) r.len = p.seq_lens[r.s];
+        }
+        return r;
+    };
+    Request mine{-1, 0, 0, -1, -1};
+    if constexpr (kOne) mine = read(tid);
+    auto get = [&](int k) {
+        if constexpr (kOne) return mine;
+        Request r = read(k);
+        if (k < p.num) {
+            r.start = p.start[k];
+            r.rank = p.rank[k];
+        }
+        return r;
+    };
+    auto put = [&](int k, const Request& r) {
+        if constexpr (kOne) {
+            mine = r;
+        } else if (k < p.num) {
+            p.start[k] = r.start;
+            p.rank[k] = r.rank;
+        }
+    };
+    const int last = kOne ? 1 : p.num;      // (passes begin at 0, 1,024 ...)
+    for (int k0 = 0; k0 < last; k0 += kPlanThreads) {
+        const int s = kOne ? mine.s : read(k0 + tid).s;
+        if (s >= 0) claim[s] = 0x7FFFFFFF;
     }
     __syncthreads();
-    for (int k = tid; k < p.num; k += kPlanThreads) {
-        const int s = p.slots[k];
-        if (s >= 0 && s < p.num_slots) atomicMin(claim + s, k);
+    for (int k0 = 0; k0 < last; k0 += kPlanThreads) {
+        const int s = kOne ? mine.s : read(k0 + tid).s;
+        if (s >= 0) atomicMin(claim + s, k0 + tid);
     }
     __syncthreads();
     // the checks, on lengths, tables and counts as they were before the call
     const int64_t most = static_cast<int64_t>(p.width) * p.page_size;
-    for (int k = tid; k < p.num; k += kPlanThreads) {
-        const int s = p.slots[k], n = p.new_lens[k];
-        const bool in = s >= 0 && s < p.num_slots;
-        const int have = in ? p.seq_lens[s] : 0, len = p.lens ? p.lens[k] : have;
-        const int first = in ? *static_cast<volatile int*>(claim + s) : -1;
-        int start = -1, err = 0;
-        if (first != k) {
-            err = NVFP4KV_DEVERR_BAD_SLOT;
-        } else if (n < 0 || len < 0 || len > have) {
-            err = NVFP4KV_DEVERR_SEQ_LEN;
-        } else if (static_cast<int64_t>(len) + n > most) {
-            err = NVFP4KV_DEVERR_CAPACITY;
-        } else {
-            start = len;
-            if (n > 0 && len % p.page_size != 0) {      // the new tokens begin in a page that others may read
-                const int pg = p.tables[s * p.stride + len / p.page_size];
-                if (pg < 0 || pg >= p.num_pages || __ldcg(p.refs + pg) != 1) {
-                    err = NVFP4KV_DEVERR_BAD_PAGE;
-                    start = -1;
-                }
-            }
+    for (int k0 = 0; k0 < last; k0 += kPlanThreads) {
+        const int k = k0 + tid;
+        if (k >= p.num) break;
+        Request r = kOne ? mine : read(k);
+        const bool first = r.s >= 0 && *static_cast<volatile int*>(claim + r.s) == k;
+        const bool fits = r.n >= 0 && r.len >= 0 && static_cast<int64_t>(r.len) + r.n <= most;
+        const int have = first ? p.seq_lens[r.s] : 0;
+        int pg = 0, count = 1;
+        const bool inside = first && fits && r.n > 0 && r.len % p.page_size != 0;      // it begins in a page that others may read
+        if (inside) {
+            pg = p.tables[r.s * p.stride + r.len / p.page_size];
+            count = pg >= 0 && pg < p.num_pages ? __ldcg(p.refs + pg) : 0;
         }
+        const int err = !first ? NVFP4KV_DEVERR_BAD_SLOT
+                        : r.n < 0 || r.len < 0 || r.len > have ? NVFP4KV_DEVERR_SEQ_LEN
+                        : !fits ? NVFP4KV_DEVERR_CAPACITY : inside && count != 1 ? NVFP4KV_DEVERR_BAD_PAGE : 0;
         if (err) set_error(p.err, err);
-        starts[k] = start;
+        else r.start = r.len;
+        put(k, r);
     }
     __syncthreads();
-    // pages of tokens that are taken back: a request per warp
+    // pages of tokens that are taken back: a few by the request's thread, many by a warp
     if (p.lens) {
-        for (int k0 = 0; k0 < p.num; k0 += kPlanThreads) {
-            const int k = k0 + 32 * lane + warp, start = k < p.num ? starts[k] : -1;
-            int s = 0, j0 = 0, j1 = 0;
-            if (start >= 0) {
-                s = p.slots[k];
-                j0 = pages_of(start, p.page_size);
-                j1 = min(pages_of(p.seq_lens[s], p.page_size), p.width);
+        auto take_back = [&](int32_t* row, int j) {
+            const int pg = row[j];
+            row[j] = -1;
+            if (pg >= 0) release_page(p.refs, p.num_pages, pg, p.err);
+        };
+        for (int k0 = 0; k0 < last; k0 += kPlanThreads) {
+            const int k = k0 + tid;
+            const Request r = get(k);
+            if (tid == 0) many = 0;
+            __syncthreads();
+            if (r.start >= 0) {
+                int32_t* row = p.tables + r.s * p.stride;
+                const int j0 = pages_of(r.start, p.page_size), j1 = min(pages_of(p.seq_lens[r.s], p.page_size), p.width);
+                if (j1 - j0 > 2) list[atomicAdd(&many, 1)] = k;
+                else
+                    for (int j = j0; j < j1; ++j) take_back(row, j);
             }
-            for (uint32_t todo = __ballot_sync(0xFFFFFFFFu, j0 < j1); todo; todo &= todo - 1) {
-                const int l = __ffs(todo) - 1;
-                int32_t* row = p.tables + __shfl_sync(0xFFFFFFFFu, s, l) * p.stride;
-                const int end = __shfl_sync(0xFFFFFFFFu, j1, l);
-                for (int j = __shfl_sync(0xFFFFFFFFu, j0, l) + lane; j < end; j += 32) {
-                    const int pg = row[j];
-                    row[j] = -1;
-                    if (pg >= 0) release_page(p.refs, p.num_pages, pg, p.err);
-                }
+            __syncthreads();
+            for (int i = warp; i < many; i += 32) {
+                const int s = p.slots[list[i]], j1 = min(pages_of(p.seq_lens[s], p.page_size), p.width);
+                for (int j = pages_of(p.lens[list[i]], p.page_size) + lane; j < j1; j += 32) take_back(p.tables + s * p.stride, j);
             }
+            __syncthreads();
         }
-        __syncthreads();
     }
     // running sums of tokens and pages
     int64_t tokens = 0, pages = 0;
-    for (int k0 = 0; k0 < p.num; k0 += kPlanThreads) {
-        const int k = k0 + tid, start = k < p.num ? starts[k] : -1, n = start >= 0 ? p.new_lens[k] : 0;
-        const int need = start >= 0 ? pages_of(start + n, p.page_size) - pages_of(start, p.page_size) : 0;
+    for (int k0 = 0; k0 < last; k0 += kPlanThreads) {
+        const int k = k0 + tid;
+        Request r = get(k);
+        const int n = r.start >= 0 ? r.n : 0, need = r.start >= 0 ? pages_of(r.start + n, p.page_size) - pages_of(r.start, p.page_size) : 0;
         int64_t sum_n, sum_p;
         const int64_t at_n = tokens + block_exclusive_scan64(n, sums64[0], &sum_n);
         const int64_t at_p = pages + block_exclusive_scan64(need, sums64[1], &sum_p);
-        if (k < p.num) {
-            // (-2: taken back, but not extended)
-            if (start >= 0 && n > 0 && at_n + n > p.num_tokens) ranks[k] = -2;
-            else ranks[k] = need == 0 ? -1 : static_cast<int>(at_p + need <= p.num_pages ? at_p : p.num_pages);
-        }
+        // (-2: taken back, but not extended)
+        if (n > 0 && at_n + n > p.num_tokens) r.rank = -2;
+        else r.rank = need == 0 ? -1 : static_cast<int>(at_p + need <= p.num_pages ? at_p : p.num_pages);
+        put(k, r);
         tokens += sum_n;
         pages += sum_p;
-        __syncthreads();
+        if (!kOne) __syncthreads();
     }
     // the lowest free pages, 16 counts a thread and step
     constexpr int kPer = 16;
@@ -385,95 +470,88 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(const __grid_
                 if (i0 + j < p.num_pages && __ldcg(p.refs + i0 + j) == 0) zero |= 1u << j;
         }
         int total;
-        int at = found + block_exclusive_scan(__popc(zero), sums, &total);
+        int at = found + block_exclusive_scan(__popc(zero), sums[0], &total);
         for (; zero && at < want; zero &= zero - 1, ++at) p.free_list[at] = static_cast<int>(i0) + __ffs(zero) - 1;
         found += total;
         __syncthreads();
     }
     // who gets them, and where their tokens begin
-    int64_t done = 0;
-    for (int k0 = 0; k0 < p.num; k0 += kPlanThreads) {
+    int done = 0;
+    for (int k0 = 0; k0 < last; k0 += kPlanThreads) {
         const int k = k0 + tid;
-        int start = -1, n = 0, rank = -1;
+        Request r = get(k);
         bool ok = false;
-        if (k < p.num && (start = starts[k]) >= 0) {
-            n = p.new_lens[k];
-            rank = ranks[k];
-            const int need = pages_of(start + n, p.page_size) - pages_of(start, p.page_size);
-            ok = rank != -2 && (need == 0 || static_cast<int64_t>(rank) + need <= found);
+        if (r.start >= 0) {
+            const int need = pages_of(r.start + r.n, p.page_size) - pages_of(r.start, p.page_size);
+            ok = r.rank != -2 && (need == 0 || static_cast<int64_t>(r.rank) + need <= found);
             if (!ok) set_error(p.err, NVFP4KV_DEVERR_CAPACITY);
         }
-        int64_t sum;
-        const int64_t at = done + block_exclusive_scan64(ok ? n : 0, sums64[2], &sum);
+        int sum;      // (at most num_tokens)
+        const int at = done + block_exclusive_scan(ok ? r.n : 0, sums[1], &sum);
         if (k < p.num) {
-            p.cu[k] = static_cast<int>(at);
-            p.out_lens[k] = ok ? start + n : 0;
-            if (start >= 0) p.seq_lens[p.slots[k]] = ok ? start + n : start;
-            p.start[k] = ok ? start : -1;
-            p.rank[k] = rank;
+            p.cu[k] = at;
+            p.out_lens[k] = ok ? r.start + r.n : 0;
+            if (r.start >= 0) p.seq_lens[r.s] = ok ? r.start + r.n : r.start;
+            p.start[k] = ok ? r.start : -1;
+            p.rank[k] = r.rank;
         }
         done += sum;
-        __syncthreads();
+        if (!kOne) __syncthreads();
     }
-    if (tid == 0) p.cu[p.num] = static_cast<int>(done);
-    griddep_launch_dependents();
+    if (tid == 0) p.cu[p.num] = done;
 }
 
+// The first tokens of the requests in shared memory, for a search whose steps depend on one another,
+// where they fit.
+constexpr int kSharedRequests = 2048;
+__device__ __forceinline__ const int* stage_cu(const ExtendArgs& p, int* cu_s) {
+    if (p.num > kSharedRequests) return p.cu;
+    for (int k = threadIdx.x; k <= p.num; k += blockDim.x) cu_s[k] = p.cu[k];
+    __syncthreads();
+    return cu_s;
+}
+
+// A step in one launch: the first block of a cluster plans, all of them write.  For steps of up to
+// kOneLaunch words of tables and rows: a launch less is 2.4 us of 24 on the host; on the GPU 16 tables of
+// 2,048 entries take 9.5 us so and 8.0 in two launches, 16 of 4,688 with 32,768 tokens 14.4 and 11, 480
+// prompts of 670,000 tokens 105 and 11.
+constexpr int kStepBlocks = 8;
+constexpr int64_t kOneLaunch = 65536;
+__global__ void __cluster_dims__(kStepBlocks, 1, 1) __launch_bounds__(kPlanThreads) extend_step_kernel(const __grid_constant__ ExtendArgs p) {
+    __shared__ int cu_s[kSharedRequests + 1];
+    griddep_wait();
+    if (blockIdx.x == 0) extend_plan<true>(p);
+    cluster_sync();
+    const int lane = threadIdx.x & 31, warp = blockIdx.x * (kPlanThreads / 32) + (threadIdx.x >> 5), warps = kStepBlocks * kPlanThreads / 32;
+    // (a table per warp, or a piece of one where there are few)
+    const int parts = p.num < warps ? warps / max(p.num, 1) : 1, each = (p.width + parts - 1) / parts;
+    for (int w = warp; w < p.num * parts; w += warps) {
+        const int k = w / parts, j0 = (w - k * parts) * each;
+        write_rows(p, k, j0, min(j0 + each, p.width), lane, 32, p.start[k], p.rank[k]);
+    }
+    const int64_t each_t = (p.num_tokens + kStepBlocks - 1) / kStepBlocks, t0 = blockIdx.x * each_t;
+    if (t0 < p.num_tokens) write_tokens(p, t0, min(t0 + each_t, p.num_tokens), stage_cu(p, cu_s), p.start, p.rank);
+}
+
+// Larger steps: planned by one block, written by as many as there is work for.
+template <bool kOne>
+__global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(const __grid_constant__ ExtendArgs p) {
+    griddep_launch_dependents();
+    griddep_wait();
+    extend_plan<kOne>(p);
+}
 // The first row_blocks blocks: the tables of a request, 1,024 entries each; the others: tokens.
 constexpr int kRowEntries = 1024, kTokensPerBlock = 1024;
 __global__ void __launch_bounds__(256) extend_apply_kernel(const __grid_constant__ ExtendArgs p, int chunks, int64_t row_blocks) {
+    __shared__ int cu_s[kSharedRequests + 1];
     griddep_wait();
     if (blockIdx.x < row_blocks) {
         const int k = static_cast<int>(blockIdx.x / chunks), j0 = static_cast<int>(blockIdx.x % chunks) * kRowEntries;
-        const int start = p.start[k];
-        int32_t* to = p.out_tables + static_cast<int64_t>(k) * p.width;
-        if (start < 0) {
-            for (int j = j0 + threadIdx.x; j < min(j0 + kRowEntries, p.width); j += blockDim.x) to[j] = -1;
-            return;
-        }
-        int32_t* row = p.tables + p.slots[k] * p.stride;
-        const int first = pages_of(start, p.page_size), last = pages_of(p.out_lens[k], p.page_size), rank = p.rank[k];
-        for (int j = j0 + threadIdx.x; j < min(j0 + kRowEntries, p.width); j += blockDim.x) {
-            int pg;
-            if (j >= first && j < last) {
-                pg = p.free_list[rank + j - first];
-                row[j] = pg;
-                p.refs[pg] = 1;
-            } else {
-                pg = row[j];
-            }
-            to[j] = pg;
-        }
+        write_rows(p, k, j0, min(j0 + kRowEntries, p.width), threadIdx.x, 256, p.start[k], p.rank[k]);
         return;
     }
     const int64_t t0 = (blockIdx.x - row_blocks) * kTokensPerBlock;
-    __shared__ int cu_s[kSharedRequests + 1];
-    const int* cu = p.cu;
-    if (p.num <= kSharedRequests) {      // (a search of dependent steps, on the chip)
-        for (int k = threadIdx.x; k <= p.num; k += blockDim.x) cu_s[k] = p.cu[k];
-        __syncthreads();
-        cu = cu_s;
-    }
-    const int live = cu[p.num];
-    for (int64_t t = t0 + threadIdx.x; t < min(t0 + kTokensPerBlock, p.num_tokens); t += blockDim.x) {
-        int64_t slot = -1;
-        int pos = 0;
-        if (t < live) {
-            int lo = 0, hi = p.num - 1;      // the last request that begins at or before t (empty ones end before it)
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) / 2;
-                if (cu[mid] <= t) lo = mid;
-                else hi = mid - 1;
-            }
-            const int start = p.start[lo];
-            pos = start + static_cast<int>(t) - cu[lo];
-            const int j = pos / p.page_size, first = pages_of(start, p.page_size);
-            const int pg = j < first ? p.tables[p.slots[lo] * p.stride + j] : p.free_list[p.rank[lo] + j - first];
-            slot = static_cast<int64_t>(pg) * p.page_size + pos % p.page_size;
-        }
-        p.slot_mapping[t] = slot;
-        p.positions[t] = pos;
-    }
+    write_tokens(p, t0, min(t0 + kTokensPerBlock, p.num_tokens), stage_cu(p, cu_s), p.start, p.rank);
 }
 
 // ------------------------------------------------------------------ forking
@@ -931,9 +1009,14 @@ extern "C" int nvfp4kv_extend_pages(int32_t* block_tables, int64_t tables_stride
     const int64_t row_blocks = static_cast<int64_t>(num) * chunks;
     const int64_t blocks = row_blocks + (num_tokens + kTokensPerBlock - 1) / kTokensPerBlock;
     if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "nvfp4kv_extend_pages: too many requests for one call");
-    cudaError_t e = launch_dependent(extend_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
-    if (e == cudaSuccess && blocks > 0)
-        e = launch_dependent(extend_apply_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a, chunks, row_blocks);
+    cudaError_t e;
+    if (num <= kPlanThreads && static_cast<int64_t>(num) * table_width + 3 * num_tokens <= kOneLaunch) {
+        e = launch_dependent(extend_step_kernel, dim3(kStepBlocks), dim3(kPlanThreads), 0, st, a);
+    } else {
+        e = launch_dependent(num <= kPlanThreads ? extend_plan_kernel<true> : extend_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, st, a);
+        if (e == cudaSuccess && blocks > 0)
+            e = launch_dependent(extend_apply_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a, chunks, row_blocks);
+    }
     if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_extend_pages launch failed: %s", cudaGetErrorString(e));
     return check_launch("nvfp4kv_extend_pages");
 }
