@@ -93,7 +93,7 @@ constexpr int SM_LSUM = SM_RED + 2 * 4 * 64 * 4;             // 4 x 64 f32
 constexpr int SM_QS = SM_LSUM + 4 * 64 * 4;                  // 4 x 64 f32: score factor (log2 units) of a row
 constexpr int SM_FLAGS = SM_QS + 4 * 64 * 4;                 // [0] TMEM base, [1] abort
 constexpr int SM_WORK = SM_FLAGS + 16;                       // a Work per warp, and one with the range's first part
-constexpr int kWorkBytes = 160;
+constexpr int kWorkBytes = 192;
 constexpr int SM_BARS = SM_WORK + (kThreads / 32 + 1) * kWorkBytes;
 constexpr int B_FULL = 0;                      // [kStages] leader: stage landed in both CTAs
 constexpr int B_EMPTY = B_FULL + kStages;      // [kStages] both: the MMAs have read the stage
@@ -264,10 +264,16 @@ __device__ __forceinline__ Seq load_seq(const PrefillParams& p, int b) {
     s.units = (s.rows + kUnitRows - 1) / kUnitRows;
     return s;
 }
+// The new token of a row of the sequence: row / heads.
+__device__ __forceinline__ int token_of(const PrefillParams& p, int row) {
+    int tok = p.heads == 1 ? row : static_cast<int>(__umulhi(row, p.heads_magic));      // the quotient, or one more
+    tok -= tok * p.heads > row;
+    return tok;
+}
 // Tokens that unit k of the sequence sees: those of its last row.
 __device__ __forceinline__ int unit_end(const PrefillParams& p, const Seq& s, int k) {
     const int last = min(s.rows, (k + 1) * kUnitRows) - 1;
-    return max(0, min(s.L, s.L - s.n + last / p.heads + 1));
+    return max(0, min(s.L, s.L - s.n + token_of(p, last) + 1));
 }
 template <bool kWindow>
 __device__ __forceinline__ int tiles_to(const PrefillParams& p, int end) {
@@ -330,6 +336,9 @@ struct Range {
     int64_t left;       // weight still to do
     int b, k, offset;   // sequence, unit, weight of the unit done before
     int image0;         // image blocks of the sequences before b
+    int loaded;         // whether what follows is sequence b's
+    Seq seq;
+    int image_rows, gap0;
 };
 // Where pair `pair` of p.pairs begins.  Run by one warp, a sequence per lane (and pass, past 32).
 template <bool kWindow>
@@ -352,7 +361,7 @@ __device__ __forceinline__ Range find_range(const PrefillParams& p, int pair) {
         lo = total * pair / p.pairs;
         hi = total * (pair + 1) / p.pairs;
     }
-    Range r{hi - lo, 0, 0, 0, 0};
+    Range r{hi - lo, 0, 0, 0, 0, 0, {}, 0, 0};
     if (hi <= lo) return r;
     int64_t before = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
@@ -414,20 +423,27 @@ __device__ __forceinline__ int tiles_in(int weight) { return max(weight - kUnitW
 template <bool kWindow>
 __device__ __forceinline__ bool next_part_of(const PrefillParams& p, Range& r, Part& t) {
     while (r.left > 0) {
-        const Seq s = load_seq(p, r.b);
-        t.image_rows = image_rows_of<kWindow>(p, s);
+        if (!r.loaded) {
+            r.seq = load_seq(p, r.b);
+            r.image_rows = image_rows_of<kWindow>(p, r.seq);
+            r.gap0 = kWindow && r.seq.units > 0 ? unit_gap(p, unit_end(p, r.seq, 0)) : 0;
+            r.loaded = 1;
+        }
+        const Seq& s = r.seq;
         if (r.k >= s.units) {
             ++r.b;
             r.k = 0;
             r.offset = 0;
-            r.image0 += (t.image_rows + kImageTok - 1) / kImageTok;
+            r.image0 += (r.image_rows + kImageTok - 1) / kImageTok;
+            r.loaded = 0;
             continue;
         }
+        t.image_rows = r.image_rows;
         t.end = unit_end(p, s, r.k);
         const int tiles = tiles_to<kWindow>(p, t.end);
         if (kWindow) {
             t.gap = unit_gap(p, t.end);
-            t.lift = t.gap - unit_gap(p, unit_end(p, s, 0));
+            t.lift = t.gap - r.gap0;
         }
         const int weight = kTileWeight * tiles + kUnitWeight, begin = r.offset;
         const int take = static_cast<int>(r.left < weight - begin ? r.left : weight - begin);
@@ -631,8 +647,7 @@ __device__ __forceinline__ void load_q(const PrefillParams& p, const volatile Pa
         q.rope[j] = 0;
         const int row = row0 + r + j * step;
         if (row < rows && r + j * step < half) {
-            int tok = p.heads == 1 ? row : static_cast<int>(__umulhi(row, p.heads_magic));      // row / heads, or one more
-            tok -= tok * p.heads > row;
+            const int tok = token_of(p, row);
             const __nv_bfloat16* src = p.q + static_cast<int64_t>(first + tok) * p.q_st + static_cast<int64_t>(row - tok * p.heads) * p.q_sh;
             q.u[j][0] = ldg_nc_v4(src + 16 * lane);
             q.u[j][1] = ldg_nc_v4(src + 16 * lane + 8);
