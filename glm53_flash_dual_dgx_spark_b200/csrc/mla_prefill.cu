@@ -65,6 +65,10 @@ namespace nvfp4kv {
 namespace {
 
 constexpr int kRope = NVFP4KV_ROPE;
+// The kernels' forms.  kAll: every token up to a row's own.  kWindowed: a window and sinks.  kDirect: those
+// with queries of several units a sequence: Q stays bf16, and goes from q straight into its operand; the
+// image holds every latent twice, in bf16 for QK and in fp16 for PV.
+enum Form { kAll, kWindowed, kDirect };
 constexpr int kDim = kLatent + kRope;
 constexpr int kUnitRows = 128;                  // query rows of a unit
 constexpr int kCtaRows = 64;
@@ -138,6 +142,8 @@ struct PrefillParams {
     uint32_t heads_magic;      // ceil(2^32 / heads)
     int pairs;
     float scale_log2, out_scale;
+    float factor;              // kDirect: what turns a score into log2 units, and what it is turned by before that
+    float turn;                // (1, -1 for a negative scale, 0 for none)
     __nv_bfloat16* out;
     int64_t o_st, o_sh;
     float* lse;
@@ -145,7 +151,7 @@ struct PrefillParams {
     float* part_ml;     // [pairs][2][128][2]: reference (log2 units), sum
     float* part_o;      // [pairs][2][64 chunks of 8 dims][128 rows][8]
     uint8_t* q_scratch; // [pairs][2 CTAs][kQBytes]: the next part's Q
-    uint8_t* image;     // [blocks][8 or 9 atoms][128 tokens x 128 B]
+    uint8_t* image;     // [blocks][8 or 9 atoms; kDirect: and 8 for PV][128 tokens x 128 B]
     uint32_t* image_bits;   // [blocks][8]: 128 bits of tokens that exist, 128 of those that hold a NaN
     int32_t* err;
 };
@@ -237,7 +243,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // Instruction descriptors: fp32 accumulators, M = 128 (a pair's rows), N = 256.
 constexpr uint32_t kIdescQk = idesc_f16_f32(128, 256, false, false);
-constexpr uint32_t kIdescRope = kIdescQk | (1u << 7) | (1u << 10);      // both operands bf16
+constexpr uint32_t kIdescBf16 = kIdescQk | (1u << 7) | (1u << 10);      // both operands bf16
 constexpr uint32_t kIdescPv = idesc_f16_f32(128, 256, false, true);
 
 // A warpgroup's registers per thread from here on (a decrease may not go up, nor an increase down).
@@ -536,6 +542,13 @@ __device__ __forceinline__ uint4 dequant8(uint32_t code, uint32_t scale2) {
     return make_uint4(hmul2_u32(h[0], scale2), hmul2_u32(h[1], scale2), hmul2_u32(h[2], scale2), hmul2_u32(h[3], scale2));
 }
 
+// Two fp16 as bf16; exact for a code times its scale (5 bits).
+__device__ __forceinline__ uint32_t half2_to_bf162(uint32_t h) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    const __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&b);
+}
+
 // ------------------------------------------------------------------ image
 // The image: every token of the sequences with new ones dequantised, as the ring stages the attention
 // kernel copies.  Block = 128 tokens: [8 latent atoms (+ the rope part)][128 tokens x 128 B], 128-byte
@@ -545,8 +558,9 @@ __device__ __forceinline__ uint4 dequant8(uint32_t code, uint32_t scale2) {
 // rows.  The blocks of the grid take pieces of 32 tokens in turn (their number is on the device), a
 // row per thread, six blocks on an SM: 24.2 us for 91K tokens (143 MB read and written, 5.9 TB/s;
 // with four rows a thread and two blocks 26.6, and 5.4 against 3.4 for 2.4K tokens).
-template <bool kWindow>
+template <Form kForm>
 __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_constant__ PrefillParams p) {
+    constexpr bool kWindow = kForm != kAll;
     __shared__ uint32_t bits[2];      // of the piece's tokens: those that exist, those that hold a NaN
     __shared__ int b_s, pos_s, total_s;
     griddep_wait();                   // first: what starts now counts on all before this grid being done
@@ -601,7 +615,7 @@ __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_cons
             }
             if (p.rope) rope = ldg_nc_v4(p.rope + row * kRope + 8 * lp);
         }
-        const int atoms = p.rope ? 9 : 8;
+        const int k_atoms = p.rope ? 9 : 8, atoms = k_atoms + (kForm == kDirect ? 8 : 0);
         uint8_t* dst = p.image + static_cast<int64_t>(block) * atoms * kStageBytes + piece * 4096 + r0 * 128 + ((lp ^ (r0 & 7)) << 4);
         bool nan = false;
 #pragma unroll
@@ -613,7 +627,14 @@ __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_cons
                 const bool bad = ((scale[h] >> (s & 2 ? 8 : 0)) & 0x7F) == 0x7F;
                 nan |= bad;
                 const uint4 v = dequant8(word[s], __byte_perm(s2, s2, s & 2 ? 0x3232 : 0x1010));
-                *reinterpret_cast<uint4*>(dst + (4 * h + s) * kStageBytes) = bad ? make_uint4(0, 0, 0, 0) : v;
+                const uint4 w = bad ? make_uint4(0, 0, 0, 0) : v;
+                if constexpr (kForm == kDirect) {
+                    *reinterpret_cast<uint4*>(dst + (k_atoms + 4 * h + s) * kStageBytes) = w;
+                    *reinterpret_cast<uint4*>(dst + (4 * h + s) * kStageBytes) =
+                        make_uint4(half2_to_bf162(w.x), half2_to_bf162(w.y), half2_to_bf162(w.z), half2_to_bf162(w.w));
+                } else {
+                    *reinterpret_cast<uint4*>(dst + (4 * h + s) * kStageBytes) = w;
+                }
             }
         }
         if (p.rope) *reinterpret_cast<uint4*>(dst + 8 * kStageBytes) = rope;
@@ -708,9 +729,42 @@ __device__ __forceinline__ void store_q(const PrefillParams& p, uint8_t* base, f
 // The first n bits of a word.
 __device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; }
 
-template <bool kWindow>
+// kDirect: the unit's rows of q into the operand as they are, 16 bytes at a time, zeros past the unit.  Run by
+// the threads tid, tid + nt, ... ; they wait for their copies and make them visible to the tensor core.
+__device__ __forceinline__ void copy_q(const PrefillParams& p, const volatile Part& t, int cta, uint8_t* base, int tid, int nt) {
+    const int half = t.half, row0 = t.block * kUnitRows + half * cta, rows = t.rows, first = t.first, pieces = p.rope ? 72 : 64;
+    const uint32_t dst0 = smem_u32(base);
+    for (int u = tid; u < kCtaRows * 8; u += nt) {      // (a piece of all atoms at a time: eight threads a row)
+        const int r = u >> 3, c0 = u & 7, row = row0 + r;
+        const bool real = r < half && row < rows;
+        const int tok = real ? token_of(p, row) : 0;
+        const __nv_bfloat16* src = p.q + static_cast<int64_t>(first + tok) * p.q_st + static_cast<int64_t>(real ? row - tok * p.heads : 0) * p.q_sh;
+        const uint32_t bytes = real ? 16 : 0;
+#pragma unroll
+        for (int k = 0; k < 9; ++k) {
+            const int c = c0 + 8 * k;                    // dims 8 c .. of the row
+            if (c >= pieces) break;
+            // latent half c / 32, piece (c / 4) % 8 of atom c % 4; the rope part in order
+            const int atom = k < 8 ? 4 * (c >> 5) + (c & 3) : 8, at = k < 8 ? (c >> 2) & 7 : c0;
+            cp_async16_zfill(dst0 + atom * (kCtaRows * 128) + r * 128 + ((at ^ (r & 7)) << 4), src + 8 * c, bytes);
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    fence_proxy_async_smem();
+}
+// The same rows into L2.
+__device__ __forceinline__ void prefetch_q(const PrefillParams& p, const volatile Part& t, int cta, int tid) {
+    const int row = t.block * kUnitRows + t.half * cta + tid;
+    if (tid >= t.half || row >= t.rows) return;
+    const int tok = token_of(p, row);
+    const __nv_bfloat16* src = p.q + static_cast<int64_t>(t.first + tok) * p.q_st + static_cast<int64_t>(row - tok * p.heads) * p.q_sh;
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"((p.rope ? kDim : kLatent) * 2) : "memory");
+}
+
+template <Form kForm>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
+    constexpr bool kWindow = kForm != kAll;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const uint32_t sbase = smem_u32(smem);
@@ -775,7 +829,8 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
     if (warp == kMmaWarp) pair_tmem_alloc(sbase + SM_FLAGS, kTmemCols);
     const int k_stages = p.rope ? 9 : 8;
     // A stage of a part's ring: K stage c.s of tile c.i, or V stage c.s - k_stages of tile c.i - 1.
-    const int64_t image_bytes = static_cast<int64_t>(k_stages) * kStageBytes;
+    const int64_t image_bytes = static_cast<int64_t>(k_stages + (kForm == kDirect ? kVStages : 0)) * kStageBytes;
+    const int v_atom = kForm == kDirect ? k_stages : 0;      // the image's first one for PV
     // (with a window, `last` is the sequence's last run of 64 image rows, `lift` in such runs)
     auto copy_stage = [&](const Cursor& c, int image, int last, int tile0, int lift, int slot) {
         const uint32_t dst = sbase + SM_RING + slot * kStageBytes, landed = bar(B_LAND + slot);
@@ -793,7 +848,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                     bulk_copy_g2s(dst + 8192, run(g + 1) + c.s * kStageBytes, 8192, landed);
                 } else {
                     const int v = c.s - k_stages;
-                    const uint8_t* src = run(4 * (tile0 + c.i - 1) + (v >> 1)) + (4 * cta + 2 * (v & 1)) * kStageBytes;
+                    const uint8_t* src = run(4 * (tile0 + c.i - 1) + (v >> 1)) + (v_atom + 4 * cta + 2 * (v & 1)) * kStageBytes;
                     bulk_copy_g2s(dst, src, 8192, landed);
                     bulk_copy_g2s(dst + 8192, src + kStageBytes, 8192, landed);
                 }
@@ -820,7 +875,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         QRows q;
         constexpr int kWarps = kThreads / 32;
         static_assert(kWarps * kQRows == kCtaRows, "one round of rows");
-        load_q(p, t1, cta, warp, kWarps, q);
+        if constexpr (kForm != kDirect) load_q(p, t1, cta, warp, kWarps, q);
         if (warp == kCopyWarp0 || warp == kCopyWarp0 + 1) {
             griddep_wait();           // the image kernel's writes
             early = kStages;          // (a tile has more)
@@ -829,8 +884,13 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             for (int u = 0; u < kStages; ++u, advance(c, k_stages, t1.n_tiles))
                 if ((u & 1) == warp - kCopyWarp0) copy_stage(c, t1.image, last_block(t1.image, t1.image_rows), t1.tile0, t1.lift / 64, u);
         }
-        store_q(p, smem + SM_Q, reinterpret_cast<float*>(smem + SM_QS), warp, kWarps, q);
-        fence_proxy_async_smem();
+        if constexpr (kForm == kDirect) {      // (the other warps)
+            if (warp < kCopyWarp0 || warp == kRelayWarp)
+                copy_q(p, t1, cta, smem + SM_Q, warp == kRelayWarp ? threadIdx.x - 64 : threadIdx.x, kThreads - 64);
+        } else {
+            store_q(p, smem + SM_Q, reinterpret_cast<float*>(smem + SM_QS), warp, kWarps, q);
+            fence_proxy_async_smem();
+        }
     }
     tc_fence_before();
     cluster_sync();
@@ -847,11 +907,15 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 const uint64_t dk = smem_desc_sw128(sbase + SM_RING, 16, 1024);
                 const uint64_t dv = smem_desc_sw128(sbase + SM_RING, 8192, 1024);
                 int stages = 0, parts = 0, tile = 0;      // so far
+                // (kDirect: the Q warps say how many tiles the next part has, 0 after the last, when its Q is there;
+                // looking parts up here took 2,000 to 5,000 cycles a part between its MMAs)
+                int told = kForm == kDirect ? first->part.n_tiles : 0;
+                bool more = kForm == kDirect ? told > 0 : advance_part(work);
 #pragma unroll 1
-                for (bool more = advance_part(work); more && !*abort_flag; more = next_part<kWindow>(p, work)) {
-                    const int n_tiles = t.n_tiles;
+                for (; more && !*abort_flag; more = kForm == kDirect ? told > 0 : next_part<kWindow>(p, work)) {
+                    const int n_tiles = kForm == kDirect ? told : t.n_tiles;
                     if (n_tiles == 0) continue;
-                    if (parts > 0) mbar_wait(bar(B_Q_FULL), (parts - 1) & 1, abort_flag, p.err);
+                    if (kForm != kDirect && parts > 0) mbar_wait(bar(B_Q_FULL), (parts - 1) & 1, abort_flag, p.err);
                     // One thread runs the part.  Only about one MMA is queued behind the running one, so all that
                     // comes between two MMAs has 64 cycles to hide in: the next stage's barrier is looked at in
                     // the middle of a stage.  (A wait per stage by the whole warp: 375 cycles a stage where the
@@ -883,7 +947,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                                 tc_fence_after();
 #pragma unroll 1
                                 for (int j = 0; j < k_stages; ++j)
-                                    stage(d, dq + ((j * kCtaRows * 128) >> 4), dk + ((slot * kStageBytes) >> 4), 2, j == 8 ? kIdescRope : kIdescQk, j == 0);
+                                    stage(d, dq + ((j * kCtaRows * 128) >> 4), dk + ((slot * kStageBytes) >> 4), 2, kForm == kDirect || j == 8 ? kIdescBf16 : kIdescQk, j == 0);
                                 pair_commit(bar(B_S_FULL + (at & 1)));
                                 if (i == n_tiles - 1) pair_commit(bar(B_Q_FREE));
                             }
@@ -903,6 +967,10 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                     stages += n_tiles * (k_stages + kVStages);
                     tile += n_tiles;
                     ++parts;
+                    if constexpr (kForm == kDirect) {
+                        if (!mbar_wait(bar(B_Q_FULL), (parts - 1) & 1, abort_flag, p.err)) break;
+                        told = flags[2 + (parts & 1)];
+                    }
                 }
                 if (elect_one()) pair_commit(bar(B_DRAIN));
                 __syncwarp();
@@ -958,7 +1026,17 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
 #pragma unroll 1
         for (bool more = advance_part(work); more; more = next_part<kWindow>(p, work)) {
             if (t.n_tiles == 0) continue;
-            if (parts > 0) {                     // (the first part's is there)
+            if (kForm == kDirect && parts > 0) {
+                prefetch_q(p, t, cta, threadIdx.x - 32 * kQWarp0);
+                wait_phase(bar(B_Q_FREE), (parts - 1) & 1, abort_flag, p.err);
+                copy_q(p, t, cta, smem + SM_Q, threadIdx.x - 32 * kQWarp0, 32 * kQWarps);
+                named_bar_sync(3, 32 * kQWarps);
+                if (warp == kQWarp0 && lane == 0) {
+                    if (cta == 0) flags[2 + (parts & 1)] = t.n_tiles;
+                    leader_arrive(bar(B_Q_FULL));
+                }
+                __syncwarp();
+            } else if (kForm != kDirect && parts > 0) {      // (the first part's is there)
                 // Converted into the workspace while the last part runs, and copied from there once its last QK
                 // is done: converted only then, the MMAs waited 10,000 cycles a part for it (8 chunks of 777
                 // tokens took 6 % longer).
@@ -991,6 +1069,14 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             }
             ++parts;
         }
+        if (kForm == kDirect && parts > 0) {         // no more
+            wait_phase(bar(B_Q_FREE), (parts - 1) & 1, abort_flag, p.err);      // (the last Q's arrival has been seen)
+            if (warp == kQWarp0 && lane == 0) {
+                if (cta == 0) flags[2 + (parts & 1)] = 0;
+                leader_arrive(bar(B_Q_FULL));
+            }
+            __syncwarp();
+        }
     } else {
         set_registers<kRegsSoftmax>();
         // ============================================================ softmax
@@ -1012,7 +1098,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 const int grow = t.block * kUnitRows + t.half * cta + row;    // row of the sequence
                 if (grow < t.rows && row < t.half) lim = min(t.L, t.L - t.n + grow / p.heads + 1);
             }
-            float factor = 1.0f, m_ref = -INFINITY, l = 0.0f;
+            float factor = kForm == kDirect ? p.factor : 1.0f, m_ref = -INFINITY, l = 0.0f;
             // bits of the quarter's tokens that exist, and of those that hold a NaN, loaded a tile ahead
             auto load_bits = [&](int i, uint2 (&w)[2]) {
                 const int tok0 = (tile0 + i) * kTile + 64 * q4;
@@ -1044,7 +1130,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 }
                 wait_phase(bar(B_S_FULL + (tile & 1)), (tile >> 1) & 1, abort_flag, p.err);
                 tc_fence_after();
-                if (i == 0) factor = reinterpret_cast<const float*>(smem + SM_QS)[64 * (parts & 3) + row];
+                if (kForm != kDirect && i == 0) factor = reinterpret_cast<const float*>(smem + SM_QS)[64 * (parts & 3) + row];
                 float x[64];
                 tmem_ld32(tmem + kTS + 128 * (tile & 1) + 64 * ch + lanes, reinterpret_cast<uint32_t*>(x));
                 tmem_ld32(tmem + kTS + 128 * (tile & 1) + 64 * ch + 32 + lanes, reinterpret_cast<uint32_t*>(x) + 32);
@@ -1052,6 +1138,10 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) leader_arrive(bar(B_S_FREE + (tile & 1)));
+                if (kForm == kDirect && p.turn != 1.0f) {
+#pragma unroll
+                    for (int k = 0; k < 64; ++k) x[k] *= p.turn;
+                }
                 if (!__all_sync(0xFFFFFFFFu, see >= 64 && (have.x & have.y) == 0xFFFFFFFFu && (nan.x | nan.y) == 0)) {
 #pragma unroll
                     for (int k = 0; k < 64; ++k) {
@@ -1332,6 +1422,7 @@ struct PrefillPlan {
     int group;               // sequences per pass over the workspace
     int pairs, image_blocks;
     int sink_rows, max_tiles;
+    Form form;
     size_t image_bytes, bits_bytes, q_bytes, o_bytes, ml_bytes, ws_bytes;
 };
 
@@ -1354,8 +1445,10 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
         image_rows = kTile * most + longest < image_rows ? kTile * most + longest : image_rows;
     }
     pl.max_tiles = static_cast<int>(tiles);
+    pl.form = window <= 0 ? kAll : longest * num_heads > kUnitRows ? kDirect : kWindowed;
+    const size_t block_bytes = static_cast<size_t>(pl.form == kDirect ? 17 : 9) * kStageBytes;
     const int64_t one = (image_rows + kImageTok - 1) / kImageTok;
-    const int64_t cap = static_cast<int64_t>(kImageCap / (9 * kStageBytes));
+    const int64_t cap = static_cast<int64_t>(kImageCap / block_bytes);
     const int64_t fit = one > 0 ? cap / one : batch;
     pl.group = static_cast<int>(fit < 1 ? 1 : (fit < batch ? fit : batch));
     // no more pairs than leave each less than a tile's weight: what a group can have
@@ -1369,31 +1462,31 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
     pl.pairs = static_cast<int>(pairs < 1 ? 1 : pairs);
     const int64_t blocks = one * pl.group;
     pl.image_blocks = static_cast<int>(blocks);
-    pl.image_bytes = static_cast<size_t>(blocks) * 9 * kStageBytes;
+    pl.image_bytes = static_cast<size_t>(blocks) * block_bytes;
     pl.bits_bytes = round256(static_cast<size_t>(blocks) * 32);
     pl.o_bytes = static_cast<size_t>(pl.pairs) * 2 * kUnitRows * kLatent * sizeof(float);
     pl.ml_bytes = static_cast<size_t>(pl.pairs) * 2 * kUnitRows * 2 * sizeof(float);
-    pl.q_bytes = static_cast<size_t>(pl.pairs) * 2 * kQBytes;
+    pl.q_bytes = pl.form == kDirect ? 0 : static_cast<size_t>(pl.pairs) * 2 * kQBytes;
     pl.ws_bytes = pl.image_bytes + pl.bits_bytes + pl.q_bytes + pl.o_bytes + pl.ml_bytes + round256(static_cast<size_t>(pl.pairs) * 2 * sizeof(PartInfo));
     return pl;
 }
 
-template <bool kWindow>
+template <Form kForm>
 int set_smem_limit() {
     static int done[64] = {0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return fail(NVFP4KV_ECUDA, "cudaGetDevice failed");
     if (dev >= 0 && dev < 64 && done[dev]) return NVFP4KV_OK;
-    const cudaError_t e = cudaFuncSetAttribute(mla_prefill_kernel<kWindow>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    const cudaError_t e = cudaFuncSetAttribute(mla_prefill_kernel<kForm>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "mla_prefill: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) done[dev] = 1;
     return NVFP4KV_OK;
 }
 
 // The launches of a call, a group of sequences at a time.
-template <bool kWindow>
+template <Form kForm>
 int launch_prefill(const PrefillParams& all, const PrefillPlan& pl, cudaStream_t st) {
-    int rc = set_smem_limit<kWindow>();
+    int rc = set_smem_limit<kForm>();
     if (rc != NVFP4KV_OK) return rc;
     for (int b0 = 0; b0 < all.batch; b0 += pl.group) {
         PrefillParams p = all;
@@ -1406,12 +1499,12 @@ int launch_prefill(const PrefillParams& all, const PrefillPlan& pl, cudaStream_t
         if (pl.image_blocks > 0) {
             const int most = 8 * device_sm_count();
             const int blocks = kImagePieces * pl.image_blocks;
-            e = launch_dependent(prefill_image_kernel<kWindow>, dim3(blocks < most ? blocks : most), dim3(256), 0, st, p);
+            e = launch_dependent(prefill_image_kernel<kForm>, dim3(blocks < most ? blocks : most), dim3(256), 0, st, p);
             if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill image launch failed: %s", cudaGetErrorString(e));
             // its set-up overlaps the image kernel; all else it reads was there before that one
-            e = launch_dependent(mla_prefill_kernel<kWindow>, grid, dim3(kThreads), kSmemBytes, st, p);
+            e = launch_dependent(mla_prefill_kernel<kForm>, grid, dim3(kThreads), kSmemBytes, st, p);
         } else {
-            mla_prefill_kernel<kWindow><<<grid, kThreads, kSmemBytes, st>>>(p);
+            mla_prefill_kernel<kForm><<<grid, kThreads, kSmemBytes, st>>>(p);
         }
         if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill launch failed: %s", cudaGetErrorString(e));
         if ((rc = check_launch("nvfp4kv_mla_prefill")) != NVFP4KV_OK) return rc;
@@ -1484,7 +1577,10 @@ int prefill_call(const void* q, int64_t q_stride_t, int64_t q_stride_h, const ui
     p.parts = reinterpret_cast<PartInfo*>(ws += pl.ml_bytes);
     p.window = window; p.sinks = sinks; p.sink_rows = pl.sink_rows; p.max_tiles = pl.max_tiles;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    return window > 0 ? launch_prefill<true>(p, pl, st) : launch_prefill<false>(p, pl, st);
+    p.turn = p.scale_log2 > 0.0f ? 1.0f : p.scale_log2 < 0.0f ? -1.0f : 0.0f;
+    p.factor = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2);
+    if (pl.form == kDirect) return launch_prefill<kDirect>(p, pl, st);
+    return pl.form == kWindowed ? launch_prefill<kWindowed>(p, pl, st) : launch_prefill<kAll>(p, pl, st);
 }
 
 // A window that hides nothing is none; otherwise it and the sinks lie within max_seq_len.
