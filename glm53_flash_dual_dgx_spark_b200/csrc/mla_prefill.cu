@@ -1418,14 +1418,340 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_const
     }
 }
 
+// ------------------------------------------------------------------ few rows in a window
+// Single tokens and short drafts over windows leave the kernels above waiting for one another: an image
+// that is read once, ranges, and 256-token tiles in pairs.  Here a CTA takes 64 query rows of one sequence
+// and at most 128 of the tokens that any of them sees, from the pool's rows to its part of the output:
+// latents and Q to shared memory as fp16 (the tile is B of both products: tokens x dims for QK, dims x
+// tokens for PV), one S, one P, one O, with M = 128 of which the upper half is whatever lies behind the
+// rows and is not read.  Parts of a unit meet in a second kernel.  What bounds it is the latency of that
+// chain (rows from HBM, two conversions, two products, the parts' way through L2).
+constexpr int kFewTokens = 128, kFewThreads = 512, kFewMaxParts = 64;
+constexpr int SF_Q = 0;                                       // 9 dim atoms x [64 rows x 128 B]; then P: 2 token atoms
+constexpr int SF_KV = SF_Q + 9 * kCtaRows * 128;              // 9 dim atoms x [128 tokens x 128 B]
+constexpr int SF_RED = SF_KV + 9 * kFewTokens * 128;          // 4 x 64 f32: row maxima of the token quarters, then sums
+constexpr int SF_QS = SF_RED + 2 * 4 * 64 * 4;                // 64 f32: score factor of a row
+constexpr int SF_BITS = SF_QS + 64 * 4;                       // 4 words of tokens that exist, 4 of those with a NaN
+constexpr int SF_FLAGS = SF_BITS + 32;                        // [0] TMEM base, [1] abort
+constexpr int SF_BARS = SF_FLAGS + 16;                        // [0] S complete, [1] O complete
+constexpr int kFewSmemBytes = SF_BARS + 16 + 1024;
+static_assert(kFewSmemBytes <= 232448, "shared memory budget");
+constexpr uint32_t kIdescFewQk = idesc_f16_f32(128, kFewTokens, false, false);
+constexpr uint32_t kIdescFewRope = kIdescFewQk | (1u << 7) | (1u << 10);
+constexpr uint32_t kIdescFewPv = idesc_f16_f32(128, 256, false, true);
+
+// What 64 rows from row 64 k on see: the first `sinks` tokens, then [lo, end).
+struct FewUnit {
+    int rows;             // of the unit
+    int sinks, lo, end;
+    int tokens, parts;    // parts >= 1
+};
+__device__ __forceinline__ FewUnit few_unit(const PrefillParams& p, const Seq& s, int k) {
+    FewUnit u;
+    const int r0 = kCtaRows * k, last = min(s.rows, r0 + kCtaRows) - 1;
+    u.rows = last + 1 - r0;
+    u.end = max(0, min(s.L, s.L - s.n + token_of(p, last) + 1));
+    u.lo = max(0, min(u.end, s.L - s.n + token_of(p, r0) + 1 - p.window));
+    u.sinks = min(p.sinks, u.lo);
+    u.tokens = u.sinks + u.end - u.lo;
+    u.parts = max(1, (u.tokens + kFewTokens - 1) / kFewTokens);
+    return u;
+}
+
+// Block x = part + few_parts (unit + few_units sequence).  Part s of a unit, when there are several, goes
+// to part_o [unit][few_parts][64 chunks of 8 dims][64 rows][8] and part_ml [unit][few_parts][64][2].
+__global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __grid_constant__ PrefillParams p, int few_units, int few_parts) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const uint32_t sbase = smem_u32(smem);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int part = blockIdx.x % few_parts, unit = blockIdx.x / few_parts, k = unit % few_units, b = unit / few_units;
+    volatile int* flags = reinterpret_cast<volatile int*>(smem + SF_FLAGS);
+    volatile int* abort_flag = flags + 1;
+    uint32_t* bits = reinterpret_cast<uint32_t*>(smem + SF_BITS);
+    const uint32_t bar = sbase + SF_BARS;
+    griddep_launch_dependents();
+    griddep_wait();
+    const Seq seq = load_seq(p, b);
+    if (kCtaRows * k >= seq.rows) return;
+    const FewUnit u = few_unit(p, seq, k);
+    if (part >= u.parts) return;
+    // Q and the part's pool rows on their way
+    Part t;
+    t.block = k >> 1;
+    t.half = kCtaRows;
+    t.rows = seq.rows;
+    t.first = seq.first;
+    QRows q;
+    load_q(p, t, k & 1, warp, kFewThreads / 32, q);
+    const int lp = tid & 7, r0 = tid >> 3, u0 = kFewTokens * part;
+    uint4 code[2][2], rope[2];
+    uint16_t scale[2][2];
+    bool have[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int l = u0 + r0 + 64 * i, pos = l < u.sinks ? l : u.lo + l - u.sinks;
+        const int64_t row = l < u.tokens ? pool_row(p, p.tables + b * p.tables_stride, pos, u.end) : -1;
+        have[i] = row >= 0;
+        if (l < u.tokens && row < 0 && lp == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
+        rope[i] = code[i][0] = code[i][1] = make_uint4(0, 0, 0, 0);
+        scale[i][0] = scale[i][1] = 0;
+        if (have[i]) {
+            const uint8_t* src = p.pool + row * kRowBytes;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                code[i][h] = ldg_nc_v4(src + 128 * h + 16 * lp);
+                scale[i][h] = __ldg(reinterpret_cast<const uint16_t*>(src + 256 + 16 * h + 2 * lp));
+            }
+            if (p.rope) rope[i] = ldg_nc_v4(p.rope + row * kRope + 8 * lp);
+        }
+    }
+    if (tid < 8) bits[tid] = 0;
+    if (tid == 32) {
+        flags[1] = 0;
+        mbar_init(bar, 1);
+        mbar_init(bar + 8, 1);
+        mbar_fence_init();
+    }
+    if (warp == 2) {
+        tmem_alloc(sbase + SF_FLAGS, kTmemCols);
+        tmem_relinquish();
+    }
+    __syncthreads();
+    store_q(p, smem + SF_Q, reinterpret_cast<float*>(smem + SF_QS), warp, kFewThreads / 32, q);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = r0 + 64 * i;
+        uint8_t* dst = smem + SF_KV + r * 128 + ((lp ^ (r & 7)) << 4);
+        bool nan = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t word[4] = {code[i][h].x, code[i][h].y, code[i][h].z, code[i][h].w};
+            const uint32_t s2 = e4m3x2_to_f16x2(scale[i][h]);
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const bool bad = ((scale[i][h] >> (a & 2 ? 8 : 0)) & 0x7F) == 0x7F;
+                nan |= bad;
+                const uint4 v = dequant8(word[a], __byte_perm(s2, s2, a & 2 ? 0x3232 : 0x1010));
+                *reinterpret_cast<uint4*>(dst + (4 * h + a) * (kFewTokens * 128)) = bad ? make_uint4(0, 0, 0, 0) : v;
+            }
+        }
+        if (p.rope) *reinterpret_cast<uint4*>(dst + 8 * (kFewTokens * 128)) = rope[i];
+        if (nan) atomicOr(&bits[4 + (r >> 5)], 1u << (r & 31));
+        if (lp == 0 && have[i]) atomicOr(&bits[r >> 5], 1u << (r & 31));
+    }
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = static_cast<uint32_t>(flags[0]);
+    if (warp == 2) {
+        if (elect_one()) {
+            const uint64_t dq = smem_desc_sw128(sbase + SF_Q, 16, 1024), dk = smem_desc_sw128(sbase + SF_KV, 16, 1024);
+            const int atoms = p.rope ? 9 : 8;
+            for (int j = 0; j < atoms; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    tc_mma_f16(tmem, dq + ((j * kCtaRows * 128) >> 4) + 2 * i, dk + ((j * kFewTokens * 128) >> 4) + 2 * i,
+                               j == 8 ? kIdescFewRope : kIdescFewQk, j > 0 || i > 0);
+            tc_commit(bar);
+        }
+        __syncwarp();
+    }
+    mbar_wait(bar, 0, abort_flag, p.err);
+    tc_fence_after();
+    // softmax: eight warps, 32 rows x 32 tokens each (a row's quarters in warps 4 apart)
+    const int sp = warp & 3, cg = warp >> 2, row = 32 * (sp & 1) + lane;
+    const uint32_t lanes = static_cast<uint32_t>(32 * (sp & 1)) << 16;
+    float* red = reinterpret_cast<float*>(smem + SF_RED);
+    float m_ref = -INFINITY;
+    if (sp < 2) {
+        int lim = 0;
+        if (row < u.rows) lim = min(seq.L, seq.L - seq.n + token_of(p, kCtaRows * k + row) + 1);
+        const float factor = reinterpret_cast<const float*>(smem + SF_QS)[row];
+        float x[32];
+        tmem_ld32(tmem + 32 * cg + lanes, reinterpret_cast<uint32_t*>(x));
+        tmem_wait_ld();
+        // local tokens l < sinks lie at l, the others at l + off
+        const int l0 = u0 + 32 * cg, off = l0 + u.lo - u.sinks;
+        const uint32_t first = bits_below(u.sinks - l0);
+        const uint32_t see = bits[cg] & ((first & bits_below(lim - l0)) |
+                                         (~first & bits_below(lim - off) & (~bits_below(lim - p.window - off) | bits_below(p.sinks - off))));
+        const uint32_t nan = bits[4 + cg];
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            if ((nan >> i) & 1u) x[i] = __int_as_float(0x7FFFFFFF);
+            if (!((see >> i) & 1u)) x[i] = -INFINITY;
+            m = fmaxf(m, x[i]);
+        }
+        red[64 * cg + row] = factor * m;
+        named_bar_sync(1, 256);
+        m = fmaxf(fmaxf(red[row], red[64 + row]), fmaxf(red[128 + row], red[192 + row]));
+        if (m > -INFINITY) m_ref = m - kTopLog2;
+        const float base = m_ref == -INFINITY ? 0.0f : m_ref;
+        uint32_t pk[16];
+        float l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float a = ex2_approx(fmaf(x[2 * i], factor, -base)), c = ex2_approx(fmaf(x[2 * i + 1], factor, -base));
+            l += a + c;
+            pk[i] = pack_half2(a, c);
+        }
+        red[256 + 64 * cg + row] = l;
+        uint8_t* dst = smem + SF_Q + (cg >> 1) * (kCtaRows * 128) + row * 128;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint4*>(dst + (((4 * (cg & 1) + c) ^ (row & 7)) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+        fence_proxy_async_smem();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 2) {
+        if (elect_one()) {
+            const uint64_t dp = smem_desc_sw128(sbase + SF_Q, 16, 1024);
+            const int steps = (min(kFewTokens, u.tokens - u0) + 15) / 16;
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+                const uint64_t dv = smem_desc_sw128(sbase + SF_KV + 4 * h * (kFewTokens * 128), kFewTokens * 128, 1024);
+                for (int i = 0; i < steps; ++i)
+                    tc_mma_f16(tmem + 256 * h, dp + (((i >> 2) * kCtaRows * 128) >> 4) + 2 * (i & 3), dv + 128 * i, kIdescFewPv, i > 0);
+            }
+            tc_commit(bar + 8);
+        }
+        __syncwarp();
+    }
+    if (u.tokens > u0) mbar_wait(bar + 8, 0, abort_flag, p.err);
+    tc_fence_after();
+    if (sp < 2) {
+        const float l = (red[256 + row] + red[320 + row]) + (red[384 + row] + red[448 + row]);
+        const bool any = l > 0.0f || l != l, whole = u.parts == 1, real = row < u.rows;
+        const int grow = kCtaRows * k + row, tok = real ? token_of(p, grow) : 0, head = grow - tok * p.heads;
+        const int64_t slot = static_cast<int64_t>(unit) * few_parts + part;
+        const float mul = whole ? (any ? p.out_scale / l : 0.0f) : 1.0f;
+        if (cg == 0 && real) {
+            if (!whole) *reinterpret_cast<float2*>(p.part_ml + 2 * (slot * kCtaRows + row)) = make_float2(m_ref, l);
+            else if (p.lse) p.lse[static_cast<int64_t>(seq.first + tok) * p.heads + head] = any ? 0.69314718055994531f * (m_ref + log2f(l)) : -INFINITY;
+        }
+        // columns 128 cg + 64 a + 8 j + e: dim 256 (cg / 2) + 32 j + 16 (cg % 2) + 8 a + e
+        __nv_bfloat16* out = p.out + static_cast<int64_t>(seq.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh + 256 * (cg >> 1) + 16 * (cg & 1);
+        float* part_o = p.part_o + (slot * 64 + 16 * cg) * (8 * kCtaRows) + 8 * row;
+#pragma unroll 1
+        for (int j = 0; j < 8; j += 2) {
+            uint32_t o[2][16];
+            tmem_ld16(tmem + 128 * cg + 8 * j + lanes, o[0]);
+            tmem_ld16(tmem + 128 * cg + 64 + 8 * j + lanes, o[1]);
+            tmem_wait_ld();
+            if (!real || (!whole && !any)) continue;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (whole) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t* src = &o[i >> 2][8 * h + 2 * (i & 3)];
+                        const __nv_bfloat162 two = any ? __floats2bfloat162_rn(__uint_as_float(src[0]) * mul, __uint_as_float(src[1]) * mul)
+                                                       : __floats2bfloat162_rn(0.0f, 0.0f);
+                        w[i] = *reinterpret_cast<const uint32_t*>(&two);
+                    }
+                    *reinterpret_cast<uint4*>(out + 32 * (j + h)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(out + 32 * (j + h) + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                } else {
+                    st_global_v8(part_o + (j + h) * (8 * kCtaRows), &o[0][8 * h]);
+                    st_global_v8(part_o + (8 + j + h) * (8 * kCtaRows), &o[1][8 * h]);
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    if (*abort_flag && warp == 2) {      // after a timed-out wait the products in flight end before their memory goes
+        mbar_drain_wait(bar, 0);
+        if (u.tokens > u0) mbar_drain_wait(bar + 8, 0);
+    }
+    __syncthreads();
+    if (warp == 2) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Merges the parts of the units that have several: four rows of a unit a block, a row's weights by a warp,
+// 8 dims of a row by a thread.
+__global__ void __launch_bounds__(256) mla_window_few_combine_kernel(const __grid_constant__ PrefillParams p, int few_units, int few_parts) {
+    __shared__ float wts[kFewMaxParts][4], invs[4];
+    const int unit = blockIdx.x / (kCtaRows / 4), row0 = blockIdx.x % (kCtaRows / 4) * 4, k = unit % few_units, b = unit / few_units;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    griddep_wait();
+    const Seq seq = load_seq(p, b);
+    const int grow0 = kCtaRows * k + row0;
+    if (grow0 >= seq.rows) return;
+    const FewUnit u = few_unit(p, seq, k);
+    if (u.parts == 1) return;
+    const int64_t slot0 = static_cast<int64_t>(unit) * few_parts;
+    if (warp < 4) {
+        const bool real = grow0 + warp < seq.rows;
+        float2 ml[kFewMaxParts / 32];
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kFewMaxParts / 32; ++i) {
+            const int s = 32 * i + lane;
+            ml[i] = make_float2(-INFINITY, 0.0f);
+            if (real && s < u.parts) ml[i] = *reinterpret_cast<const float2*>(p.part_ml + 2 * ((slot0 + s) * kCtaRows + row0 + warp));
+            if (ml[i].y > 0.0f) m = fmaxf(m, ml[i].x);
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+#pragma unroll
+        for (int i = 0; i < kFewMaxParts / 32; ++i) {
+            float w = ml[i].y > 0.0f ? exp2f(ml[i].x - m) : 0.0f;
+            if (ml[i].y != ml[i].y) w = ml[i].y;      // a NaN counts whatever its part's maximum, which no NaN raises
+            if (w != 0.0f) l += w * ml[i].y;
+            wts[32 * i + lane][warp] = w;
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+        if (lane == 0) {
+            const bool any = l > 0.0f || l != l;
+            invs[warp] = any ? p.out_scale / l : 0.0f;
+            if (p.lse && real)      // (row = token x heads + head)
+                p.lse[static_cast<int64_t>(seq.first) * p.heads + grow0 + warp] = any ? 0.69314718055994531f * (m + log2f(l)) : -INFINITY;
+        }
+    }
+    __syncthreads();
+    const int chunk = tid >> 2, j = tid & 3, row = grow0 + j;
+    float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    const float* src = p.part_o + (slot0 * 64 + chunk) * (8 * kCtaRows) + 8 * (row0 + j);
+#pragma unroll 4
+    for (int s = 0; s < u.parts; ++s) {
+        const float w = wts[s][j];
+        if (w == 0.0f) continue;      // (a part that saw no token wrote no O)
+        const float4 a = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * (64 * 8 * kCtaRows));
+        const float4 c = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * (64 * 8 * kCtaRows) + 4);
+        acc[0] = fmaf(w, a.x, acc[0]); acc[1] = fmaf(w, a.y, acc[1]); acc[2] = fmaf(w, a.z, acc[2]); acc[3] = fmaf(w, a.w, acc[3]);
+        acc[4] = fmaf(w, c.x, acc[4]); acc[5] = fmaf(w, c.y, acc[5]); acc[6] = fmaf(w, c.z, acc[6]); acc[7] = fmaf(w, c.w, acc[7]);
+    }
+    if (row >= seq.rows) return;
+    const float inv = invs[j];
+    // chunk 16 g + 8 a + i: dims 256 (g / 2) + 32 i + 16 (g % 2) + 8 a ..
+    const int dim = 256 * (chunk >> 5) + 32 * (chunk & 7) + 16 * ((chunk >> 4) & 1) + 8 * ((chunk >> 3) & 1);
+    const int tok = token_of(p, row), head = row - tok * p.heads;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 two = __floats2bfloat162_rn(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+        w[i] = *reinterpret_cast<const uint32_t*>(&two);
+    }
+    *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(seq.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh + dim) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 struct PrefillPlan {
     int group;               // sequences per pass over the workspace
     int pairs, image_blocks;
     int sink_rows, max_tiles;
     Form form;
+    int few_units, few_parts;   // > 0: units a sequence and parts a unit of the kernels for few rows
     size_t image_bytes, bits_bytes, q_bytes, o_bytes, ml_bytes, ws_bytes;
 };
 
+constexpr int64_t kFewWaves = 3;
 // Images take at most this, or one sequence's; a larger batch runs in groups of sequences.
 constexpr size_t kImageCap = size_t(1) << 30;
 
@@ -1439,6 +1765,22 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
         // a unit's rows belong to at most `span` tokens, and see no more than the sinks and the window - 1 +
         // span last tokens up to its end, which is rounded up to a multiple of 64
         const int64_t by_rows = (num_heads + kUnitRows - 2) / num_heads + 1, span = by_rows < longest ? by_rows : longest;
+        // few rows: as many parts as a wave or three of CTAs
+        const int64_t rows = longest * num_heads, few_units = (rows + kCtaRows - 1) / kCtaRows;
+        const int64_t of_64 = (num_heads + kCtaRows - 2) / num_heads + 1, few_span = of_64 < longest ? of_64 : longest;
+        int64_t seen = static_cast<int64_t>(sinks) + window - 1 + few_span;
+        seen = seen < max_seq_len ? seen : max_seq_len;
+        const int64_t few_parts = seen > kFewTokens ? (seen + kFewTokens - 1) / kFewTokens : 1;
+        if (few_parts <= kFewMaxParts && few_units * few_parts * batch <= kFewWaves * device_sm_count()) {
+            pl.few_units = static_cast<int>(few_units);
+            pl.few_parts = static_cast<int>(few_parts);
+            const size_t slots = few_parts > 1 ? static_cast<size_t>(batch) * few_units * few_parts : 0;
+            pl.group = batch;
+            pl.o_bytes = slots * kCtaRows * kLatent * sizeof(float);
+            pl.ml_bytes = round256(slots * kCtaRows * 2 * sizeof(float));
+            pl.ws_bytes = pl.o_bytes + pl.ml_bytes;
+            return pl;
+        }
         pl.sink_rows = (sinks + 63) / 64 * 64;
         const int64_t most = (pl.sink_rows + static_cast<int64_t>(window) - 1 + span + 63 + kTile - 1) / kTile;
         tiles = most < tiles ? most : tiles;
@@ -1471,13 +1813,13 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
     return pl;
 }
 
-template <Form kForm>
-int set_smem_limit() {
+template <auto kKernel>
+int set_smem_limit(int bytes) {
     static int done[64] = {0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return fail(NVFP4KV_ECUDA, "cudaGetDevice failed");
     if (dev >= 0 && dev < 64 && done[dev]) return NVFP4KV_OK;
-    const cudaError_t e = cudaFuncSetAttribute(mla_prefill_kernel<kForm>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    const cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "mla_prefill: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) done[dev] = 1;
     return NVFP4KV_OK;
@@ -1486,7 +1828,7 @@ int set_smem_limit() {
 // The launches of a call, a group of sequences at a time.
 template <Form kForm>
 int launch_prefill(const PrefillParams& all, const PrefillPlan& pl, cudaStream_t st) {
-    int rc = set_smem_limit<kForm>();
+    int rc = set_smem_limit<mla_prefill_kernel<kForm>>(kSmemBytes);
     if (rc != NVFP4KV_OK) return rc;
     for (int b0 = 0; b0 < all.batch; b0 += pl.group) {
         PrefillParams p = all;
@@ -1515,6 +1857,17 @@ int launch_prefill(const PrefillParams& all, const PrefillPlan& pl, cudaStream_t
         if ((rc = check_launch("nvfp4kv_mla_prefill combine")) != NVFP4KV_OK) return rc;
     }
     return NVFP4KV_OK;
+}
+
+int launch_few(const PrefillParams& p, const PrefillPlan& pl, cudaStream_t st) {
+    const int rc = set_smem_limit<mla_window_few_kernel>(kFewSmemBytes);
+    if (rc != NVFP4KV_OK) return rc;
+    const int units = p.batch * pl.few_units;
+    cudaError_t e = launch_dependent(mla_window_few_kernel, dim3(units * pl.few_parts), dim3(kFewThreads), kFewSmemBytes, st, p, pl.few_units, pl.few_parts);
+    if (e == cudaSuccess && pl.few_parts > 1)
+        e = launch_dependent(mla_window_few_combine_kernel, dim3(units * (kCtaRows / 4)), dim3(256), 0, st, p, pl.few_units, pl.few_parts);
+    if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill_window launch failed: %s", cudaGetErrorString(e));
+    return check_launch("nvfp4kv_mla_prefill_window");
 }
 
 int workspace_call(int batch, int total_q, int num_heads, int max_q_len, int max_seq_len, int window, int sinks, size_t* bytes) {
@@ -1579,6 +1932,7 @@ int prefill_call(const void* q, int64_t q_stride_t, int64_t q_stride_h, const ui
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     p.turn = p.scale_log2 > 0.0f ? 1.0f : p.scale_log2 < 0.0f ? -1.0f : 0.0f;
     p.factor = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2);
+    if (pl.few_units > 0) return launch_few(p, pl, st);
     if (pl.form == kDirect) return launch_prefill<kDirect>(p, pl, st);
     return pl.form == kWindowed ? launch_prefill<kWindowed>(p, pl, st) : launch_prefill<kAll>(p, pl, st);
 }
