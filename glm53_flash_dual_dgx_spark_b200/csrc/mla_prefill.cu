@@ -1422,15 +1422,21 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_const
 // Single tokens and short drafts over windows leave the kernels above waiting for one another: an image
 // that is read once, ranges, and 256-token tiles in pairs.  Here a CTA takes 64 query rows of one sequence
 // and at most 128 of the tokens that any of them sees, from the pool's rows to its part of the output:
-// latents and Q to shared memory as fp16 (the tile is B of both products: tokens x dims for QK, dims x
-// tokens for PV), one S, one P, one O, with M = 128 of which the upper half is whatever lies behind the
-// rows and is not read.  Parts of a unit meet in a second kernel.  What bounds it is the latency of that
-// chain (rows from HBM, two conversions, two products, the parts' way through L2).
+// latents and Q to shared memory as fp16, S = Q K^T with M = 128 (its upper half is whatever lies behind
+// the rows, and not read), and O^T = V^T P^T, 128 dims at a time, whose 64 columns are the rows: the same
+// tile is B of the first product and A of the second.  Parts of a unit meet in a second kernel.
+//
+// What bounds it is the latency of that chain: of 22,600 cycles for 16 single tokens of 64 heads with a
+// window of 1,024 (144 CTAs), 4,600 until Q and the pool's rows are asked for, 4,800 for them to come and
+// be converted, 2,700 for QK, 3,300 for the softmax, 2,000 for PV and 4,600 for the parts (19 MB) into L2.
+// With O = P V and 64 rows on M, the upper half of PV was wasted and half of the warps held no row of O:
+// 28.3 us a call, now 23.5 (a plan over both kernels; the second one's look at the lengths before it waits
+// and eight parts in flight 1.1 of that).
 constexpr int kFewTokens = 128, kFewThreads = 512, kFewMaxParts = 64;
 constexpr int SF_Q = 0;                                       // 9 dim atoms x [64 rows x 128 B]; then P: 2 token atoms
 constexpr int SF_KV = SF_Q + 9 * kCtaRows * 128;              // 9 dim atoms x [128 tokens x 128 B]
 constexpr int SF_RED = SF_KV + 9 * kFewTokens * 128;          // 4 x 64 f32: row maxima of the token quarters, then sums
-constexpr int SF_QS = SF_RED + 2 * 4 * 64 * 4;                // 64 f32: score factor of a row
+constexpr int SF_QS = SF_RED + 2 * 4 * 64 * 4;                // 64 f32: score factor of a row, then what O is multiplied by
 constexpr int SF_BITS = SF_QS + 64 * 4;                       // 4 words of tokens that exist, 4 of those with a NaN
 constexpr int SF_FLAGS = SF_BITS + 32;                        // [0] TMEM base, [1] abort
 constexpr int SF_BARS = SF_FLAGS + 16;                        // [0] S complete, [1] O complete
@@ -1438,7 +1444,11 @@ constexpr int kFewSmemBytes = SF_BARS + 16 + 1024;
 static_assert(kFewSmemBytes <= 232448, "shared memory budget");
 constexpr uint32_t kIdescFewQk = idesc_f16_f32(128, kFewTokens, false, false);
 constexpr uint32_t kIdescFewRope = kIdescFewQk | (1u << 7) | (1u << 10);
-constexpr uint32_t kIdescFewPv = idesc_f16_f32(128, 256, false, true);
+constexpr uint32_t kIdescFewPv = idesc_f16_f32(128, kCtaRows, true, false);
+constexpr uint32_t kTFewO = 128;                              // TMEM: S, then O^T in four blocks of 128 dims x 64 rows
+constexpr int kFewGroup = 8;                                  // rows that lie together in a part, and of a block that merges
+// The dim of lane l of O^T's block m: atom c / 64, column c % 64 of c = 128 m + l.
+__device__ __forceinline__ int few_dim(int c) { return 256 * (c >> 8) + 32 * ((c >> 3) & 7) + 8 * ((c >> 6) & 3) + (c & 7); }
 
 // What 64 rows from row 64 k on see: the first `sinks` tokens, then [lo, end).
 struct FewUnit {
@@ -1459,7 +1469,7 @@ __device__ __forceinline__ FewUnit few_unit(const PrefillParams& p, const Seq& s
 }
 
 // Block x = part + few_parts (unit + few_units sequence).  Part s of a unit, when there are several, goes
-// to part_o [unit][few_parts][64 chunks of 8 dims][64 rows][8] and part_ml [unit][few_parts][64][2].
+// to part_o [unit][few_parts][8 groups of rows][512 (as few_dim)][8 rows] and part_ml [unit][few_parts][64][2].
 __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __grid_constant__ PrefillParams p, int few_units, int few_parts) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -1608,85 +1618,96 @@ __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    const bool any_tokens = u.tokens > u0;
     if (warp == 2) {
         if (elect_one()) {
             const uint64_t dp = smem_desc_sw128(sbase + SF_Q, 16, 1024);
             const int steps = (min(kFewTokens, u.tokens - u0) + 15) / 16;
 #pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-                const uint64_t dv = smem_desc_sw128(sbase + SF_KV + 4 * h * (kFewTokens * 128), kFewTokens * 128, 1024);
+            for (int m = 0; m < 4; ++m) {
+                const uint64_t dv = smem_desc_sw128(sbase + SF_KV + 2 * m * (kFewTokens * 128), kFewTokens * 128, 1024);
                 for (int i = 0; i < steps; ++i)
-                    tc_mma_f16(tmem + 256 * h, dp + (((i >> 2) * kCtaRows * 128) >> 4) + 2 * (i & 3), dv + 128 * i, kIdescFewPv, i > 0);
+                    tc_mma_f16(tmem + kTFewO + kCtaRows * m, dv + 128 * i, dp + (((i >> 2) * kCtaRows * 128) >> 4) + 2 * (i & 3), kIdescFewPv, i > 0);
             }
             tc_commit(bar + 8);
         }
         __syncwarp();
     }
-    if (u.tokens > u0) mbar_wait(bar + 8, 0, abort_flag, p.err);
-    tc_fence_after();
-    if (sp < 2) {
+    const bool whole = u.parts == 1;
+    const int64_t slot = static_cast<int64_t>(unit) * few_parts + part;
+    float* mul = reinterpret_cast<float*>(smem + SF_QS);
+    if (sp < 2 && cg == 0) {
         const float l = (red[256 + row] + red[320 + row]) + (red[384 + row] + red[448 + row]);
-        const bool any = l > 0.0f || l != l, whole = u.parts == 1, real = row < u.rows;
-        const int grow = kCtaRows * k + row, tok = real ? token_of(p, grow) : 0, head = grow - tok * p.heads;
-        const int64_t slot = static_cast<int64_t>(unit) * few_parts + part;
-        const float mul = whole ? (any ? p.out_scale / l : 0.0f) : 1.0f;
-        if (cg == 0 && real) {
+        const bool any = l > 0.0f || l != l;
+        mul[row] = any ? p.out_scale / l : 0.0f;
+        if (row < u.rows) {
             if (!whole) *reinterpret_cast<float2*>(p.part_ml + 2 * (slot * kCtaRows + row)) = make_float2(m_ref, l);
-            else if (p.lse) p.lse[static_cast<int64_t>(seq.first + tok) * p.heads + head] = any ? 0.69314718055994531f * (m_ref + log2f(l)) : -INFINITY;
+            else if (p.lse)      // (row = token x heads + head)
+                p.lse[static_cast<int64_t>(seq.first) * p.heads + kCtaRows * k + row] = any ? 0.69314718055994531f * (m_ref + log2f(l)) : -INFINITY;
         }
-        // columns 128 cg + 64 a + 8 j + e: dim 256 (cg / 2) + 32 j + 16 (cg % 2) + 8 a + e
-        __nv_bfloat16* out = p.out + static_cast<int64_t>(seq.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh + 256 * (cg >> 1) + 16 * (cg & 1);
-        float* part_o = p.part_o + (slot * 64 + 16 * cg) * (8 * kCtaRows) + 8 * row;
-#pragma unroll 1
-        for (int j = 0; j < 8; j += 2) {
-            uint32_t o[2][16];
-            tmem_ld16(tmem + 128 * cg + 8 * j + lanes, o[0]);
-            tmem_ld16(tmem + 128 * cg + 64 + 8 * j + lanes, o[1]);
-            tmem_wait_ld();
-            if (!real || (!whole && !any)) continue;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (whole) {
-                    uint32_t w[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t* src = &o[i >> 2][8 * h + 2 * (i & 3)];
-                        const __nv_bfloat162 two = any ? __floats2bfloat162_rn(__uint_as_float(src[0]) * mul, __uint_as_float(src[1]) * mul)
-                                                       : __floats2bfloat162_rn(0.0f, 0.0f);
-                        w[i] = *reinterpret_cast<const uint32_t*>(&two);
-                    }
-                    *reinterpret_cast<uint4*>(out + 32 * (j + h)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    *reinterpret_cast<uint4*>(out + 32 * (j + h) + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-                } else {
-                    st_global_v8(part_o + (j + h) * (8 * kCtaRows), &o[0][8 * h]);
-                    st_global_v8(part_o + (8 + j + h) * (8 * kCtaRows), &o[1][8 * h]);
-                }
-            }
-        }
-        tc_fence_before();
     }
+    if (any_tokens) mbar_wait(bar + 8, 0, abort_flag, p.err);
+    tc_fence_after();
+    __syncthreads();
+    // a thread's dim of 64 rows (warp: lanes 32 (warp % 4) .. of block warp / 4)
+    const int c = 128 * cg + 32 * sp + lane;
+    const uint32_t o_addr = tmem + kTFewO + kCtaRows * cg + (static_cast<uint32_t>(32 * sp) << 16);
+    if (!whole) {
+        float* dst = p.part_o + (slot * (kCtaRows / kFewGroup) * kLatent + c) * kFewGroup;
+#pragma unroll
+        for (int g = 0; g < kCtaRows / kFewGroup; g += 4) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + kFewGroup * g, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st_global_v8(dst + (g + i) * (kLatent * kFewGroup), o + 8 * i);
+        }
+    } else {
+        // through shared memory (the latents' place: every product is done) to rows of the output
+        __nv_bfloat16* rows = reinterpret_cast<__nv_bfloat16*>(smem + SF_KV);
+        const int dim = few_dim(c);
+#pragma unroll
+        for (int g = 0; g < kCtaRows; g += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + g, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                rows[(g + i) * kLatent + dim] = __float2bfloat16_rn(any_tokens ? __uint_as_float(o[i]) * mul[g + i] : 0.0f);
+        }
+        __syncthreads();
+        for (int i = tid; i < u.rows * (kLatent / 8); i += kFewThreads) {
+            const int r = i / (kLatent / 8), d = 8 * (i % (kLatent / 8)), grow = kCtaRows * k + r, tok = token_of(p, grow), head = grow - tok * p.heads;
+            *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(seq.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh + d) =
+                *reinterpret_cast<const uint4*>(rows + r * kLatent + d);
+        }
+    }
+    tc_fence_before();
     if (*abort_flag && warp == 2) {      // after a timed-out wait the products in flight end before their memory goes
         mbar_drain_wait(bar, 0);
-        if (u.tokens > u0) mbar_drain_wait(bar + 8, 0);
+        if (any_tokens) mbar_drain_wait(bar + 8, 0);
     }
     __syncthreads();
     if (warp == 2) tmem_dealloc(tmem, kTmemCols);
 }
 
-// Merges the parts of the units that have several: four rows of a unit a block, a row's weights by a warp,
-// 8 dims of a row by a thread.
-__global__ void __launch_bounds__(256) mla_window_few_combine_kernel(const __grid_constant__ PrefillParams p, int few_units, int few_parts) {
-    __shared__ float wts[kFewMaxParts][4], invs[4];
-    const int unit = blockIdx.x / (kCtaRows / 4), row0 = blockIdx.x % (kCtaRows / 4) * 4, k = unit % few_units, b = unit / few_units;
+// Merges the parts of the units that have several: eight rows of a unit a block, a row's weights by a warp,
+// a dim of the rows by a thread.
+__global__ void __launch_bounds__(kLatent) mla_window_few_combine_kernel(const __grid_constant__ PrefillParams p, int few_units, int few_parts) {
+    __shared__ float wts[kFewMaxParts][kFewGroup], invs[kFewGroup];
+    __shared__ __align__(16) __nv_bfloat16 rows[kFewGroup][kLatent];
+    constexpr int kGroups = kCtaRows / kFewGroup;
+    const int unit = blockIdx.x / kGroups, group = blockIdx.x % kGroups, k = unit % few_units, b = unit / few_units;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    griddep_wait();
+    // (the lengths were there before the kernel before this one)
     const Seq seq = load_seq(p, b);
-    const int grow0 = kCtaRows * k + row0;
+    const int grow0 = kCtaRows * k + kFewGroup * group;
     if (grow0 >= seq.rows) return;
     const FewUnit u = few_unit(p, seq, k);
     if (u.parts == 1) return;
     const int64_t slot0 = static_cast<int64_t>(unit) * few_parts;
-    if (warp < 4) {
+    griddep_wait();
+    if (warp < kFewGroup) {
         const bool real = grow0 + warp < seq.rows;
         float2 ml[kFewMaxParts / 32];
         float m = -INFINITY, l = 0.0f;
@@ -1694,7 +1715,7 @@ __global__ void __launch_bounds__(256) mla_window_few_combine_kernel(const __gri
         for (int i = 0; i < kFewMaxParts / 32; ++i) {
             const int s = 32 * i + lane;
             ml[i] = make_float2(-INFINITY, 0.0f);
-            if (real && s < u.parts) ml[i] = *reinterpret_cast<const float2*>(p.part_ml + 2 * ((slot0 + s) * kCtaRows + row0 + warp));
+            if (real && s < u.parts) ml[i] = *reinterpret_cast<const float2*>(p.part_ml + 2 * ((slot0 + s) * kCtaRows + kFewGroup * group + warp));
             if (ml[i].y > 0.0f) m = fmaxf(m, ml[i].x);
         }
 #pragma unroll
@@ -1716,30 +1737,24 @@ __global__ void __launch_bounds__(256) mla_window_few_combine_kernel(const __gri
         }
     }
     __syncthreads();
-    const int chunk = tid >> 2, j = tid & 3, row = grow0 + j;
-    float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    const float* src = p.part_o + (slot0 * 64 + chunk) * (8 * kCtaRows) + 8 * (row0 + j);
-#pragma unroll 4
+    float acc[kFewGroup] = {};
+    const float* src = p.part_o + ((slot0 * kGroups + group) * kLatent + tid) * kFewGroup;
+#pragma unroll 8
     for (int s = 0; s < u.parts; ++s) {
-        const float w = wts[s][j];
-        if (w == 0.0f) continue;      // (a part that saw no token wrote no O)
-        const float4 a = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * (64 * 8 * kCtaRows));
-        const float4 c = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * (64 * 8 * kCtaRows) + 4);
-        acc[0] = fmaf(w, a.x, acc[0]); acc[1] = fmaf(w, a.y, acc[1]); acc[2] = fmaf(w, a.z, acc[2]); acc[3] = fmaf(w, a.w, acc[3]);
-        acc[4] = fmaf(w, c.x, acc[4]); acc[5] = fmaf(w, c.y, acc[5]); acc[6] = fmaf(w, c.z, acc[6]); acc[7] = fmaf(w, c.w, acc[7]);
-    }
-    if (row >= seq.rows) return;
-    const float inv = invs[j];
-    // chunk 16 g + 8 a + i: dims 256 (g / 2) + 32 i + 16 (g % 2) + 8 a ..
-    const int dim = 256 * (chunk >> 5) + 32 * (chunk & 7) + 16 * ((chunk >> 4) & 1) + 8 * ((chunk >> 3) & 1);
-    const int tok = token_of(p, row), head = row - tok * p.heads;
-    uint32_t w[4];
+        const float4 a = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * (kCtaRows * kLatent));
+        const float4 c = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(s) * (kCtaRows * kLatent) + 4);
+        const float v[kFewGroup] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 two = __floats2bfloat162_rn(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-        w[i] = *reinterpret_cast<const uint32_t*>(&two);
+        for (int i = 0; i < kFewGroup; ++i) acc[i] = fmaf(wts[s][i], v[i], acc[i]);
     }
-    *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(seq.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh + dim) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+    for (int i = 0; i < kFewGroup; ++i) rows[i][few_dim(tid)] = __float2bfloat16_rn(acc[i] * invs[i]);
+    __syncthreads();
+    const int r = tid / (kLatent / 8), d = 8 * (tid % (kLatent / 8)), row = grow0 + r;
+    if (row >= seq.rows) return;
+    const int tok = token_of(p, row), head = row - tok * p.heads;
+    *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(seq.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh + d) =
+        *reinterpret_cast<const uint4*>(&rows[r][d]);
 }
 
 struct PrefillPlan {
@@ -1751,7 +1766,6 @@ struct PrefillPlan {
     size_t image_bytes, bits_bytes, q_bytes, o_bytes, ml_bytes, ws_bytes;
 };
 
-constexpr int64_t kFewWaves = 3;
 // Images take at most this, or one sequence's; a larger batch runs in groups of sequences.
 constexpr size_t kImageCap = size_t(1) << 30;
 
@@ -1765,13 +1779,15 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
         // a unit's rows belong to at most `span` tokens, and see no more than the sinks and the window - 1 +
         // span last tokens up to its end, which is rounded up to a multiple of 64
         const int64_t by_rows = (num_heads + kUnitRows - 2) / num_heads + 1, span = by_rows < longest ? by_rows : longest;
-        // few rows: as many parts as a wave or three of CTAs
+        // The kernels for few rows, where their CTAs run at the same time.  In one wave they take 23.5 us for 16
+        // single tokens of 64 heads with a window of 1,024 (the others 29.4), 17.9 for 2 x 32 tokens with 128 (27.3);
+        // with 192 CTAs 32.8 against 27.3, with 576 75.9 against 63.8.
         const int64_t rows = longest * num_heads, few_units = (rows + kCtaRows - 1) / kCtaRows;
         const int64_t of_64 = (num_heads + kCtaRows - 2) / num_heads + 1, few_span = of_64 < longest ? of_64 : longest;
         int64_t seen = static_cast<int64_t>(sinks) + window - 1 + few_span;
         seen = seen < max_seq_len ? seen : max_seq_len;
         const int64_t few_parts = seen > kFewTokens ? (seen + kFewTokens - 1) / kFewTokens : 1;
-        if (few_parts <= kFewMaxParts && few_units * few_parts * batch <= kFewWaves * device_sm_count()) {
+        if (few_parts <= kFewMaxParts && few_units * few_parts * batch <= device_sm_count()) {
             pl.few_units = static_cast<int>(few_units);
             pl.few_parts = static_cast<int>(few_parts);
             const size_t slots = few_parts > 1 ? static_cast<size_t>(batch) * few_units * few_parts : 0;
@@ -1865,7 +1881,7 @@ int launch_few(const PrefillParams& p, const PrefillPlan& pl, cudaStream_t st) {
     const int units = p.batch * pl.few_units;
     cudaError_t e = launch_dependent(mla_window_few_kernel, dim3(units * pl.few_parts), dim3(kFewThreads), kFewSmemBytes, st, p, pl.few_units, pl.few_parts);
     if (e == cudaSuccess && pl.few_parts > 1)
-        e = launch_dependent(mla_window_few_combine_kernel, dim3(units * (kCtaRows / 4)), dim3(256), 0, st, p, pl.few_units, pl.few_parts);
+        e = launch_dependent(mla_window_few_combine_kernel, dim3(units * (kCtaRows / kFewGroup)), dim3(kLatent), 0, st, p, pl.few_units, pl.few_parts);
     if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill_window launch failed: %s", cudaGetErrorString(e));
     return check_launch("nvfp4kv_mla_prefill_window");
 }
