@@ -1090,36 +1090,38 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         int parts = 0, tile = 0;                 // parts with tiles, and tiles, so far
         bool first_part = true;
         griddep_wait();                          // the image kernel's token bits
+        // bits of the quarter's tokens that exist, and of those that hold a NaN: loaded a tile ahead, a part's
+        // first ones while the last PV of the part before runs
+        auto load_bits = [&](const volatile Part& t, int i, uint2 (&w)[2]) {
+            const int tok0 = (t.tile0 + i) * kTile + 64 * q4;
+            if constexpr (kWindow) {
+                const int row0 = min(tok0 < p.sink_rows ? tok0 : tok0 + t.lift, t.image_rows - 1);
+                const uint32_t* src = p.image_bits + 8 * static_cast<int64_t>(t.image + row0 / kImageTok) + (row0 & 64) / 32;
+                w[0] = *reinterpret_cast<const uint2*>(src);
+                w[1] = *reinterpret_cast<const uint2*>(src + 4);
+                return;
+            }
+            const uint32_t* src = p.image_bits + 8 * static_cast<int64_t>(t.image + min(tok0, t.L - 1) / kImageTok) + ((tok0 & (kImageTok - 1)) >> 5);
+            w[0] = *reinterpret_cast<const uint2*>(src);
+            w[1] = *reinterpret_cast<const uint2*>(src + 4);
+        };
+        uint2 ahead[2];
+        const volatile Part& next = work->ahead;
 #pragma unroll 1
         while (advance_part(work)) {
-            const int n_tiles = t.n_tiles, tile0 = t.tile0, image = t.image, gap = kWindow ? t.gap : 0, lift = kWindow ? t.lift : 0;
+            const int n_tiles = t.n_tiles, tile0 = t.tile0, gap = kWindow ? t.gap : 0;
             int lim = 0;                                                      // tokens the row sees
             {
                 const int grow = t.block * kUnitRows + t.half * cta + row;    // row of the sequence
-                if (grow < t.rows && row < t.half) lim = min(t.L, t.L - t.n + grow / p.heads + 1);
+                if (grow < t.rows && row < t.half) lim = min(t.L, t.L - t.n + token_of(p, grow) + 1);
             }
             float factor = kForm == kDirect ? p.factor : 1.0f, m_ref = -INFINITY, l = 0.0f;
-            // bits of the quarter's tokens that exist, and of those that hold a NaN, loaded a tile ahead
-            auto load_bits = [&](int i, uint2 (&w)[2]) {
-                const int tok0 = (tile0 + i) * kTile + 64 * q4;
-                if constexpr (kWindow) {
-                    const int row0 = min(tok0 < p.sink_rows ? tok0 : tok0 + lift, t.image_rows - 1);
-                    const uint32_t* src = p.image_bits + 8 * static_cast<int64_t>(image + row0 / kImageTok) + (row0 & 64) / 32;
-                    w[0] = *reinterpret_cast<const uint2*>(src);
-                    w[1] = *reinterpret_cast<const uint2*>(src + 4);
-                    return;
-                }
-                const uint32_t* src = p.image_bits + 8 * static_cast<int64_t>(image + min(tok0, t.L - 1) / kImageTok) + ((tok0 & (kImageTok - 1)) >> 5);
-                w[0] = *reinterpret_cast<const uint2*>(src);
-                w[1] = *reinterpret_cast<const uint2*>(src + 4);
-            };
-            uint2 ahead[2];
-            if (n_tiles > 0) load_bits(0, ahead);
+            if (first_part && n_tiles > 0) load_bits(t, 0, ahead);
 #pragma unroll 1
             for (int i = 0; i < n_tiles; ++i, ++tile) {
                 uint2 have = ahead[0];
                 const uint2 nan = ahead[1];
-                if (i + 1 < n_tiles) load_bits(i + 1, ahead);
+                if (i + 1 < n_tiles) load_bits(t, i + 1, ahead);
                 int see = lim - ((tile0 + i) * kTile + 64 * q4);     // tokens of the quarter the row sees
                 if constexpr (kWindow) {
                     if (lim - see >= p.sink_rows) see -= gap;
@@ -1203,6 +1205,8 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 if (lane == 0) leader_arrive(bar(B_P_FULL));
             }
             look_ahead<kWindow>(p, work);                        // (the last PV is running)
+            __syncwarp();
+            if (*reinterpret_cast<volatile int*>(&work->more) && next.n_tiles > 0) load_bits(next, 0, ahead);
             // ---- epilogue: sums over the row's four warps, O out of TMEM
             named_bar_sync(1 + (sp & 1), 128);          // the last part's sums are read
             lsum[64 * q4 + row] = l;
@@ -1213,7 +1217,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             const bool any = l > 0.0f || l != l, whole = t.head && t.tail;
             const int unit_row = t.half * cta + row, grow = t.block * kUnitRows + unit_row;
             const bool real = grow < t.rows && row < t.half;
-            const int tok = real ? grow / p.heads : 0, head = grow - tok * p.heads;
+            const int tok = real ? token_of(p, grow) : 0, head = grow - tok * p.heads;
             const int64_t part_row = (2 * pair + (first_part ? 0 : 1)) * kUnitRows + unit_row;
             const float mul = whole ? (any ? p.out_scale / l : 0.0f) : 1.0f;
             if (q4 == 0 && real) {
