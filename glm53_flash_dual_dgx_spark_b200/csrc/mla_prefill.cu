@@ -65,10 +65,11 @@ namespace nvfp4kv {
 namespace {
 
 constexpr int kRope = NVFP4KV_ROPE;
-// The kernels' forms.  kAll: every token up to a row's own.  kWindowed: a window and sinks.  kDirect: those
-// with queries of several units a sequence: Q stays bf16, and goes from q straight into its operand; the
-// image holds every latent twice, in bf16 for QK and in fp16 for PV.
-enum Form { kAll, kWindowed, kDirect };
+// The kernels' forms.  kAll: every token up to a row's own.  kDirect: a window and sinks; units are short,
+// so Q stays bf16 and goes from q straight into its operand (converted as in kAll, it was what they waited
+// for: 10,000 cycles of 32,600 a unit of three tiles), and the image holds every latent twice, in bf16
+// for QK and in fp16 for PV.
+enum Form { kAll, kDirect };
 constexpr int kDim = kLatent + kRope;
 constexpr int kUnitRows = 128;                  // query rows of a unit
 constexpr int kCtaRows = 64;
@@ -560,7 +561,7 @@ __device__ __forceinline__ uint32_t half2_to_bf162(uint32_t h) {
 // with four rows a thread and two blocks 26.6, and 5.4 against 3.4 for 2.4K tokens).
 template <Form kForm>
 __global__ void __launch_bounds__(256, 6) prefill_image_kernel(const __grid_constant__ PrefillParams p) {
-    constexpr bool kWindow = kForm != kAll;
+    constexpr bool kWindow = kForm == kDirect;
     __shared__ uint32_t bits[2];      // of the piece's tokens: those that exist, those that hold a NaN
     __shared__ int b_s, pos_s, total_s;
     griddep_wait();                   // first: what starts now counts on all before this grid being done
@@ -764,7 +765,7 @@ __device__ __forceinline__ void prefetch_q(const PrefillParams& p, const volatil
 template <Form kForm>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
-    constexpr bool kWindow = kForm != kAll;
+    constexpr bool kWindow = kForm == kDirect;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const uint32_t sbase = smem_u32(smem);
@@ -1425,27 +1426,30 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_const
 // ------------------------------------------------------------------ few rows in a window
 // Single tokens and short drafts over windows leave the kernels above waiting for one another: an image
 // that is read once, ranges, and 256-token tiles in pairs.  Here a CTA takes 64 query rows of one sequence
-// and at most 128 of the tokens that any of them sees, from the pool's rows to its part of the output:
-// latents and Q to shared memory as fp16, S = Q K^T with M = 128 (its upper half is whatever lies behind
-// the rows, and not read), and O^T = V^T P^T, 128 dims at a time, whose 64 columns are the rows: the same
-// tile is B of the first product and A of the second.  Parts of a unit meet in a second kernel.
+// and a range of the tokens that any of them sees, 128 at a time, from the pool's rows to its part of the
+// output: latents and Q to shared memory as fp16, S = Q K^T with M = 128 (its upper half is whatever lies
+// behind the rows, and not read), and O^T += V^T P^T, 128 dims at a time, whose 64 columns are the rows:
+// the same tile is B of the first product and A of the second.  Parts of a unit meet in a second kernel.
 //
 // What bounds it is the latency of that chain: of 22,600 cycles for 16 single tokens of 64 heads with a
-// window of 1,024 (144 CTAs), 4,600 until Q and the pool's rows are asked for, 4,800 for them to come and
-// be converted, 2,700 for QK, 3,300 for the softmax, 2,000 for PV and 4,600 for the parts (19 MB) into L2.
-// With O = P V and 64 rows on M, the upper half of PV was wasted and half of the warps held no row of O:
-// 28.3 us a call, now 23.5 (a plan over both kernels; the second one's look at the lengths before it waits
-// and eight parts in flight 1.1 of that).
+// window of 1,024 (144 CTAs, a tile each), 4,600 until Q and the pool's rows are asked for, 4,800 for them
+// to come and be converted, 2,700 for QK, 3,300 for the softmax, 2,000 for PV and 4,600 for the parts (19
+// MB) into L2.  With O = P V and 64 rows on M, the upper half of PV was wasted and half of the warps held
+// no row of O: 28.3 us a call, now 23.5 (the second kernel's look at the lengths before it waits, and eight
+// parts in flight, are 1.1 of that).  The pool's rows of a tile are asked for under the tile before.
 constexpr int kFewTokens = 128, kFewThreads = 512, kFewMaxParts = 64;
-constexpr int SF_Q = 0;                                       // 9 dim atoms x [64 rows x 128 B]; then P: 2 token atoms
+constexpr int SF_Q = 0;                                       // 9 dim atoms x [64 rows x 128 B]
 constexpr int SF_KV = SF_Q + 9 * kCtaRows * 128;              // 9 dim atoms x [128 tokens x 128 B]
-constexpr int SF_RED = SF_KV + 9 * kFewTokens * 128;          // 4 x 64 f32: row maxima of the token quarters, then sums
+constexpr int SF_P = SF_KV + 8 * kFewTokens * 128;            // 2 token atoms x [64 rows x 128 B], where the rope part was
+constexpr int SF_RED = SF_KV + 9 * kFewTokens * 128;          // 4 x 64 f32: row maxima of the token quarters; 4 x 64: their sums
 constexpr int SF_QS = SF_RED + 2 * 4 * 64 * 4;                // 64 f32: score factor of a row, then what O is multiplied by
-constexpr int SF_BITS = SF_QS + 64 * 4;                       // 4 words of tokens that exist, 4 of those with a NaN
+constexpr int SF_ALPHA = SF_QS + 64 * 4;                      // 64 f32: what O is multiplied by before a tile
+constexpr int SF_BITS = SF_ALPHA + 64 * 4;                    // 4 words of tokens that exist, 4 of those with a NaN
 constexpr int SF_FLAGS = SF_BITS + 32;                        // [0] TMEM base, [1] abort
-constexpr int SF_BARS = SF_FLAGS + 16;                        // [0] S complete, [1] O complete
-constexpr int kFewSmemBytes = SF_BARS + 16 + 1024;
+constexpr int SF_BARS = SF_FLAGS + 16;                        // [0] S complete, [1] O complete, [2] everything
+constexpr int kFewSmemBytes = SF_BARS + 24 + 1024;
 static_assert(kFewSmemBytes <= 232448, "shared memory budget");
+static_assert(2 * kCtaRows * 128 <= kFewTokens * 128, "P takes the rope part's place");
 constexpr uint32_t kIdescFewQk = idesc_f16_f32(128, kFewTokens, false, false);
 constexpr uint32_t kIdescFewRope = kIdescFewQk | (1u << 7) | (1u << 10);
 constexpr uint32_t kIdescFewPv = idesc_f16_f32(128, kCtaRows, true, false);
@@ -1458,9 +1462,9 @@ __device__ __forceinline__ int few_dim(int c) { return 256 * (c >> 8) + 32 * ((c
 struct FewUnit {
     int rows;             // of the unit
     int sinks, lo, end;
-    int tokens, parts;    // parts >= 1
+    int tokens, tiles, parts;    // both >= 1; part s: tiles [s tiles / parts, (s + 1) tiles / parts)
 };
-__device__ __forceinline__ FewUnit few_unit(const PrefillParams& p, const Seq& s, int k) {
+__device__ __forceinline__ FewUnit few_unit(const PrefillParams& p, const Seq& s, int k, int most) {
     FewUnit u;
     const int r0 = kCtaRows * k, last = min(s.rows, r0 + kCtaRows) - 1;
     u.rows = last + 1 - r0;
@@ -1468,7 +1472,8 @@ __device__ __forceinline__ FewUnit few_unit(const PrefillParams& p, const Seq& s
     u.lo = max(0, min(u.end, s.L - s.n + token_of(p, r0) + 1 - p.window));
     u.sinks = min(p.sinks, u.lo);
     u.tokens = u.sinks + u.end - u.lo;
-    u.parts = max(1, (u.tokens + kFewTokens - 1) / kFewTokens);
+    u.tiles = max(1, (u.tokens + kFewTokens - 1) / kFewTokens);
+    u.parts = min(u.tiles, most);
     return u;
 }
 
@@ -1488,9 +1493,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __
     griddep_wait();
     const Seq seq = load_seq(p, b);
     if (kCtaRows * k >= seq.rows) return;
-    const FewUnit u = few_unit(p, seq, k);
+    const FewUnit u = few_unit(p, seq, k, few_parts);
     if (part >= u.parts) return;
-    // Q and the part's pool rows on their way
+    const int tile0 = part * u.tiles / u.parts, tile1 = (part + 1) * u.tiles / u.parts;
+    // Q on its way
     Part t;
     t.block = k >> 1;
     t.half = kCtaRows;
@@ -1498,33 +1504,38 @@ __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __
     t.first = seq.first;
     QRows q;
     load_q(p, t, k & 1, warp, kFewThreads / 32, q);
-    const int lp = tid & 7, r0 = tid >> 3, u0 = kFewTokens * part;
+    // a tile's pool rows: eight threads a row, two rows a thread
+    const int lp = tid & 7, r0 = tid >> 3;
     uint4 code[2][2], rope[2];
     uint16_t scale[2][2];
     bool have[2];
+    auto load_rows = [&](int tile) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int l = u0 + r0 + 64 * i, pos = l < u.sinks ? l : u.lo + l - u.sinks;
-        const int64_t row = l < u.tokens ? pool_row(p, p.tables + b * p.tables_stride, pos, u.end) : -1;
-        have[i] = row >= 0;
-        if (l < u.tokens && row < 0 && lp == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
-        rope[i] = code[i][0] = code[i][1] = make_uint4(0, 0, 0, 0);
-        scale[i][0] = scale[i][1] = 0;
-        if (have[i]) {
-            const uint8_t* src = p.pool + row * kRowBytes;
+        for (int i = 0; i < 2; ++i) {
+            const int l = kFewTokens * tile + r0 + 64 * i, pos = l < u.sinks ? l : u.lo + l - u.sinks;
+            const int64_t row = l < u.tokens ? pool_row(p, p.tables + b * p.tables_stride, pos, u.end) : -1;
+            have[i] = row >= 0;
+            if (l < u.tokens && row < 0 && lp == 0) set_error(p.err, NVFP4KV_DEVERR_BAD_PAGE);
+            rope[i] = code[i][0] = code[i][1] = make_uint4(0, 0, 0, 0);
+            scale[i][0] = scale[i][1] = 0;
+            if (have[i]) {
+                const uint8_t* src = p.pool + row * kRowBytes;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                code[i][h] = ldg_nc_v4(src + 128 * h + 16 * lp);
-                scale[i][h] = __ldg(reinterpret_cast<const uint16_t*>(src + 256 + 16 * h + 2 * lp));
+                for (int h = 0; h < 2; ++h) {
+                    code[i][h] = ldg_nc_v4(src + 128 * h + 16 * lp);
+                    scale[i][h] = __ldg(reinterpret_cast<const uint16_t*>(src + 256 + 16 * h + 2 * lp));
+                }
+                if (p.rope) rope[i] = ldg_nc_v4(p.rope + row * kRope + 8 * lp);
             }
-            if (p.rope) rope[i] = ldg_nc_v4(p.rope + row * kRope + 8 * lp);
         }
-    }
+    };
+    load_rows(tile0);
     if (tid < 8) bits[tid] = 0;
     if (tid == 32) {
         flags[1] = 0;
         mbar_init(bar, 1);
         mbar_init(bar + 8, 1);
+        mbar_init(bar + 16, 1);
         mbar_fence_init();
     }
     if (warp == 2) {
@@ -1532,116 +1543,157 @@ __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __
         tmem_relinquish();
     }
     __syncthreads();
-    store_q(p, smem + SF_Q, reinterpret_cast<float*>(smem + SF_QS), warp, kFewThreads / 32, q);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = r0 + 64 * i;
-        uint8_t* dst = smem + SF_KV + r * 128 + ((lp ^ (r & 7)) << 4);
-        bool nan = false;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t word[4] = {code[i][h].x, code[i][h].y, code[i][h].z, code[i][h].w};
-            const uint32_t s2 = e4m3x2_to_f16x2(scale[i][h]);
-#pragma unroll
-            for (int a = 0; a < 4; ++a) {
-                const bool bad = ((scale[i][h] >> (a & 2 ? 8 : 0)) & 0x7F) == 0x7F;
-                nan |= bad;
-                const uint4 v = dequant8(word[a], __byte_perm(s2, s2, a & 2 ? 0x3232 : 0x1010));
-                *reinterpret_cast<uint4*>(dst + (4 * h + a) * (kFewTokens * 128)) = bad ? make_uint4(0, 0, 0, 0) : v;
-            }
-        }
-        if (p.rope) *reinterpret_cast<uint4*>(dst + 8 * (kFewTokens * 128)) = rope[i];
-        if (nan) atomicOr(&bits[4 + (r >> 5)], 1u << (r & 31));
-        if (lp == 0 && have[i]) atomicOr(&bits[r >> 5], 1u << (r & 31));
-    }
-    fence_proxy_async_smem();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
     const uint32_t tmem = static_cast<uint32_t>(flags[0]);
-    if (warp == 2) {
-        if (elect_one()) {
-            const uint64_t dq = smem_desc_sw128(sbase + SF_Q, 16, 1024), dk = smem_desc_sw128(sbase + SF_KV, 16, 1024);
-            const int atoms = p.rope ? 9 : 8;
-            for (int j = 0; j < atoms; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    tc_mma_f16(tmem, dq + ((j * kCtaRows * 128) >> 4) + 2 * i, dk + ((j * kFewTokens * 128) >> 4) + 2 * i,
-                               j == 8 ? kIdescFewRope : kIdescFewQk, j > 0 || i > 0);
-            tc_commit(bar);
-        }
-        __syncwarp();
-    }
-    mbar_wait(bar, 0, abort_flag, p.err);
-    tc_fence_after();
+    store_q(p, smem + SF_Q, reinterpret_cast<float*>(smem + SF_QS), warp, kFewThreads / 32, q);
     // softmax: eight warps, 32 rows x 32 tokens each (a row's quarters in warps 4 apart)
     const int sp = warp & 3, cg = warp >> 2, row = 32 * (sp & 1) + lane;
     const uint32_t lanes = static_cast<uint32_t>(32 * (sp & 1)) << 16;
+    // O: a dim of 64 rows a thread (warp: lanes 32 sp .. of block cg)
+    const int c = 128 * cg + 32 * sp + lane;
+    const uint32_t o_addr = tmem + kTFewO + kCtaRows * cg + (static_cast<uint32_t>(32 * sp) << 16);
     float* red = reinterpret_cast<float*>(smem + SF_RED);
-    float m_ref = -INFINITY;
-    if (sp < 2) {
-        int lim = 0;
-        if (row < u.rows) lim = min(seq.L, seq.L - seq.n + token_of(p, kCtaRows * k + row) + 1);
-        const float factor = reinterpret_cast<const float*>(smem + SF_QS)[row];
-        float x[32];
-        tmem_ld32(tmem + 32 * cg + lanes, reinterpret_cast<uint32_t*>(x));
-        tmem_wait_ld();
-        // local tokens l < sinks lie at l, the others at l + off
-        const int l0 = u0 + 32 * cg, off = l0 + u.lo - u.sinks;
-        const uint32_t first = bits_below(u.sinks - l0);
-        const uint32_t see = bits[cg] & ((first & bits_below(lim - l0)) |
-                                         (~first & bits_below(lim - off) & (~bits_below(lim - p.window - off) | bits_below(p.sinks - off))));
-        const uint32_t nan = bits[4 + cg];
-        float m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            if ((nan >> i) & 1u) x[i] = __int_as_float(0x7FFFFFFF);
-            if (!((see >> i) & 1u)) x[i] = -INFINITY;
-            m = fmaxf(m, x[i]);
-        }
-        red[64 * cg + row] = factor * m;
-        named_bar_sync(1, 256);
-        m = fmaxf(fmaxf(red[row], red[64 + row]), fmaxf(red[128 + row], red[192 + row]));
-        if (m > -INFINITY) m_ref = m - kTopLog2;
-        const float base = m_ref == -INFINITY ? 0.0f : m_ref;
-        uint32_t pk[16];
-        float l = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float a = ex2_approx(fmaf(x[2 * i], factor, -base)), c = ex2_approx(fmaf(x[2 * i + 1], factor, -base));
-            l += a + c;
-            pk[i] = pack_half2(a, c);
-        }
-        red[256 + 64 * cg + row] = l;
-        uint8_t* dst = smem + SF_Q + (cg >> 1) * (kCtaRows * 128) + row * 128;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint4*>(dst + (((4 * (cg & 1) + c) ^ (row & 7)) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
-        fence_proxy_async_smem();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const bool any_tokens = u.tokens > u0;
-    if (warp == 2) {
-        if (elect_one()) {
-            const uint64_t dp = smem_desc_sw128(sbase + SF_Q, 16, 1024);
-            const int steps = (min(kFewTokens, u.tokens - u0) + 15) / 16;
+    float* alphas = reinterpret_cast<float*>(smem + SF_ALPHA);
+    int lim = 0;
+    if (row < u.rows) lim = min(seq.L, seq.L - seq.n + token_of(p, kCtaRows * k + row) + 1);
+    float factor = 1.0f, m_ref = -INFINITY, l = 0.0f;
+    const bool any_tokens = u.tokens > 0;      // (without, one tile of nothing, and no PV)
 #pragma unroll 1
-            for (int m = 0; m < 4; ++m) {
-                const uint64_t dv = smem_desc_sw128(sbase + SF_KV + 2 * m * (kFewTokens * 128), kFewTokens * 128, 1024);
-                for (int i = 0; i < steps; ++i)
-                    tc_mma_f16(tmem + kTFewO + kCtaRows * m, dv + 128 * i, dp + (((i >> 2) * kCtaRows * 128) >> 4) + 2 * (i & 3), kIdescFewPv, i > 0);
+    for (int tile = tile0; tile < tile1; ++tile) {
+        const int u0 = kFewTokens * tile;
+        const uint32_t phase = (tile - tile0) & 1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = r0 + 64 * i;
+            uint8_t* dst = smem + SF_KV + r * 128 + ((lp ^ (r & 7)) << 4);
+            bool nan = false;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t word[4] = {code[i][h].x, code[i][h].y, code[i][h].z, code[i][h].w};
+                const uint32_t s2 = e4m3x2_to_f16x2(scale[i][h]);
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const bool bad = ((scale[i][h] >> (a & 2 ? 8 : 0)) & 0x7F) == 0x7F;
+                    nan |= bad;
+                    const uint4 v = dequant8(word[a], __byte_perm(s2, s2, a & 2 ? 0x3232 : 0x1010));
+                    *reinterpret_cast<uint4*>(dst + (4 * h + a) * (kFewTokens * 128)) = bad ? make_uint4(0, 0, 0, 0) : v;
+                }
             }
-            tc_commit(bar + 8);
+            if (p.rope) *reinterpret_cast<uint4*>(dst + 8 * (kFewTokens * 128)) = rope[i];
+            if (nan) atomicOr(&bits[4 + (r >> 5)], 1u << (r & 31));
+            if (lp == 0 && have[i]) atomicOr(&bits[r >> 5], 1u << (r & 31));
         }
-        __syncwarp();
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        if (warp == 2) {
+            if (elect_one()) {
+                const uint64_t dq = smem_desc_sw128(sbase + SF_Q, 16, 1024), dk = smem_desc_sw128(sbase + SF_KV, 16, 1024);
+                const int atoms = p.rope ? 9 : 8;
+                for (int j = 0; j < atoms; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        tc_mma_f16(tmem, dq + ((j * kCtaRows * 128) >> 4) + 2 * i, dk + ((j * kFewTokens * 128) >> 4) + 2 * i,
+                                   j == 8 ? kIdescFewRope : kIdescFewQk, j > 0 || i > 0);
+                tc_commit(bar);
+            }
+            __syncwarp();
+        }
+        if (tile + 1 < tile1) load_rows(tile + 1);
+        mbar_wait(bar, phase, abort_flag, p.err);
+        tc_fence_after();
+        float alpha = 1.0f;
+        if (sp < 2) {
+            if (tile == tile0) factor = reinterpret_cast<const float*>(smem + SF_QS)[row];
+            float x[32];
+            tmem_ld32(tmem + 32 * cg + lanes, reinterpret_cast<uint32_t*>(x));
+            tmem_wait_ld();
+            // local tokens before `sinks` lie at their own positions, the others `off` further
+            const int l0 = u0 + 32 * cg, off = l0 + u.lo - u.sinks;
+            const uint32_t first = bits_below(u.sinks - l0);
+            const uint32_t see = bits[cg] & ((first & bits_below(lim - l0)) |
+                                             (~first & bits_below(lim - off) & (~bits_below(lim - p.window - off) | bits_below(p.sinks - off))));
+            const uint32_t nan = bits[4 + cg];
+            float m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                if ((nan >> i) & 1u) x[i] = __int_as_float(0x7FFFFFFF);
+                if (!((see >> i) & 1u)) x[i] = -INFINITY;
+                m = fmaxf(m, x[i]);
+            }
+            red[64 * cg + row] = factor * m;
+            named_bar_sync(1, 256);
+            m = fmaxf(fmaxf(red[row], red[64 + row]), fmaxf(red[128 + row], red[192 + row]));
+            // (as in the kernel above: the reference moves when a tile passes it by 2^8)
+            if (m - m_ref > kRescaleLog2 + kTopLog2) {
+                const float next = m - kTopLog2;
+                alpha = m_ref == -INFINITY ? 0.0f : ex2_approx(m_ref - next);
+                l *= alpha;
+                m_ref = next;
+            }
+            const float base = m_ref == -INFINITY ? 0.0f : m_ref;
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float a = ex2_approx(fmaf(x[2 * i], factor, -base)), b2 = ex2_approx(fmaf(x[2 * i + 1], factor, -base));
+                l += a + b2;
+                pk[i] = pack_half2(a, b2);
+            }
+            uint8_t* dst = smem + SF_P + (cg >> 1) * (kCtaRows * 128) + row * 128;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint4*>(dst + (((4 * (cg & 1) + i) ^ (row & 7)) << 4)) = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+            if (cg == 0) alphas[row] = alpha;
+            fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        const bool moved = __syncthreads_or(tile > tile0 && alpha != 1.0f);
+        tc_fence_after();
+        if (tid < 8) bits[tid] = 0;       // (read by all; the next tile's are set behind a barrier)
+        if (moved) {                      // (the PV before is complete: the tile's latents came after it)
+#pragma unroll 1
+            for (int g = 0; g < kCtaRows; g += 16) {
+                uint32_t o[16];
+                tmem_ld16(o_addr + g, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alphas[g + i]);
+                tmem_st16(o_addr + g, o);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncthreads();
+            tc_fence_after();
+        }
+        if (!any_tokens) break;
+        if (warp == 2) {
+            if (elect_one()) {
+                const uint64_t dp = smem_desc_sw128(sbase + SF_P, 16, 1024);
+                const int steps = (min(kFewTokens, u.tokens - u0) + 15) / 16;
+#pragma unroll 1
+                for (int m = 0; m < 4; ++m) {
+                    const uint64_t dv = smem_desc_sw128(sbase + SF_KV + 2 * m * (kFewTokens * 128), kFewTokens * 128, 1024);
+                    for (int i = 0; i < steps; ++i)
+                        tc_mma_f16(tmem + kTFewO + kCtaRows * m, dv + 128 * i, dp + (((i >> 2) * kCtaRows * 128) >> 4) + 2 * (i & 3), kIdescFewPv,
+                                   tile > tile0 || i > 0);
+                }
+                tc_commit(bar + 8);
+            }
+            __syncwarp();
+        }
+        if (tile + 1 < tile1) {
+            mbar_wait(bar + 8, phase, abort_flag, p.err);
+            tc_fence_after();
+            __syncthreads();              // (the bits are clear)
+        }
     }
+    if (sp < 2) red[256 + 64 * cg + row] = l;
+    __syncthreads();
     const bool whole = u.parts == 1;
     const int64_t slot = static_cast<int64_t>(unit) * few_parts + part;
     float* mul = reinterpret_cast<float*>(smem + SF_QS);
     if (sp < 2 && cg == 0) {
-        const float l = (red[256 + row] + red[320 + row]) + (red[384 + row] + red[448 + row]);
+        l = (red[256 + row] + red[320 + row]) + (red[384 + row] + red[448 + row]);
         const bool any = l > 0.0f || l != l;
         mul[row] = any ? p.out_scale / l : 0.0f;
         if (row < u.rows) {
@@ -1650,12 +1702,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __
                 p.lse[static_cast<int64_t>(seq.first) * p.heads + kCtaRows * k + row] = any ? 0.69314718055994531f * (m_ref + log2f(l)) : -INFINITY;
         }
     }
-    if (any_tokens) mbar_wait(bar + 8, 0, abort_flag, p.err);
+    if (any_tokens) mbar_wait(bar + 8, (tile1 - 1 - tile0) & 1, abort_flag, p.err);
     tc_fence_after();
     __syncthreads();
-    // a thread's dim of 64 rows (warp: lanes 32 (warp % 4) .. of block warp / 4)
-    const int c = 128 * cg + 32 * sp + lane;
-    const uint32_t o_addr = tmem + kTFewO + kCtaRows * cg + (static_cast<uint32_t>(32 * sp) << 16);
     if (!whole) {
         float* dst = p.part_o + (slot * (kCtaRows / kFewGroup) * kLatent + c) * kFewGroup;
 #pragma unroll
@@ -1687,9 +1736,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __
         }
     }
     tc_fence_before();
-    if (*abort_flag && warp == 2) {      // after a timed-out wait the products in flight end before their memory goes
-        mbar_drain_wait(bar, 0);
-        if (any_tokens) mbar_drain_wait(bar + 8, 0);
+    if (warp == 2) {      // (after a timed-out wait products may be in flight: they end before their memory goes)
+        if (elect_one()) tc_commit(bar + 16);
+        __syncwarp();
+        mbar_drain_wait(bar + 16, 0);
     }
     __syncthreads();
     if (warp == 2) tmem_dealloc(tmem, kTmemCols);
@@ -1707,7 +1757,7 @@ __global__ void __launch_bounds__(kLatent) mla_window_few_combine_kernel(const _
     const Seq seq = load_seq(p, b);
     const int grow0 = kCtaRows * k + kFewGroup * group;
     if (grow0 >= seq.rows) return;
-    const FewUnit u = few_unit(p, seq, k);
+    const FewUnit u = few_unit(p, seq, k, few_parts);
     if (u.parts == 1) return;
     const int64_t slot0 = static_cast<int64_t>(unit) * few_parts;
     griddep_wait();
@@ -1773,6 +1823,8 @@ struct PrefillPlan {
 // Images take at most this, or one sequence's; a larger batch runs in groups of sequences.
 constexpr size_t kImageCap = size_t(1) << 30;
 
+constexpr int64_t kFewWaves = 3;
+
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
 PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_len, int max_seq_len, int window, int sinks) {
@@ -1783,18 +1835,19 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
         // a unit's rows belong to at most `span` tokens, and see no more than the sinks and the window - 1 +
         // span last tokens up to its end, which is rounded up to a multiple of 64
         const int64_t by_rows = (num_heads + kUnitRows - 2) / num_heads + 1, span = by_rows < longest ? by_rows : longest;
-        // The kernels for few rows, where their CTAs run at the same time.  In one wave they take 23.5 us for 16
-        // single tokens of 64 heads with a window of 1,024 (the others 29.4), 17.9 for 2 x 32 tokens with 128 (27.3);
-        // with 192 CTAs 32.8 against 27.3, with 576 75.9 against 63.8.
+        // The kernels for few rows: where no sequence has more than one unit of 64, or there are no more than
+        // kFewWaves tiles an SM.  As many parts as there are SMs for.
         const int64_t rows = longest * num_heads, few_units = (rows + kCtaRows - 1) / kCtaRows;
         const int64_t of_64 = (num_heads + kCtaRows - 2) / num_heads + 1, few_span = of_64 < longest ? of_64 : longest;
         int64_t seen = static_cast<int64_t>(sinks) + window - 1 + few_span;
         seen = seen < max_seq_len ? seen : max_seq_len;
-        const int64_t few_parts = seen > kFewTokens ? (seen + kFewTokens - 1) / kFewTokens : 1;
-        if (few_parts <= kFewMaxParts && few_units * few_parts * batch <= device_sm_count()) {
+        const int64_t few_tiles = seen > kFewTokens ? (seen + kFewTokens - 1) / kFewTokens : 1, all_units = batch * few_units;
+        if (few_units == 1 || (few_units > 1 && all_units * few_tiles <= kFewWaves * device_sm_count())) {
+            int64_t parts = all_units > 0 ? device_sm_count() / all_units : 1;
+            parts = parts < 1 ? 1 : parts > kFewMaxParts ? kFewMaxParts : parts;
+            pl.few_parts = static_cast<int>(parts < few_tiles ? parts : few_tiles);
             pl.few_units = static_cast<int>(few_units);
-            pl.few_parts = static_cast<int>(few_parts);
-            const size_t slots = few_parts > 1 ? static_cast<size_t>(batch) * few_units * few_parts : 0;
+            const size_t slots = pl.few_parts > 1 ? static_cast<size_t>(all_units) * pl.few_parts : 0;
             pl.group = batch;
             pl.o_bytes = slots * kCtaRows * kLatent * sizeof(float);
             pl.ml_bytes = round256(slots * kCtaRows * 2 * sizeof(float));
@@ -1807,7 +1860,7 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
         image_rows = kTile * most + longest < image_rows ? kTile * most + longest : image_rows;
     }
     pl.max_tiles = static_cast<int>(tiles);
-    pl.form = window <= 0 ? kAll : longest * num_heads > kUnitRows ? kDirect : kWindowed;
+    pl.form = window > 0 ? kDirect : kAll;
     const size_t block_bytes = static_cast<size_t>(pl.form == kDirect ? 17 : 9) * kStageBytes;
     const int64_t one = (image_rows + kImageTok - 1) / kImageTok;
     const int64_t cap = static_cast<int64_t>(kImageCap / block_bytes);
@@ -1954,7 +2007,7 @@ int prefill_call(const void* q, int64_t q_stride_t, int64_t q_stride_h, const ui
     p.factor = p.scale_log2 == 0.0f ? 1.0f : fabsf(p.scale_log2);
     if (pl.few_units > 0) return launch_few(p, pl, st);
     if (pl.form == kDirect) return launch_prefill<kDirect>(p, pl, st);
-    return pl.form == kWindowed ? launch_prefill<kWindowed>(p, pl, st) : launch_prefill<kAll>(p, pl, st);
+    return launch_prefill<kAll>(p, pl, st);
 }
 
 // A window that hides nothing is none; otherwise it and the sinks lie within max_seq_len.

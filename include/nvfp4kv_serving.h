@@ -1,7 +1,8 @@
 /*
- * nvfp4kv_serving -- C ABI of the serving operators around the NVFP4 paged cache: rotary
- * positions, rotated keys into the rope side-pool, attention of a ragged chunk of new tokens
- * over the paged pool, and the upkeep of the cache's pages.  Same library (libnvfp4kv.so),
+ * nvfp4kv_serving -- C ABI of the serving operators around the NVFP4 paged cache: the tables of a
+ * step, rotary positions on one axis or several, rotated keys into the rope side-pool, attention
+ * of a ragged chunk of new tokens over the paged pool, whole or in a window, and the upkeep of the
+ * cache's pages.  Same library (libnvfp4kv.so),
  * conventions, return codes and device error bits as nvfp4kv.h.  The reference has none of
  * these: its model is NoPE and vLLM schedules its prefill and its pages.
  */

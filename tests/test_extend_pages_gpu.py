@@ -156,6 +156,21 @@ def test_a_step_matches_the_model(page, lens, new, pages, pad):
     assert rt.device_errors() == 0 and not dev[2].any() and bool((dev[0] == -1).all())
 
 
+@pytest.mark.parametrize("n", [1000, 2500])
+def test_many_requests_and_slots(n):
+    """More slots, and more requests, than the chip's own memory holds, some of them twice."""
+    m = Model(5000, 4, 16, 8000, seed=n)
+    order = torch.randperm(5000, generator=m.g)[:n].tolist()
+    order[7], order[n - 1] = order[3], order[400]
+    new = torch.randint(0, 40, (n,), generator=m.g).tolist()
+    dev = m.cuda()
+    step(m, dev, order, new, None, sum(new))
+    assert m.error == _lib.DEVERR_BAD_SLOT
+    back = [a - a // 3 for a in new]
+    step(m, dev, order, [1] * n, back, n)
+    assert m.error == _lib.DEVERR_BAD_SLOT
+
+
 def test_every_request_that_is_skipped():
     m = Model(12, 8, 16, 40, seed=2)
     for s, n in enumerate([20, 33, 16, 0, 40, 100, 5, 50]):
