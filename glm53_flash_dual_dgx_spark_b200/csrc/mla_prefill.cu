@@ -1435,8 +1435,10 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_const
 // window of 1,024 (144 CTAs, a tile each), 4,600 until Q and the pool's rows are asked for, 4,800 for them
 // to come and be converted, 2,700 for QK, 3,300 for the softmax, 2,000 for PV and 4,600 for the parts (19
 // MB) into L2.  With O = P V and 64 rows on M, the upper half of PV was wasted and half of the warps held
-// no row of O: 28.3 us a call, now 23.5 (the second kernel's look at the lengths before it waits, and eight
-// parts in flight, are 1.1 of that).  The pool's rows of a tile are asked for under the tile before.
+// no row of O: 28.3 us a call, now 23.7 (the second kernel's look at the lengths before it waits, and eight
+// parts in flight, are 1.1 of that).  The pool's rows of a tile are asked for under the tile before; a
+// further tile takes 10,300 cycles (2,200 dequantising, 2,800 QK, 2,500 softmax, whose rows lie in the
+// lanes of half of the warps, 2,100 PV).
 constexpr int kFewTokens = 128, kFewThreads = 512, kFewMaxParts = 64;
 constexpr int SF_Q = 0;                                       // 9 dim atoms x [64 rows x 128 B]
 constexpr int SF_KV = SF_Q + 9 * kCtaRows * 128;              // 9 dim atoms x [128 tokens x 128 B]
@@ -1614,13 +1616,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __
             const uint32_t see = bits[cg] & ((first & bits_below(lim - l0)) |
                                              (~first & bits_below(lim - off) & (~bits_below(lim - p.window - off) | bits_below(p.sinks - off))));
             const uint32_t nan = bits[4 + cg];
-            float m = -INFINITY;
+            if (!__all_sync(0xFFFFFFFFu, see == 0xFFFFFFFFu && nan == 0)) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                if ((nan >> i) & 1u) x[i] = __int_as_float(0x7FFFFFFF);
-                if (!((see >> i) & 1u)) x[i] = -INFINITY;
-                m = fmaxf(m, x[i]);
+                for (int i = 0; i < 32; ++i) {
+                    if ((nan >> i) & 1u) x[i] = __int_as_float(0x7FFFFFFF);
+                    if (!((see >> i) & 1u)) x[i] = -INFINITY;
+                }
             }
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx[i & 1] = max3(mx[i & 1], x[2 * i], x[2 * i + 1]);
+            float m = fmaxf(mx[0], mx[1]);
             red[64 * cg + row] = factor * m;
             named_bar_sync(1, 256);
             m = fmaxf(fmaxf(red[row], red[64 + row]), fmaxf(red[128 + row], red[192 + row]));
@@ -1633,12 +1639,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __
             }
             const float base = m_ref == -INFINITY ? 0.0f : m_ref;
             uint32_t pk[16];
+            float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+            const float2 factor2 = make_float2(factor, factor), base2 = make_float2(-base, -base);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float a = ex2_approx(fmaf(x[2 * i], factor, -base)), b2 = ex2_approx(fmaf(x[2 * i + 1], factor, -base));
-                l += a + b2;
-                pk[i] = pack_half2(a, b2);
+                const float2 e = fma2(make_float2(x[2 * i], x[2 * i + 1]), factor2, base2);
+                const float2 w = make_float2(ex2_approx(e.x), ex2_approx(e.y));
+                sum[i & 1] = add2(sum[i & 1], w);
+                pk[i] = pack_half2(w.x, w.y);
             }
+            sum[0] = add2(sum[0], sum[1]);
+            l += sum[0].x + sum[0].y;
             uint8_t* dst = smem + SF_P + (cg >> 1) * (kCtaRows * 128) + row * 128;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -1823,7 +1834,7 @@ struct PrefillPlan {
 // Images take at most this, or one sequence's; a larger batch runs in groups of sequences.
 constexpr size_t kImageCap = size_t(1) << 30;
 
-constexpr int64_t kFewWaves = 3;
+constexpr int64_t kFewWaves = 2;
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
@@ -1835,8 +1846,11 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
         // a unit's rows belong to at most `span` tokens, and see no more than the sinks and the window - 1 +
         // span last tokens up to its end, which is rounded up to a multiple of 64
         const int64_t by_rows = (num_heads + kUnitRows - 2) / num_heads + 1, span = by_rows < longest ? by_rows : longest;
-        // The kernels for few rows: where no sequence has more than one unit of 64, or there are no more than
-        // kFewWaves tiles an SM.  As many parts as there are SMs for.
+        // The kernels for few rows: where no sequence has more than one unit of 64 (64 single tokens of 64 heads
+        // with a window of 1,024 take 44.3 us there and 63.4 with an image, 16 of them 23.7 and 29.3, 256 121 and
+        // 223), or there are no more than kFewWaves tiles an SM (4 x 8 tokens of 16 heads, 512: 17.9 us against 22.0; 8 x 16 of
+        // 32, 256, 192 tiles: 23.4 and 27.5; 4 x 16 of 64, 512, 320 tiles: 31.2 and 28.4).  As many parts as there
+        // are SMs for.
         const int64_t rows = longest * num_heads, few_units = (rows + kCtaRows - 1) / kCtaRows;
         const int64_t of_64 = (num_heads + kCtaRows - 2) / num_heads + 1, few_span = of_64 < longest ? of_64 : longest;
         int64_t seen = static_cast<int64_t>(sinks) + window - 1 + few_span;

@@ -91,6 +91,30 @@ CASES = [
 ]
 
 
+# calls of more than two 128-token tiles of 64 rows an SM: the chunk kernel's own form
+LARGE = [
+    ([400], [1500], 64, 64, True, 1, 0), ([300], [700], 64, 16, True, 64, 64), ([129], [1000], 128, 64, True, 65, 63),
+    ([700], [777], 20, 64, False, 128, 4), ([100, 100, 100], [255, 256, 257], 64, 64, True, 128, 1), ([260], [1500], 128, 16, True, 255, 65),
+    ([300], [1300], 64, 256, True, 256, 0), ([300, 1, 70], [777, 64, 300], 64, 64, True, 200, 129), ([1100], [3000], 20, 64, True, 257, 200),
+    ([2900], [3000], 1, 64, True, 700, 300), ([640], [640], 64, 16, True, 17, 5), ([500], [500], 64, 64, True, 499, 0),
+    ([600, 300], [400, 0], 64, 16, True, 200, 100), ([70, 0, 233, 1], [70, 50, 520, 0], 65, 16, True, 40, 7), ([200], [9000], 64, 64, True, 4096, 4),
+    ([129, 3, 1, 77] * 3, [5000, 3, 900, 300] * 3, 32, 1, True, 1000, 128),
+]
+
+
+@pytest.mark.parametrize("new,ctx,H,page,rope,window,sinks", LARGE)
+def test_large_calls_match_the_formula(new, ctx, H, page, rope, window, sinks):
+    span = min(max(new), (H + 62) // H + 1)
+    tiles = -(-min(sinks + window - 1 + span, max(ctx)) // 128)
+    assert len(new) * -(-max(new) * H // 64) * tiles > 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    p = Windowed(new, ctx, H, page, rope, window, sinks, trim=True, seed=sum(new))
+    out, lse = p.run()
+    assert rt.device_errors() == 0
+    p.check(out, lse)
+    again = p.run()
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
 @pytest.mark.parametrize("trim", [False, True])
 @pytest.mark.parametrize("new,ctx,H,page,rope,window,sinks", CASES)
 def test_window_matches_the_formula(new, ctx, H, page, rope, window, sinks, trim):
@@ -107,10 +131,11 @@ def test_a_window_that_hides_nothing_gives_the_same_bits():
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
-def test_missing_pages_in_and_behind_the_window():
-    p = Windowed([5, 3], [900, 600], 16, 16, True, 100, 20, seed=4)
-    # sequence 0: sinks on pages 0 and 1, windows from token 796 on (page 49)
-    p.tables[0, 2:49] = -1
+@pytest.mark.parametrize("n,H", [(5, 16), (90, 128)])
+def test_missing_pages_in_and_behind_the_window(n, H):
+    p = Windowed([n, 3], [900, 600], H, 16, True, 100, 20, seed=4)
+    # sequence 0: sinks on pages 0 and 1, windows from token 801 - n on
+    p.tables[0, 2:(801 - n) // 16] = -1
     out, lse = p.run()
     assert rt.device_errors() == 0
     p.check(out, lse)
@@ -123,9 +148,10 @@ def test_missing_pages_in_and_behind_the_window():
         p.tables = keep
 
 
-def test_hidden_bytes_do_not_reach_a_row():
+@pytest.mark.parametrize("H", [16, 128])
+def test_hidden_bytes_do_not_reach_a_row(H):
     """NaN latents and rope rows in every token that no row sees, and one that only some rows see."""
-    p = Windowed([70, 1], [900, 2000], 16, 64, True, 150, 5, seed=10)
+    p = Windowed([70, 1], [900, 2000], H, 64, True, 150, 5, seed=10)
     raw, rope = p.pool.view(-1, 288), p.rope.view(-1, 64)
     live = torch.zeros(raw.shape[0], dtype=torch.bool)
     for b, (n, c) in enumerate(zip(p.new, p.ctx)):
@@ -138,32 +164,34 @@ def test_hidden_bytes_do_not_reach_a_row():
     p.check(out, lse)
 
 
+@pytest.mark.parametrize("n,H", [(33, 16), (150, 64)])
 @pytest.mark.parametrize("gain,scale", [(8.0, 1.0 / 24.0), (1.0, -0.06), (1.0, 0.0), (64.0, 0.02)])
-def test_scales_and_peaked_rows(gain, scale):
-    p = Windowed([33, 2], [900, 600], 16, 64, True, 300, 10, seed=6, q_gain=gain)
+def test_scales_and_peaked_rows(gain, scale, n, H):
+    p = Windowed([n, 2], [900, 600], H, 64, True, 300, 10, seed=6, q_gain=gain)
     p.scale = scale
     out, lse = p.run(bmm2_scale=0.5)
     p.check(out, lse, out_scale=0.5)
 
 
 def test_a_batch_whose_images_do_not_fit_runs_in_groups():
-    """The images' bound is 1 GiB: 1,200 sequences of 1,000 tokens' windows take several passes."""
-    n = 1200
-    p = Windowed([1] * n, [900 + (7 * i) % 600 for i in range(n)], 2, 64, False, 500, 4, seed=18)
+    """The images' bound is 1 GiB: 400 sequences' windows of 1,000 tokens, 3 MB each, take two passes."""
+    n = 400
+    p = Windowed([2] * n, [1100 + (7 * i) % 400 for i in range(n)], 64, 64, False, 1000, 4, seed=18)
     out, lse = p.run()
     assert rt.device_errors() == 0
     p.check(out, lse)
 
 
-def test_clamped_lengths_and_padding_rows():
+@pytest.mark.parametrize("H", [12, 600])
+def test_clamped_lengths_and_padding_rows(H):
     """Sequences past the bounds end there, flagged; rows of no sequence stay as they were."""
-    p = Windowed([20, 13], [400, 377], 12, 16, True, 60, 4, seed=12)
+    p = Windowed([20, 13], [400, 377], H, 16, True, 60, 4, seed=12)
     out, lse = p.run()
     p.check(out, lse)
     cu = torch.tensor([0, 20, 33], dtype=torch.int32, device="cuda")
     seq = torch.tensor([400, 377], dtype=torch.int32, device="cuda")
     q = torch.cat([p.q, p.q[:5]])
-    full = torch.full((38, 12, 512), 7.0, dtype=torch.bfloat16, device="cuda")
+    full = torch.full((38, H, 512), 7.0, dtype=torch.bfloat16, device="cuda")
     rt.mla_prefill(q, p.pool, None, 512, 64, p.tables.cuda(), cu, seq, 20, 400, out=full, bmm1_scale=p.scale, rope_cache=p.rope,
                    window=60, sinks=4)
     assert rt.device_errors() == 0
@@ -173,8 +201,14 @@ def test_clamped_lengths_and_padding_rows():
     rt.mla_prefill(q, p.pool, None, 512, 64, p.tables.cuda(), cu, seq, 13, 400, out=full, bmm1_scale=p.scale, rope_cache=p.rope,
                    window=60, sinks=4)
     assert rt.device_errors() == _lib.DEVERR_SEQ_LEN
-    assert bool(((full[:13].float() - out[:13].float()).abs() <= 2.0 ** -7 * out[:13].float().abs() + 2.0 ** -9).all())
     assert bool((full[13:20] == 7.0).all()) and bool((full[33:] == 7.0).all())
+    p.check(torch.cat([full[:13], out[13:20], full[20:33]]), lse)
+    # none of them, and none at all
+    full.fill_(7.0)
+    rt.mla_prefill(q, p.pool, None, 512, 64, p.tables.cuda(), cu, seq, 0, 400, out=full, bmm1_scale=p.scale, window=60)
+    assert rt.device_errors() == _lib.DEVERR_SEQ_LEN and bool((full == 7.0).all())
+    rt.mla_prefill(q, p.pool, None, 512, 64, p.tables.cuda(), cu * 0, seq, 20, 400, out=full, bmm1_scale=p.scale, window=60)
+    assert rt.device_errors() == 0 and bool((full == 7.0).all())
 
 
 def test_chunks_and_one_pass_agree():
@@ -200,14 +234,15 @@ def test_chunks_and_one_pass_agree():
     assert rt.device_errors() == 0
 
 
-def test_a_graph_follows_the_lengths_on_the_device():
-    p = Windowed([4, 6], [900, 1200], 32, 64, True, 300, 10, seed=5)
+@pytest.mark.parametrize("H", [32, 128])
+def test_a_graph_follows_the_lengths_on_the_device(H):
+    p = Windowed([4, 6], [900, 1200], H, 64, True, 300 if H == 32 else 1100, 10, seed=5)
     cu = torch.tensor([0, 4, 10], dtype=torch.int32, device="cuda")
     seq = torch.tensor([900, 1200], dtype=torch.int32, device="cuda")
     tables = p.tables.cuda()
-    out = torch.empty(10, 32, 512, dtype=torch.bfloat16, device="cuda")
+    out = torch.empty(10, H, 512, dtype=torch.bfloat16, device="cuda")
     call = lambda: rt.mla_prefill(p.q, p.pool, None, 512, 64, tables, cu, seq, 8, 1216, out=out, bmm1_scale=p.scale,  # noqa: E731
-                                  rope_cache=p.rope, window=300, sinks=10)
+                                  rope_cache=p.rope, window=p.W, sinks=10)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
