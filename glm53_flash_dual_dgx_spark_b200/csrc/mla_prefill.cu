@@ -3,6 +3,10 @@
 //   x[r, t] = bmm1_scale (q[r, :512] . k[t] + q[r, 512:] . k_rope[t]),  t <= L - n + i(r)
 //   out[r] = bmm2_scale sum_t softmax(x[r])_t k[t],   lse[r] = log sum_t exp(x[r, t])
 //
+// With a window W and sinks S only t > p - W or t < S counts, p = L - n + i(r).  What follows is the form
+// without; the windowed one (kDirect) differs in the tiles of a unit (unit_gap), the image, Q and how
+// the MMA warp learns of the next part, and calls of few rows have kernels of their own at the end.
+//
 // Rows r = (new token i, head) of one sequence share the latent rows k, which are both keys and
 // values, so the kernel is two chained matrix products over 128 rows: S = Q K^T (512 or 576 deep)
 // and O = P K (512 wide), about 2.2 kFLOP per row and token, on the tensor cores.
