@@ -1495,8 +1495,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __
     volatile int* abort_flag = flags + 1;
     uint32_t* bits = reinterpret_cast<uint32_t*>(smem + SF_BITS);
     const uint32_t bar = sbase + SF_BARS;
+    griddep_wait();                   // first: the kernel that starts now reads the lengths at once
     griddep_launch_dependents();
-    griddep_wait();
     const Seq seq = load_seq(p, b);
     if (kCtaRows * k >= seq.rows) return;
     const FewUnit u = few_unit(p, seq, k, few_parts);
@@ -1877,6 +1877,7 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
         tiles = most < tiles ? most : tiles;
         image_rows = kTile * most + longest < image_rows ? kTile * most + longest : image_rows;
     }
+    tiles = tiles < 0x7FFFFFFF / kTile ? tiles : 0x7FFFFFFF / kTile;      // (their tokens are an int on the device)
     pl.max_tiles = static_cast<int>(tiles);
     pl.form = window > 0 ? kDirect : kAll;
     const size_t block_bytes = static_cast<size_t>(pl.form == kDirect ? 17 : 9) * kStageBytes;

@@ -84,6 +84,43 @@ def test_trimmed_sequences_give_what_whole_ones_give(page, H, window, sinks):
     assert live <= sum(-(-(min(n, window + 5) + sinks) // page) + 2 for n in (363, 380, 206))
 
 
+@pytest.mark.parametrize("H,window", [(64, 900), (64, 100), (128, 900)])
+def test_attention_right_behind_the_tables(H, window):
+    """Steps whose lengths change by hundreds of tokens, nothing between their tables and the attention, and
+    nothing waited for: each as with a wait."""
+    g = torch.Generator(device="cuda").manual_seed(H + window)
+    B, page, pages = 4, 64, 80
+    latent = torch.zeros(pages, page, 288, dtype=torch.uint8, device="cuda")
+    rt.write_nvfp4(torch.randn(pages * page, 512, generator=g, device="cuda").to(torch.bfloat16), latent, torch.arange(pages * page, device="cuda"))
+    q = torch.randn(2 * B, H, 576, generator=g, device="cuda").to(torch.bfloat16)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    slots = ints([0, 1, 2, 3])
+    rows = [(ints([1 + (i + k) % 2 for k in range(B)]), ints([(37 * i + 311 * k) % 1100 for k in range(B)])) for i in range(24)]
+
+    def run(wait):
+        tables, lens, refs = torch.full((B, 18), -1, dtype=torch.int32, device="cuda"), ints([0] * B), ints([0] * pages)
+        rt.extend_pages(tables, lens, slots, ints([1140] * B), refs, page, 4 * 1140)
+        start, outs = [t.clone() for t in (tables, lens, refs)], []
+        torch.cuda.synchronize()
+        for new, keep in rows:
+            for t, t0 in zip((tables, lens, refs), start):
+                t.copy_(t0)
+            e = rt.extend_pages(tables, lens, slots, new, refs, page, 2 * B, lens=keep)
+            if wait:
+                torch.cuda.synchronize()
+            outs.append(rt.mla_prefill(q, latent, None, 512, 64, e.block_tables, e.cu_seqlens_q, e.seq_lens, 2, 1152,
+                                       bmm1_scale=1 / 24, return_lse=True, window=window, sinks=3))
+            if wait:
+                torch.cuda.synchronize()
+        return outs
+
+    want, got = run(True), run(False)
+    assert rt.device_errors() == 0
+    for i, ((a, al), (b, bl)) in enumerate(zip(want, got)):
+        n = int(rows[i][0].sum())
+        assert torch.equal(a[:n], b[:n]) and torch.equal(al[:n], bl[:n])
+
+
 def test_a_step_in_one_graph():
     """extend, rotate and write, attend, trim, captured once and replayed as the sequences grow."""
     page, H, window, sinks, T = 16, 16, 40, 5, 12
