@@ -1852,15 +1852,15 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
         const int64_t by_rows = (num_heads + kUnitRows - 2) / num_heads + 1, span = by_rows < longest ? by_rows : longest;
         // The kernels for few rows: where no sequence has more than one unit of 64 (64 single tokens of 64 heads
         // with a window of 1,024 take 44.3 us there and 63.4 with an image, 16 of them 23.7 and 29.3, 256 121 and
-        // 223), or there are no more than kFewWaves tiles an SM (4 x 8 tokens of 16 heads, 512: 17.9 us against 22.0; 8 x 16 of
-        // 32, 256, 192 tiles: 23.4 and 27.5; 4 x 16 of 64, 512, 320 tiles: 31.2 and 28.4).  As many parts as there
-        // are SMs for.
+        // 313; with one of 16,384 a token takes 40 us either way and 16 of them 103 and 187), or there are no more
+        // than kFewWaves tiles an SM (4 x 8 tokens of 16 heads, 512: 17.9 us against 22.0; 8 x 16 of 32, 256, 192
+        // tiles: 23.4 and 27.5; 4 x 16 of 64, 512, 320 tiles: 31.2 and 28.4).  As many parts as there are SMs for.
         const int64_t rows = longest * num_heads, few_units = (rows + kCtaRows - 1) / kCtaRows;
         const int64_t of_64 = (num_heads + kCtaRows - 2) / num_heads + 1, few_span = of_64 < longest ? of_64 : longest;
         int64_t seen = static_cast<int64_t>(sinks) + window - 1 + few_span;
         seen = seen < max_seq_len ? seen : max_seq_len;
         const int64_t few_tiles = seen > kFewTokens ? (seen + kFewTokens - 1) / kFewTokens : 1, all_units = batch * few_units;
-        if (few_units == 1 || (few_units > 1 && all_units * few_tiles <= kFewWaves * device_sm_count())) {
+        if (few_units == 1 || (few_units > 1 && all_units <= kFewWaves * device_sm_count() / few_tiles)) {
             int64_t parts = all_units > 0 ? device_sm_count() / all_units : 1;
             parts = parts < 1 ? 1 : parts > kFewMaxParts ? kFewMaxParts : parts;
             pl.few_parts = static_cast<int>(parts < few_tiles ? parts : few_tiles);
@@ -2029,9 +2029,13 @@ int prefill_call(const void* q, int64_t q_stride_t, int64_t q_stride_h, const ui
     return launch_prefill<kAll>(p, pl, st);
 }
 
-// A window that hides nothing is none; otherwise it and the sinks lie within max_seq_len.
+// A window that hides nothing is none; otherwise it and the sinks lie within max_seq_len.  (2^30 rows are more
+// than a GPU's memory holds, so a longer window hides no more, and positions less a window stay an int.)
+constexpr int kMaxWindow = 1 << 30;
 int check_window(const char* what, int max_seq_len, int* window, int* sinks) {
     if (*window < 1 || *sinks < 0) return fail(NVFP4KV_EINVAL, "%s: window must be >= 1 and sinks >= 0", what);
+    *window = *window < kMaxWindow ? *window : kMaxWindow;
+    *sinks = *sinks < kMaxWindow ? *sinks : kMaxWindow;
     if (max_seq_len >= 0 && static_cast<int64_t>(*window) + *sinks >= max_seq_len) *window = *sinks = 0;
     return NVFP4KV_OK;
 }

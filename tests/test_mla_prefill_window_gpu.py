@@ -131,6 +131,20 @@ def test_a_window_that_hides_nothing_gives_the_same_bits():
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+def test_the_longest_windows_and_sinks():
+    """Positions before a sequence's start (length 5 with 60 new tokens) less a window of nearly 2^31."""
+    most = 2 ** 31 - 1
+    for window, sinks in ((most - 50, 0), (most - 50, 20), (1, most - 50), (700, most - 800)):
+        p = Windowed([60, 3], [5, 900], 1, 1024, True, window, sinks, seed=6)
+        tables = torch.full((2, 1 << 21), -1, dtype=torch.int32, device="cuda")
+        tables[:, : p.tables.shape[1]] = p.tables
+        cu = torch.tensor([0, 60, 63], dtype=torch.int32, device="cuda")
+        out, lse = rt.mla_prefill(p.q, p.pool, None, 512, 64, tables, cu, torch.tensor(p.ctx, dtype=torch.int32, device="cuda"),
+                                  60, most, bmm1_scale=p.scale, rope_cache=p.rope, return_lse=True, window=window, sinks=sinks)
+        assert rt.device_errors() == 0
+        p.check(out, lse)
+
+
 @pytest.mark.parametrize("n,H", [(5, 16), (90, 128)])
 def test_missing_pages_in_and_behind_the_window(n, H):
     p = Windowed([n, 3], [900, 600], H, 16, True, 100, 20, seed=4)
