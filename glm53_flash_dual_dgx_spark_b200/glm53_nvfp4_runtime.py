@@ -879,7 +879,7 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
             _require_on(query.get_device(), t, name)
     if isinstance(bmm1_scale, torch.Tensor) or isinstance(bmm2_scale, torch.Tensor):
         raise TypeError("bmm1_scale / bmm2_scale must be Python floats (a device scalar would need a sync)")
-    if window < 0 or sinks < 0 or (sinks and not window):
+    if (window or sinks) and (window <= 0 or sinks < 0):
         raise ValueError("window and sinks must be >= 0, and sinks need a window")
     qs = query.stride()
     if query.dtype is not torch.bfloat16 or len(qs) != 3 or qs[2] != 1:
@@ -938,10 +938,17 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
         if ws is None or ws.get_device() != index or not ws.is_contiguous() or ws.data_ptr() % 256 \
                 or ws.numel() * ws.element_size() < need:
             ws = _stream_buffer(index, "prefill_ws", need, torch.uint8)
-        _call("nvfp4kv_mla_prefill_window" if window else "nvfp4kv_mla_prefill", index, query.data_ptr(), qs[0], qs[1],
-              kv_cache.data_ptr(), rows, rope, block_tables.data_ptr(), ts[0], cu.data_ptr(), sl.data_ptr(), B, T, H, D,
-              kv_lora_rank, page_size, int(max_q_len), int(max_seq_len), *((window, sinks) if window else ()), bmm1_scale,
-              bmm2_scale, out.data_ptr(), os[0], os[1], None if lse is None else lse.data_ptr(), ws.data_ptr(), need)
+        lse_ptr = None if lse is None else lse.data_ptr()
+        if window:
+            _call("nvfp4kv_mla_prefill_window", index, query.data_ptr(), qs[0], qs[1], kv_cache.data_ptr(), rows, rope,
+                  block_tables.data_ptr(), ts[0], cu.data_ptr(), sl.data_ptr(), B, T, H, D, kv_lora_rank, page_size,
+                  int(max_q_len), int(max_seq_len), window, sinks, bmm1_scale, bmm2_scale, out.data_ptr(), os[0], os[1],
+                  lse_ptr, ws.data_ptr(), need)
+        else:
+            _call("nvfp4kv_mla_prefill", index, query.data_ptr(), qs[0], qs[1], kv_cache.data_ptr(), rows, rope,
+                  block_tables.data_ptr(), ts[0], cu.data_ptr(), sl.data_ptr(), B, T, H, D, kv_lora_rank, page_size,
+                  int(max_q_len), int(max_seq_len), bmm1_scale, bmm2_scale, out.data_ptr(), os[0], os[1], lse_ptr,
+                  ws.data_ptr(), need)
     return (out, lse) if return_lse else out
 
 
