@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -110,6 +111,8 @@ SERVING_SIGNATURES = {
     "nvfp4kv_trim_pages": (_I, [_P, _I64, _I, _I64, _P, _P, _I, _I, _I, _I, _P, _I64, _P, _P]),
     "nvfp4kv_compact_pages": (_I, [_P, _P, _I, _P, _I64, _I, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _P]),
     "nvfp4kv_compact_workspace_ints": (_I, [_I64, ctypes.POINTER(_I64)]),
+    "nvfp4kv_packed_entry": (_I, [ctypes.c_char_p, ctypes.POINTER(_I), ctypes.POINTER(_I)]),
+    "nvfp4kv_call_packed": (_I, [_I, _I, ctypes.c_char_p]),
 }
 
 
@@ -143,3 +146,12 @@ def check(rc: int, what: str) -> None:
     if rc != OK:
         msg = lib().nvfp4kv_last_error()
         raise Nvfp4kvError(f"{what} failed ({rc}): {msg.decode() if msg else ''}")
+
+
+def packed(name: str):
+    """(number, arguments, the function that packs them) of a serving entry for nvfp4kv_call_packed."""
+    entry, num = ctypes.c_int(0), ctypes.c_int(0)
+    check(lib().nvfp4kv_packed_entry(name.encode(), ctypes.byref(entry), ctypes.byref(num)), name)
+    form = "".join("d" if t is _F else "q" for t in SERVING_SIGNATURES[name][1])
+    assert len(form) == num.value, name
+    return entry.value, num.value, struct.Struct("=" + form).pack

@@ -21,7 +21,7 @@ LIB = os.path.join(HERE, "libnvfp4kv.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 SOURCES = ["abi_common.cu", "nvfp4_append.cu", "nvfp4_gather.cu", "nvfp4_rope.cu", "nvfp4_indexer.cu", "nvfp4_mla_decode.cu",
-           "nvfp4_mla_decode_fp4.cu", "nvfp4_mla_decode_static.cu", "rotary.cu", "cache_pages.cu", "mla_prefill.cu"]
+           "nvfp4_mla_decode_fp4.cu", "nvfp4_mla_decode_static.cu", "rotary.cu", "cache_pages.cu", "mla_prefill.cu", "packed_calls.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
               "-I", INCLUDE]

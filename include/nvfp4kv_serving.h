@@ -233,6 +233,13 @@ int nvfp4kv_compact_pages(const void* const* caches, const int64_t* page_bytes, 
 /* int32 workspace size of nvfp4kv_compact_pages. */
 int nvfp4kv_compact_workspace_ints(int64_t num_pages, int64_t* ints);
 
+/* An entry above that takes a stream, by its number, with its arguments in `args`, 8 bytes each and in
+ * order: int64 for numbers, pointers and streams, double for floats.  For callers whose foreign calls
+ * convert one argument at a time.  nvfp4kv_packed_entry gives an entry's number and how many
+ * arguments it has; they do not change while the library is loaded. */
+int nvfp4kv_packed_entry(const char* name, int* entry, int* num_args);
+int nvfp4kv_call_packed(int entry, int num_args, const void* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -136,3 +136,60 @@ def test_cpu_tensors_are_refused():
         rt.extend_pages(i(0).view(1, 1), i(0), i(0), i(1), i(0), 16, 1)
     with pytest.raises(ValueError, match="CUDA"):
         rt.trim_pages(i(0).view(1, 1), i(0), i(0), i(0), 16)
+
+
+# ------------------------------------------------------------------ packed calls
+def packed_refused(name, args):
+    number, num, pack = _lib.packed(name)
+    words = [0 if a is None else ctypes.addressof(a) if isinstance(a, ctypes.Array) else a for a in args]
+    lib = _lib.lib()
+    return lib.nvfp4kv_call_packed(number, num, pack(*words)), lib.nvfp4kv_last_error().decode()
+
+
+def test_every_entry_with_a_stream_has_a_packed_form():
+    numbers = set()
+    for name, (_, types) in _lib.SERVING_SIGNATURES.items():
+        if "_workspace_" in name or "packed" in name:
+            with pytest.raises(_lib.Nvfp4kvError, match="no entry"):
+                _lib.packed(name)
+        else:
+            number, num, _ = _lib.packed(name)
+            assert num == len(types)
+            numbers.add(number)
+    assert numbers == set(range(len(numbers)))
+
+
+@pytest.mark.parametrize("name,case,change", [
+    ("nvfp4kv_rope_axes", ROPE, dict(A=2)), ("nvfp4kv_rope_axes", ROPE, dict(D=600, r=258, off=0)), ("nvfp4kv_rope_axes", ROPE, dict(T=0)),
+    ("nvfp4kv_rope_axes", ROPE, dict(T=-1)), ("nvfp4kv_append_rope_rotated_axes", WRITE, dict(qo=32, qoh=32)),
+    ("nvfp4kv_append_rope_rotated_axes", WRITE, dict(T=0)), ("nvfp4kv_mla_prefill_window", PREFILL, dict(rows=100)),
+    ("nvfp4kv_mla_prefill_window", PREFILL, dict(rows=(1 << 40) + 1)), ("nvfp4kv_mla_prefill_window", PREFILL, dict(T=0)),
+    ("nvfp4kv_extend_pages", EXTEND, dict(ws=None)), ("nvfp4kv_trim_pages", TRIM, dict(width=9)), ("nvfp4kv_trim_pages", TRIM, dict(num=0)),
+])
+def test_a_packed_call_is_the_call(name, case, change):
+    args = list((case | change).values())
+    want = refused(name, *args)
+    got = packed_refused(name, args)
+    assert got[0] == want[0] and (got[0] == _lib.OK or got == want)
+
+
+def test_packed_calls_refuse():
+    lib = _lib.lib()
+    number, num, pack = _lib.packed("nvfp4kv_trim_pages")
+    for change in (dict(num=1 << 31), dict(win=-(1 << 31) - 1), dict(page=1 << 40)):      # (a foreign call would cut them off)
+        rc, msg = packed_refused("nvfp4kv_trim_pages", (TRIM | change).values())
+        assert rc == _lib.EINVAL and "does not fit" in msg and str(list(TRIM).index(next(iter(change)))) in msg
+    for entry, n, words in ((-1, num, b""), (1000, num, b""), (number, num - 1, b""), (number, num, None)):
+        assert lib.nvfp4kv_call_packed(entry, n, words) == _lib.EINVAL
+    out = ctypes.c_int(0)
+    assert lib.nvfp4kv_packed_entry(None, ctypes.byref(out), ctypes.byref(out)) == _lib.EINVAL
+    assert lib.nvfp4kv_packed_entry(b"nvfp4kv_append", ctypes.byref(out), ctypes.byref(out)) == _lib.EINVAL
+    assert lib.nvfp4kv_packed_entry(b"nvfp4kv_rope", None, ctypes.byref(out)) == _lib.EINVAL
+
+
+def test_an_argument_of_another_type_is_a_type_error(monkeypatch):
+    monkeypatch.setitem(rt._bufs, ("err", 0), torch.zeros(1, dtype=torch.int32))
+    monkeypatch.setattr(rt, "_raw_stream", lambda index: 0)
+    for bad in (1.5, None, "16", 1 << 70):
+        with pytest.raises(TypeError, match="nvfp4kv_trim_pages"):
+            rt._call("nvfp4kv_trim_pages", 0, *list((TRIM | dict(page=bad)).values())[:-2])
