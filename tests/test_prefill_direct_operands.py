@@ -1,7 +1,7 @@
 """CPU: the form of the chunk attention kernel whose Q warps copy Q straight into its operand and tell the
 MMA warp of the next part (queries of several units in a window), as the model of test_prefill_operands
-with those two roles as mla_prefill.cu has them there: a change of a wait, an arrival or a role has to be
-made here too.
+with those two roles, and the MMA warp's wait for the output of the part before, as mla_prefill.cu has
+them there: a change of a wait, an arrival or a role has to be made here too.
 
 The number of the next part's tiles goes through two words, written before the arrival that says its Q is
 there; 0 after the last part, once its last QK is done."""
@@ -35,6 +35,8 @@ class Direct(Model):
         j, n = 0, self.parts[0]
         while n > 0:
             for i in range(n + 1):
+                if i == 1 and j > 0:
+                    yield from self.wait("O_FREE", self.o_free, j - 1)
                 if i < n:
                     if tile >= 2:
                         yield from self.wait("S_FREE", self.s_free[tile & 1], (tile >> 1) - 1)
@@ -50,8 +52,6 @@ class Direct(Model):
                         self.pipe.append(("commit", both(self.q_free)))
                 if i > 0:
                     yield from self.wait("P_FULL", self.p_full, tile - 1)
-                    if i == 1 and j > 0:
-                        yield from self.wait("O_FREE", self.o_free, j - 1)
                     for k in range(V_STAGES):
                         yield from stage("pv", j, tile - 1, i == 1 and k == 0)
 
