@@ -26,16 +26,18 @@ template <typename T> struct Vec {
     static constexpr int kN = 16 / sizeof(T);
     T v[kN];
 };
-template <typename T> __device__ __forceinline__ Vec<T> load_vec(const T* p) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+template <typename T, bool kStream = false> __device__ __forceinline__ Vec<T> load_vec(const T* p) {
+    const uint4* src = reinterpret_cast<const uint4*>(p);
+    const uint4 u = kStream ? __ldcs(src) : *src;
     Vec<T> r;
     memcpy(&r, &u, 16);
     return r;
 }
-template <typename T> __device__ __forceinline__ void store_vec(T* p, const Vec<T>& r) {
+template <typename T, bool kStream = false> __device__ __forceinline__ void store_vec(T* p, const Vec<T>& r) {
     uint4 u;
     memcpy(&u, &r, 16);
-    *reinterpret_cast<uint4*>(p) = u;
+    if (kStream) __stcs(reinterpret_cast<uint4*>(p), u);
+    else *reinterpret_cast<uint4*>(p) = u;
 }
 
 __device__ __forceinline__ int64_t load_index(const void* p, bool i64, int64_t i) {
@@ -142,9 +144,11 @@ __device__ __forceinline__ uint32_t quotient(uint32_t n, const SmallDiv& v) { re
 // With several axes, a block gathers the cos | sin rows of its `num` tokens from t0 on in shared memory
 // once, so that its units read them as 16-byte vectors like a row of the table, whichever way the
 // axes are spread over the pairs (loaded pair by pair in every unit they took as many load slots as the
-// values themselves: 8,192 tokens x 32 heads x 128 bf16 42 us, now 28.3, with one axis 29.1).  It comes
-// before the units' own loads: behind them their addresses stay in registers, and fewer blocks fit
-// (31.6 us; the gradient of 2,049 x 20 x 192 fp32 13.1 us against 11.3).  rows [num][rotary], turns [num].
+// values themselves: 8,192 tokens x 32 heads x 128 bf16 42 us; now 21.9, as much as a plain copy).  It
+// comes before the units' own loads: behind them their addresses stay in registers, and fewer blocks fit
+// (31.6 us against 28.3 before the vectors were marked as streaming; with the vectors through shared
+// memory by asynchronous copies, asked for before the gathering, 34.5).  The schedulers issue in two of
+// three cycles, so the index arithmetic counts.  rows [num][rotary], turns [num].
 __device__ __forceinline__ void gather_rows(float* rows, uint8_t* turns, int num, int64_t t0, int64_t tokens, const void* positions,
                                             bool i64, const Axes& axes, const SmallDiv& half, const float* table, int64_t max_positions) {
     const int h = static_cast<int>(half.d);
@@ -156,9 +160,18 @@ __device__ __forceinline__ void gather_rows(float* rows, uint8_t* turns, int num
         const float* src = table + (pos >= 0 && pos < max_positions ? pos : 0) * (2 * h) + i;
         rows[2 * h * k + i] = __ldg(src);
         rows[2 * h * k + h + i] = __ldg(src + h);
-        if (i == 0) turns[k] = all_in_table(positions, i64, t, axes, max_positions);
     }
+    // (by the threads that have no pair, where there are some: in the loop above, by the first pair's lane, every
+    // warp waited for it; 65,536 tokens x 1 head x 128 bf16 took 32 us, so 24.4)
+    for (int k = blockDim.x - 1 - threadIdx.x; k < num && t0 + k < tokens; k += blockDim.x)
+        turns[k] = all_in_table(positions, i64, t0 + k, axes, max_positions);
     __syncthreads();
+}
+
+// The same for any dividend: the product's upper half is the quotient, or one more.
+__device__ __forceinline__ uint32_t any_quotient(uint32_t n, const SmallDiv& v) {
+    const uint32_t q = quotient(n, v);
+    return q - (static_cast<int>(n - q * v.d) < 0);
 }
 
 inline SmallDiv small_div(uint32_t d) { return {d, static_cast<uint32_t>(((1ull << 32) + d - 1) / d)}; }
@@ -184,17 +197,21 @@ constexpr int kRopeSteps = 2;
 // A unit is a 16-byte vector of a head (a rotated one of the half layout: the pair of vectors that
 // turn together).  The units of the call are dealt flat, two to a thread and 256 apart: every warp
 // moves 512 contiguous bytes, every block is full, and two loads in flight per thread are enough at
-// the occupancy that leaves (8,192 tokens x 64 heads x 576 bf16, 1.2 GB: 188 us = 6.4 TB/s, as much
+// the occupancy that leaves (8,192 tokens x 64 heads x 576 bf16, 1.2 GB: 181 us = 6.7 TB/s, as much
 // as a plain copy; 8 % more with one, 1 % more with four, 20 % more with blocks of whole heads, whose
-// last steps are part empty).  The gradient of 2,049 tokens x 32 heads x 128 fp32 takes 12 us.
+// last steps are part empty).  The gradient of 2,049 tokens x 32 heads x 128 fp32 takes 10 us.
+//
+// With several axes the vectors are marked as streaming: with new inputs each time, 8,192 tokens x 32
+// heads x 128 bf16 26.1 -> 24.4 us, the gradient of 2,049 x 20 x 192 fp32 14.9 -> 12.4 (marks on the
+// loads or the stores alone gain a tenth of that); six blocks fit in the half layout, 27.6 -> 26.1.
 template <typename T, bool kInterleaved, bool kAxes>
-__global__ void __launch_bounds__(256, kAxes ? (kInterleaved ? 7 : 5) : (kInterleaved && sizeof(T) == 2 ? 8 : 4)) rope_vec_kernel(const __grid_constant__ RopeArgs p) {
+__global__ void __launch_bounds__(256, kAxes ? (kInterleaved ? 8 : 6) : (kInterleaved && sizeof(T) == 2 ? 8 : 4)) rope_vec_kernel(const __grid_constant__ RopeArgs p) {
     constexpr int N = Vec<T>::kN;
     const int64_t u0 = static_cast<int64_t>(blockIdx.x) * (256 * kRopeSteps);
     int64_t row0, t0;       // the block's first head row, its token
     if (p.total < (1ll << 32)) {
-        row0 = static_cast<uint32_t>(u0) / p.units.d;
-        t0 = static_cast<uint32_t>(row0) / p.by_heads.d;
+        row0 = any_quotient(static_cast<uint32_t>(u0), p.units);
+        t0 = any_quotient(static_cast<uint32_t>(row0), p.by_heads);
     } else {
         row0 = u0 / p.units.d;
         t0 = row0 / p.by_heads.d;
@@ -221,8 +238,8 @@ __global__ void __launch_bounds__(256, kAxes ? (kInterleaved ? 7 : 5) : (kInterl
         at[k] = t[k] * p.o_st + h * p.o_sh + d;
         if (u0 + threadIdx.x + 256 * k < p.total) {
             const T* xp = static_cast<const T*>(p.x) + t[k] * p.x_st + h * p.x_sh + d;
-            a[k] = load_vec(xp);
-            if (!kInterleaved && r[k] >= 0) b[k] = load_vec(xp + half);
+            a[k] = load_vec<T, kAxes>(xp);
+            if (!kInterleaved && r[k] >= 0) b[k] = load_vec<T, kAxes>(xp + half);
         } else {
             r[k] = -2;
         }
@@ -242,10 +259,10 @@ __global__ void __launch_bounds__(256, kAxes ? (kInterleaved ? 7 : 5) : (kInterl
                 if (g.turn) a[k] = rotate_pairs<T, kAxes>(a[k], cs, half, sign);
             } else {
                 if (g.turn) rotate_halves<T, kAxes>(a[k], b[k], cs, half, sign);
-                store_vec(op + half, b[k]);
+                store_vec<T, kAxes>(op + half, b[k]);
             }
         }
-        store_vec(op, a[k]);
+        store_vec<T, kAxes>(op, a[k]);
     }
 }
 
@@ -354,7 +371,7 @@ struct RopeAppendArgs {
 // 8 bf16, as one 16-byte access or element by element.  The accesses are marked as streaming: a step's
 // rows pass once, while the table rows of its positions come back with every layer, and should stay
 // in L2 (32,768 tokens x 16 heads over a table of 77 MB: 28.0 us against 33.3 without the marks, and
-// 29.8 with the next blocks' table rows prefetched instead).
+// 29.8 with the next blocks' table rows prefetched instead; with the units below 25.2).
 template <bool kVec> __device__ __forceinline__ Vec<__nv_bfloat16> get8(const __nv_bfloat16* p) {
     if constexpr (kVec) {
         const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
@@ -379,16 +396,18 @@ template <bool kVec> __device__ __forceinline__ void put8(__nv_bfloat16* p, cons
     }
 }
 
-// The units (8 dims of a row, half layout: 8 and their partners) of all rows, dealt flat as in
-// rope_vec_kernel, two a thread (37.7 us with one, 42 with four, before the streaming marks); a
-// token's rows are its key and the heads of its query.  What bounds it is the latency of a block's
-// three dependent accesses (position, table row, store) at full occupancy, then HBM.
+// The units (8 dims of a row and the 8 that lie 32 further) of all rows, dealt flat as in
+// rope_vec_kernel, one a thread, in the half layout two (with several axes 31 us against 37 with one;
+// interleaved, two units of 8 dims instead of one of 16 cost the index arithmetic twice, 33.8 against
+// 32.2); a token's rows are its key and the heads of its query.  What bounds it is the issue of the
+// index arithmetic and the latency of a block's dependent accesses (position, table row, store) at full
+// occupancy, then HBM.
 template <bool kInterleaved, bool kVec, bool kAxes>
 __device__ __forceinline__ void rope_append_rotated(const RopeAppendArgs& p) {
     using V = Vec<__nv_bfloat16>;
-    constexpr int kU = kInterleaved ? 8 : 4, kSteps = kAppendSteps, kRows = 256 / kU;      // rows of a block and step
+    constexpr int kU = 4, kSteps = kInterleaved ? 1 : kAppendSteps, kRows = 256 / kU;      // rows of a block and step
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kRows * kSteps);
-    const int64_t t0 = row0 < (1ll << 32) ? static_cast<int64_t>(static_cast<uint32_t>(row0) / p.rows_of_token.d) : row0 / p.rows_of_token.d;
+    const int64_t t0 = row0 < (1ll << 32) ? static_cast<int64_t>(any_quotient(static_cast<uint32_t>(row0), p.rows_of_token)) : row0 / p.rows_of_token.d;
     const uint32_t first = static_cast<uint32_t>(row0 - t0 * p.rows_of_token.d);
     const int u = threadIdx.x % kU;
     griddep_wait();
@@ -408,7 +427,7 @@ __device__ __forceinline__ void rope_append_rotated(const RopeAppendArgs& p) {
         if (t[k] >= p.tokens) continue;
         const __nv_bfloat16* src = h[k] < 0 ? p.k + t[k] * p.k_st : p.q + t[k] * p.q_st + h[k] * p.q_sh;
         a[k] = get8<kVec>(src + 8 * u);
-        if (!kInterleaved) b[k] = get8<kVec>(src + 32 + 8 * u);
+        b[k] = get8<kVec>(src + 32 + 8 * u);
     }
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
@@ -429,12 +448,15 @@ __device__ __forceinline__ void rope_append_rotated(const RopeAppendArgs& p) {
         } else {
             dst = p.qo + t[k] * p.qo_st + h[k] * p.qo_sh;
         }
-        if (kInterleaved) {
-            if (g.turn) a[k] = rotate_pairs<__nv_bfloat16, kAxes>(a[k], g.row + 4 * u, 32, 1.0f);
-        } else {
-            if (g.turn) rotate_halves<__nv_bfloat16, kAxes>(a[k], b[k], g.row + 8 * u, 32, 1.0f);
-            put8<kVec>(dst + 32 + 8 * u, b[k]);
+        if (g.turn) {
+            if (kInterleaved) {
+                a[k] = rotate_pairs<__nv_bfloat16, kAxes>(a[k], g.row + 4 * u, 32, 1.0f);
+                b[k] = rotate_pairs<__nv_bfloat16, kAxes>(b[k], g.row + 16 + 4 * u, 32, 1.0f);
+            } else {
+                rotate_halves<__nv_bfloat16, kAxes>(a[k], b[k], g.row + 8 * u, 32, 1.0f);
+            }
         }
+        put8<kVec>(dst + 32 + 8 * u, b[k]);
         put8<kVec>(dst + 8 * u, a[k]);
     }
 }
@@ -444,9 +466,10 @@ __global__ void __launch_bounds__(256) rope_append_rotated_kernel(const __grid_c
     rope_append_rotated<kInterleaved, kVec, false>(p);
 }
 // (more blocks on an SM hide the gathering: 43 us with the angles loaded pair by pair, 36 gathered
-// beside the rows' loads with 5 blocks, 31.6 gathered before them with 8, the table's own rows 26)
+// beside the rows' loads with 5 blocks, 31.6 gathered before them with 8, now 27.7; one axis, which reads
+// the table's own rows, 25)
 template <bool kInterleaved, bool kVec>
-__global__ void __launch_bounds__(256, kInterleaved && kVec ? 8 : kVec ? 5 : 4) rope_append_axes_kernel(const __grid_constant__ RopeAppendArgs p) {
+__global__ void __launch_bounds__(256, kInterleaved && kVec ? 8 : kVec ? 6 : 4) rope_append_axes_kernel(const __grid_constant__ RopeAppendArgs p) {
     rope_append_rotated<kInterleaved, kVec, true>(p);
 }
 
