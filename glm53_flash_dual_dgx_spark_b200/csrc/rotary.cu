@@ -346,7 +346,7 @@ int launch_rope(RopeArgs a, int64_t tokens, bool interleaved, cudaStream_t st) {
     return check_launch("nvfp4kv_rope");
 }
 
-constexpr int kAppendSteps = 2;
+constexpr int kAppendRows = 64, kHalfSteps = 2;      // rows of a block and step (four threads a row); steps in the half layout
 
 struct RopeAppendArgs {
     const __nv_bfloat16* k;
@@ -405,7 +405,7 @@ template <bool kVec> __device__ __forceinline__ void put8(__nv_bfloat16* p, cons
 template <bool kInterleaved, bool kVec, bool kAxes>
 __device__ __forceinline__ void rope_append_rotated(const RopeAppendArgs& p) {
     using V = Vec<__nv_bfloat16>;
-    constexpr int kU = 4, kSteps = kInterleaved ? 1 : kAppendSteps, kRows = 256 / kU;      // rows of a block and step
+    constexpr int kRows = kAppendRows, kU = 256 / kRows, kSteps = kInterleaved ? 1 : kHalfSteps;
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kRows * kSteps);
     const int64_t t0 = row0 < (1ll << 32) ? static_cast<int64_t>(any_quotient(static_cast<uint32_t>(row0), p.rows_of_token)) : row0 / p.rows_of_token.d;
     const uint32_t first = static_cast<uint32_t>(row0 - t0 * p.rows_of_token.d);
@@ -582,7 +582,7 @@ int append_rotated_call(const char* what, const void* k_pe, int64_t num_tokens, 
                                 (q_stride_t | q_stride_h | qo_stride_t | qo_stride_h) % 8 == 0));
     const uint32_t per_token = a.heads + 1;
     a.rows_of_token = small_div(per_token);
-    const int64_t per_block = kAppendSteps * 256 / (interleaved ? 8 : 4), blocks = (num_tokens * per_token + per_block - 1) / per_block;
+    const int64_t per_block = kAppendRows * (interleaved ? 1 : kHalfSteps), blocks = (num_tokens * per_token + per_block - 1) / per_block;
     if (blocks > 0x7FFFFFFF) return fail(NVFP4KV_EINVAL, "%s: too many rows for one call", what);
     const dim3 grid(static_cast<unsigned>(blocks));
     size_t smem = 0;
