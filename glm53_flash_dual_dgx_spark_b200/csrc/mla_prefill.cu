@@ -1775,11 +1775,12 @@ __global__ void __launch_bounds__(kLatent) mla_window_few_combine_kernel(const _
     // (the lengths were there before the kernel before this one)
     const Seq seq = load_seq(p, b);
     const int grow0 = kCtaRows * k + kFewGroup * group;
-    if (grow0 >= seq.rows) return;
-    const FewUnit u = few_unit(p, seq, k, few_parts);
+    FewUnit u;
+    u.parts = 1;
+    if (grow0 < seq.rows) u = few_unit(p, seq, k, few_parts);
+    griddep_wait();                   // whatever there is to merge: this grid ends after the one before it
     if (u.parts == 1) return;
     const int64_t slot0 = static_cast<int64_t>(unit) * few_parts;
-    griddep_wait();
     if (warp < kFewGroup) {
         const bool real = grow0 + warp < seq.rows;
         float2 ml[kFewMaxParts / 32];

@@ -280,6 +280,23 @@ def test_a_graph_follows_the_lengths_on_the_device(H):
     assert rt.device_errors() == 0
 
 
+def test_what_follows_a_call_without_parts_reads_its_output():
+    """Tables wide enough for several parts of a unit, sequences short enough for one: nothing is merged,
+    and the next kernels still find the output."""
+    p = Windowed([1] * 8, [100, 1, 128, 77, 5, 120, 64, 90], 64, 64, True, 1000, 4, seed=21)
+    cu = torch.arange(9, dtype=torch.int32, device="cuda")
+    seq = torch.tensor(p.ctx, dtype=torch.int32, device="cuda")
+    tables = torch.nn.functional.pad(p.tables.cuda(), (0, 64), value=-1)
+    first = None
+    for _ in range(200):
+        out = torch.full((8, 64, 512), 7.0, dtype=torch.bfloat16, device="cuda")
+        rt.mla_prefill(p.q, p.pool, None, 512, 64, tables, cu, seq, 1, 4096, out=out, bmm1_scale=p.scale, rope_cache=p.rope, window=1000, sinks=4)
+        after = out.clone()
+        first = after if first is None else first
+        assert torch.equal(after, first)
+    p.check(first, p.run()[1])
+
+
 def test_long_context():
     """A window at the end of 300,000 tokens whose other pages are gone."""
     p = Windowed([3], [1000], 16, 64, True, 600, 20, seed=21)
