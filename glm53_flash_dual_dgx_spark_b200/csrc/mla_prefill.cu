@@ -1499,12 +1499,31 @@ __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __
     volatile int* abort_flag = flags + 1;
     uint32_t* bits = reinterpret_cast<uint32_t*>(smem + SF_BITS);
     const uint32_t bar = sbase + SF_BARS;
+    // (what needs no input comes before the wait: 0.5 us of 16)
+    if (tid < 8) bits[tid] = 0;
+    if (tid == 32) {
+        flags[1] = 0;
+        mbar_init(bar, 1);
+        mbar_init(bar + 8, 1);
+        mbar_init(bar + 16, 1);
+        mbar_fence_init();
+    }
+    if (warp == 2) {
+        tmem_alloc(sbase + SF_FLAGS, kTmemCols);
+        tmem_relinquish();
+    }
+    __syncthreads();
+    const uint32_t tmem = static_cast<uint32_t>(flags[0]);
     griddep_wait();                   // first: the kernel that starts now reads the lengths at once
     griddep_launch_dependents();
     const Seq seq = load_seq(p, b);
-    if (kCtaRows * k >= seq.rows) return;
-    const FewUnit u = few_unit(p, seq, k, few_parts);
-    if (part >= u.parts) return;
+    FewUnit u;
+    u.parts = 0;
+    if (kCtaRows * k < seq.rows) u = few_unit(p, seq, k, few_parts);
+    if (part >= u.parts) {
+        if (warp == 2) tmem_dealloc(tmem, kTmemCols);
+        return;
+    }
     const int tile0 = part * u.tiles / u.parts, tile1 = (part + 1) * u.tiles / u.parts;
     // Q on its way
     Part t;
@@ -1540,20 +1559,6 @@ __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __
         }
     };
     load_rows(tile0);
-    if (tid < 8) bits[tid] = 0;
-    if (tid == 32) {
-        flags[1] = 0;
-        mbar_init(bar, 1);
-        mbar_init(bar + 8, 1);
-        mbar_init(bar + 16, 1);
-        mbar_fence_init();
-    }
-    if (warp == 2) {
-        tmem_alloc(sbase + SF_FLAGS, kTmemCols);
-        tmem_relinquish();
-    }
-    __syncthreads();
-    const uint32_t tmem = static_cast<uint32_t>(flags[0]);
     store_q(p, smem + SF_Q, reinterpret_cast<float*>(smem + SF_QS), warp, kFewThreads / 32, q);
     // softmax: eight warps, 32 rows x 32 tokens each (a row's quarters in warps 4 apart)
     const int sp = warp & 3, cg = warp >> 2, row = 32 * (sp & 1) + lane;
@@ -1772,6 +1777,7 @@ __global__ void __launch_bounds__(kLatent) mla_window_few_combine_kernel(const _
     constexpr int kGroups = kCtaRows / kFewGroup;
     const int unit = blockIdx.x / kGroups, group = blockIdx.x % kGroups, k = unit % few_units, b = unit / few_units;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    griddep_launch_dependents();
     // (the lengths were there before the kernel before this one)
     const Seq seq = load_seq(p, b);
     const int grow0 = kCtaRows * k + kFewGroup * group;
