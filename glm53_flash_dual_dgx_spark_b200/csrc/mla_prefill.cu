@@ -1437,13 +1437,14 @@ __global__ void __launch_bounds__(128) prefill_combine_kernel(const __grid_const
 // and a range of the tokens that any of them sees, 128 at a time, from the pool's rows to its part of the
 // output: latents and Q to shared memory as fp16, S = Q K^T with M = 128 (its upper half is whatever lies
 // behind the rows, and not read), and O^T += V^T P^T, 128 dims at a time, whose 64 columns are the rows:
-// the same tile is B of the first product and A of the second.  Parts of a unit meet in a second kernel.
+// the same tile is B of the first product and A of the second.  Parts of a unit meet in a second kernel,
+// or in the cluster that they are (few_joined).
 //
 // What bounds it is the latency of that chain: of 22,600 cycles for 16 single tokens of 64 heads with a
 // window of 1,024 (144 CTAs, a tile each), 4,600 until Q and the pool's rows are asked for, 4,800 for them
 // to come and be converted, 2,700 for QK, 3,300 for the softmax, 2,000 for PV and 4,600 for the parts (19
 // MB) into L2.  With O = P V and 64 rows on M, the upper half of PV was wasted and half of the warps held
-// no row of O: 28.3 us a call, now 23.7 (the second kernel's look at the lengths before it waits, and eight
+// no row of O: 28.3 us a call, now 23.3 (the second kernel's look at the lengths before it waits, and eight
 // parts in flight, are 1.1 of that).  The pool's rows of a tile are asked for under the tile before; a
 // further tile takes 10,300 cycles (2,200 dequantising, 2,800 QK, 2,500 softmax, whose rows lie in the
 // lanes of half of the warps, 2,100 PV).
@@ -1487,8 +1488,17 @@ __device__ __forceinline__ FewUnit few_unit(const PrefillParams& p, const Seq& s
     return u;
 }
 
+constexpr int kFewJoined = 8;                                 // parts of a unit whose CTAs are a cluster, at most
+constexpr int kFewPieces = 8;                                 // a CTA's share of the merge: eight rows of another's part each
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(addr));
+}
+
 // Block x = part + few_parts (unit + few_units sequence).  Part s of a unit, when there are several, goes
 // to part_o [unit][few_parts][8 groups of rows][512 (as few_dim)][8 rows] and part_ml [unit][few_parts][64][2].
+// kJoined: the parts of a unit are a cluster, and each merges its share of the unit's rows.
+template <bool kJoined>
 __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __grid_constant__ PrefillParams p, int few_units, int few_parts) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -1729,6 +1739,95 @@ __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __
     if (any_tokens) mbar_wait(bar + 8, (tile1 - 1 - tile0) & 1, abort_flag, p.err);
     tc_fence_after();
     __syncthreads();
+    // kJoined: CTA `part` merges row groups part, part + parts ...: its own share of them is still in tensor
+    // memory, the others' are asked for, up to eight pieces at a time, before the weights are known.
+    auto join_parts = [&] {
+        const int parts = u.parts, others = parts - 1, groups = (u.rows + kFewGroup - 1) / kFewGroup;
+        const int mine = groups > part ? (groups - part + parts - 1) / parts : 0, pieces = mine * others;
+        const int64_t slot0 = static_cast<int64_t>(unit) * few_parts;
+        float* wts = reinterpret_cast<float*>(smem + SF_Q);      // [row][part]
+        float* invs = wts + kCtaRows * kFewJoined;
+        __nv_bfloat16* rows = reinterpret_cast<__nv_bfloat16*>(smem + SF_KV);
+        float4 v[kFewPieces][2];
+        int at_g = 0, at_s = 0;         // of the next piece
+        auto ask = [&](int first) {
+#pragma unroll
+            for (int j = 0; j < kFewPieces; ++j) {
+                if (first + j < pieces) {
+                    const int s = at_s + (at_s >= part);
+                    const float4* src = reinterpret_cast<const float4*>(
+                        p.part_o + (((slot0 + s) * (kCtaRows / kFewGroup) + part + at_g * parts) * kLatent + c) * kFewGroup);
+                    v[j][0] = __ldcg(src);
+                    v[j][1] = __ldcg(src + 1);
+                }
+                if (++at_s == others) {
+                    at_s = 0;
+                    ++at_g;
+                }
+            }
+        };
+        ask(0);
+        {      // weights of all rows: eight parts of four rows a warp
+            const int r = 4 * warp + (lane >> 3), s = lane & 7;
+            const bool real = r < u.rows;
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (real && s < parts) ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * ((slot0 + s) * kCtaRows + r)));
+            float m = ml.y > 0.0f ? ml.x : -INFINITY;
+#pragma unroll
+            for (int o = 4; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            float w = ml.y > 0.0f ? exp2f(ml.x - m) : 0.0f;
+            if (ml.y != ml.y) w = ml.y;      // a NaN counts whatever its part's maximum, which no NaN raises
+            float sum = w != 0.0f ? w * ml.y : 0.0f;
+#pragma unroll
+            for (int o = 4; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+            wts[r * kFewJoined + s] = w;
+            if (s == 0) {
+                const bool any = sum > 0.0f || sum != sum;
+                invs[r] = any ? p.out_scale / sum : 0.0f;
+                if (p.lse && real && part == 0)      // (row = token x heads + head)
+                    p.lse[static_cast<int64_t>(seq.first) * p.heads + kCtaRows * k + r] = any ? 0.69314718055994531f * (m + log2f(sum)) : -INFINITY;
+            }
+        }
+        __syncthreads();
+        float acc[kFewGroup];
+        int g = 0, s = 0;
+#pragma unroll 1
+        for (int first = 0; first < pieces; first += kFewPieces) {
+            if (first > 0) ask(first);
+#pragma unroll
+            for (int j = 0; j < kFewPieces; ++j) {
+                if (first + j < pieces) {
+                    const float* w = wts + kFewGroup * (part + g * parts) * kFewJoined;
+                    if (s == 0) {
+                        uint32_t o[8];
+                        tmem_ld8(o_addr + kFewGroup * (part + g * parts), o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < kFewGroup; ++i) acc[i] = w[i * kFewJoined + part] * __uint_as_float(o[i]);
+                    }
+                    const int from = s + (s >= part);
+                    const float x[kFewGroup] = {v[j][0].x, v[j][0].y, v[j][0].z, v[j][0].w, v[j][1].x, v[j][1].y, v[j][1].z, v[j][1].w};
+#pragma unroll
+                    for (int i = 0; i < kFewGroup; ++i) acc[i] = fmaf(w[i * kFewJoined + from], x[i], acc[i]);
+                    if (++s == others) {
+#pragma unroll
+                        for (int i = 0; i < kFewGroup; ++i)
+                            rows[(kFewGroup * g + i) * kLatent + few_dim(c)] = __float2bfloat16_rn(acc[i] * invs[kFewGroup * (part + g * parts) + i]);
+                        s = 0;
+                        ++g;
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        for (int i = tid; i < mine * kFewGroup * (kLatent / 8); i += kFewThreads) {
+            const int r = i / (kLatent / 8), d = 8 * (i % (kLatent / 8)), row = kFewGroup * (part + r / kFewGroup * parts) + r % kFewGroup;
+            if (row >= u.rows) continue;
+            const int grow = kCtaRows * k + row, tok = token_of(p, grow), head = grow - tok * p.heads;
+            *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(seq.first + tok) * p.o_st + static_cast<int64_t>(head) * p.o_sh + d) =
+                *reinterpret_cast<const uint4*>(rows + r * kLatent + d);
+        }
+    };
     if (!whole) {
         float* dst = p.part_o + (slot * (kCtaRows / kFewGroup) * kLatent + c) * kFewGroup;
 #pragma unroll
@@ -1737,7 +1836,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) mla_window_few_kernel(const __
             tmem_ld32(o_addr + kFewGroup * g, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) st_global_v8(dst + (g + i) * (kLatent * kFewGroup), o + 8 * i);
+            for (int i = 0; i < 4; ++i)
+                if (!kJoined || (g + i) % u.parts != part) st_global_v8(dst + (g + i) * (kLatent * kFewGroup), o + 8 * i);
+        }
+        if constexpr (kJoined) {
+            cluster_sync();
+            join_parts();
         }
     } else {
         // through shared memory (the latents' place: every product is done) to rows of the output
@@ -1962,13 +2066,70 @@ int launch_prefill(const PrefillParams& all, const PrefillPlan& pl, cudaStream_t
     return NVFP4KV_OK;
 }
 
+// How many clusters of n blocks of the kernel for few rows run at once (0: none, or not known).
+int few_clusters(int n) {
+    static int known[64][kFewJoined + 1];      // (one more than the number)
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (known[dev][n] == 0) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(n);
+        cfg.blockDim = dim3(kFewThreads);
+        cfg.dynamicSmemBytes = kFewSmemBytes;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = n;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        if (cudaOccupancyMaxActiveClusters(&clusters, mla_window_few_kernel<true>, &cfg) != cudaSuccess) {
+            (void)cudaGetLastError();
+            clusters = 0;
+        }
+        known[dev][n] = clusters + 1;
+    }
+    return known[dev][n] - 1;
+}
+
+// Whether the parts of a unit run as a cluster and merge themselves.  Where the CTAs fill most of the SMs, the
+// second kernel waits for the slowest of all and reads every part while no SM computes: 64 single tokens
+// of 64 heads in 2 parts 18.1 us against 20.6, 30 in 4 parts 18.3 against 19.3, 15 in 8 parts 18.6
+// against 22.1.  With fewer CTAs it is faster, its rows spread over more SMs (12 CTAs 15.7 against 16.9, 64
+// 17.3 against 17.9), and where a CTA's share is more than kFewPieces pieces (16 tokens in 6 parts 19.3
+// against 19.6).
+bool few_joined(int units, int parts) {
+    constexpr int kGroups = kCtaRows / kFewGroup;
+    return parts > 1 && parts <= kFewJoined && (kGroups + parts - 1) / parts * (parts - 1) <= kFewPieces &&
+           8 * units * parts >= 5 * device_sm_count() && units <= few_clusters(parts);
+}
+
 int launch_few(const PrefillParams& p, const PrefillPlan& pl, cudaStream_t st) {
-    const int rc = set_smem_limit<mla_window_few_kernel>(kFewSmemBytes);
+    int rc = set_smem_limit<mla_window_few_kernel<false>>(kFewSmemBytes);
+    if (rc == NVFP4KV_OK) rc = set_smem_limit<mla_window_few_kernel<true>>(kFewSmemBytes);
     if (rc != NVFP4KV_OK) return rc;
     const int units = p.batch * pl.few_units;
-    cudaError_t e = launch_dependent(mla_window_few_kernel, dim3(units * pl.few_parts), dim3(kFewThreads), kFewSmemBytes, st, p, pl.few_units, pl.few_parts);
-    if (e == cudaSuccess && pl.few_parts > 1)
-        e = launch_dependent(mla_window_few_combine_kernel, dim3(units * (kCtaRows / kFewGroup)), dim3(kLatent), 0, st, p, pl.few_units, pl.few_parts);
+    cudaError_t e;
+    if (few_joined(units, pl.few_parts)) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(units * pl.few_parts);
+        cfg.blockDim = dim3(kFewThreads);
+        cfg.dynamicSmemBytes = kFewSmemBytes;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = pl.few_parts;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+        e = cudaLaunchKernelEx(&cfg, mla_window_few_kernel<true>, p, pl.few_units, pl.few_parts);
+    } else {
+        e = launch_dependent(mla_window_few_kernel<false>, dim3(units * pl.few_parts), dim3(kFewThreads), kFewSmemBytes, st, p, pl.few_units, pl.few_parts);
+        if (e == cudaSuccess && pl.few_parts > 1)
+            e = launch_dependent(mla_window_few_combine_kernel, dim3(units * (kCtaRows / kFewGroup)), dim3(kLatent), 0, st, p, pl.few_units, pl.few_parts);
+    }
     if (e != cudaSuccess) return fail(NVFP4KV_ECUDA, "nvfp4kv_mla_prefill_window launch failed: %s", cudaGetErrorString(e));
     return check_launch("nvfp4kv_mla_prefill_window");
 }

@@ -280,6 +280,38 @@ def test_a_graph_follows_the_lengths_on_the_device(H):
     assert rt.device_errors() == 0
 
 
+# units of up to 64 rows in 2 to 8 parts each, with enough of them to fill most of the SMs; shorter sequences
+# among them have fewer parts, one or none
+JOINED = [
+    ([1] * 64, [250, 64, 1, 700] * 16, 64, 64, True, 200, 4), ([3] * 30, [900, 500, 3, 2, 0, 260] * 5, 20, 16, True, 500, 0),
+    ([1] * 15, [1100, 1500, 600] * 5, 64, 64, True, 1000, 20), ([1] * 24, [700, 130, 4000, 512] * 6, 64, 256, True, 600, 10),
+    ([64] * 37, [600] * 30 + [64, 100, 200, 300, 30, 0, 1], 1, 64, False, 300, 1), ([1, 0] * 50, [300, 300, 200, 64] * 25, 8, 1, True, 250, 4),
+    ([8] * 4, [500, 2000, 505, 700], 64, 64, True, 500, 0), ([1] * 19, [1300, 900] * 9 + [40], 63, 64, True, 800, 70),
+]
+
+
+@pytest.mark.parametrize("trim", [False, True])
+@pytest.mark.parametrize("new,ctx,H,page,rope,window,sinks", JOINED)
+def test_many_units_of_several_parts(new, ctx, H, page, rope, window, sinks, trim):
+    p = Windowed(new, ctx, H, page, rope, window, sinks, trim=trim, seed=len(new))
+    out, lse = p.run()
+    assert rt.device_errors() == 0
+    p.check(out, lse)
+    for _ in range(5):
+        again = p.run()
+        assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
+def test_missing_pages_and_nan_scales_in_some_parts():
+    p = Windowed([1] * 64, [250, 200, 255, 256] * 16, 64, 16, True, 250, 4, seed=8)
+    p.pool.view(-1, 288)[p.slots(3)[17], 256] = 0x7F        # a token of sequence 3's first part
+    p.tables[5, 12] = -1                                    # tokens 192 .. 207: the second part of sequence 5
+    p.tables[9, :8] = p.pages                               # all but what lies behind the window of its first part
+    out, lse = p.run()
+    assert rt.device_errors() == _lib.DEVERR_BAD_PAGE
+    p.check(out, lse)
+
+
 def test_what_follows_a_call_without_parts_reads_its_output():
     """Tables wide enough for several parts of a unit, sequences short enough for one: nothing is merged,
     and the next kernels still find the output."""
