@@ -1965,11 +1965,11 @@ PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_l
         // a unit's rows belong to at most `span` tokens, and see no more than the sinks and the window - 1 +
         // span last tokens up to its end, which is rounded up to a multiple of 64
         const int64_t by_rows = (num_heads + kUnitRows - 2) / num_heads + 1, span = by_rows < longest ? by_rows : longest;
-        // The kernels for few rows: where no sequence has more than one unit of 64 (64 single tokens of 64 heads
-        // with a window of 1,024 take 44.3 us there and 63.4 with an image, 16 of them 23.7 and 29.3, 256 121 and
-        // 313; with one of 16,384 a token takes 40 us either way and 16 of them 103 and 187), or there are no more
-        // than kFewWaves tiles an SM (4 x 8 tokens of 16 heads, 512: 17.9 us against 22.0; 8 x 16 of 32, 256, 192
-        // tiles: 23.4 and 27.5; 4 x 16 of 64, 512, 320 tiles: 31.2 and 28.4).  As many parts as there are SMs for.
+        // The kernels for few rows: where no sequence has more than one unit of 64 (single tokens of 64 heads with a
+        // window of 1,024: 1 takes 17.0 us there and 19.0 with an image, 16 23.5 and 32, 64 40 and 84, 256 115 and
+        // 312; with a window of 16,384 a token takes 40 us either way and 16 of them 103 and 187), or there are no
+        // more than kFewWaves tiles an SM (4 x 8 tokens of 16 heads, 512: 16.8 us against 22.3; 8 x 16 of 32, 256,
+        // 192 tiles: 22.3 and 27.5; 4 x 16 of 64, 512, 320 tiles: 28.4 and 28.4).  As many parts as there are SMs for.
         const int64_t rows = longest * num_heads, few_units = (rows + kCtaRows - 1) / kCtaRows;
         const int64_t of_64 = (num_heads + kCtaRows - 2) / num_heads + 1, few_span = of_64 < longest ? of_64 : longest;
         int64_t seen = static_cast<int64_t>(sinks) + window - 1 + few_span;
