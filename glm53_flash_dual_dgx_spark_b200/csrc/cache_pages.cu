@@ -512,7 +512,7 @@ __device__ __forceinline__ const int* stage_cu(const ExtendArgs& p, int* cu_s) {
 }
 
 // A step in one launch: the first block of a cluster plans, all of them write.  For steps of up to
-// kOneLaunch words of tables and rows: a launch less is 2.4 us of 24 on the host; on the GPU 16 tables of
+// kOneLaunch words of tables and rows: a launch less is 2.4 us of 19 on the host; on the GPU 16 tables of
 // 2,048 entries take 9.5 us so and 8.0 in two launches, 16 of 4,688 with 32,768 tokens 14.4 and 11, 480
 // prompts of 670,000 tokens 105 and 11.
 constexpr int kStepBlocks = 8;
