@@ -1080,8 +1080,8 @@ def trim_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, slots: torch.
                page_size: int, window: int = 0, sinks: int = 0) -> None:
     """Gives back pages of the sequences in ``slots`` that no later step reads, in place: with
     ``window`` those behind the window of the next token, but for the first ``sinks`` tokens (their
-    entries become -2), and those past the sequence's end (-1).  Where drafts may still be taken back,
-    give a window that is longer by their number."""
+    entries become -2), and those past the sequence's end (-1).  Where drafts may still be taken back, or
+    cached tokens asked for again, give a window that is longer by their number."""
     _require_cuda(block_tables, "block_tables")
     index, st = block_tables.get_device(), block_tables.stride()
     if not _tables(index, block_tables, st, seq_lens, slots, ref_counts):

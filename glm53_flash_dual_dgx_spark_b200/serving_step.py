@@ -87,8 +87,9 @@ def run(heads: int = 64, prompt: int = 700, steps: int = 3, chunk: int = 256, se
         T = sum(new)
         q, kv, kr = draw(T, heads, rt.LATENT + rt.ROPE), draw(T, rt.LATENT), draw(T, rt.ROPE)
         out = attend(cache, tables, q, max(new), cos_sin, positions, kv, kr, scale, axes, **seen)
-        if window:
-            rt.trim_pages(cache.tables, cache.lens, torch.tensor(slots, dtype=torch.int32, device=device), cache.refs, PAGE, **seen)
+        if window:      # (a token more than the next one sees: the reads below ask for the last one again)
+            rt.trim_pages(cache.tables, cache.lens, torch.tensor(slots, dtype=torch.int32, device=device), cache.refs, PAGE,
+                          window=window + 1, sinks=sinks)
         return out, q
 
     # chunked prefill of both prompts

@@ -210,7 +210,8 @@ int nvfp4kv_extend_workspace_ints(int num, int64_t num_slots, int64_t num_pages,
 /* Gives back pages of the sequences in slots[k] (k < num) that no later step reads: with window >
  * 0 those whose tokens are all at or past `sinks` and behind the window of the next token, at
  * position seq_len (their entries become NVFP4KV_PAGE_TRIMMED), and those that begin at or past
- * seq_len (-1).  Where tokens may still be taken back, window has to be longer by their number.
+ * seq_len (-1).  Where tokens may still be taken back or asked for again, window has to be longer by
+ * their number.
  * Bad slots and pages as in nvfp4kv_free_pages. */
 int nvfp4kv_trim_pages(int32_t* block_tables, int64_t tables_stride, int table_width, int64_t num_slots,
                        const int32_t* seq_lens, const int32_t* slots, int num, int page_size, int window,

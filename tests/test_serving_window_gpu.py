@@ -23,6 +23,15 @@ def test_serving_loop(heads, prompt, window, sinks, image):
     assert torch.equal(got["out"], whole["out"]) == (not window or prompt <= window)
 
 
+@pytest.mark.parametrize("window", [255, 256])
+def test_serving_loop_wherever_the_window_begins_in_a_page(window):
+    for prompt in range(500, 564, 3):
+        got = serving_step.run(heads=2, prompt=prompt, steps=3, window=window, sinks=4)
+        assert got["device_errors"] == 0 and got["fork_equals_parent"] and got["compaction_keeps_outputs"], prompt
+    got = serving_step.run(heads=2, prompt=700, steps=3, window=256, sinks=4)
+    assert got["device_errors"] == 0
+
+
 class Twin:
     """The same growing sequences twice: with pages placed on the device and trimmed behind the window, and
     in a pool where every sequence has its pages for good."""
