@@ -216,9 +216,10 @@ trim_pages_kernel(int32_t* tables, int64_t stride, int width, int64_t num_slots,
     }
     int32_t* row = tables + slot * stride;
     const int len = max(0, seq_lens[slot]);
-    const int end = len / page + (len % page != 0);                            // pages of the sequence
+    // (both within the table, so that a thread's index, of pages of one token too, stays an int)
+    const int end = min(width, len / page + (len % page != 0));                // pages of the sequence
     // pages [lo, hi): all of their tokens are sinks' successors and older than the window
-    const int lo = sinks / page + (sinks % page != 0), hi = window > 0 && len >= window ? (len - window + 1) / page : 0;
+    const int lo = min(width, sinks / page + (sinks % page != 0)), hi = window > 0 && len >= window ? (len - window + 1) / page : 0;
     auto take = [&](int j, int mark) {
         const int p = row[j];
         if (p >= 0 && atomicCAS(row + j, p, mark) == p) release_page(refs, num_pages, p, err);
