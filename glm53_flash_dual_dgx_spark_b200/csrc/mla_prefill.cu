@@ -1965,6 +1965,10 @@ constexpr size_t kImageCap = size_t(1) << 30;
 
 constexpr int64_t kFewWaves = 2;
 
+// Sequences end here at the latest: a position and what its tile, its image block or the rounding of a unit's end
+// adds to it (up to 256) stay an int.  A multiple of every page size.
+constexpr int kMostTokens = 0x7FFFF000;
+
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
 PrefillPlan make_prefill_plan(int batch, int total_q, int num_heads, int max_q_len, int max_seq_len, int window, int sinks) {
@@ -2189,7 +2193,8 @@ int prefill_call(const void* q, int64_t q_stride_t, int64_t q_stride_h, const ui
     p.q = static_cast<const __nv_bfloat16*>(q); p.q_st = q_stride_t; p.q_sh = q_stride_h;
     p.pool = pool; p.rope = static_cast<const uint16_t*>(rope_pool); p.num_pages = pool_rows / page_size;
     p.tables = tables; p.tables_stride = tables_stride; p.cu = cu_seqlens_q; p.seq_lens = seq_lens;
-    p.batch = batch; p.total_q = total_q; p.heads = num_heads; p.max_q_len = max_q_len; p.max_seq_len = max_seq_len;
+    p.batch = batch; p.total_q = total_q; p.heads = num_heads; p.max_q_len = max_q_len;
+    p.max_seq_len = max_seq_len < kMostTokens ? max_seq_len : kMostTokens;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
     p.scale_log2 = bmm1_scale * 1.4426950408889634f; p.out_scale = bmm2_scale;
     p.out = static_cast<__nv_bfloat16*>(out); p.o_st = out_stride_t; p.o_sh = out_stride_h;

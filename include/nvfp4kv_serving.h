@@ -92,8 +92,9 @@ int nvfp4kv_append_rope_rotated_axes(const void* k_pe, int64_t num_tokens, int64
  *    (the rope side-pool, may be NULL) dims [512, 576) meet its rows.
  * tables [batch, >= ceil(max_seq_len / page_size)] page ids (row stride tables_stride).
  *    seq_lens and cu_seqlens_q stay on the device; max_q_len and max_seq_len bound them.  What
- *    goes past them sets NVFP4KV_DEVERR_SEQ_LEN: a sequence ends at max_seq_len tokens, and of
- *    more than max_q_len new tokens only the first max_q_len get their rows of out and lse.
+ *    goes past them sets NVFP4KV_DEVERR_SEQ_LEN: a sequence ends at max_seq_len tokens (and at
+ *    2^31 - 4,096), and of more than max_q_len new tokens only the first max_q_len get their rows of
+ *    out and lse.
  * out: bf16 [total_q, num_heads, 512] with strides (out_stride_t, out_stride_h), multiples of
  *    8, 16-byte aligned: softmax(bmm1_scale * q.k) . v * bmm2_scale.  A row that sees no token
  *    is zeros.  lse (may be NULL): fp32 [total_q, num_heads], the natural log of the sum of
