@@ -640,6 +640,14 @@ def _require_on(index: int, t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must be on cuda:{index} like the others")
 
 
+def _whole(x, name: str) -> int:
+    """x as an int that is equal to it (half a token cut off a window would be none at all)."""
+    n = int(x)
+    if n != x:
+        raise TypeError(f"{name} must be whole numbers, not {x!r}")
+    return n
+
+
 def _vector(t: torch.Tensor) -> torch.Tensor:
     return t if t.dim() == 1 and t.is_contiguous() else t.reshape(-1).contiguous()
 
@@ -683,7 +691,7 @@ def rope_axes(sections, rotary_dim: int = ROPE, dealt: bool = False) -> tuple[in
     """The axis of each of the rotary_dim / 2 pairs, for ``axes`` of the rotary operators: sections[a]
     pairs turn by axis a (time, height, width ...; at most 4), in sections one after the other, or
     ``dealt``: a pair to each axis in turn that has some left."""
-    left = [int(n) for n in sections]
+    left = [_whole(n, "sections") for n in sections]
     if not 1 <= len(left) <= _lib.MAX_AXES or min(left) < 0 or 2 * sum(left) != rotary_dim:
         raise ValueError(f"sections must be 1 to {_lib.MAX_AXES} numbers of pairs that add up to rotary_dim / 2")
     if not dealt:
@@ -704,7 +712,7 @@ def _axes(axes, num: int, rotary_dim: int):
     """The host array of a call's pair axes."""
     array = _pair_axes.get((axes, num, rotary_dim)) if type(axes) is tuple else None
     if array is None:
-        axes = tuple(int(a) for a in axes)
+        axes = tuple(_whole(a, "axes") for a in axes)
         if len(axes) != rotary_dim // 2 or not all(0 <= a < num for a in axes):
             raise ValueError(f"axes must be {rotary_dim // 2} numbers in [0, {num}), one for each rotated pair")
         if len(_pair_axes) >= 256:
@@ -853,6 +861,14 @@ def write_nvfp4_rope_rotated(k_pe: torch.Tensor, rope_cache: torch.Tensor, slot_
 
 
 # ------------------------------------------------------------------ chunk attention
+def _window(window, sinks) -> tuple[int, int]:
+    """A window and its sinks as C ints (what is longer than a sequence hides nothing)."""
+    window, sinks = _whole(window, "window"), _whole(sinks, "sinks")
+    if window < 0 or sinks < 0 or (sinks and not window):
+        raise ValueError("window and sinks must be >= 0, and sinks need a window")
+    return min(window, 0x7FFFFFFF), min(sinks, 0x7FFFFFFF)
+
+
 def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: torch.Tensor | None,
                 kv_lora_rank: int, qk_rope_head_dim: int, block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor,
                 seq_lens: torch.Tensor, max_q_len: int, max_seq_len: int, out: torch.Tensor | None = None,
@@ -887,8 +903,8 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
             _require_on(query.get_device(), t, name)
     if isinstance(bmm1_scale, torch.Tensor) or isinstance(bmm2_scale, torch.Tensor):
         raise TypeError("bmm1_scale / bmm2_scale must be Python floats (a device scalar would need a sync)")
-    if (window or sinks) and (window <= 0 or sinks < 0):
-        raise ValueError("window and sinks must be >= 0, and sinks need a window")
+    if window or sinks:
+        window, sinks = _window(window, sinks)
     qs = query.stride()
     if query.dtype is not torch.bfloat16 or len(qs) != 3 or qs[2] != 1:
         raise ValueError("query must be bf16 [T, H, D] with a contiguous last dimension")
@@ -924,8 +940,6 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
         rope = rope_cache.data_ptr()
     lse = query.new_empty((T, H), dtype=torch.float32) if return_lse else None
     if T > 0 and B > 0:
-        if window:      # (as C ints: what is longer than a sequence hides nothing)
-            window, sinks = min(int(window), 0x7FFFFFFF), min(int(sinks), 0x7FFFFFFF)
         key = ("prefill", B, T, H, max_q_len, max_seq_len, window, sinks, index)
         need = _ws_sizes.get(key)
         if need is None:
@@ -1089,11 +1103,9 @@ def trim_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, slots: torch.
     S, width = block_tables.shape
     if seq_lens.numel() != S:
         raise ValueError("seq_lens must have one entry per row of block_tables")
-    if window < 0 or sinks < 0 or (sinks and not window):
-        raise ValueError("window and sinks must be >= 0, and sinks need a window")
+    window, sinks = _window(window, sinks)
     _call("nvfp4kv_trim_pages", index, block_tables.data_ptr(), st[0], width, S, seq_lens.data_ptr(), slots.data_ptr(),
-          slots.numel(), page_size, min(int(window), 0x7FFFFFFF), min(int(sinks), 0x7FFFFFFF), ref_counts.data_ptr(),
-          ref_counts.numel())
+          slots.numel(), page_size, window, sinks, ref_counts.data_ptr(), ref_counts.numel())
 
 
 def copy_pages(caches, src: torch.Tensor, dst: torch.Tensor) -> None:
