@@ -42,13 +42,6 @@ class Cache:
         return rt.extend_pages(self.tables, self.lens, torch.tensor(slots, dtype=torch.int32, device=dev),
                                torch.tensor(new, dtype=torch.int32, device=dev), self.refs, PAGE, sum(new))
 
-    def extend(self, slot: int, n: int) -> torch.Tensor:
-        """Pages for n more tokens of one sequence; their pool slots."""
-        tables = self.step([slot], [n])
-        if int(tables.cu_seqlens_q[1]) < n:
-            raise RuntimeError("the cache is full")
-        return tables.slot_mapping
-
 
 def attend(cache: Cache, tables: rt.StepTables, q, max_new, cos_sin, positions, kv_c, k_pe, scale, axes=None, window=0, sinks=0):
     """One layer's step for the new tokens of `tables`: append, rotate, attend."""
@@ -92,6 +85,10 @@ def run(heads: int = 64, prompt: int = 700, steps: int = 3, chunk: int = 256, se
                           window=window + 1, sinks=sinks)
         return out, q
 
+    def check(want):      # (a request that finds no page is skipped; looked at after many steps, since it waits for the device)
+        if cache.lens.tolist() != want:
+            raise RuntimeError(f"the cache is full: sequences of {cache.lens.tolist()} tokens instead of {want}")
+
     # chunked prefill of both prompts
     done = [0, 0]
     while done != lens:
@@ -99,6 +96,7 @@ def run(heads: int = 64, prompt: int = 700, steps: int = 3, chunk: int = 256, se
         slots = [s for s, n in enumerate(new) if n]
         out, q = step(slots, [n for n in new if n])
         done = [d + n for d, n in zip(done, new)]
+    check(lens + [0] * samples)
     # samples of the first prompt: full pages shared, the last one copied
     src = torch.zeros(samples, dtype=torch.int32, device=device)
     dst = torch.arange(2, 2 + samples, dtype=torch.int32, device=device)
@@ -109,6 +107,7 @@ def run(heads: int = 64, prompt: int = 700, steps: int = 3, chunk: int = 256, se
     shared = int((cache.refs > 1).sum())
     for _ in range(steps):                      # every sequence decodes a token
         step(list(range(2 + samples)), [1] * (2 + samples))
+    check([n + steps for n in lens + [prompt] * samples])
     # the second prompt and two samples end; the rest moves to the front of the pool
     before = read(cache, [0, 2], torch.cat([probe, probe]), [1, 1], scale, **seen)
     rt.free_pages(cache.tables, cache.lens, torch.tensor([1, 3, 4], dtype=torch.int32, device=device), cache.refs)
