@@ -1100,9 +1100,10 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         bool first_part = true;
         griddep_wait();                          // the image kernel's token bits
         // bits of the quarter's tokens that exist, and of those that hold a NaN: loaded a tile ahead, a part's
-        // first ones while the last PV of the part before runs
-        auto load_bits = [&](const volatile Part& t, int i, uint2 (&w)[2]) {
-            const int tok0 = (t.tile0 + i) * kTile + 64 * q4;
+        // first ones while the last PV of the part before runs (without a window with the part's place in
+        // registers: read from `t` it held up every tile, 2,048 tokens of 64 heads over 16,384 2,898 us against 2,891)
+        auto load_bits = [&](const volatile Part& t, int tile0, int image, int L, int i, uint2 (&w)[2]) {
+            const int tok0 = ((kWindow ? t.tile0 : tile0) + i) * kTile + 64 * q4;
             if constexpr (kWindow) {
                 const int row0 = min(tok0 < p.sink_rows ? tok0 : tok0 + t.lift, t.image_rows - 1);
                 const uint32_t* src = p.image_bits + 8 * static_cast<int64_t>(t.image + row0 / kImageTok) + (row0 & 64) / 32;
@@ -1110,7 +1111,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
                 w[1] = *reinterpret_cast<const uint2*>(src + 4);
                 return;
             }
-            const uint32_t* src = p.image_bits + 8 * static_cast<int64_t>(t.image + min(tok0, t.L - 1) / kImageTok) + ((tok0 & (kImageTok - 1)) >> 5);
+            const uint32_t* src = p.image_bits + 8 * static_cast<int64_t>(image + min(tok0, L - 1) / kImageTok) + ((tok0 & (kImageTok - 1)) >> 5);
             w[0] = *reinterpret_cast<const uint2*>(src);
             w[1] = *reinterpret_cast<const uint2*>(src + 4);
         };
@@ -1118,19 +1119,19 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
         const volatile Part& next = work->ahead;
 #pragma unroll 1
         while (advance_part(work)) {
-            const int n_tiles = t.n_tiles, tile0 = t.tile0, gap = kWindow ? t.gap : 0;
+            const int n_tiles = t.n_tiles, tile0 = t.tile0, image = t.image, L = t.L, gap = kWindow ? t.gap : 0;
             int lim = 0;                                                      // tokens the row sees
             {
                 const int grow = t.block * kUnitRows + t.half * cta + row;    // row of the sequence
                 if (grow < t.rows && row < t.half) lim = min(t.L, t.L - t.n + token_of(p, grow) + 1);
             }
             float factor = kForm == kDirect ? p.factor : 1.0f, m_ref = -INFINITY, l = 0.0f;
-            if (first_part && n_tiles > 0) load_bits(t, 0, ahead);
+            if (first_part && n_tiles > 0) load_bits(t, tile0, image, L, 0, ahead);
 #pragma unroll 1
             for (int i = 0; i < n_tiles; ++i, ++tile) {
                 uint2 have = ahead[0];
                 const uint2 nan = ahead[1];
-                if (i + 1 < n_tiles) load_bits(t, i + 1, ahead);
+                if (i + 1 < n_tiles) load_bits(t, tile0, image, L, i + 1, ahead);
                 int see = lim - ((tile0 + i) * kTile + 64 * q4);     // tokens of the quarter the row sees
                 if constexpr (kWindow) {
                     if (lim - see >= p.sink_rows) see -= gap;
@@ -1215,7 +1216,7 @@ mla_prefill_kernel(const __grid_constant__ PrefillParams p) {
             }
             look_ahead<kWindow>(p, work);                        // (the last PV is running)
             __syncwarp();
-            if (*reinterpret_cast<volatile int*>(&work->more) && next.n_tiles > 0) load_bits(next, 0, ahead);
+            if (*reinterpret_cast<volatile int*>(&work->more) && next.n_tiles > 0) load_bits(next, next.tile0, next.image, next.L, 0, ahead);
             // ---- epilogue: sums over the row's four warps, O out of TMEM
             named_bar_sync(1 + (sp & 1), 128);          // the last part's sums are read
             lsum[64 * q4 + row] = l;
