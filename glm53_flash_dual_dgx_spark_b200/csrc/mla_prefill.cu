@@ -72,7 +72,8 @@ constexpr int kRope = NVFP4KV_ROPE;
 // The kernels' forms.  kAll: every token up to a row's own.  kDirect: a window and sinks; units are short,
 // so Q stays bf16 and goes from q straight into its operand (converted as in kAll, it was what they waited
 // for: 10,000 cycles of 32,600 a unit of three tiles), and the image holds every latent twice, in bf16
-// for QK and in fp16 for PV.
+// for QK and in fp16 for PV.  Without a power of two per row, products of the latent part stay within fp32 for
+// queries up to 2^106 (values up to 2,688, 512 of them) and keep all their bits down to 2^-92.
 enum Form { kAll, kDirect };
 constexpr int kDim = kLatent + kRope;
 constexpr int kUnitRows = 128;                  // query rows of a unit

@@ -197,9 +197,9 @@ constexpr int kRopeSteps = 2;
 // A unit is a 16-byte vector of a head (a rotated one of the half layout: the pair of vectors that
 // turn together).  The units of the call are dealt flat, two to a thread and 256 apart: every warp
 // moves 512 contiguous bytes, every block is full, and two loads in flight per thread are enough at
-// the occupancy that leaves (8,192 tokens x 64 heads x 576 bf16, 1.2 GB: 181 us = 6.7 TB/s, as much
-// as a plain copy; 8 % more with one, 1 % more with four, 20 % more with blocks of whole heads, whose
-// last steps are part empty).  The gradient of 2,049 tokens x 32 heads x 128 fp32 takes 10 us.
+// the occupancy that leaves (8,192 tokens x 64 heads x 576 bf16, 1.2 GB: 180 us = 6.7 TB/s, where a
+// plain copy of the same tensors takes 184.5; 8 % more with one, 1 % more with four, 20 % more with
+// blocks of whole heads, whose last steps are part empty).  The gradient of 2,049 tokens x 32 heads x 128 fp32 takes 10 us.
 //
 // With several axes the vectors are marked as streaming: with new inputs each time, 8,192 tokens x 32
 // heads x 128 bf16 26.1 -> 24.4 us, the gradient of 2,049 x 20 x 192 fp32 14.9 -> 12.4 (marks on the
@@ -269,7 +269,8 @@ __global__ void __launch_bounds__(256, kAxes ? (kInterleaved ? 8 : 6) : (kInterl
 // Any strides, alignment and sizes: one element (a rotated dim: its pair) per thread and step, for rows
 // that no 16-byte access can take (views at an odd offset, heads of odd sizes).  It is bound by its
 // 2- or 4-byte accesses and a division per element: 8,192 tokens x 64 heads x 192 bf16, shifted by 3,
-// take 388 us where the bytes take 62 (1.0 TB/s; fp32 2.1).  A caller that can align its rows should.
+// take 395 us where the bytes take 62 (1.0 TB/s; fp32 2.1), with three axes, whose positions every pair
+// looks up, 510.  A caller that can align its rows should.
 template <typename T, bool kInterleaved, bool kAxes>
 __global__ void __launch_bounds__(256) rope_elem_kernel(const __grid_constant__ RopeArgs p, int head_blocks, int heads_per_block) {
     const int64_t t = blockIdx.x / head_blocks;

@@ -889,7 +889,8 @@ def mla_prefill(query: torch.Tensor, kv_cache: torch.Tensor, workspace_buffer: t
     was in ``out`` before, and anything where the call allocates it.
 
     ``window`` > 0: the query at position p sees only tokens t > p - window, and the first ``sinks``
-    of its sequence.  What no new token sees is not read, and its pages may be gone (trim_pages)."""
+    of its sequence.  What no new token sees is not read, and its pages may be gone (trim_pages).
+    A call of many rows then takes the queries as they are: past 2^106 products can pass fp32's range."""
     try:      # (the whole host side of a call is about as long as a short batch on the device)
         index = query.get_device()
         together = index >= 0 and kv_cache.get_device() == block_tables.get_device() == cu_seqlens_q.get_device() \

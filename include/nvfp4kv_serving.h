@@ -127,6 +127,8 @@ int nvfp4kv_mla_prefill_workspace_size(int batch, int total_q, int num_heads, in
  * window, and those with t < sinks.  window >= 1, sinks >= 0.  Tokens that no query of the call
  * sees are never read, and their pages may be missing (nvfp4kv_trim_pages gives them back) without
  * an error.  The workspace holds images of what the windows cover, not of whole contexts.
+ * Where there are images (many query rows), q is used as it is, without the power of two that each row
+ * is scaled by elsewhere: queries past 2^106 can pass fp32's range there.
  */
 int nvfp4kv_mla_prefill_window(const void* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* pool,
                                int64_t pool_rows, const void* rope_pool, const int32_t* tables,
